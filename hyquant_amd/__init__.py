@@ -1,7 +1,8 @@
 """MI355X-native (gfx950) implementation of HyQuant's hybrid-precision
 attention hot path: per-token KV quantisation (2/4/8 bits), the fused
 four-segment split-K decode, the vertical-line selector, the freeze / flush
-of the decode cache and the hybrid INT8-QK prefill, exposed through the C ABI
+of the decode cache, the hybrid INT8-QK prefill and a paged 4-bit cache with
+the attention that reads it, exposed through the C ABI
 of libhyq.so (include/hyq.h)."""
 
 from .decode_d_stage import (  # noqa: F401
@@ -26,6 +27,13 @@ from .d_stage_cache import (  # noqa: F401
     splitk_decode_attention_k4v4,
     splitk_decode_attention_k4v4_mma,
 )
+from .paged import (  # noqa: F401
+    PagedBatch,
+    paged_append,
+    paged_attention,
+    paged_batch,
+    paged_gather,
+)
 from .cache_io import load_cache, save_cache  # noqa: F401
 
 __all__ = [
@@ -47,4 +55,9 @@ __all__ = [
     "splitk_decode_attention_k4v4",
     "splitk_decode_attention_k4v4_mma",
     "d_stage_decode_attention",
+    "PagedBatch",
+    "paged_batch",
+    "paged_append",
+    "paged_gather",
+    "paged_attention",
 ]

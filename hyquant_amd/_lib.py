@@ -55,6 +55,11 @@ EXPORTS = (
     "hyq_prefill_hybrid",
     "hyq_prefill_unified",
     "hyq_prefill_hybrid_fp8qk",
+    "hyq_paged_batch",
+    "hyq_paged_append",
+    "hyq_paged_gather",
+    "hyq_paged_attention_workspace_size",
+    "hyq_paged_attention",
 )
 
 
@@ -113,6 +118,24 @@ class PrefillParams(Structure):
         ("window", c_int32), ("smooth_k", c_int32), ("pv_mode", c_int32),
         ("sm_scale", c_double),
         ("dtype_fp16", c_int32),
+    ]
+
+
+class PagedParams(Structure):
+    """Mirror of `hyq_paged_params` (include/hyq.h)."""
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+        ("out", c_void_p), ("o_stride_t", c_int64), ("o_stride_h", c_int64),
+        ("lse", c_void_p),
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("p_stride_page", c_int64), ("p_stride_head", c_int64),
+        ("k_scale", c_void_p), ("v_scale", c_void_p), ("s_stride_page", c_int64), ("s_stride_head", c_int64),
+        ("block_table", c_void_p), ("bt_stride", c_int64),
+        ("seq_lens", c_void_p), ("cu_seqlens", c_void_p),
+        ("num_pages", c_int64),
+        ("page_size", c_int32), ("max_pages", c_int32), ("num_requests", c_int32), ("num_tokens", c_int32),
+        ("kv_heads", c_int32), ("kv_repeat", c_int32), ("head_dim", c_int32), ("window", c_int32),
+        ("sm_scale", c_float),
+        ("dtype_fp16", c_int32), ("zero_tail", c_int32),
     ]
 
 
@@ -187,6 +210,19 @@ def _declare(lib):
     lib.hyq_prefill_unified.argtypes = [POINTER(PrefillParams), c_void_p, c_size_t, c_void_p]
     lib.hyq_prefill_hybrid_fp8qk.restype = c_int
     lib.hyq_prefill_hybrid_fp8qk.argtypes = [POINTER(PrefillParams), c_void_p, c_size_t, c_void_p]
+    lib.hyq_paged_batch.restype = c_int
+    lib.hyq_paged_batch.argtypes = [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32,
+                                    c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.hyq_paged_append.restype = c_int
+    lib.hyq_paged_append.argtypes = ([c_void_p, c_int64, c_int64] * 2 + [c_int32, c_void_p, c_int64, c_int32, c_int32]
+                                     + [c_void_p, c_void_p, c_int64, c_int64] * 2 + [c_int64, c_int32, c_void_p])
+    lib.hyq_paged_gather.restype = c_int
+    lib.hyq_paged_gather.argtypes = ([c_void_p, c_int64, c_int32, c_int32] + [c_void_p, c_void_p, c_int64, c_int64] * 2
+                                     + [c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p])
+    lib.hyq_paged_attention_workspace_size.restype = c_size_t
+    lib.hyq_paged_attention_workspace_size.argtypes = [POINTER(PagedParams)]
+    lib.hyq_paged_attention.restype = c_int
+    lib.hyq_paged_attention.argtypes = [POINTER(PagedParams), c_void_p, c_size_t, c_void_p]
 
 
 def lib():

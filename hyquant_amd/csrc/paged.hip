@@ -1,0 +1,953 @@
+// The paged 4-bit KV cache: batch layout, append, read-back and attention
+// over block tables.
+//
+// Cache: int8 [pages, key heads, page, D/2] codes of hyq_quant_pack's 4-bit
+// format (the even channel in the low nibble) and fp16 [pages, key heads,
+// page] scales, K and V alike; token j of request r sits in page
+// block_table[r][j / page] at row j % page.  Pages are a power of two of 16
+// to 256 tokens, so a 16-token tile never crosses a page and every tile's
+// rows are one base address plus 32-bit lane offsets; bases are 64-bit.
+#include "hyq_common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace hyq {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int MAX_REQUESTS = 16384;      // two int32 prefix arrays of a batch fit in LDS
+constexpr int MIN_PAGE = 16, MAX_PAGE = 256;
+
+bool ok_page(int page) { return page >= MIN_PAGE && page <= MAX_PAGE && (page & (page - 1)) == 0; }
+int log2i(int x) {
+    int l = 0;
+    while ((1 << l) < x) ++l;
+    return l;
+}
+
+// ---------------------------------------------------------------------------
+// batch layout
+// ---------------------------------------------------------------------------
+// cu = prefix sums of the new tokens, first = prefix sums of the pages that
+// each request takes, ceil(len / page) - ceil(ctx / page); token t of request
+// r has position ctx_r + t - cu_r.  Every workgroup scans the R lengths by
+// itself (they stay in the L2) and keeps both prefix arrays in LDS, so the
+// layout is one launch; token and page entries then find their request by a
+// binary search.  A new page's id comes from the free list, never from the
+// table entry another workgroup writes.  Bound: the chain lengths -> scan ->
+// search -> table -> store, a few microseconds.
+constexpr int BT = 256;                  // threads
+constexpr int BATCH_TOKENS = 1024;       // tokens per workgroup
+
+struct BatchArgs {
+    const int32_t* ctx;
+    const int32_t* fresh;
+    int32_t* table;
+    int64_t bt_stride;
+    const int32_t* free_pages;
+    int32_t *cu, *lens, *used;
+    int64_t *slots, *positions;
+    int32_t R, max_pages, num_free, page_log2, tokens;
+};
+
+__device__ __forceinline__ int ceil_pages(int tokens, int page_log2) {
+    return static_cast<int>((static_cast<uint32_t>(tokens) + (1u << page_log2) - 1u) >> page_log2);
+}
+
+// the last i in [0, n] with a[i] <= x (a[0] <= x, a ascending)
+template <typename T>
+__device__ __forceinline__ int last_at_most(const T* a, int n, T x) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_incl_scan(T v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(BT) void paged_batch_kernel(BatchArgs a) {
+    extern __shared__ int32_t lds[];
+    int32_t* const cu = lds;                       // [R + 1]
+    int32_t* const first = lds + a.R + 1;          // [R + 1]
+    __shared__ int32_t wsum[2][BT / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int base_t = 0, base_p = 0;
+    for (int r0 = 0; r0 < a.R; r0 += BT) {
+        const int r = r0 + tid;
+        int n = 0, p = 0;
+        if (r < a.R) {
+            const int c = max(a.ctx[r], 0);
+            n = max(a.fresh[r], 0);
+            p = ceil_pages(c + n, a.page_log2) - ceil_pages(c, a.page_log2);
+        }
+        const int in = wave_incl_scan(n, lane), ip = wave_incl_scan(p, lane);
+        if (lane == 63) { wsum[0][w] = in; wsum[1][w] = ip; }
+        __syncthreads();
+        int bt = base_t, bp = base_p;
+#pragma unroll
+        for (int i = 0; i < BT / 64; ++i) {
+            if (i < w) { bt += wsum[0][i]; bp += wsum[1][i]; }
+            base_t += wsum[0][i];
+            base_p += wsum[1][i];
+        }
+        if (r < a.R) { cu[r] = bt + in - n; first[r] = bp + ip - p; }
+        __syncthreads();
+    }
+    if (tid == 0) { cu[a.R] = base_t; first[a.R] = base_p; }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int r = tid; r <= a.R; r += BT) {
+            a.cu[r] = cu[r];
+            if (r < a.R) a.lens[r] = max(a.ctx[r], 0) + max(a.fresh[r], 0);
+        }
+        if (tid == 0) a.used[0] = base_p;
+    }
+    // the pages taken: entry i of the free list goes to request r at table
+    // column ceil(ctx / page) + i - first[r]
+    for (int i = blockIdx.x * BT + tid; i < base_p; i += gridDim.x * BT) {
+        const int r = last_at_most(first, a.R - 1, i);
+        const int col = ceil_pages(max(a.ctx[r], 0), a.page_log2) + i - first[r];
+        if (static_cast<uint32_t>(col) < static_cast<uint32_t>(a.max_pages))
+            a.table[r * a.bt_stride + col] = i < a.num_free ? a.free_pages[i] : -1;
+    }
+    const int page = 1 << a.page_log2;
+    for (int t = blockIdx.x * BT + tid; t < a.tokens; t += gridDim.x * BT) {
+        int64_t slot = -1, pos = -1;
+        if (t < base_t) {
+            const int r = last_at_most(cu, a.R - 1, t);
+            const int c = max(a.ctx[r], 0);
+            const int x = c + t - cu[r];
+            const int col = x >> a.page_log2, old = ceil_pages(c, a.page_log2);
+            int id = -1;
+            if (static_cast<uint32_t>(col) < static_cast<uint32_t>(a.max_pages)) {
+                const int i = first[r] + col - old;
+                id = col < old ? a.table[r * a.bt_stride + col]
+                     : static_cast<uint32_t>(i) < static_cast<uint32_t>(a.num_free) ? a.free_pages[i] : -1;
+            }
+            pos = x;
+            if (id >= 0) slot = (static_cast<int64_t>(id) << a.page_log2) + (x & (page - 1));
+        }
+        a.slots[t] = slot;
+        a.positions[t] = pos;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// append and read back
+// ---------------------------------------------------------------------------
+struct RowArgs {
+    const uint16_t *k, *v;               // [tokens, key heads, D]
+    int64_t kt, kh, vt, vh;
+    uint16_t *ok, *ov;                   // the read-back's rows, contiguous
+    const int64_t* slots;
+    int8_t *kp, *vp;
+    int64_t ps_page, ps_head;
+    uint16_t *ks, *vs;
+    int64_t ss_page, ss_head;
+    int64_t num_slots;
+    uint32_t rows, heads;                // rows = tokens * heads
+    int32_t page_log2, lpt_log2;
+};
+
+// hyq_quant_pack's 4-bit rows (quant_row_codes) into their slots: D/8 lanes
+// of 8 channels own a row, blockIdx.y picks K or V, one launch for both.
+// HBM-bound: 2D bytes read and D/2 + 2 written per row.
+template <bool F16>
+__global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
+    const int lpt = 1 << a.lpt_log2, sub = threadIdx.x & (lpt - 1);
+    const uint32_t row = blockIdx.x * (256u >> a.lpt_log2) + (threadIdx.x >> a.lpt_log2);
+    const bool is_v = blockIdx.y != 0;
+    const uint32_t rr = row < a.rows ? row : a.rows - 1;
+    const uint32_t t = rr / a.heads, h = rr - t * a.heads;
+    const uint16_t* src = is_v ? a.v + t * a.vt + h * a.vh : a.k + t * a.kt + h * a.kh;
+    const int64_t slot = a.slots[t];
+    const uint4 raw = reinterpret_cast<const uint4*>(src)[sub];
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (F16) {
+            x[2 * i] = f16_bits_to_f32(static_cast<uint16_t>(w[i]));
+            x[2 * i + 1] = f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16));
+        } else {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    for (int m = 1; m < lpt; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
+    amax = fmaxf(amax, 1e-5f);
+    _Float16 s16;
+    uint32_t c[8];
+    quant_row_codes<4>(x, amax, s16, c);
+    if (row >= a.rows || slot < 0 || slot >= a.num_slots) return;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word |= (c[i] & 15u) << (4 * i);
+    const int64_t page = slot >> a.page_log2, off = slot & ((1 << a.page_log2) - 1);
+    int8_t* dst = (is_v ? a.vp : a.kp) + page * a.ps_page + h * a.ps_head + ((off * 4) << a.lpt_log2);
+    reinterpret_cast<uint32_t*>(dst)[sub] = word;
+    if (sub == 0) (is_v ? a.vs : a.ks)[page * a.ss_page + h * a.ss_head + off] = __builtin_bit_cast(uint16_t, s16);
+}
+
+// Rows of the cache by slot as bf16 or fp16 values, code * scale rounded once
+// (the product is exact in fp32); slots outside the pool give zero rows.
+// HBM-bound: D/2 + 2 bytes read and 2D written per row.
+template <bool F16>
+__global__ __launch_bounds__(256) void paged_gather_kernel(RowArgs a) {
+    const int lpt = 1 << a.lpt_log2, sub = threadIdx.x & (lpt - 1);
+    const uint32_t row = blockIdx.x * (256u >> a.lpt_log2) + (threadIdx.x >> a.lpt_log2);
+    if (row >= a.rows) return;
+    const bool is_v = blockIdx.y != 0;
+    const uint32_t t = row / a.heads, h = row - t * a.heads;
+    const int64_t slot = a.slots[t];
+    uint32_t o[4] = {0, 0, 0, 0};
+    if (slot >= 0 && slot < a.num_slots) {
+        const int64_t page = slot >> a.page_log2, off = slot & ((1 << a.page_log2) - 1);
+        const int8_t* src = (is_v ? a.vp : a.kp) + page * a.ps_page + h * a.ps_head + ((off * 4) << a.lpt_log2);
+        const uint32_t word = reinterpret_cast<const uint32_t*>(src)[sub];
+        const float s = f16_bits_to_f32((is_v ? a.vs : a.ks)[page * a.ss_page + h * a.ss_head + off]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = static_cast<float>(static_cast<int>(word << (28 - 8 * i)) >> 28) * s;
+            const float hi = static_cast<float>(static_cast<int>(word << (24 - 8 * i)) >> 28) * s;
+            o[i] = F16 ? f32_to_f16_bits(lo) | (static_cast<uint32_t>(f32_to_f16_bits(hi)) << 16) : pack_bf16x2(lo, hi);
+        }
+    }
+    reinterpret_cast<uint4*>((is_v ? a.ov : a.ok) + (static_cast<int64_t>(row) * 8 << a.lpt_log2))[sub] =
+        make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// ---------------------------------------------------------------------------
+// attention: the schedule
+// ---------------------------------------------------------------------------
+// Query rows of a request are its new tokens times the G query heads of a KV
+// head, row = token * G + head, cut into tiles of TILE rows; a tile's keys may
+// be cut into pieces, whose partial results a merge launch joins.  The
+// schedule is the same for every KV head (blockIdx.y of the attention).  It
+// is made on the device from the lengths, so that nothing is read back and a
+// captured graph follows the lengths it is replayed with.
+constexpr int TILE = 16;                 // query rows per tile
+constexpr int GROUP = 32;                // keys per wavefront step
+constexpr int PLAN_T = 1024;
+constexpr int SLOTS = 1024;              // pieces wanted over all KV heads while tiles are few
+constexpr int MIN_UNITS = 4;             // GROUP steps per piece, at least (one per wavefront)
+
+struct Item {
+    int32_t req, q0, qlen, len;          // request, its first token, its new tokens, its keys
+    int32_t row0;                        // first row of the tile within the request
+    int32_t key0, key1;                  // keys of this piece
+    int32_t part;                        // partial slot, -1: the tile is whole
+};
+struct Join {
+    int32_t q0, row0, rows, part, pieces, pad[3];
+};
+struct Counts {
+    int32_t items, joins, tokens, pad;   // tokens: those of all requests
+};
+
+struct PlanArgs {
+    const int32_t* lens;
+    const int32_t* cu;
+    int32_t R, T, G, window, capacity;   // capacity: keys that a block table row can name
+    int32_t target;                      // pieces per KV head wanted
+    int32_t max_items, max_parts, max_joins;
+    Counts* counts;
+    Item* items;
+    Join* joins;
+};
+
+struct Req {
+    int32_t q0, qlen, len, tiles, units; // units: the longest tile's GROUP-key steps
+};
+
+// first key that row position pos sees
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
+
+__device__ __forceinline__ Req request(const PlanArgs& a, int r) {
+    Req q{};
+    if (r >= a.R) return q;
+    q.q0 = r;
+    q.qlen = 1;
+    if (a.cu) {
+        q.q0 = min(max(a.cu[r], 0), a.T);
+        q.qlen = min(max(a.cu[r + 1], q.q0), a.T) - q.q0;
+    }
+    q.len = min(max(a.lens[r], 0), a.capacity);
+    const int rows = q.qlen * a.G;
+    q.tiles = (rows + TILE - 1) / TILE;
+    // the rows of a tile see at most window + TILE keys between them
+    const int keys = a.window > 0 && a.window < q.len - TILE ? a.window + TILE : q.len;
+    q.units = keys / GROUP + 2;          // from a GROUP boundary to a GROUP boundary
+    return q;
+}
+
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    if (lane == 0) red[w] = v;
+    __syncthreads();
+    int64_t s = 0;
+    for (int i = 0; i < PLAN_T / 64; ++i) s += red[i];
+    __syncthreads();
+    return s;
+}
+
+__global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
+    __shared__ int64_t red[PLAN_T / 64];
+    // items, partial slots and joins before each request of a round (64 bits:
+    // lengths that make no sense may add up to anything)
+    __shared__ int64_t start[3][PLAN_T + 1];
+    __shared__ int64_t wsum[3][PLAN_T / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int64_t work = 0;
+    for (int r = tid; r < a.R; r += PLAN_T) {
+        const Req q = request(a, r);
+        work += static_cast<int64_t>(q.tiles) * q.units;
+    }
+    work = block_sum(work, red);
+    const int64_t per = max(static_cast<int64_t>(MIN_UNITS), (work + a.target - 1) / a.target);   // units per piece
+    int64_t base[3] = {0, 0, 0};
+    for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
+        const Req q = request(a, r0 + tid);
+        const int64_t pieces = (q.units + per - 1) / per;
+        const int64_t n[3] = {q.tiles * pieces, pieces > 1 ? q.tiles * pieces : 0, pieces > 1 ? q.tiles : 0};
+        int64_t incl[3], total[3] = {0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            incl[k] = wave_incl_scan(n[k], lane);
+            if (lane == 63) wsum[k][w] = incl[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            int64_t before = 0;
+            for (int i = 0; i < PLAN_T / 64; ++i) {
+                if (i < w) before += wsum[k][i];
+                total[k] += wsum[k][i];
+            }
+            start[k][tid] = before + incl[k] - n[k];
+        }
+        __syncthreads();
+        const int nr = min(PLAN_T, a.R - r0);
+        for (int64_t i = tid; i < total[0] && base[0] + i < a.max_items; i += PLAN_T) {
+            const int k = last_at_most(start[0], nr - 1, i);
+            const Req x = request(a, r0 + k);
+            const int pc = static_cast<int>((x.units + per - 1) / per);
+            const int local = static_cast<int>(i - start[0][k]), tile = local / pc, piece = local - tile * pc;
+            const int row0 = tile * TILE, row1 = min(row0 + TILE, x.qlen * a.G);
+            const int p0 = x.len - x.qlen + row0 / a.G, p1 = x.len - x.qlen + (row1 - 1) / a.G;   // first and last position
+            const int lo = first_key(p0, a.window) / GROUP, hi = (max(p1, -1) + GROUP) / GROUP;   // GROUP steps
+            const int64_t steps = max(hi - lo, 0);
+            const int64_t part = base[1] + start[1][k] + local;
+            const bool split = pc > 1 && part < a.max_parts;
+            Item it{r0 + k, x.q0, x.qlen, x.len, row0, 0, 0, split ? static_cast<int>(part) : -1};
+            it.key0 = (lo + static_cast<int>(steps * piece / pc)) * GROUP;
+            it.key1 = min(p1 + 1, (lo + static_cast<int>(steps * (piece + 1) / pc)) * GROUP);
+            a.items[base[0] + i] = it;
+            const int64_t j = base[2] + start[2][k] + tile;
+            if (split && piece == 0 && j < a.max_joins)
+                a.joins[j] = Join{x.q0, row0, row1 - row0, it.part, pc, {0, 0, 0}};
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) base[k] += total[k];
+        __syncthreads();
+    }
+    if (tid == 0)
+        *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))),
+                           static_cast<int32_t>(min(base[2], static_cast<int64_t>(a.max_joins))), a.cu ? min(max(a.cu[a.R], 0), a.T) : a.T, 0};
+}
+
+// ---------------------------------------------------------------------------
+// attention: 16 query rows per workgroup
+// ---------------------------------------------------------------------------
+struct AttnArgs {
+    const uint16_t* q;
+    int64_t q_t, q_h;
+    uint16_t* out;
+    int64_t o_t, o_h;
+    float* lse;
+    int64_t l_t;
+    const int8_t *kp, *vp;
+    int64_t ps_page, ps_head;
+    const uint16_t *ks, *vs;
+    int64_t ss_page, ss_head;
+    const int32_t* table;
+    int64_t bt_stride;
+    const Counts* counts;
+    const Item* items;
+    const Join* joins;
+    float* part;                         // [slot][key head][TILE][D] sums, then [slot][key head][TILE][2] (m, l)
+    float* ml;
+    int32_t G, heads, page_log2, num_pages, window, tokens, zero_tail;
+    float scale;                         // sm_scale * log2(e)
+};
+
+constexpr float M_INIT = -1.0e30f;
+constexpr float SLACK = 8.0f;            // the running maximum moves when a score passes it by this (log2 units)
+constexpr int WAVES = 4;
+constexpr float LN2 = 0.69314718055994531f;
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+__device__ __forceinline__ uint32_t nib2(uint32_t x, int s, uint32_t magic) { return ((x >> s) & 0x000f000fu) ^ magic; }
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float xmax16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xmax32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float col_max(float v) { return xmax32(xmax16(v)); }
+__device__ __forceinline__ float col_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int I>
+__device__ __forceinline__ float quad_bcast(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), I * 0x55, 0xf, 0xf, true));
+}
+
+// 16-bit words of a row as floats (exact)
+template <bool F16>
+__device__ __forceinline__ float half_at(uint32_t w, int hi) {
+    if constexpr (F16) return f16_bits_to_f32(static_cast<uint16_t>(hi ? w >> 16 : w));
+    else return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+}
+
+// The power of two that brings the largest finite row maximum of a tile to
+// [2^14, 2^15), so that fp16 holds the queries exactly down to 2^-38 of it;
+// returned as the exponent to subtract, in [-100, 100].
+__device__ __forceinline__ int q_exponent(float amax) {
+    const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127;
+    return min(max(e, -100), 100) - 14;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+template <int D>
+struct Raw {
+    uint32_t k[2][D / 32];               // tile t: row c's channels (D/4) kb .. of token 16t + 4(c & 3) + (c >> 2)
+    uint32_t v[8];                       // slot e: token 4e + kb, 8 channels
+    uint32_t sk[2], sv[2];               // tile t: scale bits of token 16t + 4(c & 3) + kb
+    int first;                           // first token of the group
+    int ok;                              // bit t: tile t's page is inside the pool
+};
+
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
+    constexpr int NB = D / 16;           // PV products per group
+    constexpr int KW = D / 32;           // QK products (and K dwords) per tile
+    constexpr int ROWB = D / 2;          // packed bytes per token
+    __shared__ float red[WAVES][TILE][D + 4];
+    __shared__ float redm[WAVES][TILE], redl[WAVES][TILE];
+    if (static_cast<int>(blockIdx.x) >= a.counts->items) return;
+    const Item it = a.items[blockIdx.x];
+    const int head = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, kb = lane >> 4;
+    const int nrows = min(TILE, it.qlen * a.G - it.row0);
+
+    // ---- queries: B operands, row c's channels (D/4) kb + 8m + [0,4,1,5,2,6,3,7] ----
+    const int row = it.row0 + min(c, nrows - 1);
+    const int tok = row / a.G, hq = row - tok * a.G;
+    const uint16_t* qp = a.q + (static_cast<int64_t>(it.q0) + tok) * a.q_t + (static_cast<int64_t>(head) * a.G + hq) * a.q_h + (D / 4) * kb;
+    float amax = 0.f;
+    u32x4 qr[KW];
+#pragma unroll
+    for (int m = 0; m < KW; ++m) {
+        qr[m] = *reinterpret_cast<const u32x4*>(qp + 8 * m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(half_at<F16>(qr[m][i], 0)), fabsf(half_at<F16>(qr[m][i], 1))));
+    }
+    amax = col_max(amax);
+    if (!(amax < INFINITY)) amax = 0.f;
+    amax = max16_dpp(amax);
+    const int qe = q_exponent(amax);
+    const float qs = pow2(-qe);
+    f16x8 qop[KW];
+#pragma unroll
+    for (int m = 0; m < KW; ++m) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = half_at<F16>(qr[m][i >> 1], i & 1) * qs;
+        qop[m] = f16x8{static_cast<_Float16>(f[0]), static_cast<_Float16>(f[4]), static_cast<_Float16>(f[1]), static_cast<_Float16>(f[5]),
+                       static_cast<_Float16>(f[2]), static_cast<_Float16>(f[6]), static_cast<_Float16>(f[3]), static_cast<_Float16>(f[7])};
+    }
+    const float qk = a.scale * pow2(qe) * 16777216.0f;     // K operands are codes * 2^-24
+    f32x4 kbias = {0.f, 0.f, 0.f, 0.f};
+    {
+        const u32x4 half = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};
+#pragma unroll
+        for (int m = 0; m < KW; ++m) kbias = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, half), qop[m], kbias, 0, 0, 0);
+        kbias = -kbias;
+    }
+    // this lane's row sees the keys [lo, hi]
+    const int pos = it.len - it.qlen + tok;
+    const int lo = first_key(pos, a.window), hi = pos;
+    const int tok1 = (it.row0 + nrows - 1) / a.G;
+    const int all_hi = it.len - it.qlen + it.row0 / a.G;                    // every row sees keys up to here
+    const int all_lo = first_key(it.len - it.qlen + tok1, a.window);        // and from here
+
+    float m_run = M_INIT, l_run = 0.f;
+    f32x4 acc[NB], ones = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
+    const int page_mask = (1 << a.page_log2) - 1;
+    const int32_t* trow = a.table + it.req * a.bt_stride;
+    const int steps = (max(it.key1 - it.key0, 0) + GROUP - 1) / GROUP;
+    const int mine = steps > w && a.num_pages > 0 ? (steps - w + WAVES - 1) / WAVES : 0;       // this wavefront's groups w, w + 4, ...
+    const uint32_t klane = (4 * (c & 3) + (c >> 2)) * ROWB + (ROWB / 4) * kb;
+    const uint32_t vlane = kb * ROWB + (D == 128 ? 4 * c : 4 * (c & 7));
+    const uint32_t slane = (4 * (c & 3) + kb) * 2;
+
+    // page ids of this wavefront's next 32 groups, tile t of group i in lane 2i + t
+    auto ids_at = [&](int i0) -> int {
+        const int t = it.key0 + GROUP * (w + WAVES * (i0 + (lane >> 1))) + 16 * (lane & 1);
+        return trow[min(t, it.key1 - 1) >> a.page_log2];
+    };
+    int ids = mine > 0 ? ids_at(0) : 0;
+    auto load = [&](Raw<D>& r, int i) {
+        r.first = it.key0 + GROUP * (w + WAVES * i);
+        r.ok = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + t);
+            const bool ok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages);
+            r.ok |= ok ? 1 << t : 0;
+            const int64_t pg = ok ? id : 0;
+            const int t0 = (min(r.first + 16 * t, it.key1 - 1) & page_mask) & ~15;
+            const int8_t* kb_ = a.kp + pg * a.ps_page + hk + t0 * ROWB;
+            const int8_t* vb_ = a.vp + pg * a.ps_page + hk + t0 * ROWB;
+            if constexpr (D == 128) {
+                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb_ + klane));
+                r.k[t][0] = x[0]; r.k[t][1] = x[1]; r.k[t][2] = x[2]; r.k[t][3] = x[3];
+            } else {
+                const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kb_ + klane));
+                r.k[t][0] = x[0]; r.k[t][1] = x[1];
+            }
+            const char* ksb = reinterpret_cast<const char*>(a.ks + pg * a.ss_page + hs + t0);
+            const char* vsb = reinterpret_cast<const char*>(a.vs + pg * a.ss_page + hs + t0);
+            r.sk[t] = *reinterpret_cast<const uint16_t*>(ksb + slane);
+            r.sv[t] = *reinterpret_cast<const uint16_t*>(vsb + slane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                r.v[4 * t + e] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb_ + vlane + 4 * e * ROWB));
+        }
+    };
+    auto compute = [&](const Raw<D>& r) {
+        float s[8];
+        const float sk[2] = {f16_bits_to_f32(static_cast<uint16_t>(r.sk[0])) * qk, f16_bits_to_f32(static_cast<uint16_t>(r.sk[1])) * qk};
+        const float sv[2] = {f16_bits_to_f32(static_cast<uint16_t>(r.sv[0])), f16_bits_to_f32(static_cast<uint16_t>(r.sv[1]))};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 x = kbias;
+#pragma unroll
+            for (int m = 0; m < KW; ++m) {
+                const uint32_t kw = r.k[t][m];
+                const u32x4 o = {nib2(kw, 0, 0x00080008u), nib2(kw, 4, 0x00080008u), nib2(kw, 8, 0x00080008u), nib2(kw, 12, 0x00080008u)};
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, o), qop[m], x, 0, 0, 0);
+            }
+            s[4 * t + 0] = x[0] * quad_bcast<0>(sk[t]);
+            s[4 * t + 1] = x[1] * quad_bcast<1>(sk[t]);
+            s[4 * t + 2] = x[2] * quad_bcast<2>(sk[t]);
+            s[4 * t + 3] = x[3] * quad_bcast<3>(sk[t]);
+        }
+        // masked keys: behind the row's own position or before its window,
+        // past the piece, or in a page outside the pool.  Their scores and
+        // their P' are selected, not multiplied away: the scales there may be
+        // anything.
+        uint32_t dead = 0;
+        const bool edge = r.first + GROUP - 1 > min(all_hi, it.key1 - 1) || r.first < all_lo || r.ok != 3;
+        if (edge) {
+            const int top = min(hi, it.key1 - 1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int j = r.first + 4 * e + kb;
+                if (j > top || j < lo || !((r.ok >> (e >> 2)) & 1)) {
+                    s[e] = -INFINITY;
+                    dead |= 1u << e;
+                }
+            }
+        }
+        float mx = vmax3(s[0], s[1], s[2]);
+        mx = vmax3(mx, s[3], s[4]);
+        mx = vmax3(mx, s[5], s[6]);
+        mx = vmax2(mx, s[7]);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + SLACK)) {
+            mx = col_max(mx);
+            const float mnew = fmaxf(m_run, mx);
+            const float alpha = fast_exp2(m_run - mnew);
+            l_run *= alpha;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) acc[nb] *= alpha;
+            ones *= alpha;
+            m_run = mnew;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            s[e] = fast_exp2(s[e] - m_run);
+            l_run += s[e];
+        }
+        float p[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            p[4 * t + 0] = s[4 * t + 0] * quad_bcast<0>(sv[t]);
+            p[4 * t + 1] = s[4 * t + 1] * quad_bcast<1>(sv[t]);
+            p[4 * t + 2] = s[4 * t + 2] * quad_bcast<2>(sv[t]);
+            p[4 * t + 3] = s[4 * t + 3] * quad_bcast<3>(sv[t]);
+        }
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = (dead >> e) & 1 ? 0.f : p[e];
+        }
+        const u32x4 pw = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+        const bf16x8 pop = __builtin_bit_cast(bf16x8, pw);
+        bf16x8 plo;
+        if constexpr (F16) {             // an fp16 model's output keeps 11 bits: P' as the sum of two bf16 numbers
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] -= half_at<false>(pw[i >> 1], i & 1);
+            const u32x4 pl = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+            plo = __builtin_bit_cast(bf16x8, pl);
+        }
+        uint32_t vlo[4], vhi[4];
+#pragma unroll
+        for (int pr = 0; pr < 4; ++pr) {
+            uint32_t x = r.v[2 * pr], y = r.v[2 * pr + 1];
+            if constexpr (D == 64) {     // rows 8..15 of a product are the upper four channels of a dword
+                x = c >= 8 ? x >> 16 : x;
+                y = c >= 8 ? y >> 16 : y;
+            }
+            vlo[pr] = perm(y, x, 0x05040100u);
+            vhi[pr] = perm(y, x, 0x07060302u);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const uint32_t* src = nb < 4 ? vlo : vhi;
+            const int sh = 4 * (nb & 3);
+            const u32x4 o = {nib2(src[0], sh, 0x43084308u), nib2(src[1], sh, 0x43084308u), nib2(src[2], sh, 0x43084308u), nib2(src[3], sh, 0x43084308u)};
+            acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), pop, acc[nb], 0, 0, 0);
+            if constexpr (F16) acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), plo, acc[nb], 0, 0, 0);
+        }
+        const u32x4 onesw = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), pop, ones, 0, 0, 0);
+        if constexpr (F16) ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), plo, ones, 0, 0, 0);
+    };
+    Raw<D> r;
+    for (int i = 0; i < mine; ++i) {
+        if (i > 0 && (i & 31) == 0) ids = ids_at(i);
+        load(r, i);
+        compute(r);
+    }
+
+    // ---- the four wavefronts' results, joined through LDS ----
+    l_run = col_sum(l_run);
+    if (kb == 0) { redm[w][c] = m_run; redl[w][c] = l_run; }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * kb + i;
+            const int ch = D == 128 ? 8 * j + nb : 8 * (j & 7) + 4 * (j >> 3) + nb;
+            red[w][c][ch] = acc[nb][i] - 136.0f * ones[i];
+        }
+    __syncthreads();
+    for (int e = tid; e < nrows * (D / 4); e += 64 * WAVES) {
+        const int rw = e / (D / 4), ch = 4 * (e - rw * (D / 4));
+        float m = redm[0][rw];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) m = fmaxf(m, redm[i][rw]);
+        float l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            const float f = fast_exp2(redm[i][rw] - m);
+            l += f * redl[i][rw];
+            o += f * *reinterpret_cast<const f32x4*>(&red[i][rw][ch]);
+        }
+        if (it.part >= 0) {
+            const int64_t slot = static_cast<int64_t>(it.part) * a.heads + head;
+            *reinterpret_cast<f32x4*>(a.part + (slot * TILE + rw) * D + ch) = o;
+            if (ch == 0) { a.ml[(slot * TILE + rw) * 2] = m; a.ml[(slot * TILE + rw) * 2 + 1] = l; }
+        } else {
+            const int rr = it.row0 + rw, tk = rr / a.G;
+            const int64_t h = static_cast<int64_t>(head) * a.G + rr - tk * a.G, t = static_cast<int64_t>(it.q0) + tk;
+            const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;       // no key: zeros; NaN stays NaN
+            o *= inv;
+            u32x2 ow;
+            if constexpr (F16) {
+                ow[0] = f32_to_f16_bits(o[0]) | (static_cast<uint32_t>(f32_to_f16_bits(o[1])) << 16);
+                ow[1] = f32_to_f16_bits(o[2]) | (static_cast<uint32_t>(f32_to_f16_bits(o[3])) << 16);
+            } else {
+                ow[0] = pack_bf16x2(o[0], o[1]);
+                ow[1] = pack_bf16x2(o[2], o[3]);
+            }
+            *reinterpret_cast<u32x2*>(a.out + t * a.o_t + h * a.o_h + ch) = ow;
+            if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        }
+    }
+}
+
+// Joins the pieces of the split tiles: grid (joins, key heads), thread (row, 4
+// channels).  By zero_tail it also clears the rows behind the last request.
+template <int D, bool F16>
+__global__ __launch_bounds__(TILE * D / 4) void paged_join_kernel(AttnArgs a) {
+    if (a.zero_tail) {
+        const int64_t total = static_cast<int64_t>(a.tokens - a.counts->tokens) * a.G * (D / 4);   // of one KV head
+        for (int64_t e = static_cast<int64_t>(blockIdx.x) * (TILE * D / 4) + threadIdx.x; e < total; e += static_cast<int64_t>(gridDim.x) * (TILE * D / 4)) {
+            const int64_t row = e / (D / 4), t = row / a.G, h = blockIdx.y * static_cast<int64_t>(a.G) + row - t * a.G;
+            const int ch = 4 * static_cast<int>(e - row * (D / 4));
+            if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (a.counts->tokens + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
+            if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(a.counts->tokens + t) * a.l_t + h] = -INFINITY;
+        }
+    }
+    if (static_cast<int>(blockIdx.x) >= a.counts->joins) return;
+    const Join jn = a.joins[blockIdx.x];
+    const int head = blockIdx.y, rw = threadIdx.x / (D / 4), ch = 4 * (threadIdx.x - rw * (D / 4));
+    if (rw >= jn.rows) return;
+    float m = M_INIT;
+    for (int i = 0; i < jn.pieces; ++i) m = fmaxf(m, a.ml[(((static_cast<int64_t>(jn.part) + i) * a.heads + head) * TILE + rw) * 2]);
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < jn.pieces; ++i) {
+        const int64_t at = ((static_cast<int64_t>(jn.part) + i) * a.heads + head) * TILE + rw;
+        const float f = fast_exp2(a.ml[at * 2] - m);
+        l += f * a.ml[at * 2 + 1];
+        o += f * *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
+    }
+    const int rr = jn.row0 + rw, tk = rr / a.G;
+    const int64_t h = static_cast<int64_t>(head) * a.G + rr - tk * a.G, t = static_cast<int64_t>(jn.q0) + tk;
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+    o *= inv;
+    u32x2 ow;
+    if constexpr (F16) {
+        ow[0] = f32_to_f16_bits(o[0]) | (static_cast<uint32_t>(f32_to_f16_bits(o[1])) << 16);
+        ow[1] = f32_to_f16_bits(o[2]) | (static_cast<uint32_t>(f32_to_f16_bits(o[3])) << 16);
+    } else {
+        ow[0] = pack_bf16x2(o[0], o[1]);
+        ow[1] = pack_bf16x2(o[2], o[3]);
+    }
+    *reinterpret_cast<u32x2*>(a.out + t * a.o_t + h * a.o_h + ch) = ow;
+    if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct Sizes {
+    int64_t target, items, joins, parts;
+    size_t off_items, off_joins, off_part, off_ml, bytes;
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// A request's tiles are cut into ceil(units / per) pieces with per >=
+// total / target: at most target + tiles in all, at most 2 target of them in
+// tiles that are cut (units > per), which are at most target; the tiles are
+// at most rows / TILE + requests.
+Sizes sizes_of(const hyq_paged_params& p) {
+    Sizes s{};
+    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_repeat;
+    const int64_t tiles = rows / TILE + std::min<int64_t>(p.num_requests, p.num_tokens);
+    s.target = std::max<int64_t>(1, SLOTS / p.kv_heads);
+    s.items = s.target + tiles;
+    s.joins = std::min(tiles, s.target);
+    s.parts = std::min(s.items, 2 * s.target);
+    s.off_items = 256;
+    s.off_joins = up256(s.off_items + s.items * sizeof(Item));
+    s.off_part = up256(s.off_joins + s.joins * sizeof(Join));
+    s.off_ml = up256(s.off_part + static_cast<size_t>(s.parts) * p.kv_heads * TILE * p.head_dim * 4);
+    s.bytes = up256(s.off_ml + static_cast<size_t>(s.parts) * p.kv_heads * TILE * 2 * 4);
+    return s;
+}
+
+int check_pool(const char* what, int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t kv_heads, const void* kp,
+               const void* vp, const void* ks, const void* vs, int64_t ps_page, int64_t ps_head, int64_t ss_page,
+               int64_t ss_head) {
+    const std::string w = std::string(what) + ": ";
+    if (head_dim != 64 && head_dim != 128) return fail(HYQ_ENOTSUP, w + "head_dim must be 64 or 128, got " + std::to_string(head_dim));
+    if (!ok_page(page_size)) return fail(HYQ_ENOTSUP, w + "page_size must be a power of two from 16 to 256, got " + std::to_string(page_size));
+    if (num_pages < 0 || num_pages > (int64_t{1} << 30)) return fail(HYQ_EINVAL, w + "num_pages out of range");
+    if (kv_heads < 1 || kv_heads > 65535) return fail(HYQ_EINVAL, w + "key heads out of range");
+    if (num_pages == 0) return HYQ_OK;
+    if (!kp || !vp || !ks || !vs) return fail(HYQ_EINVAL, w + "null cache pointer");
+    if (!aligned(kp, 16) || !aligned(vp, 16) || ps_page % 16 || ps_head % 16)
+        return fail(HYQ_EINVAL, w + "code pages must be 16-byte aligned with strides divisible by 16");
+    if (!aligned(ks, 2) || !aligned(vs, 2)) return fail(HYQ_EINVAL, w + "scales misaligned");
+    return HYQ_OK;
+}
+
+int check_attention(const hyq_paged_params* p) {
+    const char* w = "hyq_paged_attention";
+    if (!p) return fail(HYQ_EINVAL, std::string(w) + ": null parameters");
+    const std::string s = std::string(w) + ": ";
+    if (int st = check_pool(w, p->head_dim, p->page_size, p->num_pages, p->kv_heads, p->k_pages, p->v_pages, p->k_scale, p->v_scale,
+                            p->p_stride_page, p->p_stride_head, p->s_stride_page, p->s_stride_head))
+        return st;
+    if (p->kv_repeat < 1 || p->kv_repeat > 1024) return fail(HYQ_ENOTSUP, s + "kv_repeat must be 1 to 1024");
+    if (p->num_requests < 0 || p->num_tokens < 0 || p->max_pages < 0 || p->window < 0)
+        return fail(HYQ_EINVAL, s + "negative size");
+    if (static_cast<int64_t>(p->num_tokens) * p->kv_repeat > (int64_t{1} << 30))
+        return fail(HYQ_ENOTSUP, s + "more than 2^30 query rows per key head");
+    if (static_cast<int64_t>(p->max_pages) * p->page_size > (int64_t{1} << 30))
+        return fail(HYQ_ENOTSUP, s + "a block table row names more than 2^30 tokens");
+    if (p->num_requests > (1 << 20)) return fail(HYQ_ENOTSUP, s + "more than 2^20 requests");
+    if (p->dtype_fp16 != 0 && p->dtype_fp16 != 1) return fail(HYQ_EINVAL, s + "dtype_fp16 must be 0 or 1");
+    if (p->zero_tail < 0 || p->zero_tail > 3) return fail(HYQ_EINVAL, s + "zero_tail must be 0 to 3");
+    if (!(p->sm_scale == p->sm_scale) || std::isinf(p->sm_scale)) return fail(HYQ_EINVAL, s + "sm_scale must be finite");
+    if (p->num_requests == 0 || p->num_tokens == 0) return HYQ_OK;
+    if (!p->cu_seqlens && p->num_tokens != p->num_requests)
+        return fail(HYQ_EINVAL, s + "without cu_seqlens every request has one token");
+    if (!p->q || !p->out || !p->seq_lens || (p->max_pages > 0 && !p->block_table)) return fail(HYQ_EINVAL, s + "null pointer");
+    if (!aligned(p->q, 16) || p->q_stride_t % 8 || p->q_stride_h % 8)
+        return fail(HYQ_EINVAL, s + "q must be 16-byte aligned with strides divisible by 8");
+    if (!aligned(p->out, 8) || p->o_stride_t % 4 || p->o_stride_h % 4)
+        return fail(HYQ_EINVAL, s + "out must be 8-byte aligned with strides divisible by 4");
+    if (!aligned(p->seq_lens, 4) || !aligned(p->cu_seqlens, 4) || !aligned(p->block_table, 4) || !aligned(p->lse, 4))
+        return fail(HYQ_EINVAL, s + "lengths, table and lse must be 4-byte aligned");
+    return HYQ_OK;
+}
+
+template <int D, bool F16>
+void launch_attention(const AttnArgs& a, const Sizes& s, hipStream_t st) {
+    paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
+    paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(s.joins), a.heads), dim3(TILE * D / 4), 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace hyq
+
+using namespace hyq;
+
+extern "C" int hyq_paged_batch(const int32_t* context_lens, const int32_t* new_lens, int32_t num_requests,
+                               int32_t* block_table, int64_t bt_stride, int32_t max_pages, const int32_t* free_pages,
+                               int32_t num_free, int32_t page_size, int32_t num_tokens, int32_t* cu_seqlens,
+                               int32_t* seq_lens, int64_t* slots, int64_t* positions, int32_t* pages_used, void* stream) {
+    if (num_requests < 0 || num_tokens < 0 || max_pages < 0 || num_free < 0) return fail(HYQ_EINVAL, "hyq_paged_batch: negative size");
+    if (num_requests > MAX_REQUESTS)
+        return fail(HYQ_ENOTSUP, "hyq_paged_batch: at most " + std::to_string(MAX_REQUESTS) + " requests, got " + std::to_string(num_requests));
+    if (!ok_page(page_size))
+        return fail(HYQ_ENOTSUP, "hyq_paged_batch: page_size must be a power of two from 16 to 256, got " + std::to_string(page_size));
+    if (!cu_seqlens || !pages_used || (num_requests && (!context_lens || !new_lens || !seq_lens)) ||
+        (num_requests && max_pages && !block_table) || (num_free && !free_pages) || (num_tokens && (!slots || !positions)))
+        return fail(HYQ_EINVAL, "hyq_paged_batch: null pointer");
+    if (!aligned(context_lens, 4) || !aligned(new_lens, 4) || !aligned(block_table, 4) || !aligned(free_pages, 4) ||
+        !aligned(cu_seqlens, 4) || !aligned(seq_lens, 4) || !aligned(pages_used, 4) || !aligned(slots, 8) || !aligned(positions, 8))
+        return fail(HYQ_EINVAL, "hyq_paged_batch: misaligned pointer");
+    BatchArgs a{context_lens, new_lens, block_table, bt_stride, free_pages, cu_seqlens, seq_lens, pages_used, slots, positions,
+                num_requests, max_pages, num_free, log2i(page_size), num_tokens};
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(512, 1 + (static_cast<int64_t>(num_tokens) - 1) / BATCH_TOKENS));
+    const size_t lds = 2 * (static_cast<size_t>(num_requests) + 1) * sizeof(int32_t);
+    if (lds > 64 * 1024 - 64)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_batch_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+    paged_batch_kernel<<<dim3(blocks), dim3(BT), lds, static_cast<hipStream_t>(stream)>>>(a);
+    return check_launch("hyq_paged_batch");
+}
+
+extern "C" int hyq_paged_append(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
+                                int64_t v_stride_h, int32_t is_fp16, const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
+                                int32_t head_dim, int8_t* k_pages, int8_t* v_pages, int64_t p_stride_page, int64_t p_stride_head,
+                                uint16_t* k_scale, uint16_t* v_scale, int64_t s_stride_page, int64_t s_stride_head,
+                                int64_t num_pages, int32_t page_size, void* stream) {
+    if (int st = check_pool("hyq_paged_append", head_dim, page_size, num_pages, kv_heads, k_pages, v_pages, k_scale, v_scale, p_stride_page,
+                            p_stride_head, s_stride_page, s_stride_head))
+        return st;
+    if (num_tokens < 0) return fail(HYQ_EINVAL, "hyq_paged_append: negative size");
+    if (is_fp16 != 0 && is_fp16 != 1) return fail(HYQ_EINVAL, "hyq_paged_append: is_fp16 must be 0 or 1");
+    if (num_tokens == 0 || num_pages == 0) return HYQ_OK;
+    if (!k || !v || !slots) return fail(HYQ_EINVAL, "hyq_paged_append: null pointer");
+    if (!aligned(k, 16) || !aligned(v, 16) || (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 || !aligned(slots, 8))
+        return fail(HYQ_EINVAL, "hyq_paged_append: rows must be 16-byte aligned with strides divisible by 8");
+    const int64_t rows = num_tokens * kv_heads;
+    if (num_tokens > (int64_t{1} << 30) || rows > (int64_t{1} << 30)) return fail(HYQ_ENOTSUP, "hyq_paged_append: more than 2^30 rows");
+    RowArgs a{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, nullptr, nullptr, slots, k_pages, v_pages, p_stride_page, p_stride_head,
+              k_scale, v_scale, s_stride_page, s_stride_head, num_pages * page_size, static_cast<uint32_t>(rows),
+              static_cast<uint32_t>(kv_heads), log2i(page_size), log2i(head_dim / 8)};
+    const int64_t per = 256 >> a.lpt_log2;
+    const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), 2);
+    if (is_fp16) paged_append_kernel<true><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+    else paged_append_kernel<false><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+    return check_launch("hyq_paged_append");
+}
+
+extern "C" int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads, int32_t head_dim, const int8_t* k_pages,
+                                const int8_t* v_pages, int64_t p_stride_page, int64_t p_stride_head, const uint16_t* k_scale,
+                                const uint16_t* v_scale, int64_t s_stride_page, int64_t s_stride_head, int64_t num_pages,
+                                int32_t page_size, int32_t out_fp16, uint16_t* k_out, uint16_t* v_out, void* stream) {
+    if (int st = check_pool("hyq_paged_gather", head_dim, page_size, num_pages, kv_heads, k_pages, v_pages, k_scale, v_scale, p_stride_page,
+                            p_stride_head, s_stride_page, s_stride_head))
+        return st;
+    if (num_tokens < 0) return fail(HYQ_EINVAL, "hyq_paged_gather: negative size");
+    if (out_fp16 != 0 && out_fp16 != 1) return fail(HYQ_EINVAL, "hyq_paged_gather: out_fp16 must be 0 or 1");
+    if (num_tokens == 0) return HYQ_OK;
+    if (!k_out || !v_out || !slots) return fail(HYQ_EINVAL, "hyq_paged_gather: null pointer");
+    if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(slots, 8)) return fail(HYQ_EINVAL, "hyq_paged_gather: misaligned pointer");
+    const int64_t rows = num_tokens * kv_heads;
+    if (num_tokens > (int64_t{1} << 30) || rows > (int64_t{1} << 30)) return fail(HYQ_ENOTSUP, "hyq_paged_gather: more than 2^30 rows");
+    RowArgs a{nullptr, nullptr, 0, 0, 0, 0, k_out, v_out, slots, const_cast<int8_t*>(k_pages), const_cast<int8_t*>(v_pages), p_stride_page,
+              p_stride_head, const_cast<uint16_t*>(k_scale), const_cast<uint16_t*>(v_scale), s_stride_page, s_stride_head,
+              num_pages * page_size, static_cast<uint32_t>(rows), static_cast<uint32_t>(kv_heads), log2i(page_size), log2i(head_dim / 8)};
+    const int64_t per = 256 >> a.lpt_log2;
+    const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), 2);
+    if (out_fp16) paged_gather_kernel<true><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+    else paged_gather_kernel<false><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+    return check_launch("hyq_paged_gather");
+}
+
+extern "C" size_t hyq_paged_attention_workspace_size(const hyq_paged_params* p) {
+    if (check_attention(p) != HYQ_OK || p->num_requests == 0 || p->num_tokens == 0) return 0;
+    return sizes_of(*p).bytes;
+}
+
+extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int st = check_attention(p)) return st;
+    if (p->num_requests == 0 || p->num_tokens == 0) return HYQ_OK;
+    const Sizes s = sizes_of(*p);
+    if (!workspace || workspace_bytes < s.bytes)
+        return fail(HYQ_ENOSPC, "hyq_paged_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(s.bytes) + " needed");
+    if (!aligned(workspace, 256)) return fail(HYQ_EINVAL, "hyq_paged_attention: workspace must be 256-byte aligned");
+    char* ws = static_cast<char*>(workspace);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    PlanArgs pl{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, p->window,
+                p->max_pages * p->page_size, static_cast<int32_t>(s.target), static_cast<int32_t>(s.items),
+                static_cast<int32_t>(s.parts), static_cast<int32_t>(s.joins), reinterpret_cast<Counts*>(ws), reinterpret_cast<Item*>(ws + s.off_items),
+                reinterpret_cast<Join*>(ws + s.off_joins)};
+    paged_plan_kernel<<<dim3(1), dim3(PLAN_T), 0, st>>>(pl);
+    AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
+               p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head, p->k_scale,
+               p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, pl.counts, pl.items, pl.joins,
+               reinterpret_cast<float*>(ws + s.off_part), reinterpret_cast<float*>(ws + s.off_ml), p->kv_repeat, p->kv_heads,
+               log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->num_tokens, p->zero_tail, p->sm_scale * 1.44269504f};
+    if (p->head_dim == 128) {
+        if (p->dtype_fp16) launch_attention<128, true>(a, s, st);
+        else launch_attention<128, false>(a, s, st);
+    } else {
+        if (p->dtype_fp16) launch_attention<64, true>(a, s, st);
+        else launch_attention<64, false>(a, s, st);
+    }
+    return check_launch("hyq_paged_attention");
+}

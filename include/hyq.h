@@ -397,6 +397,109 @@ int hyq_prefill_hybrid_fp8qk(const hyq_prefill_params* params, void* workspace, 
 int hyq_prefill_unified(const hyq_prefill_params* params, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/*
+ * The paged 4-bit KV cache (no counterpart in the reference, whose caches are
+ * one tensor per sequence, src/ops/d_stage_kv_cache.py): the keys and values
+ * of many requests in pages of a common pool,
+ *   k_pages, v_pages  int8 [num_pages, kv_heads, page_size, head_dim / 2], hyq_quant_pack's
+ *                     4-bit rows, strides (p_stride_page, p_stride_head, head_dim / 2), the
+ *                     same for K and V; 16-byte aligned, strides divisible by 16
+ *   k_scale, v_scale  fp16 [num_pages, kv_heads, page_size], strides (s_stride_page,
+ *                     s_stride_head, 1), the same for K and V
+ * page_size: a power of two from 16 to 256; head_dim 64 or 128.  Token j of
+ * request r is row j % page_size of page block_table[r][j / page_size]; its
+ * slot is that page's id * page_size + that row.
+ */
+
+/*
+ * The layout of a step's batch, from device lengths:
+ *   context_lens, new_lens  int32 [num_requests]: tokens a request has in the cache, and the
+ *                           tokens that this step adds (0 allowed); negative counts as 0
+ *   block_table  int32 [num_requests, max_pages] stride bt_stride: entries of the pages that a
+ *                request holds are read; the entries [ceil(ctx / page), ceil((ctx + new) /
+ *                page)) are written, the others left as they are
+ *   free_pages   int32 [num_free]: page ids, taken in order, request by request
+ * writes
+ *   cu_seqlens   int32 [num_requests + 1]  prefix sums of new_lens
+ *   seq_lens     int32 [num_requests]      context + new
+ *   slots, positions  int64 [num_tokens]   of each new token; -1 past the last
+ *   pages_used   int32 [1]                 pages that the step needs (also where that is more
+ *                                          than num_free: the entries of those that there are
+ *                                          not become -1, and so do their tokens' slots, as
+ *                                          where a row would need more than max_pages)
+ * Tokens past num_tokens are left out.  At most 16384 requests; the new
+ * lengths' sum below 2^31.
+ */
+int hyq_paged_batch(const int32_t* context_lens, const int32_t* new_lens, int32_t num_requests,
+                    int32_t* block_table, int64_t bt_stride, int32_t max_pages, const int32_t* free_pages,
+                    int32_t num_free, int32_t page_size, int32_t num_tokens, int32_t* cu_seqlens,
+                    int32_t* seq_lens, int64_t* slots, int64_t* positions, int32_t* pages_used, void* stream);
+
+/*
+ * New rows into their slots: bit for bit hyq_quant_pack's codes and scales.
+ *   k, v   bf16 (is_fp16 = 0) or fp16 [num_tokens, kv_heads, head_dim], strides (t, h, 1),
+ *          16-byte aligned, strides divisible by 8
+ *   slots  int64 [num_tokens]; a slot outside [0, num_pages * page_size) writes nothing.
+ *          Precondition: no slot is named twice (it would hold some mixture of the rows).
+ */
+int hyq_paged_append(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v,
+                     int64_t v_stride_t, int64_t v_stride_h, int32_t is_fp16, const int64_t* slots,
+                     int64_t num_tokens, int32_t kv_heads, int32_t head_dim, int8_t* k_pages, int8_t* v_pages,
+                     int64_t p_stride_page, int64_t p_stride_head, uint16_t* k_scale, uint16_t* v_scale,
+                     int64_t s_stride_page, int64_t s_stride_head, int64_t num_pages, int32_t page_size, void* stream);
+
+/*
+ * Rows of the cache by slot: k_out, v_out bf16 (out_fp16 = 0) or fp16
+ * [num_tokens, kv_heads, head_dim] contiguous = RNE(code * scale); zero rows
+ * for slots outside the pool.
+ */
+int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads, int32_t head_dim,
+                     const int8_t* k_pages, const int8_t* v_pages, int64_t p_stride_page, int64_t p_stride_head,
+                     const uint16_t* k_scale, const uint16_t* v_scale, int64_t s_stride_page, int64_t s_stride_head,
+                     int64_t num_pages, int32_t page_size, int32_t out_fp16, uint16_t* k_out, uint16_t* v_out,
+                     void* stream);
+
+/*
+ * Causal attention of a ragged batch of new tokens over the pages.  Request r
+ * has the tokens [cu_seqlens[r], cu_seqlens[r + 1]) of q (token r alone where
+ * cu_seqlens is NULL), the last of its seq_lens[r] cached tokens: its token i
+ * is at position p = seq_lens[r] - (its tokens) + i and sees the keys j <= p,
+ * with window > 0 only those with j > p - window:
+ *   out = softmax_j(sm_scale q . k_j) v_j,  lse = ln sum_j exp(sm_scale q . k_j)
+ * A row that sees no key is 0 (lse -inf).  The codes enter the products as
+ * exact operands: the K scale multiplies the fp32 score, the V scale the
+ * weight, which is then rounded to bf16 (for an fp16 model to the sum of two
+ * bf16 numbers).
+ *   q     bf16 or fp16 [num_tokens, kv_heads * kv_repeat, head_dim] strides (t, h, 1),
+ *         16-byte aligned, strides divisible by 8; out the same type, 8-byte aligned,
+ *         strides divisible by 4
+ *   lse   float [num_tokens, kv_heads * kv_repeat] contiguous, or NULL
+ * Lengths beyond max_pages * page_size count as that, negative ones as 0; keys
+ * in pages outside [0, num_pages) are left out; cu_seqlens is clamped to
+ * [0, num_tokens].  Rows of tokens behind the last request are left as they
+ * are, but with bit 0 of zero_tail out is set to 0 there, with bit 1 lse to -inf.
+ * The workspace needs no initialisation; calls that share one must be ordered
+ * on one stream.
+ */
+typedef struct hyq_paged_params {
+    const void* q; int64_t q_stride_t, q_stride_h;
+    void* out; int64_t o_stride_t, o_stride_h;
+    float* lse;
+    const int8_t* k_pages; const int8_t* v_pages; int64_t p_stride_page, p_stride_head;
+    const uint16_t* k_scale; const uint16_t* v_scale; int64_t s_stride_page, s_stride_head;
+    const int32_t* block_table; int64_t bt_stride;
+    const int32_t* seq_lens;
+    const int32_t* cu_seqlens;
+    int64_t num_pages;
+    int32_t page_size, max_pages, num_requests, num_tokens;
+    int32_t kv_heads, kv_repeat, head_dim, window;
+    float sm_scale;
+    int32_t dtype_fp16, zero_tail;
+} hyq_paged_params;
+
+size_t hyq_paged_attention_workspace_size(const hyq_paged_params* p);
+int hyq_paged_attention(const hyq_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
