@@ -238,176 +238,6 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(RowArgs a) {
         make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// ---------------------------------------------------------------------------
-// attention: the schedule
-// ---------------------------------------------------------------------------
-// Query rows of a request are its new tokens times the G query heads of a KV
-// head, row = token * G + head, cut into tiles of TILE rows; a tile's keys may
-// be cut into pieces, whose partial results a merge launch joins.  The
-// schedule is the same for every KV head (blockIdx.y of the attention).  It
-// is made on the device from the lengths, so that nothing is read back and a
-// captured graph follows the lengths it is replayed with.
-constexpr int TILE = 16;                 // query rows per tile
-constexpr int GROUP = 32;                // keys per wavefront step
-constexpr int PLAN_T = 1024;
-constexpr int SLOTS = 1024;              // pieces wanted over all KV heads while tiles are few
-constexpr int MIN_UNITS = 4;             // GROUP steps per piece, at least (one per wavefront)
-
-struct Item {
-    int32_t req, q0, qlen, len;          // request, its first token, its new tokens, its keys
-    int32_t row0;                        // first row of the tile within the request
-    int32_t key0, key1;                  // keys of this piece
-    int32_t part;                        // partial slot, -1: the tile is whole
-};
-struct Join {
-    int32_t q0, row0, rows, part, pieces, pad[3];
-};
-struct Counts {
-    int32_t items, joins, tokens, pad;   // tokens: those of all requests
-};
-
-struct PlanArgs {
-    const int32_t* lens;
-    const int32_t* cu;
-    int32_t R, T, G, window, capacity;   // capacity: keys that a block table row can name
-    int32_t target;                      // pieces per KV head wanted
-    int32_t max_items, max_parts, max_joins;
-    Counts* counts;
-    Item* items;
-    Join* joins;
-};
-
-struct Req {
-    int32_t q0, qlen, len, tiles, units; // units: the longest tile's GROUP-key steps
-};
-
-// first key that row position pos sees
-__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
-
-__device__ __forceinline__ Req request(const PlanArgs& a, int r) {
-    Req q{};
-    if (r >= a.R) return q;
-    q.q0 = r;
-    q.qlen = 1;
-    if (a.cu) {
-        q.q0 = min(max(a.cu[r], 0), a.T);
-        q.qlen = min(max(a.cu[r + 1], q.q0), a.T) - q.q0;
-    }
-    q.len = min(max(a.lens[r], 0), a.capacity);
-    const int rows = q.qlen * a.G;
-    q.tiles = (rows + TILE - 1) / TILE;
-    // the rows of a tile see at most window + TILE keys between them
-    const int keys = a.window > 0 && a.window < q.len - TILE ? a.window + TILE : q.len;
-    q.units = keys / GROUP + 2;          // from a GROUP boundary to a GROUP boundary
-    return q;
-}
-
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    if (lane == 0) red[w] = v;
-    __syncthreads();
-    int64_t s = 0;
-    for (int i = 0; i < PLAN_T / 64; ++i) s += red[i];
-    __syncthreads();
-    return s;
-}
-
-__global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
-    __shared__ int64_t red[PLAN_T / 64];
-    // items, partial slots and joins before each request of a round (64 bits:
-    // lengths that make no sense may add up to anything)
-    __shared__ int64_t start[3][PLAN_T + 1];
-    __shared__ int64_t wsum[3][PLAN_T / 64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int64_t work = 0;
-    for (int r = tid; r < a.R; r += PLAN_T) {
-        const Req q = request(a, r);
-        work += static_cast<int64_t>(q.tiles) * q.units;
-    }
-    work = block_sum(work, red);
-    const int64_t per = max(static_cast<int64_t>(MIN_UNITS), (work + a.target - 1) / a.target);   // units per piece
-    int64_t base[3] = {0, 0, 0};
-    for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
-        const Req q = request(a, r0 + tid);
-        const int64_t pieces = (q.units + per - 1) / per;
-        const int64_t n[3] = {q.tiles * pieces, pieces > 1 ? q.tiles * pieces : 0, pieces > 1 ? q.tiles : 0};
-        int64_t incl[3], total[3] = {0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            incl[k] = wave_incl_scan(n[k], lane);
-            if (lane == 63) wsum[k][w] = incl[k];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            int64_t before = 0;
-            for (int i = 0; i < PLAN_T / 64; ++i) {
-                if (i < w) before += wsum[k][i];
-                total[k] += wsum[k][i];
-            }
-            start[k][tid] = before + incl[k] - n[k];
-        }
-        __syncthreads();
-        const int nr = min(PLAN_T, a.R - r0);
-        for (int64_t i = tid; i < total[0] && base[0] + i < a.max_items; i += PLAN_T) {
-            const int k = last_at_most(start[0], nr - 1, i);
-            const Req x = request(a, r0 + k);
-            const int pc = static_cast<int>((x.units + per - 1) / per);
-            const int local = static_cast<int>(i - start[0][k]), tile = local / pc, piece = local - tile * pc;
-            const int row0 = tile * TILE, row1 = min(row0 + TILE, x.qlen * a.G);
-            const int p0 = x.len - x.qlen + row0 / a.G, p1 = x.len - x.qlen + (row1 - 1) / a.G;   // first and last position
-            const int lo = first_key(p0, a.window) / GROUP, hi = (max(p1, -1) + GROUP) / GROUP;   // GROUP steps
-            const int64_t steps = max(hi - lo, 0);
-            const int64_t part = base[1] + start[1][k] + local;
-            const bool split = pc > 1 && part < a.max_parts;
-            Item it{r0 + k, x.q0, x.qlen, x.len, row0, 0, 0, split ? static_cast<int>(part) : -1};
-            it.key0 = (lo + static_cast<int>(steps * piece / pc)) * GROUP;
-            it.key1 = min(p1 + 1, (lo + static_cast<int>(steps * (piece + 1) / pc)) * GROUP);
-            a.items[base[0] + i] = it;
-            const int64_t j = base[2] + start[2][k] + tile;
-            if (split && piece == 0 && j < a.max_joins)
-                a.joins[j] = Join{x.q0, row0, row1 - row0, it.part, pc, {0, 0, 0}};
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) base[k] += total[k];
-        __syncthreads();
-    }
-    if (tid == 0)
-        *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))),
-                           static_cast<int32_t>(min(base[2], static_cast<int64_t>(a.max_joins))), a.cu ? min(max(a.cu[a.R], 0), a.T) : a.T, 0};
-}
-
-// ---------------------------------------------------------------------------
-// attention: 16 query rows per workgroup
-// ---------------------------------------------------------------------------
-struct AttnArgs {
-    const uint16_t* q;
-    int64_t q_t, q_h;
-    uint16_t* out;
-    int64_t o_t, o_h;
-    float* lse;
-    int64_t l_t;
-    const int8_t *kp, *vp;
-    int64_t ps_page, ps_head;
-    const uint16_t *ks, *vs;
-    int64_t ss_page, ss_head;
-    const int32_t* table;
-    int64_t bt_stride;
-    const Counts* counts;
-    const Item* items;
-    const Join* joins;
-    float* part;                         // [slot][key head][TILE][D] sums, then [slot][key head][TILE][2] (m, l)
-    float* ml;
-    int32_t G, heads, page_log2, num_pages, window, tokens, zero_tail;
-    float scale;                         // sm_scale * log2(e)
-};
-
-constexpr float M_INIT = -1.0e30f;
-constexpr float SLACK = 8.0f;            // the running maximum moves when a score passes it by this (log2 units)
-constexpr int WAVES = 4;
-constexpr float LN2 = 0.69314718055994531f;
-
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 __device__ __forceinline__ uint32_t nib2(uint32_t x, int s, uint32_t magic) { return ((x >> s) & 0x000f000fu) ^ magic; }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -431,6 +261,263 @@ __device__ __forceinline__ float quad_bcast(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), I * 0x55, 0xf, 0xf, true));
 }
 
+// ---------------------------------------------------------------------------
+// attention: the schedule
+// ---------------------------------------------------------------------------
+// Query rows of a request are its new tokens times the G query heads of a KV
+// head, row = token * G + head, cut into tiles of TILE rows; a tile's keys may
+// be cut into pieces, whose partial results a join launch adds up.  The
+// schedule is the same for every KV head.  It is made on the device from the
+// lengths, so that nothing is read back and a captured graph follows the
+// lengths it is replayed with: up to 64 requests every wavefront finds its own
+// item (lane r looks at request r; one load, two wavefront scans), more are
+// laid out by a launch before.
+constexpr int TILE = 16;                 // query rows per tile
+constexpr int GROUP = 32;                // keys per wavefront step
+constexpr int PLAN_T = 1024;
+constexpr int INLINE_R = 64;             // requests of a schedule without a launch of its own
+constexpr int SLOTS = 1024;              // pieces wanted over all KV heads while tiles are few
+constexpr int MIN_UNITS = 8;             // GROUP steps per piece, at least (two per wavefront)
+
+struct Item {
+    int32_t req, q0, qlen, len;          // request, its first token, its new tokens, its keys
+    int32_t row0;                        // first row of the tile within the request
+    int32_t key0, key1;                  // keys of this piece
+    int32_t part;                        // partial slot, -1: the tile is whole
+};
+struct Join {
+    int32_t q0, row0, rows, part, pieces, pad[3];
+};
+struct Counts {
+    int32_t items, joins, pad[2];
+};
+
+struct PlanArgs {
+    const int32_t* lens;
+    const int32_t* cu;
+    int32_t R, T, G, window, capacity;   // capacity: keys that a block table row can name
+    int32_t target;                      // pieces per KV head wanted
+    int32_t max_items, max_parts, max_joins;
+    Counts* counts;
+    Item* items;
+    Join* joins;
+};
+
+struct Req {
+    int32_t q0, qlen, len, tiles, units; // units: the longest tile's GROUP-key steps
+};
+
+// first key that a row at position pos sees
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
+
+__device__ __forceinline__ Req request(const PlanArgs& a, int r) {
+    Req q{};
+    if (r >= a.R) return q;
+    q.q0 = r;
+    q.qlen = 1;
+    if (a.cu) {
+        q.q0 = min(max(a.cu[r], 0), a.T);
+        q.qlen = min(max(a.cu[r + 1], q.q0), a.T) - q.q0;
+    }
+    q.len = min(max(a.lens[r], 0), a.capacity);
+    q.tiles = (q.qlen * a.G + TILE - 1) / TILE;
+    // the rows of a tile see at most window + TILE keys between them
+    const int keys = a.window > 0 && a.window < q.len - TILE ? a.window + TILE : q.len;
+    q.units = keys / GROUP + 2;          // from a GROUP boundary to a GROUP boundary
+    return q;
+}
+
+// GROUP steps per piece so that the pieces of all tiles are at most target +
+// tiles: at least work / target (the float sum's rounding is far below 2^-14)
+__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work) {
+    const float per = ceilf(work * (1.0f + 0x1p-14f) / static_cast<float>(a.target));
+    return static_cast<int>(fminf(fmaxf(per, static_cast<float>(MIN_UNITS)), 0x1p30f));
+}
+__device__ __forceinline__ int pieces_of(const Req& x, int per) {
+    return static_cast<int>((static_cast<uint32_t>(x.units) + static_cast<uint32_t>(per) - 1u) / static_cast<uint32_t>(per));
+}
+
+// Piece `piece` of pc of tile `tile` of a request
+__device__ __forceinline__ Item make_item(const PlanArgs& a, const Req& x, int r, int tile, int piece, int pc,
+                                          int part) {
+    const int row0 = tile * TILE, row1 = min(row0 + TILE, x.qlen * a.G);
+    const int p0 = x.len - x.qlen + row0 / a.G, p1 = x.len - x.qlen + (row1 - 1) / a.G;   // first and last position
+    const int lo = first_key(p0, a.window) / GROUP, hi = (max(p1, -1) + GROUP) / GROUP;   // GROUP steps
+    const int steps = max(hi - lo, 0), each = static_cast<int>((static_cast<uint32_t>(steps) + pc - 1u) / pc);
+    Item it{r, x.q0, x.qlen, x.len, row0, 0, 0, part};
+    it.key0 = (lo + min(steps, piece * each)) * GROUP;
+    it.key1 = min(p1 + 1, (lo + min(steps, (piece + 1) * each)) * GROUP);
+    return it;
+}
+__device__ __forceinline__ Join make_join(const PlanArgs& a, const Req& x, int tile, int pc, int part) {
+    return Join{x.q0, tile * TILE, min(TILE, x.qlen * a.G - tile * TILE), part, pc, {0, 0, 0}};
+}
+
+// inclusive sums over the wavefront by DPP row shifts and broadcasts
+__device__ __forceinline__ int scan_dpp(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);    // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);    // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = col_sum(sum16_dpp(v));
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
+// The schedule of up to 64 requests in one wavefront's registers.  32 bits are
+// enough whatever the lengths: 64 requests of at most 2^22 tiles each and the
+// target's pieces on top.
+struct Plan64 {
+    Req x;                               // of request `lane`
+    int items, parts, joins;             // before it
+    int pc;
+};
+__device__ __forceinline__ Plan64 plan64(const PlanArgs& a, int lane) {
+    Plan64 p;
+    p.x = request(a, lane);
+    const int per = units_per_piece(a, wave_sum(static_cast<float>(p.x.tiles) * static_cast<float>(p.x.units)));
+    p.pc = pieces_of(p.x, per);
+    const int n = p.x.tiles * p.pc, split = p.pc > 1 ? 1 : 0;
+    p.items = scan_dpp(n) - n;
+    p.parts = scan_dpp(split * n) - split * n;
+    p.joins = scan_dpp(split * p.x.tiles) - split * p.x.tiles;
+    return p;
+}
+// lane `k`'s request, the same in every lane
+__device__ __forceinline__ Req lane_req(const Req& x, int k) {
+    return Req{__builtin_amdgcn_readlane(x.q0, k), __builtin_amdgcn_readlane(x.qlen, k), __builtin_amdgcn_readlane(x.len, k),
+               __builtin_amdgcn_readlane(x.tiles, k), __builtin_amdgcn_readlane(x.units, k)};
+}
+// the lane whose range [start, start + n) holds i (ranges laid end to end), -1: none
+__device__ __forceinline__ int lane_of(int start, int n, int i) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(start <= i && i < start + n);
+    return m ? __builtin_ctzll(m) : -1;
+}
+
+// This workgroup's item / join; false: it has none
+__device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int lane, Item& it) {
+    if (a.R > INLINE_R) {
+        if (i >= a.counts->items) return false;
+        it = a.items[i];
+        return true;
+    }
+    const Plan64 p = plan64(a, lane);
+    const int k = lane_of(p.items, p.x.tiles * p.pc, i);
+    if (k < 0) return false;
+    const int pc = __builtin_amdgcn_readlane(p.pc, k), local = i - __builtin_amdgcn_readlane(p.items, k);
+    const int part = __builtin_amdgcn_readlane(p.parts, k) + local;
+    it = make_item(a, lane_req(p.x, k), k, local / pc, local % pc, pc, pc > 1 && part < a.max_parts ? part : -1);
+    return true;
+}
+__device__ __forceinline__ bool find_join(const PlanArgs& a, int j, int lane, Join& jn) {
+    if (a.R > INLINE_R) {
+        if (j >= a.counts->joins) return false;
+        jn = a.joins[j];
+        return true;
+    }
+    const Plan64 p = plan64(a, lane);
+    const int k = lane_of(p.joins, p.pc > 1 ? p.x.tiles : 0, j);
+    if (k < 0) return false;
+    const int pc = __builtin_amdgcn_readlane(p.pc, k), tile = j - __builtin_amdgcn_readlane(p.joins, k);
+    const int part = __builtin_amdgcn_readlane(p.parts, k) + tile * pc;
+    if (part + pc > a.max_parts) return false;
+    jn = make_join(a, lane_req(p.x, k), tile, pc, part);
+    return true;
+}
+
+__global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
+    // items, partial slots and joins before each request of a round (64 bits:
+    // lengths that make no sense may add up to anything)
+    __shared__ int64_t start[3][PLAN_T];
+    __shared__ int64_t wsum[3][PLAN_T / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ float fsum[PLAN_T / 64];
+    float work = 0.f;
+    for (int r = tid; r < a.R; r += PLAN_T) {
+        const Req q = request(a, r);
+        work += static_cast<float>(q.tiles) * static_cast<float>(q.units);
+    }
+    work = wave_sum(work);
+    if (lane == 0) fsum[w] = work;
+    __syncthreads();
+    work = 0.f;
+    for (int i = 0; i < PLAN_T / 64; ++i) work += fsum[i];
+    __syncthreads();
+    const int per = units_per_piece(a, work);
+    int64_t base[3] = {0, 0, 0};
+    for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
+        const Req q = request(a, r0 + tid);
+        const int64_t pieces = pieces_of(q, per);
+        const int64_t n[3] = {q.tiles * pieces, pieces > 1 ? q.tiles * pieces : 0, pieces > 1 ? q.tiles : 0};
+        int64_t incl[3], total[3] = {0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            incl[k] = wave_incl_scan(n[k], lane);
+            if (lane == 63) wsum[k][w] = incl[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            int64_t before = 0;
+            for (int i = 0; i < PLAN_T / 64; ++i) {
+                if (i < w) before += wsum[k][i];
+                total[k] += wsum[k][i];
+            }
+            start[k][tid] = before + incl[k] - n[k];
+        }
+        __syncthreads();
+        const int nr = min(PLAN_T, a.R - r0);
+        for (int64_t i = tid; i < total[0] && base[0] + i < a.max_items; i += PLAN_T) {
+            const int k = last_at_most(start[0], nr - 1, i);
+            const Req x = request(a, r0 + k);
+            const int pc = pieces_of(x, per), local = static_cast<int>(i - start[0][k]), tile = local / pc, piece = local - tile * pc;
+            const int64_t part = base[1] + start[1][k] + local;
+            const bool split = pc > 1 && part < a.max_parts;
+            a.items[base[0] + i] = make_item(a, x, r0 + k, tile, piece, pc, split ? static_cast<int>(part) : -1);
+            const int64_t j = base[2] + start[2][k] + tile;
+            if (split && piece == 0 && j < a.max_joins) a.joins[j] = make_join(a, x, tile, pc, static_cast<int>(part));
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) base[k] += total[k];
+        __syncthreads();
+    }
+    if (tid == 0)
+        *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))),
+                           static_cast<int32_t>(min(base[2], static_cast<int64_t>(a.max_joins))), {0, 0}};
+}
+
+// ---------------------------------------------------------------------------
+// attention: 16 query rows per workgroup
+// ---------------------------------------------------------------------------
+struct AttnArgs {
+    const uint16_t* q;
+    int64_t q_t, q_h;
+    uint16_t* out;
+    int64_t o_t, o_h;
+    float* lse;
+    int64_t l_t;
+    const int8_t *kp, *vp;
+    int64_t ps_page, ps_head;
+    const uint16_t *ks, *vs;
+    int64_t ss_page, ss_head;
+    const int32_t* table;
+    int64_t bt_stride;
+    PlanArgs plan;
+    float* part;                         // [slot][key head][TILE][D] sums, then [slot][key head][TILE][2] (m, l)
+    float* ml;
+    int32_t G, heads, page_log2, num_pages, window, zero_tail;
+    float scale;                         // sm_scale * log2(e)
+};
+
+constexpr float M_INIT = -1.0e30f;
+constexpr float SLACK = 8.0f;            // the running maximum moves when a score passes it by this (log2 units)
+constexpr int WAVES = 4;
+constexpr float LN2 = 0.69314718055994531f;
+
 // 16-bit words of a row as floats (exact)
 template <bool F16>
 __device__ __forceinline__ float half_at(uint32_t w, int hi) {
@@ -446,6 +533,25 @@ __device__ __forceinline__ int q_exponent(float amax) {
     return min(max(e, -100), 100) - 14;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// out (and lse) of a row from its sums: a row without keys is zero, NaN stays NaN
+template <bool F16>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int q0, int rr, int head, int ch, float m, float l, f32x4 o) {
+    const int tk = rr / a.G;
+    const int64_t h = static_cast<int64_t>(head) * a.G + rr - tk * a.G, t = static_cast<int64_t>(q0) + tk;
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+    o *= inv;
+    u32x2 ow;
+    if constexpr (F16) {
+        ow[0] = f32_to_f16_bits(o[0]) | (static_cast<uint32_t>(f32_to_f16_bits(o[1])) << 16);
+        ow[1] = f32_to_f16_bits(o[2]) | (static_cast<uint32_t>(f32_to_f16_bits(o[3])) << 16);
+    } else {
+        ow[0] = pack_bf16x2(o[0], o[1]);
+        ow[1] = pack_bf16x2(o[2], o[3]);
+    }
+    *reinterpret_cast<u32x2*>(a.out + t * a.o_t + h * a.o_h + ch) = ow;
+    if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
 
 template <int D>
 struct Raw {
@@ -463,10 +569,10 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
     constexpr int ROWB = D / 2;          // packed bytes per token
     __shared__ float red[WAVES][TILE][D + 4];
     __shared__ float redm[WAVES][TILE], redl[WAVES][TILE];
-    if (static_cast<int>(blockIdx.x) >= a.counts->items) return;
-    const Item it = a.items[blockIdx.x];
-    const int head = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = blockIdx.y;
+    Item it;
+    if (!find_item(a.plan, blockIdx.x, lane, it)) return;
     const int c = lane & 15, kb = lane >> 4;
     const int nrows = min(TILE, it.qlen * a.G - it.row0);
 
@@ -694,65 +800,77 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
             *reinterpret_cast<f32x4*>(a.part + (slot * TILE + rw) * D + ch) = o;
             if (ch == 0) { a.ml[(slot * TILE + rw) * 2] = m; a.ml[(slot * TILE + rw) * 2 + 1] = l; }
         } else {
-            const int rr = it.row0 + rw, tk = rr / a.G;
-            const int64_t h = static_cast<int64_t>(head) * a.G + rr - tk * a.G, t = static_cast<int64_t>(it.q0) + tk;
-            const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;       // no key: zeros; NaN stays NaN
-            o *= inv;
-            u32x2 ow;
-            if constexpr (F16) {
-                ow[0] = f32_to_f16_bits(o[0]) | (static_cast<uint32_t>(f32_to_f16_bits(o[1])) << 16);
-                ow[1] = f32_to_f16_bits(o[2]) | (static_cast<uint32_t>(f32_to_f16_bits(o[3])) << 16);
-            } else {
-                ow[0] = pack_bf16x2(o[0], o[1]);
-                ow[1] = pack_bf16x2(o[2], o[3]);
-            }
-            *reinterpret_cast<u32x2*>(a.out + t * a.o_t + h * a.o_h + ch) = ow;
-            if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+            store_row<F16>(a, it.q0, it.row0 + rw, head, ch, m, l, o);
         }
     }
 }
 
-// Joins the pieces of the split tiles: grid (joins, key heads), thread (row, 4
-// channels).  By zero_tail it also clears the rows behind the last request.
+// Adds up the pieces of the split tiles: one workgroup per tile and KV head.
+// A row is 4 channels a lane of D/4; while rows are fewer than the lane
+// groups, several groups share a row's pieces and meet in LDS.  Four pieces
+// are in flight per group.  By zero_tail it also clears the rows behind the
+// last request.
+constexpr int JOIN_T = 1024;
 template <int D, bool F16>
-__global__ __launch_bounds__(TILE * D / 4) void paged_join_kernel(AttnArgs a) {
-    if (a.zero_tail) {
-        const int64_t total = static_cast<int64_t>(a.tokens - a.counts->tokens) * a.G * (D / 4);   // of one KV head
-        for (int64_t e = static_cast<int64_t>(blockIdx.x) * (TILE * D / 4) + threadIdx.x; e < total; e += static_cast<int64_t>(gridDim.x) * (TILE * D / 4)) {
-            const int64_t row = e / (D / 4), t = row / a.G, h = blockIdx.y * static_cast<int64_t>(a.G) + row - t * a.G;
+__global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
+    constexpr int LG = JOIN_T / (D / 4);    // lane groups
+    __shared__ float so[LG][D];
+    __shared__ float sm[LG], sl[LG];
+    const int tid = threadIdx.x, head = blockIdx.y;
+    if (a.zero_tail && a.plan.cu) {
+        const int64_t first = min(max(a.plan.cu[a.plan.R], 0), a.plan.T);
+        const int64_t total = (a.plan.T - first) * a.G * (D / 4);   // of one KV head
+        for (int64_t e = static_cast<int64_t>(blockIdx.x) * JOIN_T + tid; e < total; e += static_cast<int64_t>(gridDim.x) * JOIN_T) {
+            const int64_t row = e / (D / 4), t = row / a.G, h = head * static_cast<int64_t>(a.G) + row - t * a.G;
             const int ch = 4 * static_cast<int>(e - row * (D / 4));
-            if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (a.counts->tokens + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
-            if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(a.counts->tokens + t) * a.l_t + h] = -INFINITY;
+            if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (first + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
+            if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(first + t) * a.l_t + h] = -INFINITY;
         }
     }
-    if (static_cast<int>(blockIdx.x) >= a.counts->joins) return;
-    const Join jn = a.joins[blockIdx.x];
-    const int head = blockIdx.y, rw = threadIdx.x / (D / 4), ch = 4 * (threadIdx.x - rw * (D / 4));
-    if (rw >= jn.rows) return;
-    float m = M_INIT;
-    for (int i = 0; i < jn.pieces; ++i) m = fmaxf(m, a.ml[(((static_cast<int64_t>(jn.part) + i) * a.heads + head) * TILE + rw) * 2]);
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < jn.pieces; ++i) {
-        const int64_t at = ((static_cast<int64_t>(jn.part) + i) * a.heads + head) * TILE + rw;
-        const float f = fast_exp2(a.ml[at * 2] - m);
-        l += f * a.ml[at * 2 + 1];
-        o += f * *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
+    Join jn;
+    if (!find_join(a.plan, blockIdx.x, tid & 63, jn)) return;
+    const int share = jn.rows <= LG / 8 ? 8 : jn.rows <= LG / 4 ? 4 : jn.rows <= LG / 2 ? 2 : 1;
+    const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4)), sub = g % share;
+    for (int r0 = 0; r0 < jn.rows; r0 += LG / share) {
+        const int rw = r0 + g / share;
+        float m = M_INIT, l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        if (rw < jn.rows) {
+            constexpr int DEEP = 4;
+            for (int i0 = sub; i0 < jn.pieces; i0 += DEEP * share) {
+                float mi[DEEP], li[DEEP];
+                f32x4 oi[DEEP];
+#pragma unroll
+                for (int j = 0; j < DEEP; ++j) {
+                    const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * TILE + rw;
+                    mi[j] = a.ml[at * 2];
+                    li[j] = a.ml[at * 2 + 1];
+                    oi[j] = *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
+                }
+#pragma unroll
+                for (int j = 0; j < DEEP; ++j) {
+                    if (i0 + j * share >= jn.pieces) break;
+                    const float mn = fmaxf(m, mi[j]), f = fast_exp2(m - mn), fi = fast_exp2(mi[j] - mn);
+                    o = o * f + oi[j] * fi;
+                    l = l * f + li[j] * fi;
+                    m = mn;
+                }
+            }
+        }
+        if (share > 1) {                 // (one round of the loop: rows <= LG / share)
+            *reinterpret_cast<f32x4*>(&so[g][ch]) = o;
+            if (ch == 0) { sm[g] = m; sl[g] = l; }
+            __syncthreads();
+            if (sub != 0) return;
+            for (int i = 1; i < share; ++i) {
+                const float mn = fmaxf(m, sm[g + i]), f = fast_exp2(m - mn), fi = fast_exp2(sm[g + i] - mn);
+                o = o * f + *reinterpret_cast<const f32x4*>(&so[g + i][ch]) * fi;
+                l = l * f + sl[g + i] * fi;
+                m = mn;
+            }
+        }
+        if (rw < jn.rows) store_row<F16>(a, jn.q0, jn.row0 + rw, head, ch, m, l, o);
     }
-    const int rr = jn.row0 + rw, tk = rr / a.G;
-    const int64_t h = static_cast<int64_t>(head) * a.G + rr - tk * a.G, t = static_cast<int64_t>(jn.q0) + tk;
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    o *= inv;
-    u32x2 ow;
-    if constexpr (F16) {
-        ow[0] = f32_to_f16_bits(o[0]) | (static_cast<uint32_t>(f32_to_f16_bits(o[1])) << 16);
-        ow[1] = f32_to_f16_bits(o[2]) | (static_cast<uint32_t>(f32_to_f16_bits(o[3])) << 16);
-    } else {
-        ow[0] = pack_bf16x2(o[0], o[1]);
-        ow[1] = pack_bf16x2(o[2], o[3]);
-    }
-    *reinterpret_cast<u32x2*>(a.out + t * a.o_t + h * a.o_h + ch) = ow;
-    if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 // ---------------------------------------------------------------------------
@@ -811,8 +929,8 @@ int check_attention(const hyq_paged_params* p) {
     if (p->kv_repeat < 1 || p->kv_repeat > 1024) return fail(HYQ_ENOTSUP, s + "kv_repeat must be 1 to 1024");
     if (p->num_requests < 0 || p->num_tokens < 0 || p->max_pages < 0 || p->window < 0)
         return fail(HYQ_EINVAL, s + "negative size");
-    if (static_cast<int64_t>(p->num_tokens) * p->kv_repeat > (int64_t{1} << 30))
-        return fail(HYQ_ENOTSUP, s + "more than 2^30 query rows per key head");
+    if (static_cast<int64_t>(p->num_tokens) * p->kv_repeat > (int64_t{1} << 26))
+        return fail(HYQ_ENOTSUP, s + "more than 2^26 query rows per key head");
     if (static_cast<int64_t>(p->max_pages) * p->page_size > (int64_t{1} << 30))
         return fail(HYQ_ENOTSUP, s + "a block table row names more than 2^30 tokens");
     if (p->num_requests > (1 << 20)) return fail(HYQ_ENOTSUP, s + "more than 2^20 requests");
@@ -835,7 +953,7 @@ int check_attention(const hyq_paged_params* p) {
 template <int D, bool F16>
 void launch_attention(const AttnArgs& a, const Sizes& s, hipStream_t st) {
     paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
-    paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(s.joins), a.heads), dim3(TILE * D / 4), 0, st>>>(a);
+    paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(s.joins), a.heads), dim3(JOIN_T), 0, st>>>(a);
 }
 
 }  // namespace
@@ -936,12 +1054,12 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
                 p->max_pages * p->page_size, static_cast<int32_t>(s.target), static_cast<int32_t>(s.items),
                 static_cast<int32_t>(s.parts), static_cast<int32_t>(s.joins), reinterpret_cast<Counts*>(ws), reinterpret_cast<Item*>(ws + s.off_items),
                 reinterpret_cast<Join*>(ws + s.off_joins)};
-    paged_plan_kernel<<<dim3(1), dim3(PLAN_T), 0, st>>>(pl);
+    if (p->num_requests > INLINE_R) paged_plan_kernel<<<dim3(1), dim3(PLAN_T), 0, st>>>(pl);
     AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
                p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head, p->k_scale,
-               p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, pl.counts, pl.items, pl.joins,
+               p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, pl,
                reinterpret_cast<float*>(ws + s.off_part), reinterpret_cast<float*>(ws + s.off_ml), p->kv_repeat, p->kv_heads,
-               log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->num_tokens, p->zero_tail, p->sm_scale * 1.44269504f};
+               log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail, p->sm_scale * 1.44269504f};
     if (p->head_dim == 128) {
         if (p->dtype_fp16) launch_attention<128, true>(a, s, st);
         else launch_attention<128, false>(a, s, st);
