@@ -272,12 +272,25 @@ __device__ __forceinline__ float quad_bcast(float x) {
 // lengths it is replayed with: up to 64 requests every wavefront finds its own
 // item (lane r looks at request r; one load, two wavefront scans), more are
 // laid out by a launch before.
-constexpr int TILE = 16;                 // query rows per tile
-constexpr int GROUP = 32;                // keys per wavefront step
+// Requests of at most 16 rows (decode steps) and larger ones (chunks) have a
+// kernel and a schedule each: a tile of 16 rows is bound by the cache's bytes,
+// one of CHUNK rows by the products.
 constexpr int PLAN_T = 1024;
 constexpr int INLINE_R = 64;             // requests of a schedule without a launch of its own
-constexpr int SLOTS = 1024;              // pieces wanted over all KV heads while tiles are few
-constexpr int MIN_UNITS = 8;             // GROUP steps per piece, at least (two per wavefront)
+constexpr int CHUNK_WAVES = 8;
+constexpr int CHUNK = 32 * CHUNK_WAVES;  // rows of a chunk tile
+struct Narrow {
+    static constexpr int TILE = 16, GROUP = 32;   // query rows per tile, keys per step
+    static constexpr int MIN_UNITS = 8;  // steps per piece, at least (two per wavefront)
+    static constexpr int SLOTS = 1024;   // pieces wanted over all KV heads
+    static constexpr int ENOUGH = 1 << 30;        // tiles over all KV heads that are not cut any more
+};
+struct Wide {
+    static constexpr int TILE = CHUNK, GROUP = 64;
+    static constexpr int MIN_UNITS = 4;
+    static constexpr int SLOTS = 512;
+    static constexpr int ENOUGH = 224;
+};
 
 struct Item {
     int32_t req, q0, qlen, len;          // request, its first token, its new tokens, its keys
@@ -296,6 +309,7 @@ struct PlanArgs {
     const int32_t* lens;
     const int32_t* cu;
     int32_t R, T, G, window, capacity;   // capacity: keys that a block table row can name
+    int32_t enough;                      // tiles of one KV head that are not cut any more
     int32_t target;                      // pieces per KV head wanted
     int32_t max_items, max_parts, max_joins;
     Counts* counts;
@@ -310,6 +324,7 @@ struct Req {
 // first key that a row at position pos sees
 __device__ __forceinline__ int first_key(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
+template <typename K>
 __device__ __forceinline__ Req request(const PlanArgs& a, int r) {
     Req q{};
     if (r >= a.R) return q;
@@ -320,37 +335,42 @@ __device__ __forceinline__ Req request(const PlanArgs& a, int r) {
         q.qlen = min(max(a.cu[r + 1], q.q0), a.T) - q.q0;
     }
     q.len = min(max(a.lens[r], 0), a.capacity);
-    q.tiles = (q.qlen * a.G + TILE - 1) / TILE;
+    const int rows = q.qlen * a.G;
+    q.tiles = (rows <= Narrow::TILE) == (K::TILE == Narrow::TILE) ? (rows + K::TILE - 1) / K::TILE : 0;
     // the rows of a tile see at most window + TILE keys between them
-    const int keys = a.window > 0 && a.window < q.len - TILE ? a.window + TILE : q.len;
-    q.units = keys / GROUP + 2;          // from a GROUP boundary to a GROUP boundary
+    const int keys = a.window > 0 && a.window < q.len - K::TILE ? a.window + K::TILE : q.len;
+    q.units = keys / K::GROUP + 2;       // from a GROUP boundary to a GROUP boundary
     return q;
 }
 
 // GROUP steps per piece so that the pieces of all tiles are at most target +
 // tiles: at least work / target (the float sum's rounding is far below 2^-14)
-__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work) {
+template <typename K>
+__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work, float tiles) {
+    if (tiles >= static_cast<float>(a.enough)) return 1 << 30;
     const float per = ceilf(work * (1.0f + 0x1p-14f) / static_cast<float>(a.target));
-    return static_cast<int>(fminf(fmaxf(per, static_cast<float>(MIN_UNITS)), 0x1p30f));
+    return static_cast<int>(fminf(fmaxf(per, static_cast<float>(K::MIN_UNITS)), 0x1p30f));
 }
 __device__ __forceinline__ int pieces_of(const Req& x, int per) {
     return static_cast<int>((static_cast<uint32_t>(x.units) + static_cast<uint32_t>(per) - 1u) / static_cast<uint32_t>(per));
 }
 
 // Piece `piece` of pc of tile `tile` of a request
+template <typename K>
 __device__ __forceinline__ Item make_item(const PlanArgs& a, const Req& x, int r, int tile, int piece, int pc,
                                           int part) {
-    const int row0 = tile * TILE, row1 = min(row0 + TILE, x.qlen * a.G);
+    const int row0 = tile * K::TILE, row1 = min(row0 + K::TILE, x.qlen * a.G);
     const int p0 = x.len - x.qlen + row0 / a.G, p1 = x.len - x.qlen + (row1 - 1) / a.G;   // first and last position
-    const int lo = first_key(p0, a.window) / GROUP, hi = (max(p1, -1) + GROUP) / GROUP;   // GROUP steps
+    const int lo = first_key(p0, a.window) / K::GROUP, hi = (max(p1, -1) + K::GROUP) / K::GROUP;   // GROUP steps
     const int steps = max(hi - lo, 0), each = static_cast<int>((static_cast<uint32_t>(steps) + pc - 1u) / pc);
     Item it{r, x.q0, x.qlen, x.len, row0, 0, 0, part};
-    it.key0 = (lo + min(steps, piece * each)) * GROUP;
-    it.key1 = min(p1 + 1, (lo + min(steps, (piece + 1) * each)) * GROUP);
+    it.key0 = (lo + min(steps, piece * each)) * K::GROUP;
+    it.key1 = min(p1 + 1, (lo + min(steps, (piece + 1) * each)) * K::GROUP);
     return it;
 }
+template <typename K>
 __device__ __forceinline__ Join make_join(const PlanArgs& a, const Req& x, int tile, int pc, int part) {
-    return Join{x.q0, tile * TILE, min(TILE, x.qlen * a.G - tile * TILE), part, pc, {0, 0, 0}};
+    return Join{x.q0, tile * K::TILE, min(K::TILE, x.qlen * a.G - tile * K::TILE), part, pc, {0, 0, 0}};
 }
 
 // inclusive sums over the wavefront by DPP row shifts and broadcasts
@@ -376,10 +396,12 @@ struct Plan64 {
     int items, parts, joins;             // before it
     int pc;
 };
+template <typename K>
 __device__ __forceinline__ Plan64 plan64(const PlanArgs& a, int lane) {
     Plan64 p;
-    p.x = request(a, lane);
-    const int per = units_per_piece(a, wave_sum(static_cast<float>(p.x.tiles) * static_cast<float>(p.x.units)));
+    p.x = request<K>(a, lane);
+    const float tiles = static_cast<float>(p.x.tiles);
+    const int per = units_per_piece<K>(a, wave_sum(tiles * static_cast<float>(p.x.units)), wave_sum(tiles));
     p.pc = pieces_of(p.x, per);
     const int n = p.x.tiles * p.pc, split = p.pc > 1 ? 1 : 0;
     p.items = scan_dpp(n) - n;
@@ -399,58 +421,66 @@ __device__ __forceinline__ int lane_of(int start, int n, int i) {
 }
 
 // This workgroup's item / join; false: it has none
+template <typename K>
 __device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int lane, Item& it) {
     if (a.R > INLINE_R) {
         if (i >= a.counts->items) return false;
         it = a.items[i];
         return true;
     }
-    const Plan64 p = plan64(a, lane);
+    const Plan64 p = plan64<K>(a, lane);
     const int k = lane_of(p.items, p.x.tiles * p.pc, i);
     if (k < 0) return false;
     const int pc = __builtin_amdgcn_readlane(p.pc, k), local = i - __builtin_amdgcn_readlane(p.items, k);
     const int part = __builtin_amdgcn_readlane(p.parts, k) + local;
-    it = make_item(a, lane_req(p.x, k), k, local / pc, local % pc, pc, pc > 1 && part < a.max_parts ? part : -1);
+    // (a causal request's last tiles have the most keys: they go first)
+    const Req x = lane_req(p.x, k);
+    it = make_item<K>(a, x, k, x.tiles - 1 - local / pc, local % pc, pc, pc > 1 && part < a.max_parts ? part : -1);
     return true;
 }
+template <typename K>
 __device__ __forceinline__ bool find_join(const PlanArgs& a, int j, int lane, Join& jn) {
     if (a.R > INLINE_R) {
         if (j >= a.counts->joins) return false;
         jn = a.joins[j];
         return true;
     }
-    const Plan64 p = plan64(a, lane);
+    const Plan64 p = plan64<K>(a, lane);
     const int k = lane_of(p.joins, p.pc > 1 ? p.x.tiles : 0, j);
     if (k < 0) return false;
-    const int pc = __builtin_amdgcn_readlane(p.pc, k), tile = j - __builtin_amdgcn_readlane(p.joins, k);
-    const int part = __builtin_amdgcn_readlane(p.parts, k) + tile * pc;
+    const int pc = __builtin_amdgcn_readlane(p.pc, k), nth = j - __builtin_amdgcn_readlane(p.joins, k);
+    const int part = __builtin_amdgcn_readlane(p.parts, k) + nth * pc;
+    const Req x = lane_req(p.x, k);
     if (part + pc > a.max_parts) return false;
-    jn = make_join(a, lane_req(p.x, k), tile, pc, part);
+    jn = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
     return true;
 }
 
-__global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
+template <typename K>
+__device__ __forceinline__ void plan(const PlanArgs& a) {
     // items, partial slots and joins before each request of a round (64 bits:
     // lengths that make no sense may add up to anything)
     __shared__ int64_t start[3][PLAN_T];
     __shared__ int64_t wsum[3][PLAN_T / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    __shared__ float fsum[PLAN_T / 64];
-    float work = 0.f;
+    __shared__ float fsum[2][PLAN_T / 64];
+    float work = 0.f, tiles = 0.f;
     for (int r = tid; r < a.R; r += PLAN_T) {
-        const Req q = request(a, r);
+        const Req q = request<K>(a, r);
         work += static_cast<float>(q.tiles) * static_cast<float>(q.units);
+        tiles += static_cast<float>(q.tiles);
     }
     work = wave_sum(work);
-    if (lane == 0) fsum[w] = work;
+    tiles = wave_sum(tiles);
+    if (lane == 0) { fsum[0][w] = work; fsum[1][w] = tiles; }
     __syncthreads();
-    work = 0.f;
-    for (int i = 0; i < PLAN_T / 64; ++i) work += fsum[i];
+    work = tiles = 0.f;
+    for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; tiles += fsum[1][i]; }
     __syncthreads();
-    const int per = units_per_piece(a, work);
+    const int per = units_per_piece<K>(a, work, tiles);
     int64_t base[3] = {0, 0, 0};
     for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
-        const Req q = request(a, r0 + tid);
+        const Req q = request<K>(a, r0 + tid);
         const int64_t pieces = pieces_of(q, per);
         const int64_t n[3] = {q.tiles * pieces, pieces > 1 ? q.tiles * pieces : 0, pieces > 1 ? q.tiles : 0};
         int64_t incl[3], total[3] = {0, 0, 0};
@@ -473,13 +503,14 @@ __global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
         const int nr = min(PLAN_T, a.R - r0);
         for (int64_t i = tid; i < total[0] && base[0] + i < a.max_items; i += PLAN_T) {
             const int k = last_at_most(start[0], nr - 1, i);
-            const Req x = request(a, r0 + k);
-            const int pc = pieces_of(x, per), local = static_cast<int>(i - start[0][k]), tile = local / pc, piece = local - tile * pc;
+            const Req x = request<K>(a, r0 + k);
+            const int pc = pieces_of(x, per), local = static_cast<int>(i - start[0][k]), nth = local / pc, piece = local - nth * pc;
+            const int tile = x.tiles - 1 - nth;
             const int64_t part = base[1] + start[1][k] + local;
             const bool split = pc > 1 && part < a.max_parts;
-            a.items[base[0] + i] = make_item(a, x, r0 + k, tile, piece, pc, split ? static_cast<int>(part) : -1);
-            const int64_t j = base[2] + start[2][k] + tile;
-            if (split && piece == 0 && j < a.max_joins) a.joins[j] = make_join(a, x, tile, pc, static_cast<int>(part));
+            a.items[base[0] + i] = make_item<K>(a, x, r0 + k, tile, piece, pc, split ? static_cast<int>(part) : -1);
+            const int64_t j = base[2] + start[2][k] + nth;
+            if (split && piece == 0 && j < a.max_joins) a.joins[j] = make_join<K>(a, x, tile, pc, static_cast<int>(part));
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k) base[k] += total[k];
@@ -488,6 +519,11 @@ __global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs a) {
     if (tid == 0)
         *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))),
                            static_cast<int32_t>(min(base[2], static_cast<int64_t>(a.max_joins))), {0, 0}};
+}
+// block 0: the schedule of the short requests, block 1: the chunks'
+__global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs narrow, PlanArgs wide) {
+    if (blockIdx.x == 0) plan<Narrow>(narrow);
+    else plan<Wide>(wide);
 }
 
 // ---------------------------------------------------------------------------
@@ -507,7 +543,7 @@ struct AttnArgs {
     const int32_t* table;
     int64_t bt_stride;
     PlanArgs plan;
-    float* part;                         // [slot][key head][TILE][D] sums, then [slot][key head][TILE][2] (m, l)
+    float* part;                         // [slot][key head][TILE][D] sums; ml: [slot][key head][TILE][2] (m, l)
     float* ml;
     int32_t G, heads, page_log2, num_pages, window, zero_tail;
     float scale;                         // sm_scale * log2(e)
@@ -515,7 +551,7 @@ struct AttnArgs {
 
 constexpr float M_INIT = -1.0e30f;
 constexpr float SLACK = 8.0f;            // the running maximum moves when a score passes it by this (log2 units)
-constexpr int WAVES = 4;
+constexpr int WAVES = 4;                 // of the 16-row kernel
 constexpr float LN2 = 0.69314718055994531f;
 
 // 16-bit words of a row as floats (exact)
@@ -564,6 +600,7 @@ struct Raw {
 
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
+    constexpr int TILE = Narrow::TILE, GROUP = Narrow::GROUP;
     constexpr int NB = D / 16;           // PV products per group
     constexpr int KW = D / 32;           // QK products (and K dwords) per tile
     constexpr int ROWB = D / 2;          // packed bytes per token
@@ -572,7 +609,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = blockIdx.y;
     Item it;
-    if (!find_item(a.plan, blockIdx.x, lane, it)) return;
+    if (!find_item<Narrow>(a.plan, blockIdx.x, lane, it)) return;
     const int c = lane & 15, kb = lane >> 4;
     const int nrows = min(TILE, it.qlen * a.G - it.row0);
 
@@ -706,7 +743,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
         mx = vmax2(mx, s[7]);
         if (__builtin_amdgcn_ballot_w64(mx > m_run + SLACK)) {
             mx = col_max(mx);
-            const float mnew = fmaxf(m_run, mx);
+            const float mnew = mx > m_run + SLACK ? mx : m_run;        // (a row's own scores alone move its maximum)
             const float alpha = fast_exp2(m_run - mnew);
             l_run *= alpha;
 #pragma unroll
@@ -805,19 +842,362 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
     }
 }
 
-// Adds up the pieces of the split tiles: one workgroup per tile and KV head.
+// ---------------------------------------------------------------------------
+// attention: CHUNK query rows per workgroup
+// ---------------------------------------------------------------------------
+// A wavefront owns 32 rows.  The codes of 64 keys at a time are turned into
+// fp16 operands once for all rows of the workgroup and laid in LDS (K as
+// [key][channel], V transposed as [channel][key]), double-buffered: while one
+// block is multiplied, the next one's codes are already in registers.
+//   QK  S^T[key][row] = K . Q^T  with v_mfma_f32_32x32x16_f16; codes and (scaled
+//       by a power of two) queries are exact, the K scale multiplies the fp32
+//       score in the fma that subtracts the reference: t = S k_scale - M.
+//   PV  O^T[channel][row] = V^T . P'^T, P' = fp16(2^t v_scale) against the exact
+//       codes.  The reference M of a row follows max(score + log2 of the
+//       block's largest V scale), so that P' keeps to [0, 2^13] whatever the
+//       scales are; rounding P' to 11 bits once is the only rounding between
+//       the scores and the output.
+// Output register i of a lane (row l & 31, half h = l >> 5) of a 32-key tile is
+// key 8 (i >> 2) + 4 h + (i & 3); V's keys lie in LDS in the order that makes
+// registers 8s .. 8s + 7 the B operand of step s, so P never leaves its lane.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+constexpr float P_SHIFT = 6.0f;          // P' is at most 2^(P_SHIFT + SLACK_W + 1)
+constexpr float SLACK_W = 6.0f;
+constexpr int BLK = 64;                  // keys per step
+
+__device__ __forceinline__ uint32_t pk_sub1032(uint32_t x) {
+    const f16x2 b = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) - b);
+}
+// two codes of a word as fp16: 1024 + (nibble ^ 8) is exact, so is minus 1032
+__device__ __forceinline__ uint32_t codes2(uint32_t x, int s) { return pk_sub1032(nib2(x, s, 0x64086408u)); }
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+    const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+template <int D>
+struct ChunkLds {
+    uint8_t k[2][BLK * D * 2];           // [key][D / 8 chunks of 16 bytes], swizzled
+    uint8_t v[2][D * BLK * 2];           // [channel][8 chunks of 8 keys], swizzled
+    float ks[2][BLK];                    // K scale * qk
+    float vs[2][BLK];
+    float ve[2];                         // log2 bound of the block's V scales
+    int ok[2];                           // bit t: 16-key tile t's page is inside the pool
+    float red[CHUNK_WAVES];
+};
+
+// byte offsets of a 16-byte chunk: neighbouring keys' (channels') equal chunks
+// and one key's chunks fall on different banks, for the stores and the loads
+template <int D>
+__device__ __forceinline__ uint32_t k_at(int key, int x) {
+    if constexpr (D == 128) return key * 256 + ((x ^ (key & 15)) << 4);
+    else return key * 128 + ((x ^ ((key >> 1) & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t v_at(int ch, int x) {
+    const int f = ((ch >> 2) & 7) ^ ((ch << 1) & 4);
+    return ch * 128 + ((x ^ f) << 4);
+}
+
+// e with x < 2^e, x >= 0 finite
+__device__ __forceinline__ float scale_bound(float x) {
+    return static_cast<float>(static_cast<int>(__float_as_uint(fmaxf(x, 0x1p-24f)) >> 23) - 126);
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnArgs a) {
+    constexpr int KM = D / 16;           // QK products per 32 keys
+    constexpr int DT = D / 32;           // 32-channel tiles of V
+    constexpr int ROWB = D / 2;
+    constexpr int NT = 64 * CHUNK_WAVES;
+    constexpr int NV = 8 * (D / 4);      // V tasks: 8 keys x 4 channels
+    constexpr int NK = BLK * (D / 32);   // K tasks: 1 key x 32 channels
+    static_assert(NV + NK <= NT, "a thread has one task");
+    extern __shared__ uint8_t lds_raw[];
+    ChunkLds<D>& L = *reinterpret_cast<ChunkLds<D>*>(lds_raw);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = blockIdx.x % a.heads;
+    Item it;
+    if (!find_item<Wide>(a.plan, blockIdx.x / a.heads, lane, it)) return;
+    const int r32 = lane & 31, h = lane >> 5;
+    const int nrows = min(CHUNK, it.qlen * a.G - it.row0);
+
+    // ---- queries ----
+    const int rt = 32 * w + r32;                          // row within the tile
+    const int row = it.row0 + min(rt, nrows - 1);
+    const int tok = row / a.G, hq = row - tok * a.G;
+    const uint16_t* qp = a.q + (static_cast<int64_t>(it.q0) + tok) * a.q_t + (static_cast<int64_t>(head) * a.G + hq) * a.q_h + 8 * h;
+    u32x4 qr[KM];
+    float amax = 0.f;
+#pragma unroll
+    for (int m = 0; m < KM; ++m) {
+        qr[m] = *reinterpret_cast<const u32x4*>(qp + 16 * m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(half_at<F16>(qr[m][i], 0)), fabsf(half_at<F16>(qr[m][i], 1))));
+    }
+    amax = xmax32(amax);
+    if (!(amax < INFINITY)) amax = 0.f;
+    amax = xmax16(max16_dpp(amax));
+    if (lane == 0) L.red[w] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CHUNK_WAVES; ++i) amax = fmaxf(amax, L.red[i]);
+    const int qe = q_exponent(amax);
+    const float qs = pow2(-qe), qk = a.scale * pow2(qe);
+    f16x8 qop[KM];
+#pragma unroll
+    for (int m = 0; m < KM; ++m) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = half_at<F16>(qr[m][i >> 1], i & 1) * qs;
+        qop[m] = f16x8{static_cast<_Float16>(f[0]), static_cast<_Float16>(f[4]), static_cast<_Float16>(f[1]), static_cast<_Float16>(f[5]),
+                       static_cast<_Float16>(f[2]), static_cast<_Float16>(f[6]), static_cast<_Float16>(f[3]), static_cast<_Float16>(f[7])};
+    }
+    const int pos = it.len - it.qlen + tok;
+    const int lo = first_key(pos, a.window), top = min(pos, it.key1 - 1);
+    // this wavefront's rows (none: it only converts): every one sees [all_lo, all_hi], none past any_hi
+    const bool active = 32 * w < nrows;
+    const int t0 = (it.row0 + min(32 * w, nrows - 1)) / a.G, t1 = (it.row0 + min(32 * w + 31, nrows - 1)) / a.G;
+    const int all_hi = min(it.len - it.qlen + t0, it.key1 - 1), all_lo = first_key(it.len - it.qlen + t1, a.window);
+    const int any_hi = it.len - it.qlen + t1, any_lo = first_key(it.len - it.qlen + t0, a.window);
+
+    // ---- conversion tasks ----
+    const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
+    const int page_mask = (1 << a.page_log2) - 1;
+    const int32_t* trow = a.table + it.req * a.bt_stride;
+    const int nblk = a.num_pages > 0 ? (max(it.key1 - it.key0, 0) + BLK - 1) / BLK : 0;
+    const bool is_v = tid < NV, is_k = tid >= NV && tid < NV + NK;
+    // V: chunk c8 holds the keys 16 (c8 >> 1) + 4 (c8 & 1) + {0..3, 8..11}, channels 4 dq ..
+    const int c8 = tid / (D / 4), dq = tid - c8 * (D / 4);
+    const int kt = tid - NV, kkey = kt / (D / 32), kq = kt - kkey * (D / 32);
+    // scales: wavefront 0's lane j is key j for V, wavefront 1's for K
+    const int my16 = is_v ? c8 >> 1 : is_k ? kkey >> 4 : 0;       // the task's 16-key tile
+    auto page_id = [&](int blk, int t16) -> int {
+        const int t = min(it.key0 + BLK * blk + 16 * t16, it.key1 - 1);
+        return trow[t >> a.page_log2];
+    };
+    auto tile_off = [&](int blk, int t16) -> int { return (min(it.key0 + BLK * blk + 16 * t16, it.key1 - 1) & page_mask) & ~15; };
+    struct Raw64 {
+        uint32_t d[8];
+        uint32_t s;                      // scale bits (wavefronts 0 and 1)
+        int sid;                         // and their page
+    };
+    Raw64 raw{};
+    auto fetch = [&](int blk, int id, int sid) {
+        const int64_t pg = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages) ? id : 0;
+        const int off = tile_off(blk, my16);
+        if (is_v) {
+            const int8_t* b = a.vp + pg * a.ps_page + hk + (off + 4 * (c8 & 1)) * ROWB + 2 * dq;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) raw.d[e] = *reinterpret_cast<const uint16_t*>(b + ((e & 3) + 8 * (e >> 2)) * ROWB);
+        } else if (is_k) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(a.kp + pg * a.ps_page + hk + (off + (kkey & 15)) * ROWB + 16 * kq);
+            raw.d[0] = x[0]; raw.d[1] = x[1]; raw.d[2] = x[2]; raw.d[3] = x[3];
+        }
+        if (w < 2) {
+            const bool ok = static_cast<uint32_t>(sid) < static_cast<uint32_t>(a.num_pages);
+            const int64_t sp = ok ? sid : 0;
+            const int so = tile_off(blk, lane >> 4) + (lane & 15);
+            raw.s = (w == 0 ? a.vs : a.ks)[sp * a.ss_page + hs + so];
+            raw.sid = ok;
+        }
+    };
+    auto store = [&](int b, int blk) {
+        if (is_v) {
+            uint32_t pr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pr[i] = raw.d[2 * i] | (raw.d[2 * i + 1] << 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 o = {codes2(pr[0], 4 * i), codes2(pr[1], 4 * i), codes2(pr[2], 4 * i), codes2(pr[3], 4 * i)};
+                *reinterpret_cast<u32x4*>(&L.v[b][v_at(4 * dq + i, c8)]) = o;
+            }
+        } else if (is_k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 o = {codes2(raw.d[i], 0), codes2(raw.d[i], 4), codes2(raw.d[i], 8), codes2(raw.d[i], 12)};
+                *reinterpret_cast<u32x4*>(&L.k[b][k_at<D>(kkey, 4 * kq + i)]) = o;
+            }
+        }
+        if (w == 0) {
+            const float f = f16_bits_to_f32(static_cast<uint16_t>(raw.s));
+            float x = fabsf(f);
+            // keys past the piece or in no page hold anything: not in the bound
+            if (!(x < INFINITY) || it.key0 + BLK * blk + lane >= it.key1 || !raw.sid) x = 0.f;
+            x = col_max(max16_dpp(x));
+            L.vs[b][lane] = f;
+            if (lane == 0) L.ve[b] = scale_bound(x);
+        } else if (w == 1) {
+            const uint64_t m = __builtin_amdgcn_ballot_w64(raw.sid != 0);
+            L.ks[b][lane] = f16_bits_to_f32(static_cast<uint16_t>(raw.s)) * qk;
+            if (lane == 0) L.ok[b] = static_cast<int>((m & 1) | ((m >> 15) & 2) | ((m >> 30) & 4) | ((m >> 45) & 8));
+        }
+    };
+
+    float m_run = M_INIT, l_run = 0.f;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+    auto compute = [&](int b, int blk) {
+        const int j0 = it.key0 + BLK * blk;
+        f32x16 sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[t][i] = 0.f;
+#pragma unroll
+            for (int m = 0; m < KM; ++m) {
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(&L.k[b][k_at<D>(32 * t + r32, 2 * m + h)]);
+                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qop[m], sc[t], 0, 0, 0);
+            }
+        }
+        // t = score - reference (0 while the row has seen no key)
+        const int ok = __builtin_amdgcn_readfirstlane(L.ok[b]);
+        const bool unset = m_run == M_INIT;
+        const float m_use = unset ? 0.f : m_run;
+        float t[32];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&L.ks[b][8 * g + 4 * h]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[4 * g + i] = __builtin_fmaf(sc[g >> 2][4 * (g & 3) + i], x[i], -m_use);
+        }
+        float ve = L.ve[b];
+        uint32_t dead = 0;
+        const bool edge = j0 + BLK - 1 > all_hi || j0 < all_lo || ok != 15;
+        if (edge) {
+            // keys that the row does not see; its bound is over the others' V
+            // scales, so that what is hidden from a row does not touch its bits
+            float vx = 0.f;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(&L.vs[b][8 * g + 4 * h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 8 * g + 4 * h + i;
+                    if (j > top || j < lo || !((ok >> (g >> 1)) & 1)) {
+                        t[4 * g + i] = -INFINITY;
+                        dead |= 1u << (4 * g + i);
+                    } else if (fabsf(x[i]) < INFINITY) {
+                        vx = fmaxf(vx, fabsf(x[i]));
+                    }
+                }
+            }
+            ve = scale_bound(xmax32(vx));
+        }
+        float mx = vmax3(t[0], t[1], t[2]);
+#pragma unroll
+        for (int i = 3; i < 31; i += 2) mx = vmax3(mx, t[i], t[i + 1]);
+        mx = vmax2(mx, t[31]) + ve;
+        // (a row's own scores alone decide whether its reference moves)
+        if (__builtin_amdgcn_ballot_w64(unset || mx > P_SHIFT + SLACK_W)) {      // rare after the first blocks
+            mx = xmax32(mx);
+            const bool move = unset ? mx > -INFINITY : mx > P_SHIFT + SLACK_W;
+            const float up = move ? mx - P_SHIFT : 0.f;
+            const float alpha = unset ? 1.0f : fast_exp2(-up);
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= alpha;
+            m_run = move ? m_use + up : m_run;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) t[i] -= up;
+        }
+        float ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            t[i] = fast_exp2(t[i]);
+            ls += t[i];
+        }
+        l_run += ls;
+        uint32_t pw[16];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            // (lane i of a quad reads key 4h + i of the group: quad broadcasts hand out all four)
+            const float v = L.vs[b][8 * g + 4 * h + (lane & 3)];
+            t[4 * g] *= quad_bcast<0>(v);
+            t[4 * g + 1] *= quad_bcast<1>(v);
+            t[4 * g + 2] *= quad_bcast<2>(v);
+            t[4 * g + 3] *= quad_bcast<3>(v);
+        }
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) t[i] = (dead >> i) & 1 ? 0.f : t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pw[i] = pack_f16x2(t[2 * i], t[2 * i + 1]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const u32x4 pv = {pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f16x8 vf = *reinterpret_cast<const f16x8*>(&L.v[b][v_at(32 * d + r32, 2 * s + h)]);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, __builtin_bit_cast(f16x8, pv), acc[d], 0, 0, 0);
+            }
+        }
+    };
+
+    if (nblk > 0) {
+        fetch(0, page_id(0, my16), page_id(0, lane >> 4));
+        int id = page_id(1, my16), sid = page_id(1, lane >> 4);
+        store(0, 0);
+        if (nblk > 1) fetch(1, id, sid);
+        id = page_id(2, my16);
+        sid = page_id(2, lane >> 4);
+        __syncthreads();
+        for (int n = 0; n < nblk; ++n) {
+            if (n + 1 < nblk) {
+                store((n + 1) & 1, n + 1);
+                if (n + 2 < nblk) {
+                    fetch(n + 2, id, sid);
+                    id = page_id(n + 3, my16);
+                    sid = page_id(n + 3, lane >> 4);
+                }
+            }
+            const int j0 = it.key0 + BLK * n;
+            if (active && j0 <= any_hi && j0 + BLK > any_lo) compute(n & 1, n);
+            __syncthreads();
+        }
+    }
+    if (rt >= nrows) return;
+    const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+    l_run = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
+    if (it.part >= 0) {
+        const int64_t at = (static_cast<int64_t>(it.part) * a.heads + head) * CHUNK + rt;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(a.part + at * D + 32 * d + 8 * g + 4 * h) =
+                    f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        if (h == 0) { a.ml[at * 2] = m_run; a.ml[at * 2 + 1] = l_run; }
+    } else {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store_row<F16>(a, it.q0, row, head, 32 * d + 8 * g + 4 * h, m_run, l_run,
+                               f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]});
+    }
+}
+
+// Adds up the pieces of the split tiles: one workgroup per 32 rows of a tile
+// (blockIdx.z) and KV head.
 // A row is 4 channels a lane of D/4; while rows are fewer than the lane
 // groups, several groups share a row's pieces and meet in LDS.  Four pieces
 // are in flight per group.  By zero_tail it also clears the rows behind the
 // last request.
 constexpr int JOIN_T = 1024;
-template <int D, bool F16>
+template <typename K, int D, bool F16>
 __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
     constexpr int LG = JOIN_T / (D / 4);    // lane groups
     __shared__ float so[LG][D];
     __shared__ float sm[LG], sl[LG];
     const int tid = threadIdx.x, head = blockIdx.y;
-    if (a.zero_tail && a.plan.cu) {
+    if (a.zero_tail && a.plan.cu && blockIdx.z == 0) {
         const int64_t first = min(max(a.plan.cu[a.plan.R], 0), a.plan.T);
         const int64_t total = (a.plan.T - first) * a.G * (D / 4);   // of one KV head
         for (int64_t e = static_cast<int64_t>(blockIdx.x) * JOIN_T + tid; e < total; e += static_cast<int64_t>(gridDim.x) * JOIN_T) {
@@ -828,21 +1208,23 @@ __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
         }
     }
     Join jn;
-    if (!find_join(a.plan, blockIdx.x, tid & 63, jn)) return;
-    const int share = jn.rows <= LG / 8 ? 8 : jn.rows <= LG / 4 ? 4 : jn.rows <= LG / 2 ? 2 : 1;
+    if (!find_join<K>(a.plan, blockIdx.x, tid & 63, jn)) return;
+    const int first = 32 * blockIdx.z, rows = min(32, jn.rows - first);
+    if (rows <= 0) return;
+    const int share = rows <= LG / 8 ? 8 : rows <= LG / 4 ? 4 : rows <= LG / 2 ? 2 : 1;
     const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4)), sub = g % share;
-    for (int r0 = 0; r0 < jn.rows; r0 += LG / share) {
+    for (int r0 = 0; r0 < rows; r0 += LG / share) {
         const int rw = r0 + g / share;
         float m = M_INIT, l = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        if (rw < jn.rows) {
+        if (rw < rows) {
             constexpr int DEEP = 4;
             for (int i0 = sub; i0 < jn.pieces; i0 += DEEP * share) {
                 float mi[DEEP], li[DEEP];
                 f32x4 oi[DEEP];
 #pragma unroll
                 for (int j = 0; j < DEEP; ++j) {
-                    const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * TILE + rw;
+                    const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * K::TILE + first + rw;
                     mi[j] = a.ml[at * 2];
                     li[j] = a.ml[at * 2 + 1];
                     oi[j] = *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
@@ -869,7 +1251,7 @@ __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
                 m = mn;
             }
         }
-        if (rw < jn.rows) store_row<F16>(a, jn.q0, jn.row0 + rw, head, ch, m, l, o);
+        if (rw < rows) store_row<F16>(a, jn.q0, jn.row0 + first + rw, head, ch, m, l, o);
     }
 }
 
@@ -877,30 +1259,43 @@ __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 struct Sizes {
-    int64_t target, items, joins, parts;
-    size_t off_items, off_joins, off_part, off_ml, bytes;
+    int64_t target, enough, items, joins, parts;
+    size_t off_counts, off_items, off_joins, off_part, off_ml, end;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// A request's tiles are cut into ceil(units / per) pieces with per >=
-// total / target: at most target + tiles in all, at most 2 target of them in
-// tiles that are cut (units > per), which are at most target; the tiles are
-// at most rows / TILE + requests.
-Sizes sizes_of(const hyq_paged_params& p) {
+// Where a kind's schedule and partial results lie, from `at` on.  A request's
+// tiles are cut into ceil(units / per) pieces with per >= total / target: at
+// most target + tiles in all, at most 2 target of them in tiles that are cut
+// (units > per), which are at most target.  `tiles` bounds the tiles.
+template <typename K>
+Sizes sizes_of(const hyq_paged_params& p, int64_t tiles, size_t at) {
     Sizes s{};
-    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_repeat;
-    const int64_t tiles = rows / TILE + std::min<int64_t>(p.num_requests, p.num_tokens);
-    s.target = std::max<int64_t>(1, SLOTS / p.kv_heads);
-    s.items = s.target + tiles;
+    s.target = std::max<int64_t>(1, K::SLOTS / p.kv_heads);
+    s.enough = (K::ENOUGH + p.kv_heads - 1) / p.kv_heads;
+    s.items = tiles ? s.target + tiles : 0;
     s.joins = std::min(tiles, s.target);
     s.parts = std::min(s.items, 2 * s.target);
-    s.off_items = 256;
+    s.off_counts = at;
+    s.off_items = at + 256;
     s.off_joins = up256(s.off_items + s.items * sizeof(Item));
     s.off_part = up256(s.off_joins + s.joins * sizeof(Join));
-    s.off_ml = up256(s.off_part + static_cast<size_t>(s.parts) * p.kv_heads * TILE * p.head_dim * 4);
-    s.bytes = up256(s.off_ml + static_cast<size_t>(s.parts) * p.kv_heads * TILE * 2 * 4);
+    s.off_ml = up256(s.off_part + static_cast<size_t>(s.parts) * p.kv_heads * K::TILE * p.head_dim * 4);
+    s.end = up256(s.off_ml + static_cast<size_t>(s.parts) * p.kv_heads * K::TILE * 2 * 4);
     return s;
+}
+struct Both {
+    Sizes narrow, wide;
+};
+Both sizes_of(const hyq_paged_params& p) {
+    const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_repeat, R = std::min(p.num_requests, p.num_tokens);
+    // without cu_seqlens every request has kv_repeat rows
+    const bool narrow = p.kv_repeat <= Narrow::TILE, wide = p.cu_seqlens ? rows > Narrow::TILE : !narrow;
+    Both b;
+    b.narrow = sizes_of<Narrow>(p, narrow ? R : 0, 0);
+    b.wide = sizes_of<Wide>(p, wide ? rows / Wide::TILE + std::min(R, rows / (Narrow::TILE + 1)) : 0, b.narrow.end);
+    return b;
 }
 
 int check_pool(const char* what, int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t kv_heads, const void* kp,
@@ -951,9 +1346,26 @@ int check_attention(const hyq_paged_params* p) {
 }
 
 template <int D, bool F16>
-void launch_attention(const AttnArgs& a, const Sizes& s, hipStream_t st) {
-    paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
-    paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(s.joins), a.heads), dim3(JOIN_T), 0, st>>>(a);
+int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, hipStream_t st) {
+    // (the join launch also clears the rows behind the last request: once)
+    if (s.narrow.items) {
+        a.part = reinterpret_cast<float*>(ws + s.narrow.off_part);
+        a.ml = reinterpret_cast<float*>(ws + s.narrow.off_ml);
+        paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
+        paged_join_kernel<Narrow, D, F16><<<dim3(static_cast<unsigned>(s.narrow.joins), a.heads), dim3(JOIN_T), 0, st>>>(a);
+        a.zero_tail = 0;
+    }
+    if (s.wide.items) {
+        a.plan = wide;
+        a.part = reinterpret_cast<float*>(ws + s.wide.off_part);
+        a.ml = reinterpret_cast<float*>(ws + s.wide.off_ml);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_chunk_kernel<D, F16>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(ChunkLds<D>)));
+        if (e != hipSuccess) return fail(HYQ_EDEVICE, std::string("hyq_paged_attention: ") + hipGetErrorString(e));
+        paged_chunk_kernel<D, F16><<<dim3(static_cast<unsigned>(s.wide.items * a.heads)), dim3(64 * CHUNK_WAVES), sizeof(ChunkLds<D>), st>>>(a);
+        paged_join_kernel<Wide, D, F16><<<dim3(static_cast<unsigned>(s.wide.joins), a.heads, CHUNK / 32), dim3(JOIN_T), 0, st>>>(a);
+    }
+    return check_launch("hyq_paged_attention");
 }
 
 }  // namespace
@@ -1038,34 +1450,31 @@ extern "C" int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_
 
 extern "C" size_t hyq_paged_attention_workspace_size(const hyq_paged_params* p) {
     if (check_attention(p) != HYQ_OK || p->num_requests == 0 || p->num_tokens == 0) return 0;
-    return sizes_of(*p).bytes;
+    return sizes_of(*p).wide.end;
 }
 
 extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, size_t workspace_bytes, void* stream) {
     if (int st = check_attention(p)) return st;
     if (p->num_requests == 0 || p->num_tokens == 0) return HYQ_OK;
-    const Sizes s = sizes_of(*p);
-    if (!workspace || workspace_bytes < s.bytes)
-        return fail(HYQ_ENOSPC, "hyq_paged_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(s.bytes) + " needed");
+    const Both s = sizes_of(*p);
+    if (!workspace || workspace_bytes < s.wide.end)
+        return fail(HYQ_ENOSPC, "hyq_paged_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(s.wide.end) + " needed");
     if (!aligned(workspace, 256)) return fail(HYQ_EINVAL, "hyq_paged_attention: workspace must be 256-byte aligned");
     char* ws = static_cast<char*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    PlanArgs pl{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, p->window,
-                p->max_pages * p->page_size, static_cast<int32_t>(s.target), static_cast<int32_t>(s.items),
-                static_cast<int32_t>(s.parts), static_cast<int32_t>(s.joins), reinterpret_cast<Counts*>(ws), reinterpret_cast<Item*>(ws + s.off_items),
-                reinterpret_cast<Join*>(ws + s.off_joins)};
-    if (p->num_requests > INLINE_R) paged_plan_kernel<<<dim3(1), dim3(PLAN_T), 0, st>>>(pl);
-    AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
-               p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head, p->k_scale,
-               p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, pl,
-               reinterpret_cast<float*>(ws + s.off_part), reinterpret_cast<float*>(ws + s.off_ml), p->kv_repeat, p->kv_heads,
-               log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail, p->sm_scale * 1.44269504f};
-    if (p->head_dim == 128) {
-        if (p->dtype_fp16) launch_attention<128, true>(a, s, st);
-        else launch_attention<128, false>(a, s, st);
-    } else {
-        if (p->dtype_fp16) launch_attention<64, true>(a, s, st);
-        else launch_attention<64, false>(a, s, st);
-    }
-    return check_launch("hyq_paged_attention");
+    auto plan_of = [&](const Sizes& z) {
+        return PlanArgs{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, p->window, p->max_pages * p->page_size,
+                        static_cast<int32_t>(z.enough), static_cast<int32_t>(z.target), static_cast<int32_t>(z.items),
+                        static_cast<int32_t>(z.parts), static_cast<int32_t>(z.joins), reinterpret_cast<Counts*>(ws + z.off_counts),
+                        reinterpret_cast<Item*>(ws + z.off_items), reinterpret_cast<Join*>(ws + z.off_joins)};
+    };
+    const PlanArgs narrow = plan_of(s.narrow), wide = plan_of(s.wide);
+    if (p->num_requests > INLINE_R) paged_plan_kernel<<<dim3(s.wide.items ? 2 : 1), dim3(PLAN_T), 0, st>>>(narrow, wide);
+    const AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
+                     p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head,
+                     p->k_scale, p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, narrow, nullptr, nullptr,
+                     p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail,
+                     p->sm_scale * 1.44269504f};
+    if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, wide, s, ws, st) : launch_attention<128, false>(a, wide, s, ws, st);
+    return p->dtype_fp16 ? launch_attention<64, true>(a, wide, s, ws, st) : launch_attention<64, false>(a, wide, s, ws, st);
 }
