@@ -6,6 +6,10 @@
 // output and calls hyq_decode_hybrid through the pointer the Python side
 // hands over at set-up (the library ctypes loaded, whichever file that is).
 //
+// The paged cache's calls (hyquant_amd/paged.py) take the same way: each makes
+// the checks of its Python form and declines (status -1) whatever fails one,
+// so that the Python form copies, or raises.
+//
 // decode takes exactly the calls the Python fast path takes (bf16 / fp16 q
 // with unit channel stride, kv_repeat dividing the query heads, CUDA tensors,
 // the three bf16 segments with unit channel strides, equal K / V lengths and
@@ -24,6 +28,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
+#include <optional>
 
 #include "../../include/hyq.h"
 
@@ -118,7 +123,177 @@ Result run(const at::Tensor& q, int64_t bh_q, int64_t d, int64_t q_stride, at::I
     return {st, out};
 }
 
+// ---- the paged cache ---------------------------------------------------------
+
+using BatchFn = decltype(&hyq_paged_batch);
+using PagedAppendFn = decltype(&hyq_paged_append);
+using GatherFn = decltype(&hyq_paged_gather);
+using AttentionFn = decltype(&hyq_paged_attention);
+using AttentionSizeFn = decltype(&hyq_paged_attention_workspace_size);
+struct {
+    BatchFn batch = nullptr;
+    PagedAppendFn append = nullptr;
+    GatherFn gather = nullptr;
+    AttentionSizeFn size = nullptr;
+    AttentionFn attention = nullptr;
+} g_paged;
+
+bool plain(const at::Tensor& t, at::ScalarType type, int64_t dim, const at::Device& device) {
+    return t.scalar_type() == type && t.dim() == dim && t.device() == device && !at::isTensorSubclassLike(t);
+}
+// an integer tensor whose last dimension is contiguous
+bool ints(const at::Tensor& t, at::ScalarType type, int64_t dim, const at::Device& device) {
+    return plain(t, type, dim, device) && (t.stride(dim - 1) == 1 || t.numel() <= 1);
+}
+bool half(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+// rows of channels at 16-byte addresses
+bool rows16(const at::Tensor& t) {
+    return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+// a pool as _check_pool wants it (sizes and alignment are the library's to check)
+bool pool(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks, const at::Tensor& vs, const at::Device& device) {
+    if (!plain(kp, at::kChar, 4, device) || !plain(vp, at::kChar, 4, device) || !plain(ks, at::kHalf, 3, device) ||
+        !plain(vs, at::kHalf, 3, device))
+        return false;
+    if (kp.sizes() != vp.sizes() || kp.strides() != vp.strides() || ks.sizes() != vs.sizes() || ks.strides() != vs.strides())
+        return false;
+    if (ks.size(0) != kp.size(0) || ks.size(1) != kp.size(1) || ks.size(2) != kp.size(2)) return false;
+    return kp.numel() > 0 && kp.stride(3) == 1 && kp.stride(2) == kp.size(3) && ks.stride(2) == 1;
+}
+template <typename T>
+T* ptr(const at::Tensor& t) { return static_cast<T*>(t.data_ptr()); }
+
 }  // namespace
+
+void set_paged(int64_t batch, int64_t append, int64_t gather, int64_t size, int64_t attention) {
+    g_paged.batch = reinterpret_cast<BatchFn>(batch);
+    g_paged.append = reinterpret_cast<PagedAppendFn>(append);
+    g_paged.gather = reinterpret_cast<GatherFn>(gather);
+    g_paged.size = reinterpret_cast<AttentionSizeFn>(size);
+    g_paged.attention = reinterpret_cast<AttentionFn>(attention);
+}
+
+// (status, cu_seqlens, seq_lens, slots, positions, pages_used)
+std::tuple<int64_t, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_batch(
+    const at::Tensor& ctx, const at::Tensor& fresh, const at::Tensor& table, const at::Tensor& free_pages, int64_t page,
+    int64_t tokens, int64_t stream) {
+    const auto dev = ctx.device();
+    const int64_t R = ctx.dim() == 1 ? ctx.size(0) : 0;
+    if (!g_paged.batch || !dev.is_cuda() || R < 1 || tokens < 0 || tokens > INT32_MAX || page < 0 || page > INT32_MAX ||
+        !ints(ctx, at::kInt, 1, dev) || !ints(fresh, at::kInt, 1, dev) || !ints(table, at::kInt, 2, dev) ||
+        !ints(free_pages, at::kInt, 1, dev) || fresh.size(0) != R || table.size(0) != R || free_pages.size(0) > INT32_MAX)
+        return {-1, {}, {}, {}, {}, {}};
+    const c10::DeviceGuard guard(dev);
+    const auto i32 = ctx.options(), i64 = i32.dtype(at::kLong);
+    const at::Tensor cu = at::empty({R + 1}, i32), lens = at::empty({R}, i32), used = at::empty({1}, i32);
+    const at::Tensor slots = at::empty({tokens}, i64), positions = at::empty({tokens}, i64);
+    const int st = g_paged.batch(ptr<int32_t>(ctx), ptr<int32_t>(fresh), static_cast<int32_t>(R), ptr<int32_t>(table), table.stride(0),
+                                 static_cast<int32_t>(table.size(1)), ptr<int32_t>(free_pages),
+                                 static_cast<int32_t>(free_pages.size(0)), static_cast<int32_t>(page), static_cast<int32_t>(tokens),
+                                 ptr<int32_t>(cu), ptr<int32_t>(lens), ptr<int64_t>(slots), ptr<int64_t>(positions),
+                                 ptr<int32_t>(used), reinterpret_cast<void*>(stream));
+    return {st, cu, lens, slots, positions, used};
+}
+
+int64_t paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, const at::Tensor& kp, const at::Tensor& vp,
+                     const at::Tensor& ks, const at::Tensor& vs, int64_t stream) {
+    const auto dev = k.device();
+    if (!g_paged.append || !dev.is_cuda() || !half(k) || !plain(k, k.scalar_type(), 3, dev) || !plain(v, k.scalar_type(), 3, dev) ||
+        k.sizes() != v.sizes() || !pool(kp, vp, ks, vs, dev) || k.size(1) != kp.size(1) || k.size(2) != 2 * kp.size(3) ||
+        !ints(slots, at::kLong, 1, dev) || slots.size(0) != k.size(0) || k.size(0) == 0 || !rows16(k) || !rows16(v))
+        return -1;
+    const c10::DeviceGuard guard(dev);
+    return g_paged.append(ptr<uint16_t>(k), k.stride(0), k.stride(1), ptr<uint16_t>(v), v.stride(0), v.stride(1),
+                          k.scalar_type() == at::kHalf, ptr<int64_t>(slots), k.size(0), static_cast<int32_t>(kp.size(1)),
+                          static_cast<int32_t>(k.size(2)), ptr<int8_t>(kp), ptr<int8_t>(vp), kp.stride(0), kp.stride(1),
+                          ptr<uint16_t>(ks), ptr<uint16_t>(vs), ks.stride(0), ks.stride(1), kp.size(0),
+                          static_cast<int32_t>(kp.size(2)), reinterpret_cast<void*>(stream));
+}
+
+// (status, k, v)
+std::tuple<int64_t, at::Tensor, at::Tensor> paged_gather(const at::Tensor& slots, const at::Tensor& kp, const at::Tensor& vp,
+                                                         const at::Tensor& ks, const at::Tensor& vs, bool fp16, int64_t stream) {
+    const auto dev = slots.device();
+    if (!g_paged.gather || !dev.is_cuda() || !ints(slots, at::kLong, 1, dev) || slots.size(0) == 0 || !pool(kp, vp, ks, vs, dev))
+        return {-1, {}, {}};
+    const c10::DeviceGuard guard(dev);
+    const auto opt = slots.options().dtype(fp16 ? at::kHalf : at::kBFloat16);
+    const at::Tensor k = at::empty({slots.size(0), kp.size(1), 2 * kp.size(3)}, opt), v = at::empty(k.sizes(), opt);
+    const int st = g_paged.gather(ptr<int64_t>(slots), slots.size(0), static_cast<int32_t>(kp.size(1)),
+                                  static_cast<int32_t>(2 * kp.size(3)), ptr<int8_t>(kp), ptr<int8_t>(vp), kp.stride(0), kp.stride(1),
+                                  ptr<uint16_t>(ks), ptr<uint16_t>(vs), ks.stride(0), ks.stride(1), kp.size(0),
+                                  static_cast<int32_t>(kp.size(2)), fp16, ptr<uint16_t>(k), ptr<uint16_t>(v),
+                                  reinterpret_cast<void*>(stream));
+    return {st, k, v};
+}
+
+// (status, out, lse)
+std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
+                                                            const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table,
+                                                            const at::Tensor& lens, const std::optional<at::Tensor>& cu,
+                                                            const std::optional<double>& sm_scale, int64_t window,
+                                                            bool want_lse, int64_t stream) {
+    const std::tuple<int64_t, at::Tensor, at::Tensor> skip{-1, {}, {}};
+    const auto dev = q.device();
+    if (!g_paged.attention || !dev.is_cuda() || !half(q) || !plain(q, q.scalar_type(), 3, dev) || !pool(kp, vp, ks, vs, dev) ||
+        !ints(table, at::kInt, 2, dev) || !ints(lens, at::kInt, 1, dev))
+        return skip;
+    const int64_t T = q.size(0), HQ = q.size(1), D = q.size(2), R = lens.size(0), H = kp.size(1);
+    if (T == 0 || R == 0 || T > INT32_MAX || HQ == 0 || HQ % H || D != 2 * kp.size(3) || table.size(0) != R || !rows16(q) || window < 0 ||
+        window > INT32_MAX)
+        return skip;
+    if (cu ? !ints(*cu, at::kInt, 1, dev) || cu->size(0) != R + 1 : T != R) return skip;
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor out = at::empty({T, HQ, D}, q.options());
+    at::Tensor lse;
+    hyq_paged_params p{};
+    if (want_lse) {
+        lse = at::empty({T, HQ}, q.options().dtype(at::kFloat));
+        p.lse = ptr<float>(lse);
+    }
+    p.q = q.data_ptr();
+    p.q_stride_t = q.stride(0);
+    p.q_stride_h = q.stride(1);
+    p.out = out.data_ptr();
+    p.o_stride_t = HQ * D;
+    p.o_stride_h = D;
+    p.k_pages = ptr<int8_t>(kp);
+    p.v_pages = ptr<int8_t>(vp);
+    p.p_stride_page = kp.stride(0);
+    p.p_stride_head = kp.stride(1);
+    p.k_scale = ptr<uint16_t>(ks);
+    p.v_scale = ptr<uint16_t>(vs);
+    p.s_stride_page = ks.stride(0);
+    p.s_stride_head = ks.stride(1);
+    p.block_table = ptr<int32_t>(table);
+    p.bt_stride = table.stride(0);
+    p.seq_lens = ptr<int32_t>(lens);
+    p.cu_seqlens = cu ? ptr<int32_t>(*cu) : nullptr;
+    p.num_pages = kp.size(0);
+    p.page_size = static_cast<int32_t>(kp.size(2));
+    p.max_pages = static_cast<int32_t>(table.size(1));
+    p.num_requests = static_cast<int32_t>(R);
+    p.num_tokens = static_cast<int32_t>(T);
+    p.kv_heads = static_cast<int32_t>(H);
+    p.kv_repeat = static_cast<int32_t>(HQ / H);
+    p.head_dim = static_cast<int32_t>(D);
+    p.window = static_cast<int32_t>(window);
+    p.sm_scale = static_cast<float>(sm_scale ? *sm_scale : std::pow(static_cast<double>(D), -0.5));
+    p.dtype_fp16 = q.scalar_type() == at::kHalf;
+    p.zero_tail = 3;
+    const size_t need = g_paged.size(&p);
+    if (need == 0) return skip;
+    const at::Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+    const int st = g_paged.attention(&p, ws.data_ptr(), need, reinterpret_cast<void*>(stream));
+    return {st, out, lse};
+}
+
+// the paged parameter block's size and the offsets of two of its fields
+std::tuple<int64_t, int64_t, int64_t> paged_layout() {
+    return {static_cast<int64_t>(sizeof(hyq_paged_params)), static_cast<int64_t>(offsetof(hyq_paged_params, num_pages)),
+            static_cast<int64_t>(offsetof(hyq_paged_params, zero_tail))};
+}
 
 // the library entry points (addresses from ctypes)
 void set_entry(int64_t hybrid, int64_t append) {
@@ -190,10 +365,16 @@ std::tuple<int64_t, int64_t, int64_t> layout() {
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.def("signatures", [] { return 2; }, "counts up when a function of this module takes other arguments");
+    m.def("signatures", [] { return 3; }, "counts up when a function of this module takes other arguments");
     m.def("layout", &layout, "sizeof(hyq_decode_params), offsetof(seg_n), offsetof(dtype_flags)");
     m.def("set_entry", &set_entry, "the addresses of hyq_decode_hybrid and hyq_append_rows");
     m.def("decode", &decode, "fused_d_stage_decode eager fast path");
     m.def("decode_cache", &decode_cache, "a layer cache's decode step");
     m.def("append", &append, "a layer cache's staging append");
+    m.def("paged_layout", &paged_layout, "sizeof(hyq_paged_params), offsetof(num_pages), offsetof(zero_tail)");
+    m.def("set_paged", &set_paged, "the addresses of the five hyq_paged entry points");
+    m.def("paged_batch", &paged_batch, "a step's batch layout");
+    m.def("paged_append", &paged_append, "new rows into the pages");
+    m.def("paged_gather", &paged_gather, "rows of the pages");
+    m.def("paged_attention", &paged_attention, "attention over the pages");
 }

@@ -10,6 +10,7 @@
 #include "hyq_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -1345,6 +1346,18 @@ int check_attention(const hyq_paged_params* p) {
     return HYQ_OK;
 }
 
+// More than 64 KiB of LDS for a kernel, once per device (`done`: a bit for each)
+int raise_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = uint64_t{1} << (dev & 63);
+    if (e == hipSuccess && (done.load(std::memory_order_acquire) & bit)) return HYQ_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e != hipSuccess) return fail(HYQ_EDEVICE, std::string("paged attention: LDS limit: ") + hipGetErrorString(e));
+    done.fetch_or(bit, std::memory_order_release);
+    return HYQ_OK;
+}
+
 template <int D, bool F16>
 int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, hipStream_t st) {
     // (the join launch also clears the rows behind the last request: once)
@@ -1359,9 +1372,8 @@ int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, 
         a.plan = wide;
         a.part = reinterpret_cast<float*>(ws + s.wide.off_part);
         a.ml = reinterpret_cast<float*>(ws + s.wide.off_ml);
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_chunk_kernel<D, F16>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(ChunkLds<D>)));
-        if (e != hipSuccess) return fail(HYQ_EDEVICE, std::string("hyq_paged_attention: ") + hipGetErrorString(e));
+        static std::atomic<uint64_t> raised{0};
+        if (int rc = raise_lds(reinterpret_cast<const void*>(paged_chunk_kernel<D, F16>), sizeof(ChunkLds<D>), raised)) return rc;
         paged_chunk_kernel<D, F16><<<dim3(static_cast<unsigned>(s.wide.items * a.heads)), dim3(64 * CHUNK_WAVES), sizeof(ChunkLds<D>), st>>>(a);
         paged_join_kernel<Wide, D, F16><<<dim3(static_cast<unsigned>(s.wide.joins), a.heads, CHUNK / 32), dim3(JOIN_T), 0, st>>>(a);
     }
@@ -1392,8 +1404,9 @@ extern "C" int hyq_paged_batch(const int32_t* context_lens, const int32_t* new_l
                 num_requests, max_pages, num_free, log2i(page_size), num_tokens};
     const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(512, 1 + (static_cast<int64_t>(num_tokens) - 1) / BATCH_TOKENS));
     const size_t lds = 2 * (static_cast<size_t>(num_requests) + 1) * sizeof(int32_t);
+    static std::atomic<uint64_t> raised{0};
     if (lds > 64 * 1024 - 64)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_batch_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        if (int rc = raise_lds(reinterpret_cast<const void*>(paged_batch_kernel), 2 * (MAX_REQUESTS + 1) * sizeof(int32_t), raised)) return rc;
     paged_batch_kernel<<<dim3(blocks), dim3(BT), lds, static_cast<hipStream_t>(stream)>>>(a);
     return check_launch("hyq_paged_batch");
 }

@@ -309,11 +309,15 @@ def _load_fast_ext():
             # built against another torch: the Python paths take every call
             _FX = False
             return False
-        P = _lib.DecodeParams
+        P, G = _lib.DecodeParams, _lib.PagedParams
         # (a build of earlier sources has no signatures())
-        if getattr(m, "signatures", lambda: 0)() == 2 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset):
-            m.set_entry(*(ctypes.cast(f, ctypes.c_void_p).value
-                          for f in (_lib.lib().hyq_decode_hybrid, _lib.lib().hyq_append_rows)))
+        if (getattr(m, "signatures", lambda: 0)() == 3 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset)
+                and m.paged_layout() == (ctypes.sizeof(G), G.num_pages.offset, G.zero_tail.offset)):
+            L = _lib.lib()
+            at = lambda *fs: (ctypes.cast(f, ctypes.c_void_p).value for f in fs)  # noqa: E731
+            m.set_entry(*at(L.hyq_decode_hybrid, L.hyq_append_rows))
+            m.set_paged(*at(L.hyq_paged_batch, L.hyq_paged_append, L.hyq_paged_gather, L.hyq_paged_attention_workspace_size,
+                            L.hyq_paged_attention))
             mod = m
     _FX = mod
     return mod

@@ -34,6 +34,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _lib
+from . import decode_d_stage as dd
 from .decode_d_stage import _HALF, _require_gpu, _stream
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -46,6 +47,17 @@ class PagedBatch(NamedTuple):
     slots: torch.Tensor           # int64 [num_tokens], -1 past the last new token
     positions: torch.Tensor       # int64 [num_tokens], likewise
     pages_used: torch.Tensor      # int32 [1], pages the step needs
+
+
+def _fast(t: torch.Tensor):
+    """(the C++ form of the calls, t's stream), or (None, 0).  It makes the
+    checks below natively and declines whatever fails one (status -1, or the
+    library's own status): that call comes back to the Python form, which
+    copies what the kernels cannot read, or raises."""
+    fx = dd._FX if dd._FX is not None else dd._load_fast_ext()
+    if fx and isinstance(t, torch.Tensor) and t.is_cuda:
+        return fx, _stream(t.device)
+    return None, 0
 
 
 def _ints(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: torch.device) -> None:
@@ -79,6 +91,14 @@ def paged_batch(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table:
     sum; the slots and positions behind that sum are -1.  Where free_pages or
     max_pages do not suffice, the missing entries and their tokens' slots are
     -1 (pages_used tells what was needed)."""
+    fx, stream = _fast(context_lens)
+    if fx:
+        try:
+            st, *b = fx.paged_batch(context_lens, new_lens, block_table, free_pages, page_size, num_tokens, stream)
+            if st == 0:
+                return PagedBatch(*b)
+        except TypeError:                  # an argument of another type: named below
+            pass
     _require_gpu(context_lens, "context_lens")
     dev = context_lens.device
     _ints(context_lens, "context_lens", torch.int32, 1, dev)
@@ -144,6 +164,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages:
     slots (int64 [T]): bit for bit quantize_per_token's codes and scales.  A
     slot outside the pool writes nothing; the slots of one call have to be
     distinct."""
+    fx, stream = _fast(k)
+    if fx:
+        try:
+            if fx.paged_append(k, v, slots, k_pages, v_pages, k_scale, v_scale, stream) == 0:
+                return
+        except TypeError:
+            pass
     _require_gpu(k, "k")
     N, H, P, D = _check_pool(k_pages, v_pages, k_scale, v_scale, k.device)
     if k.dtype not in _HALF or v.dtype != k.dtype:
@@ -167,6 +194,14 @@ def paged_gather(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                  v_scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The K and V rows [T, H, D] of slots (int64 [T]) as bf16 or fp16: code *
     scale rounded once; zeros for slots outside the pool."""
+    fx, stream = _fast(slots)
+    if fx and dtype in _HALF:
+        try:
+            st, k, v = fx.paged_gather(slots, k_pages, v_pages, k_scale, v_scale, dtype == torch.float16, stream)
+            if st == 0:
+                return k, v
+        except TypeError:
+            pass
     _require_gpu(slots, "slots")
     _ints(slots, "slots", torch.int64, 1, slots.device)
     N, H, P, D = _check_pool(k_pages, v_pages, k_scale, v_scale, slots.device)
@@ -199,6 +234,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     log-sum-exp of the scaled scores, fp32 [T, H_Q].  A row that sees no key is
     zero (lse -inf), as are the rows behind the last request of a padded batch
     (those of an `out` that is handed in are left as they are)."""
+    fx, stream = _fast(q)
+    if fx and out is None:
+        try:
+            st, o, lse = fx.paged_attention(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens,
+                                            sm_scale, window, return_lse, stream)
+            if st == 0:
+                return (o, lse) if return_lse else o
+        except TypeError:
+            pass
     _require_gpu(q, "q")
     dev = q.device
     N, H, P, D = _check_pool(k_pages, v_pages, k_scale, v_scale, dev)
