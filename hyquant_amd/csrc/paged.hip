@@ -590,6 +590,12 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int q0, int rr, int
     if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr int NT = 2;                    // cache policy bit: non-temporal (codes are read once)
+__device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+
 template <int D>
 struct Raw {
     uint32_t k[2][D / 32];               // tile t: row c's channels (D/4) kb .. of token 16t + 4(c & 3) + (c >> 2)
@@ -600,7 +606,7 @@ struct Raw {
 };
 
 template <int D, bool F16>
-__global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
     constexpr int TILE = Narrow::TILE, GROUP = Narrow::GROUP;
     constexpr int NB = D / 16;           // PV products per group
     constexpr int KW = D / 32;           // QK products (and K dwords) per tile
@@ -614,18 +620,77 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
     const int c = lane & 15, kb = lane >> 4;
     const int nrows = min(TILE, it.qlen * a.G - it.row0);
 
-    // ---- queries: B operands, row c's channels (D/4) kb + 8m + [0,4,1,5,2,6,3,7] ----
+    // ---- the first loads: queries, page ids, then the first groups' rows ----
+    // (a decode step's tile is its one token's G rows: no division by G)
+    const bool one = it.qlen == 1;
     const int row = it.row0 + min(c, nrows - 1);
-    const int tok = row / a.G, hq = row - tok * a.G;
+    const int tok = one ? 0 : row / a.G, hq = row - tok * a.G;
     const uint16_t* qp = a.q + (static_cast<int64_t>(it.q0) + tok) * a.q_t + (static_cast<int64_t>(head) * a.G + hq) * a.q_h + (D / 4) * kb;
-    float amax = 0.f;
+    const int32_t* trow = a.table + it.req * a.bt_stride;
+    const int steps = (max(it.key1 - it.key0, 0) + GROUP - 1) / GROUP;
+    const int mine = steps > w && a.num_pages > 0 ? (steps - w + WAVES - 1) / WAVES : 0;   // this wavefront's groups w, w + 4, ...
+    // page ids of this wavefront's next 32 groups, tile t of group i in lane 2i + t
+    auto ids_at = [&](int i0) -> int {
+        const int t = it.key0 + GROUP * (w + WAVES * (i0 + (lane >> 1))) + 16 * (lane & 1);
+        return trow[min(t, it.key1 - 1) >> a.page_log2];
+    };
+    int ids = 0, ids_next = 0;
+    if (mine > 0) ids = ids_at(0);
+    if (mine > 32) ids_next = ids_at(32);
     u32x4 qr[KW];
 #pragma unroll
-    for (int m = 0; m < KW; ++m) {
-        qr[m] = *reinterpret_cast<const u32x4*>(qp + 8 * m);
+    for (int m = 0; m < KW; ++m) qr[m] = *reinterpret_cast<const u32x4*>(qp + 8 * m);
+
+    const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
+    const int page_mask = (1 << a.page_log2) - 1;
+    const uint32_t klane = (4 * (c & 3) + (c >> 2)) * ROWB + (ROWB / 4) * kb;
+    const uint32_t vlane = kb * ROWB + (D == 128 ? 4 * c : 4 * (c & 7));
+    const uint32_t slane = (4 * (c & 3) + kb) * 2;
+    // Every load goes through a buffer descriptor over its 16-token tile, of
+    // range 0 past this wavefront's groups or where the page is not in the
+    // pool: such loads give zeros and touch no memory, so the ring's loads are
+    // unconditional and their wait counts exact.
+    auto load = [&](Raw<D>& r, int i) {
+        if (i > 0 && (i & 31) == 0) {
+            ids = ids_next;
+            ids_next = mine > i + 32 ? ids_at(i + 32) : 0;
+        }
+        r.first = it.key0 + GROUP * (w + WAVES * i);
+        r.ok = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + t);
+            const bool ok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages);
+            const bool in = ok && i < mine;
+            r.ok |= ok ? 1 << t : 0;
+            const int64_t pg = ok ? id : 0;
+            const int t0 = (min(r.first + 16 * t, it.key1 - 1) & page_mask) & ~15;
+            const int64_t co = pg * a.ps_page + hk + t0 * ROWB, so = pg * a.ss_page + hs + t0;
+            const Rsrc rk = make_rsrc(a.kp + co, in ? 16 * ROWB : 0), rv = make_rsrc(a.vp + co, in ? 16 * ROWB : 0);
+            const Rsrc rks = make_rsrc(a.ks + so, in ? 32 : 0), rvs = make_rsrc(a.vs + so, in ? 32 : 0);
+            if constexpr (D == 128) {
+                const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, klane, 0, NT));
+                r.k[t][0] = x[0]; r.k[t][1] = x[1]; r.k[t][2] = x[2]; r.k[t][3] = x[3];
+            } else {
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, klane, 0, NT));
+                r.k[t][0] = x[0]; r.k[t][1] = x[1];
+            }
+            r.sk[t] = __builtin_amdgcn_raw_buffer_load_b16(rks, slane, 0, 0);
+            r.sv[t] = __builtin_amdgcn_raw_buffer_load_b16(rvs, slane, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.v[4 * t + e] = __builtin_amdgcn_raw_buffer_load_b32(rv, vlane + 4 * e * ROWB, 0, NT);
+        }
+    };
+    Raw<D> ring[3];
+    load(ring[0], 0);
+    load(ring[1], 1);
+
+    // ---- queries: B operands, row c's channels (D/4) kb + 8m + [0,4,1,5,2,6,3,7] ----
+    float amax = 0.f;
+#pragma unroll
+    for (int m = 0; m < KW; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(half_at<F16>(qr[m][i], 0)), fabsf(half_at<F16>(qr[m][i], 1))));
-    }
     amax = col_max(amax);
     if (!(amax < INFINITY)) amax = 0.f;
     amax = max16_dpp(amax);
@@ -651,8 +716,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
     // this lane's row sees the keys [lo, hi]
     const int pos = it.len - it.qlen + tok;
     const int lo = first_key(pos, a.window), hi = pos;
-    const int tok1 = (it.row0 + nrows - 1) / a.G;
-    const int all_hi = it.len - it.qlen + it.row0 / a.G;                    // every row sees keys up to here
+    const int tok0 = one ? 0 : it.row0 / a.G, tok1 = one ? 0 : (it.row0 + nrows - 1) / a.G;
+    const int all_hi = it.len - it.qlen + tok0;                             // every row sees keys up to here
     const int all_lo = first_key(it.len - it.qlen + tok1, a.window);        // and from here
 
     float m_run = M_INIT, l_run = 0.f;
@@ -660,49 +725,6 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
-    const int page_mask = (1 << a.page_log2) - 1;
-    const int32_t* trow = a.table + it.req * a.bt_stride;
-    const int steps = (max(it.key1 - it.key0, 0) + GROUP - 1) / GROUP;
-    const int mine = steps > w && a.num_pages > 0 ? (steps - w + WAVES - 1) / WAVES : 0;       // this wavefront's groups w, w + 4, ...
-    const uint32_t klane = (4 * (c & 3) + (c >> 2)) * ROWB + (ROWB / 4) * kb;
-    const uint32_t vlane = kb * ROWB + (D == 128 ? 4 * c : 4 * (c & 7));
-    const uint32_t slane = (4 * (c & 3) + kb) * 2;
-
-    // page ids of this wavefront's next 32 groups, tile t of group i in lane 2i + t
-    auto ids_at = [&](int i0) -> int {
-        const int t = it.key0 + GROUP * (w + WAVES * (i0 + (lane >> 1))) + 16 * (lane & 1);
-        return trow[min(t, it.key1 - 1) >> a.page_log2];
-    };
-    int ids = mine > 0 ? ids_at(0) : 0;
-    auto load = [&](Raw<D>& r, int i) {
-        r.first = it.key0 + GROUP * (w + WAVES * i);
-        r.ok = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int id = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + t);
-            const bool ok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages);
-            r.ok |= ok ? 1 << t : 0;
-            const int64_t pg = ok ? id : 0;
-            const int t0 = (min(r.first + 16 * t, it.key1 - 1) & page_mask) & ~15;
-            const int8_t* kb_ = a.kp + pg * a.ps_page + hk + t0 * ROWB;
-            const int8_t* vb_ = a.vp + pg * a.ps_page + hk + t0 * ROWB;
-            if constexpr (D == 128) {
-                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb_ + klane));
-                r.k[t][0] = x[0]; r.k[t][1] = x[1]; r.k[t][2] = x[2]; r.k[t][3] = x[3];
-            } else {
-                const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kb_ + klane));
-                r.k[t][0] = x[0]; r.k[t][1] = x[1];
-            }
-            const char* ksb = reinterpret_cast<const char*>(a.ks + pg * a.ss_page + hs + t0);
-            const char* vsb = reinterpret_cast<const char*>(a.vs + pg * a.ss_page + hs + t0);
-            r.sk[t] = *reinterpret_cast<const uint16_t*>(ksb + slane);
-            r.sv[t] = *reinterpret_cast<const uint16_t*>(vsb + slane);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                r.v[4 * t + e] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb_ + vlane + 4 * e * ROWB));
-        }
-    };
     auto compute = [&](const Raw<D>& r) {
         float s[8];
         const float sk[2] = {f16_bits_to_f32(static_cast<uint16_t>(r.sk[0])) * qk, f16_bits_to_f32(static_cast<uint16_t>(r.sk[1])) * qk};
@@ -801,11 +823,13 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(AttnArgs a) {
         ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), pop, ones, 0, 0, 0);
         if constexpr (F16) ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), plo, ones, 0, 0, 0);
     };
-    Raw<D> r;
-    for (int i = 0; i < mine; ++i) {
-        if (i > 0 && (i & 31) == 0) ids = ids_at(i);
-        load(r, i);
-        compute(r);
+    for (int i = 0; i < mine; i += 3) {
+        load(ring[2], i + 2);
+        compute(ring[0]);
+        load(ring[0], i + 3);
+        if (i + 1 < mine) compute(ring[1]);
+        load(ring[1], i + 4);
+        if (i + 2 < mine) compute(ring[2]);
     }
 
     // ---- the four wavefronts' results, joined through LDS ----
