@@ -284,13 +284,17 @@ struct Narrow {
     static constexpr int TILE = 16, GROUP = 32;   // query rows per tile, keys per step
     static constexpr int MIN_UNITS = 8;  // steps per piece, at least (two per wavefront)
     static constexpr int SLOTS = 1024;   // pieces wanted over all KV heads
-    static constexpr int ENOUGH = 1 << 30;        // tiles over all KV heads that are not cut any more
+    static constexpr float LONGEST = 0.f;         // (see units_per_piece)
+    static constexpr int JOIN_T = 1024, JOIN_ROWS = 16;   // threads and rows of a join's workgroup
 };
 struct Wide {
     static constexpr int TILE = CHUNK, GROUP = 64;
     static constexpr int MIN_UNITS = 4;
-    static constexpr int SLOTS = 512;
-    static constexpr int ENOUGH = 224;
+    // one workgroup a CU, a quarter of them for the pieces that rounding up adds:
+    // a second round costs more than longer pieces
+    static constexpr int SLOTS = 192;
+    static constexpr float LONGEST = 1.15f;
+    static constexpr int JOIN_T = 256, JOIN_ROWS = 8;
 };
 
 struct Item {
@@ -310,7 +314,6 @@ struct PlanArgs {
     const int32_t* lens;
     const int32_t* cu;
     int32_t R, T, G, window, capacity;   // capacity: keys that a block table row can name
-    int32_t enough;                      // tiles of one KV head that are not cut any more
     int32_t target;                      // pieces per KV head wanted
     int32_t max_items, max_parts, max_joins;
     Counts* counts;
@@ -344,12 +347,14 @@ __device__ __forceinline__ Req request(const PlanArgs& a, int r) {
     return q;
 }
 
-// GROUP steps per piece so that the pieces of all tiles are at most target +
-// tiles: at least work / target (the float sum's rounding is far below 2^-14)
+// GROUP steps per piece: the work of a slot, so that the pieces of all tiles are
+// at most target + tiles (the float sum's rounding is far below 2^-14).  Where
+// no tile is much longer than that, as in a prompt of many tiles, cutting gains
+// nothing and costs the partial results.
 template <typename K>
-__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work, float tiles) {
-    if (tiles >= static_cast<float>(a.enough)) return 1 << 30;
+__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work, float longest) {
     const float per = ceilf(work * (1.0f + 0x1p-14f) / static_cast<float>(a.target));
+    if (longest <= per * K::LONGEST) return 1 << 30;
     return static_cast<int>(fminf(fmaxf(per, static_cast<float>(K::MIN_UNITS)), 0x1p30f));
 }
 __device__ __forceinline__ int pieces_of(const Req& x, int per) {
@@ -384,6 +389,10 @@ __device__ __forceinline__ int scan_dpp(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);    // row_bcast:31 into rows 2 and 3
     return v;
 }
+__device__ __forceinline__ float wave_top(float v) {
+    v = col_max(max16_dpp(v));
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
 __device__ __forceinline__ float wave_sum(float v) {
     v = col_sum(sum16_dpp(v));
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
@@ -401,8 +410,8 @@ template <typename K>
 __device__ __forceinline__ Plan64 plan64(const PlanArgs& a, int lane) {
     Plan64 p;
     p.x = request<K>(a, lane);
-    const float tiles = static_cast<float>(p.x.tiles);
-    const int per = units_per_piece<K>(a, wave_sum(tiles * static_cast<float>(p.x.units)), wave_sum(tiles));
+    const float units = p.x.tiles ? static_cast<float>(p.x.units) : 0.f;
+    const int per = units_per_piece<K>(a, wave_sum(static_cast<float>(p.x.tiles) * units), wave_top(units));
     p.pc = pieces_of(p.x, per);
     const int n = p.x.tiles * p.pc, split = p.pc > 1 ? 1 : 0;
     p.items = scan_dpp(n) - n;
@@ -439,22 +448,22 @@ __device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int lane, It
     it = make_item<K>(a, x, k, x.tiles - 1 - local / pc, local % pc, pc, pc > 1 && part < a.max_parts ? part : -1);
     return true;
 }
+// the joins of a schedule, and join j of them (p: where requests are up to 64)
 template <typename K>
-__device__ __forceinline__ bool find_join(const PlanArgs& a, int j, int lane, Join& jn) {
-    if (a.R > INLINE_R) {
-        if (j >= a.counts->joins) return false;
-        jn = a.joins[j];
-        return true;
-    }
-    const Plan64 p = plan64<K>(a, lane);
+__device__ __forceinline__ int count_joins(const PlanArgs& a, const Plan64& p) {
+    if (a.R > INLINE_R) return a.counts->joins;
+    return min(__builtin_amdgcn_readlane(p.joins + (p.pc > 1 ? p.x.tiles : 0), 63), a.max_joins);
+}
+template <typename K>
+__device__ __forceinline__ Join find_join(const PlanArgs& a, const Plan64& p, int j) {
+    if (a.R > INLINE_R) return a.joins[j];
     const int k = lane_of(p.joins, p.pc > 1 ? p.x.tiles : 0, j);
-    if (k < 0) return false;
     const int pc = __builtin_amdgcn_readlane(p.pc, k), nth = j - __builtin_amdgcn_readlane(p.joins, k);
     const int part = __builtin_amdgcn_readlane(p.parts, k) + nth * pc;
     const Req x = lane_req(p.x, k);
-    if (part + pc > a.max_parts) return false;
-    jn = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
-    return true;
+    Join jn = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
+    if (part + pc > a.max_parts) jn.rows = 0;
+    return jn;
 }
 
 template <typename K>
@@ -465,20 +474,20 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
     __shared__ int64_t wsum[3][PLAN_T / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     __shared__ float fsum[2][PLAN_T / 64];
-    float work = 0.f, tiles = 0.f;
+    float work = 0.f, longest = 0.f;
     for (int r = tid; r < a.R; r += PLAN_T) {
         const Req q = request<K>(a, r);
         work += static_cast<float>(q.tiles) * static_cast<float>(q.units);
-        tiles += static_cast<float>(q.tiles);
+        if (q.tiles) longest = fmaxf(longest, static_cast<float>(q.units));
     }
     work = wave_sum(work);
-    tiles = wave_sum(tiles);
-    if (lane == 0) { fsum[0][w] = work; fsum[1][w] = tiles; }
+    longest = wave_top(longest);
+    if (lane == 0) { fsum[0][w] = work; fsum[1][w] = longest; }
     __syncthreads();
-    work = tiles = 0.f;
-    for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; tiles += fsum[1][i]; }
+    work = longest = 0.f;
+    for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; longest = fmaxf(longest, fsum[1][i]); }
     __syncthreads();
-    const int per = units_per_piece<K>(a, work, tiles);
+    const int per = units_per_piece<K>(a, work, longest);
     int64_t base[3] = {0, 0, 0};
     for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
         const Req q = request<K>(a, r0 + tid);
@@ -871,25 +880,26 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
 // attention: CHUNK query rows per workgroup
 // ---------------------------------------------------------------------------
 // A wavefront owns 32 rows.  The codes of 64 keys at a time are turned into
-// fp16 operands once for all rows of the workgroup and laid in LDS (K as
-// [key][channel], V transposed as [channel][key]), double-buffered: while one
-// block is multiplied, the next one's codes are already in registers.
+// fp16 operands once for all rows of the workgroup and laid in LDS, two blocks
+// ahead of the products.
 //   QK  S^T[key][row] = K . Q^T  with v_mfma_f32_32x32x16_f16; codes and (scaled
 //       by a power of two) queries are exact, the K scale multiplies the fp32
 //       score in the fma that subtracts the reference: t = S k_scale - M.
 //   PV  O^T[channel][row] = V^T . P'^T, P' = fp16(2^t v_scale) against the exact
-//       codes.  The reference M of a row follows max(score + log2 of the
-//       block's largest V scale), so that P' keeps to [0, 2^13] whatever the
-//       scales are; rounding P' to 11 bits once is the only rounding between
-//       the scores and the output.
-// Output register i of a lane (row l & 31, half h = l >> 5) of a 32-key tile is
-// key 8 (i >> 2) + 4 h + (i & 3); V's keys lie in LDS in the order that makes
-// registers 8s .. 8s + 7 the B operand of step s, so P never leaves its lane.
+//       codes, V^T by transposing LDS reads.  The reference M of a row follows
+//       max(score + log2 of the block's largest V scale), so that P' keeps to
+//       [0, 2^13] whatever the scales are; rounding P' to 11 bits once is the
+//       only rounding between the scores and the output.
+// Output register i of a lane (row l & 31, half h = l >> 5) of a 32-key product
+// is key 8 (i >> 2) + 4 h + (i & 3); registers 8s .. 8s + 7 are the B operand of
+// step s of P.V, without a shuffle.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr float P_SHIFT = 6.0f;          // P' is at most 2^(P_SHIFT + SLACK_W + 1)
 constexpr float SLACK_W = 6.0f;
-constexpr int BLK = 64;                  // keys per step
+constexpr int BLK = 64;                  // keys per block
+constexpr int BUFS = 3;                  // blocks in LDS
+constexpr float BAD = 4096.0f;
 
 __device__ __forceinline__ uint32_t pk_sub1032(uint32_t x) {
     const f16x2 b = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
@@ -902,28 +912,23 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// Bytes from a key's row of D fp16 channels to the next's.  16 lanes of a K
+// operand read (neighbouring rows, one 16-byte chunk) and 32 of a transposing V
+// read (4 rows, 64 bytes) fall on all 64 banks once by the padding, so a lane's
+// operands are one address and constants.
+template <int D> constexpr int KROW = 2 * D + 16;
+template <int D> constexpr int VROW = 2 * D + 64;
+
 template <int D>
 struct ChunkLds {
-    uint8_t k[2][BLK * D * 2];           // [key][D / 8 chunks of 16 bytes], swizzled
-    uint8_t v[2][D * BLK * 2];           // [channel][8 chunks of 8 keys], swizzled
-    float ks[2][BLK];                    // K scale * qk
-    float vs[2][BLK];
-    float ve[2];                         // log2 bound of the block's V scales
-    int ok[2];                           // bit t: 16-key tile t's page is inside the pool
+    uint8_t k[BUFS][BLK * KROW<D>];
+    uint8_t v[BUFS][BLK * VROW<D>];
+    float ks[BUFS][BLK];                 // K scale * qk
+    float vs[BUFS][BLK];                 // V scale, 0 where it is not finite or not to be looked at
+    float ve[BUFS][4];                   // per 16-key tile: log2 bound of vs, BAD more if a key needs care
+    uint32_t care[BUFS][4];              // bits 0..15: keys whose V scale is not finite; bit 16: the page is in the pool
     float red[CHUNK_WAVES];
 };
-
-// byte offsets of a 16-byte chunk: neighbouring keys' (channels') equal chunks
-// and one key's chunks fall on different banks, for the stores and the loads
-template <int D>
-__device__ __forceinline__ uint32_t k_at(int key, int x) {
-    if constexpr (D == 128) return key * 256 + ((x ^ (key & 15)) << 4);
-    else return key * 128 + ((x ^ ((key >> 1) & 7)) << 4);
-}
-__device__ __forceinline__ uint32_t v_at(int ch, int x) {
-    const int f = ((ch >> 2) & 7) ^ ((ch << 1) & 4);
-    return ch * 128 + ((x ^ f) << 4);
-}
 
 // e with x < 2^e, x >= 0 finite
 __device__ __forceinline__ float scale_bound(float x) {
@@ -935,11 +940,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     constexpr int KM = D / 16;           // QK products per 32 keys
     constexpr int DT = D / 32;           // 32-channel tiles of V
     constexpr int ROWB = D / 2;
-    constexpr int NT = 64 * CHUNK_WAVES;
-    constexpr int NV = 8 * (D / 4);      // V tasks: 8 keys x 4 channels
-    constexpr int NK = BLK * (D / 32);   // K tasks: 1 key x 32 channels
-    static_assert(NV + NK <= NT, "a thread has one task");
-    extern __shared__ uint8_t lds_raw[];
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     ChunkLds<D>& L = *reinterpret_cast<ChunkLds<D>*>(lds_raw);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = blockIdx.x % a.heads;
@@ -949,7 +950,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     const int nrows = min(CHUNK, it.qlen * a.G - it.row0);
 
     // ---- queries ----
-    const int rt = 32 * w + r32;                          // row within the tile
+    const int rt = 32 * w + r32;                          // row within the tile (behind its last: that one again)
     const int row = it.row0 + min(rt, nrows - 1);
     const int tok = row / a.G, hq = row - tok * a.G;
     const uint16_t* qp = a.q + (static_cast<int64_t>(it.q0) + tok) * a.q_t + (static_cast<int64_t>(head) * a.G + hq) * a.q_h + 8 * h;
@@ -981,145 +982,158 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     }
     const int pos = it.len - it.qlen + tok;
     const int lo = first_key(pos, a.window), top = min(pos, it.key1 - 1);
-    // this wavefront's rows (none: it only converts): every one sees [all_lo, all_hi], none past any_hi
-    const bool active = 32 * w < nrows;
+    // every row of this wavefront sees [all_lo, all_hi]
     const int t0 = (it.row0 + min(32 * w, nrows - 1)) / a.G, t1 = (it.row0 + min(32 * w + 31, nrows - 1)) / a.G;
     const int all_hi = min(it.len - it.qlen + t0, it.key1 - 1), all_lo = first_key(it.len - it.qlen + t1, a.window);
-    const int any_hi = it.len - it.qlen + t1, any_lo = first_key(it.len - it.qlen + t0, a.window);
 
-    // ---- conversion tasks ----
+    // ---- conversion ----
+    // Wavefronts 0..3 have the V codes and scales of the 16-key tiles 0..3 of a
+    // block, wavefronts 4..7 the K codes and scales: one page id and one
+    // descriptor each, of range 0 (zeros, no access) where the page is not in
+    // the pool.
+    const bool is_v = w < 4;
+    const int tile = w & 3;
     const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
     const int page_mask = (1 << a.page_log2) - 1;
     const int32_t* trow = a.table + it.req * a.bt_stride;
     const int nblk = a.num_pages > 0 ? (max(it.key1 - it.key0, 0) + BLK - 1) / BLK : 0;
-    const bool is_v = tid < NV, is_k = tid >= NV && tid < NV + NK;
-    // V: chunk c8 holds the keys 16 (c8 >> 1) + 4 (c8 & 1) + {0..3, 8..11}, channels 4 dq ..
-    const int c8 = tid / (D / 4), dq = tid - c8 * (D / 4);
-    const int kt = tid - NV, kkey = kt / (D / 32), kq = kt - kkey * (D / 32);
-    // scales: wavefront 0's lane j is key j for V, wavefront 1's for K
-    const int my16 = is_v ? c8 >> 1 : is_k ? kkey >> 4 : 0;       // the task's 16-key tile
-    auto page_id = [&](int blk, int t16) -> int {
-        const int t = min(it.key0 + BLK * blk + 16 * t16, it.key1 - 1);
-        return trow[t >> a.page_log2];
+    // lane = key of the tile * KL + 32-channel part kq (D = 64: the upper 32
+    // lanes store what the lower ones store)
+    constexpr int KL = D / 32;
+    const int cl = D == 128 ? lane : lane & 31;
+    const int kkey = cl / KL, kq = cl % KL;
+    const int8_t* const codes = is_v ? a.vp : a.kp;
+    const uint16_t* const scales = is_v ? a.vs : a.ks;
+    uint8_t* const mine = (is_v ? L.v[0] + (16 * tile + kkey) * VROW<D> : L.k[0] + (16 * tile + kkey) * KROW<D>) + 64 * kq;
+    auto tile_key = [&](int blk) { return it.key0 + BLK * blk + 16 * tile; };
+    auto page_id = [&](int blk) -> int { return trow[min(tile_key(blk), it.key1 - 1) >> a.page_log2]; };
+    u32x4 raw = {};                      // 32 codes
+    uint32_t sraw = 0;                   // scale bits (lanes 0..15)
+    bool sok = false;                    // the page is in the pool
+    auto fetch = [&](int blk, int id) __attribute__((always_inline)) {
+        id = __builtin_amdgcn_readfirstlane(id);
+        sok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages);
+        const int64_t pg = sok ? id : 0;
+        const int o = (min(tile_key(blk), it.key1 - 1) & page_mask) & ~15;
+        const Rsrc rc = make_rsrc(codes + pg * a.ps_page + hk + o * ROWB, sok ? 16 * ROWB : 0);
+        const Rsrc rs = make_rsrc(scales + pg * a.ss_page + hs + o, sok ? 32 : 0);
+        raw = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, 16 * cl, 0, 0));
+        sraw = __builtin_amdgcn_raw_buffer_load_b16(rs, 2 * lane, 0, 0);
     };
-    auto tile_off = [&](int blk, int t16) -> int { return (min(it.key0 + BLK * blk + 16 * t16, it.key1 - 1) & page_mask) & ~15; };
-    struct Raw64 {
-        uint32_t d[8];
-        uint32_t s;                      // scale bits (wavefronts 0 and 1)
-        int sid;                         // and their page
-    };
-    Raw64 raw{};
-    auto fetch = [&](int blk, int id, int sid) {
-        const int64_t pg = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages) ? id : 0;
-        const int off = tile_off(blk, my16);
+    // block blk into buffer b
+    auto store = [&](int blk, int b) __attribute__((always_inline)) {
+        uint8_t* const dst = mine + b * (is_v ? sizeof(L.v[0]) : sizeof(L.k[0]));
+        // a word's channels in the order 0, 4, 1, 5, 2, 6, 3, 7: the queries'
+        // and, for V, that of the output's rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x4*>(dst + 16 * i) = u32x4{codes2(raw[i], 0), codes2(raw[i], 4), codes2(raw[i], 8), codes2(raw[i], 12)};
+        const float f = f16_bits_to_f32(static_cast<uint16_t>(sraw));
         if (is_v) {
-            const int8_t* b = a.vp + pg * a.ps_page + hk + (off + 4 * (c8 & 1)) * ROWB + 2 * dq;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) raw.d[e] = *reinterpret_cast<const uint16_t*>(b + ((e & 3) + 8 * (e >> 2)) * ROWB);
-        } else if (is_k) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(a.kp + pg * a.ps_page + hk + (off + (kkey & 15)) * ROWB + 16 * kq);
-            raw.d[0] = x[0]; raw.d[1] = x[1]; raw.d[2] = x[2]; raw.d[3] = x[3];
-        }
-        if (w < 2) {
-            const bool ok = static_cast<uint32_t>(sid) < static_cast<uint32_t>(a.num_pages);
-            const int64_t sp = ok ? sid : 0;
-            const int so = tile_off(blk, lane >> 4) + (lane & 15);
-            raw.s = (w == 0 ? a.vs : a.ks)[sp * a.ss_page + hs + so];
-            raw.sid = ok;
-        }
-    };
-    auto store = [&](int b, int blk) {
-        if (is_v) {
-            uint32_t pr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pr[i] = raw.d[2 * i] | (raw.d[2 * i + 1] << 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u32x4 o = {codes2(pr[0], 4 * i), codes2(pr[1], 4 * i), codes2(pr[2], 4 * i), codes2(pr[3], 4 * i)};
-                *reinterpret_cast<u32x4*>(&L.v[b][v_at(4 * dq + i, c8)]) = o;
+            // keys past the piece or in no page hold anything: they count as 0
+            const bool live = lane < 16 && tile_key(blk) + lane < it.key1 && sok;
+            const bool bad = live && !(fabsf(f) < INFINITY);
+            const float x = live && !bad ? f : 0.f;
+            const uint32_t mask = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(bad));
+            const float most = max16_dpp(fabsf(x));
+            if (lane < 16) L.vs[b][16 * tile + lane] = x;
+            if (lane == 0) {
+                L.ve[b][tile] = scale_bound(most) + (mask || !sok ? BAD : 0.f);
+                L.care[b][tile] = mask | (sok ? 1u << 16 : 0u);
             }
-        } else if (is_k) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u32x4 o = {codes2(raw.d[i], 0), codes2(raw.d[i], 4), codes2(raw.d[i], 8), codes2(raw.d[i], 12)};
-                *reinterpret_cast<u32x4*>(&L.k[b][k_at<D>(kkey, 4 * kq + i)]) = o;
-            }
-        }
-        if (w == 0) {
-            const float f = f16_bits_to_f32(static_cast<uint16_t>(raw.s));
-            float x = fabsf(f);
-            // keys past the piece or in no page hold anything: not in the bound
-            if (!(x < INFINITY) || it.key0 + BLK * blk + lane >= it.key1 || !raw.sid) x = 0.f;
-            x = col_max(max16_dpp(x));
-            L.vs[b][lane] = f;
-            if (lane == 0) L.ve[b] = scale_bound(x);
-        } else if (w == 1) {
-            const uint64_t m = __builtin_amdgcn_ballot_w64(raw.sid != 0);
-            L.ks[b][lane] = f16_bits_to_f32(static_cast<uint16_t>(raw.s)) * qk;
-            if (lane == 0) L.ok[b] = static_cast<int>((m & 1) | ((m >> 15) & 2) | ((m >> 30) & 4) | ((m >> 45) & 8));
+        } else if (lane < 16) {
+            L.ks[b][16 * tile + lane] = f * qk;
         }
     };
 
     float m_run = M_INIT, l_run = 0.f;
-    f32x16 acc[DT];
+    f32x16 acc[DT], sc;
+    float t[16];                         // score - reference of 32 keys, then their weights
+    uint32_t pw[8];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-    auto compute = [&](int b, int blk) {
-        const int j0 = it.key0 + BLK * blk;
-        f32x16 sc[2];
+    // K of half x, step m: key 32 x + (l & 31), channels 16 m + 8 h ..
+    const uint8_t* const kl = L.k[0] + r32 * KROW<D> + 16 * h;
+    // V of half x, step s, tile d: within 16 lanes, lane j of the transposing
+    // read gets element j & 3 of the 8-byte pieces that the lanes 4 e + (j >> 2)
+    // address: piece q = l & 3 of channels 32 d + (l & 16) + 4 q .. of key 32 x +
+    // 16 s + 4 h + e (and 8 keys on), e = (l >> 2) & 3, which gives lane l
+    // channel 32 d + (l & 31) of the keys of its registers 8 s ..
+    const uint8_t* const vl = L.v[0] + (4 * h + ((lane >> 2) & 3)) * VROW<D> + 2 * (lane & 16) + 8 * (lane & 3);
+    auto v_operand = [&](const uint8_t* p) __attribute__((always_inline)) {
+        typedef short i16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) i16x4* LdsV;
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV)(p)));
+        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV)(p + 8 * VROW<D>)));
+        return __builtin_bit_cast(f16x8, u32x4{x[0], x[1], y[0], y[1]});
+    };
+    auto qk_product = [&](int b, int x) __attribute__((always_inline)) {
+        const uint8_t* const p = kl + b * static_cast<int>(sizeof(L.k[0]));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[t][i] = 0.f;
+        for (int m = 0; m < KM; ++m)
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(p + 32 * x * KROW<D> + 32 * m), qop[m], sc, 0, 0, 0);
+    };
+    auto pv_product = [&](int b, int x) __attribute__((always_inline)) {
+        const uint8_t* const p = vl + b * static_cast<int>(sizeof(L.v[0]));
 #pragma unroll
-            for (int m = 0; m < KM; ++m) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(&L.k[b][k_at<D>(32 * t + r32, 2 * m + h)]);
-                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qop[m], sc[t], 0, 0, 0);
-            }
+        for (int s = 0; s < 2; ++s) {
+            const u32x4 pv = {pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_operand(p + (32 * x + 16 * s) * VROW<D> + 64 * d), __builtin_bit_cast(f16x8, pv),
+                                                                acc[d], 0, 0, 0);
         }
-        // t = score - reference (0 while the row has seen no key)
-        const int ok = __builtin_amdgcn_readfirstlane(L.ok[b]);
-        const bool unset = m_run == M_INIT;
-        const float m_use = unset ? 0.f : m_run;
-        float t[32];
+    };
+    // t = scale * S - reference (0 while the row has seen no key); the lane's largest
+    auto scores = [&](int b, int x, float m_use) __attribute__((always_inline)) -> float {
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(&L.ks[b][8 * g + 4 * h]);
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 k4 = *reinterpret_cast<const f32x4*>(&L.ks[b][32 * x + 8 * g + 4 * h]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[4 * g + i] = __builtin_fmaf(sc[g >> 2][4 * (g & 3) + i], x[i], -m_use);
+            for (int i = 0; i < 4; ++i) t[4 * g + i] = __builtin_fmaf(sc[4 * g + i], k4[i], -m_use);
         }
-        float ve = L.ve[b];
-        uint32_t dead = 0;
-        const bool edge = j0 + BLK - 1 > all_hi || j0 < all_lo || ok != 15;
-        if (edge) {
-            // keys that the row does not see; its bound is over the others' V
-            // scales, so that what is hidden from a row does not touch its bits
+        float mx = vmax3(t[0], t[1], t[2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) mx = vmax3(mx, t[i], t[i + 1]);
+        return vmax2(mx, t[15]);
+    };
+    // hides what the rows do not see, and raises their reference where a
+    // score passes it
+    auto settle = [&](int b, int x, int blk, float mx, float m_use, bool unset) __attribute__((always_inline)) {
+        const int j0 = it.key0 + BLK * blk + 32 * x;
+        float ve = fmaxf(L.ve[b][2 * x], L.ve[b][2 * x + 1]);
+        if (j0 + 31 > all_hi || j0 < all_lo || __builtin_amdgcn_readfirstlane(__float_as_int(ve)) >= __float_as_int(BAD / 2)) {
+            // the row's bound is over the V scales that it sees, so that what
+            // is hidden from a row does not touch its bits; a row that sees a
+            // scale that is not finite is NaN
             float vx = 0.f;
+            mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(&L.vs[b][8 * g + 4 * h]);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v4 = *reinterpret_cast<const f32x4*>(&L.vs[b][32 * x + 8 * g + 4 * h]);
+                const uint32_t care = L.care[b][2 * x + (g >> 1)];
+                const uint32_t bad = care >> (8 * (g & 1) + 4 * h);
+                const bool in_pool = care >> 16;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = j0 + 8 * g + 4 * h + i;
-                    if (j > top || j < lo || !((ok >> (g >> 1)) & 1)) {
-                        t[4 * g + i] = -INFINITY;
-                        dead |= 1u << (4 * g + i);
-                    } else if (fabsf(x[i]) < INFINITY) {
-                        vx = fmaxf(vx, fabsf(x[i]));
-                    }
+                    const bool seen = j <= top && j >= lo && in_pool;
+                    t[4 * g + i] = seen ? t[4 * g + i] : -INFINITY;
+                    mx = fmaxf(mx, t[4 * g + i]);
+                    vx = fmaxf(vx, seen ? fabsf(v4[i]) : 0.f);
+                    if (seen && ((bad >> i) & 1)) l_run = __builtin_nanf("");
                 }
             }
             ve = scale_bound(xmax32(vx));
         }
-        float mx = vmax3(t[0], t[1], t[2]);
-#pragma unroll
-        for (int i = 3; i < 31; i += 2) mx = vmax3(mx, t[i], t[i + 1]);
-        mx = vmax2(mx, t[31]) + ve;
+        mx += ve;
         // (a row's own scores alone decide whether its reference moves)
-        if (__builtin_amdgcn_ballot_w64(unset || mx > P_SHIFT + SLACK_W)) {      // rare after the first blocks
+        if (__builtin_amdgcn_ballot_w64(unset || mx > P_SHIFT + SLACK_W)) {      // rare after the first keys
             mx = xmax32(mx);
             const bool move = unset ? mx > -INFINITY : mx > P_SHIFT + SLACK_W;
             const float up = move ? mx - P_SHIFT : 0.f;
@@ -1129,154 +1143,160 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             for (int d = 0; d < DT; ++d) acc[d] *= alpha;
             m_run = move ? m_use + up : m_run;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) t[i] -= up;
+            for (int i = 0; i < 16; ++i) t[i] -= up;
         }
-        float ls = 0.f;
+    };
+    // P' = fp16(2^t * V scale) of half x (every scale in vs is finite: a hidden
+    // key's weight of zero stays zero)
+    auto weights = [&](int b, int x) __attribute__((always_inline)) {
+        float ls[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            t[i] = fast_exp2(t[i]);
-            ls += t[i];
-        }
-        l_run += ls;
-        uint32_t pw[16];
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 v4 = *reinterpret_cast<const f32x4*>(&L.vs[b][32 * x + 8 * g + 4 * h]);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-            // (lane i of a quad reads key 4h + i of the group: quad broadcasts hand out all four)
-            const float v = L.vs[b][8 * g + 4 * h + (lane & 3)];
-            t[4 * g] *= quad_bcast<0>(v);
-            t[4 * g + 1] *= quad_bcast<1>(v);
-            t[4 * g + 2] *= quad_bcast<2>(v);
-            t[4 * g + 3] *= quad_bcast<3>(v);
-        }
-        if (edge) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) t[i] = (dead >> i) & 1 ? 0.f : t[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pw[i] = pack_f16x2(t[2 * i], t[2 * i + 1]);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const u32x4 pv = {pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const f16x8 vf = *reinterpret_cast<const f16x8*>(&L.v[b][v_at(32 * d + r32, 2 * s + h)]);
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, __builtin_bit_cast(f16x8, pv), acc[d], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                t[4 * g + i] = fast_exp2(t[4 * g + i]);
+                ls[i & 1] += t[4 * g + i];
             }
+            pw[2 * g] = pack_f16x2(t[4 * g] * v4[0], t[4 * g + 1] * v4[1]);
+            pw[2 * g + 1] = pack_f16x2(t[4 * g + 2] * v4[2], t[4 * g + 3] * v4[3]);
         }
+        l_run += ls[0] + ls[1];
+    };
+    // One step: the next 32 keys' scores are multiplied while these 32 are
+    // weighted, and formed while these are added up, so that the matrix and the
+    // vector pipe have work at the same time.
+    auto step = [&](int kb, int kx, int kblk, int vb, int vx) __attribute__((always_inline)) {
+        qk_product(kb, kx);
+        weights(vb, vx);
+        const bool unset = m_run == M_INIT;
+        const float m_use = unset ? 0.f : m_run;
+        pv_product(vb, vx);
+        const float mx = scores(kb, kx, m_use);
+        settle(kb, kx, kblk, mx, m_use, unset);
     };
 
     if (nblk > 0) {
-        fetch(0, page_id(0, my16), page_id(0, lane >> 4));
-        int id = page_id(1, my16), sid = page_id(1, lane >> 4);
+        fetch(0, page_id(0));
         store(0, 0);
-        if (nblk > 1) fetch(1, id, sid);
-        id = page_id(2, my16);
-        sid = page_id(2, lane >> 4);
+        fetch(1, page_id(1));
+        store(1, 1);
+        fetch(2, page_id(2));
+        int id = page_id(3);
         __syncthreads();
+        qk_product(0, 0);
+        settle(0, 0, 0, scores(0, 0, 0.f), 0.f, true);
+        // one wavefront of a SIMD goes first where both could issue: they drift
+        // half a step apart
+        if (w < CHUNK_WAVES / 2) __builtin_amdgcn_s_setprio(1);
+        int b0 = 0, b1 = 1, b2 = 2;      // buffers of the blocks n, n + 1, n + 2
         for (int n = 0; n < nblk; ++n) {
-            if (n + 1 < nblk) {
-                store((n + 1) & 1, n + 1);
-                if (n + 2 < nblk) {
-                    fetch(n + 2, id, sid);
-                    id = page_id(n + 3, my16);
-                    sid = page_id(n + 3, lane >> 4);
-                }
-            }
-            const int j0 = it.key0 + BLK * n;
-            if (active && j0 <= any_hi && j0 + BLK > any_lo) compute(n & 1, n);
+            store(n + 2, b2);
+            fetch(n + 3, id);
+            id = page_id(n + 4);
+            step(b0, 1, n, b0, 0);
+            step(b1, 0, n + 1, b0, 1);   // (past the last block: hidden keys)
+            const int o = b0;
+            b0 = b1;
+            b1 = b2;
+            b2 = o;
             __syncthreads();
         }
     }
     if (rt >= nrows) return;
     const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
     l_run = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
-    if (it.part >= 0) {
-        const int64_t at = (static_cast<int64_t>(it.part) * a.heads + head) * CHUNK + rt;
+    // Registers 4 g .. of a tile are the rows 8 g + 4 h ..: channels 0, 4, 1, 5 (h =
+    // 0) or 2, 6, 3, 7 of 8: two values change places between the lane's halves
+    const int64_t at = (static_cast<int64_t>(it.part) * a.heads + head) * CHUNK + rt;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<f32x4*>(a.part + at * D + 32 * d + 8 * g + 4 * h) =
-                    f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
-        if (h == 0) { a.ml[at * 2] = m_run; a.ml[at * 2 + 1] = l_run; }
-    } else {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                store_row<F16>(a, it.q0, row, head, 32 * d + 8 * g + 4 * h, m_run, l_run,
-                               f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]});
-    }
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 o = {acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+            const float x = __shfl_xor(h ? o[0] : o[1], 32, 64), y = __shfl_xor(h ? o[2] : o[3], 32, 64);
+            const f32x4 z = h ? f32x4{x, y, o[1], o[3]} : f32x4{o[0], o[2], x, y};
+            const int ch = 32 * d + 8 * g + 4 * h;
+            if (it.part >= 0) *reinterpret_cast<f32x4*>(a.part + at * D + ch) = z;
+            else store_row<F16>(a, it.q0, row, head, ch, m_run, l_run, z);
+        }
+    if (it.part >= 0 && h == 0) { a.ml[at * 2] = m_run; a.ml[at * 2 + 1] = l_run; }
 }
 
-// Adds up the pieces of the split tiles: one workgroup per 32 rows of a tile
-// (blockIdx.z) and KV head.
-// A row is 4 channels a lane of D/4; while rows are fewer than the lane
-// groups, several groups share a row's pieces and meet in LDS.  Four pieces
-// are in flight per group.  By zero_tail it also clears the rows behind the
-// last request.
-constexpr int JOIN_T = 1024;
+// Adds up the pieces of the split tiles.  A workgroup takes JOIN_ROWS rows of a
+// tile and KV head after the other; a row is 4 channels a lane of D/4, and
+// while rows are fewer than the lane groups, several groups share a row's
+// pieces and meet in LDS.  Four pieces are in flight per group.  By zero_tail
+// it also clears the rows behind the last request.
 template <typename K, int D, bool F16>
-__global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
-    constexpr int LG = JOIN_T / (D / 4);    // lane groups
+__global__ __launch_bounds__(K::JOIN_T) void paged_join_kernel(AttnArgs a) {
+    constexpr int LG = K::JOIN_T / (D / 4);        // lane groups
+    constexpr int PARTS = K::TILE / K::JOIN_ROWS;  // of a tile
     __shared__ float so[LG][D];
     __shared__ float sm[LG], sl[LG];
-    const int tid = threadIdx.x, head = blockIdx.y;
-    if (a.zero_tail && a.plan.cu && blockIdx.z == 0) {
+    const int tid = threadIdx.x;
+    const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
+    if (a.zero_tail && a.plan.cu) {
         const int64_t first = min(max(a.plan.cu[a.plan.R], 0), a.plan.T);
-        const int64_t total = (a.plan.T - first) * a.G * (D / 4);   // of one KV head
-        for (int64_t e = static_cast<int64_t>(blockIdx.x) * JOIN_T + tid; e < total; e += static_cast<int64_t>(gridDim.x) * JOIN_T) {
-            const int64_t row = e / (D / 4), t = row / a.G, h = head * static_cast<int64_t>(a.G) + row - t * a.G;
-            const int ch = 4 * static_cast<int>(e - row * (D / 4));
+        const int64_t rows = (a.plan.T - first) * a.G * a.heads;       // (token, query head)
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * LG + g; r < rows; r += static_cast<int64_t>(gridDim.x) * LG) {
+            const int64_t t = r / (a.G * a.heads), h = r - t * (a.G * a.heads);
             if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (first + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
             if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(first + t) * a.l_t + h] = -INFINITY;
         }
     }
-    Join jn;
-    if (!find_join<K>(a.plan, blockIdx.x, tid & 63, jn)) return;
-    const int first = 32 * blockIdx.z, rows = min(32, jn.rows - first);
-    if (rows <= 0) return;
-    const int share = rows <= LG / 8 ? 8 : rows <= LG / 4 ? 4 : rows <= LG / 2 ? 2 : 1;
-    const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4)), sub = g % share;
-    for (int r0 = 0; r0 < rows; r0 += LG / share) {
-        const int rw = r0 + g / share;
-        float m = M_INIT, l = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        if (rw < rows) {
-            constexpr int DEEP = 4;
-            for (int i0 = sub; i0 < jn.pieces; i0 += DEEP * share) {
-                float mi[DEEP], li[DEEP];
-                f32x4 oi[DEEP];
+    Plan64 p{};
+    if (a.plan.R <= INLINE_R) p = plan64<K>(a.plan, tid & 63);
+    const int64_t total = static_cast<int64_t>(count_joins<K>(a.plan, p)) * a.heads * PARTS;
+    for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+        const uint32_t rest = static_cast<uint32_t>(i) / a.heads;
+        const int head = static_cast<uint32_t>(i) - rest * a.heads;
+        const Join jn = find_join<K>(a.plan, p, rest / PARTS);
+        const int first = rest % PARTS * K::JOIN_ROWS, rows = min(K::JOIN_ROWS, jn.rows - first);
+        const int share = rows <= LG / 8 ? 8 : rows <= LG / 4 ? 4 : rows <= LG / 2 ? 2 : 1;
+        const int sub = g % share;
+        for (int r0 = 0; r0 < rows; r0 += LG / share) {
+            const int rw = r0 + g / share;
+            float m = M_INIT, l = 0.f;
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            if (rw < rows) {
+                constexpr int DEEP = 4;
+                for (int i0 = sub; i0 < jn.pieces; i0 += DEEP * share) {
+                    float mi[DEEP], li[DEEP];
+                    f32x4 oi[DEEP];
 #pragma unroll
-                for (int j = 0; j < DEEP; ++j) {
-                    const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * K::TILE + first + rw;
-                    mi[j] = a.ml[at * 2];
-                    li[j] = a.ml[at * 2 + 1];
-                    oi[j] = *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
-                }
+                    for (int j = 0; j < DEEP; ++j) {
+                        const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * K::TILE + first + rw;
+                        mi[j] = a.ml[at * 2];
+                        li[j] = a.ml[at * 2 + 1];
+                        oi[j] = *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
+                    }
 #pragma unroll
-                for (int j = 0; j < DEEP; ++j) {
-                    if (i0 + j * share >= jn.pieces) break;
-                    const float mn = fmaxf(m, mi[j]), f = fast_exp2(m - mn), fi = fast_exp2(mi[j] - mn);
-                    o = o * f + oi[j] * fi;
-                    l = l * f + li[j] * fi;
-                    m = mn;
+                    for (int j = 0; j < DEEP; ++j) {
+                        if (i0 + j * share >= jn.pieces) break;
+                        const float mn = fmaxf(m, mi[j]), f = fast_exp2(m - mn), fi = fast_exp2(mi[j] - mn);
+                        o = o * f + oi[j] * fi;
+                        l = l * f + li[j] * fi;
+                        m = mn;
+                    }
                 }
             }
-        }
-        if (share > 1) {                 // (one round of the loop: rows <= LG / share)
-            *reinterpret_cast<f32x4*>(&so[g][ch]) = o;
-            if (ch == 0) { sm[g] = m; sl[g] = l; }
-            __syncthreads();
-            if (sub != 0) return;
-            for (int i = 1; i < share; ++i) {
-                const float mn = fmaxf(m, sm[g + i]), f = fast_exp2(m - mn), fi = fast_exp2(sm[g + i] - mn);
-                o = o * f + *reinterpret_cast<const f32x4*>(&so[g + i][ch]) * fi;
-                l = l * f + sl[g + i] * fi;
-                m = mn;
+            if (share > 1) {             // (one round of this loop: rows <= LG / share)
+                *reinterpret_cast<f32x4*>(&so[g][ch]) = o;
+                if (ch == 0) { sm[g] = m; sl[g] = l; }
+                __syncthreads();
+                if (sub == 0) {
+                    for (int k = 1; k < share; ++k) {
+                        const float mn = fmaxf(m, sm[g + k]), f = fast_exp2(m - mn), fi = fast_exp2(sm[g + k] - mn);
+                        o = o * f + *reinterpret_cast<const f32x4*>(&so[g + k][ch]) * fi;
+                        l = l * f + sl[g + k] * fi;
+                        m = mn;
+                    }
+                }
+                __syncthreads();
             }
+            if (sub == 0 && rw < rows) store_row<F16>(a, jn.q0, jn.row0 + first + rw, head, ch, m, l, o);
         }
-        if (rw < rows) store_row<F16>(a, jn.q0, jn.row0 + first + rw, head, ch, m, l, o);
     }
 }
 
@@ -1284,7 +1304,7 @@ __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 struct Sizes {
-    int64_t target, enough, items, joins, parts;
+    int64_t target, items, joins, parts;
     size_t off_counts, off_items, off_joins, off_part, off_ml, end;
 };
 
@@ -1298,7 +1318,6 @@ template <typename K>
 Sizes sizes_of(const hyq_paged_params& p, int64_t tiles, size_t at) {
     Sizes s{};
     s.target = std::max<int64_t>(1, K::SLOTS / p.kv_heads);
-    s.enough = (K::ENOUGH + p.kv_heads - 1) / p.kv_heads;
     s.items = tiles ? s.target + tiles : 0;
     s.joins = std::min(tiles, s.target);
     s.parts = std::min(s.items, 2 * s.target);
@@ -1382,6 +1401,12 @@ int raise_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
     return HYQ_OK;
 }
 
+// at most a round of the resident workgroups (2048 threads a CU)
+template <typename K>
+unsigned join_grid(const Sizes& s, int heads) {
+    return static_cast<unsigned>(std::min<int64_t>(s.joins * heads * (K::TILE / K::JOIN_ROWS), 256 * (2048 / K::JOIN_T)));
+}
+
 template <int D, bool F16>
 int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, hipStream_t st) {
     // (the join launch also clears the rows behind the last request: once)
@@ -1389,7 +1414,7 @@ int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, 
         a.part = reinterpret_cast<float*>(ws + s.narrow.off_part);
         a.ml = reinterpret_cast<float*>(ws + s.narrow.off_ml);
         paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
-        paged_join_kernel<Narrow, D, F16><<<dim3(static_cast<unsigned>(s.narrow.joins), a.heads), dim3(JOIN_T), 0, st>>>(a);
+        paged_join_kernel<Narrow, D, F16><<<dim3(join_grid<Narrow>(s.narrow, a.heads)), dim3(Narrow::JOIN_T), 0, st>>>(a);
         a.zero_tail = 0;
     }
     if (s.wide.items) {
@@ -1399,7 +1424,7 @@ int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, 
         static std::atomic<uint64_t> raised{0};
         if (int rc = raise_lds(reinterpret_cast<const void*>(paged_chunk_kernel<D, F16>), sizeof(ChunkLds<D>), raised)) return rc;
         paged_chunk_kernel<D, F16><<<dim3(static_cast<unsigned>(s.wide.items * a.heads)), dim3(64 * CHUNK_WAVES), sizeof(ChunkLds<D>), st>>>(a);
-        paged_join_kernel<Wide, D, F16><<<dim3(static_cast<unsigned>(s.wide.joins), a.heads, CHUNK / 32), dim3(JOIN_T), 0, st>>>(a);
+        paged_join_kernel<Wide, D, F16><<<dim3(join_grid<Wide>(s.wide, a.heads)), dim3(Wide::JOIN_T), 0, st>>>(a);
     }
     return check_launch("hyq_paged_attention");
 }
@@ -1501,7 +1526,7 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto plan_of = [&](const Sizes& z) {
         return PlanArgs{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, p->window, p->max_pages * p->page_size,
-                        static_cast<int32_t>(z.enough), static_cast<int32_t>(z.target), static_cast<int32_t>(z.items),
+                        static_cast<int32_t>(z.target), static_cast<int32_t>(z.items),
                         static_cast<int32_t>(z.parts), static_cast<int32_t>(z.joins), reinterpret_cast<Counts*>(ws + z.off_counts),
                         reinterpret_cast<Item*>(ws + z.off_items), reinterpret_cast<Join*>(ws + z.off_joins)};
     };
