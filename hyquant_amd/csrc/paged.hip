@@ -270,14 +270,17 @@ __device__ __forceinline__ float quad_bcast(float x) {
 // be cut into pieces, whose partial results a join launch adds up.  The
 // schedule is the same for every KV head.  It is made on the device from the
 // lengths, so that nothing is read back and a captured graph follows the
-// lengths it is replayed with: up to 64 requests every wavefront finds its own
-// item (lane r looks at request r; one load, two wavefront scans), more are
-// laid out by a launch before.
+// lengths it is replayed with: up to 256 requests every wavefront finds its own
+// item (a lane looks at one request, or at four neighbours where there are more
+// than 64; one round of loads, a few wavefront scans), more are laid out by a
+// launch before.
 // Requests of at most 16 rows (decode steps) and larger ones (chunks) have a
 // kernel and a schedule each: a tile of 16 rows is bound by the cache's bytes,
 // one of CHUNK rows by the products.
 constexpr int PLAN_T = 1024;
-constexpr int INLINE_R = 64;             // requests of a schedule without a launch of its own
+constexpr int LANE_R = 4;                // requests of a lane, at most
+constexpr int INLINE_R = 64 * LANE_R;    // requests of a schedule without a launch of its own
+constexpr int JOIN_T = 1024;             // threads of a join's workgroup
 constexpr int CHUNK_WAVES = 8;
 constexpr int CHUNK = 32 * CHUNK_WAVES;  // rows of a chunk tile
 struct Narrow {
@@ -285,7 +288,7 @@ struct Narrow {
     static constexpr int MIN_UNITS = 8;  // steps per piece, at least (two per wavefront)
     static constexpr int SLOTS = 1024;   // pieces wanted over all KV heads
     static constexpr float LONGEST = 0.f;         // (see units_per_piece)
-    static constexpr int JOIN_T = 1024, JOIN_ROWS = 16;   // threads and rows of a join's workgroup
+    static constexpr int JOIN_ROWS = 16;          // rows of a join's workgroup
 };
 struct Wide {
     static constexpr int TILE = CHUNK, GROUP = 64;
@@ -294,7 +297,7 @@ struct Wide {
     // a second round costs more than longer pieces
     static constexpr int SLOTS = 192;
     static constexpr float LONGEST = 1.15f;
-    static constexpr int JOIN_T = 256, JOIN_ROWS = 8;
+    static constexpr int JOIN_ROWS = 32;
 };
 
 struct Item {
@@ -398,72 +401,106 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
-// The schedule of up to 64 requests in one wavefront's registers.  32 bits are
-// enough whatever the lengths: 64 requests of at most 2^22 tiles each and the
-// target's pieces on top.
-struct Plan64 {
-    Req x;                               // of request `lane`
-    int items, parts, joins;             // before it
-    int pc;
+// The schedule of up to INLINE_R requests in one wavefront's registers.  32 bits
+// are enough whatever the lengths: 256 requests of at most 2^22 tiles each and
+// the target's pieces on top.
+struct RegPlan {
+    Req x[LANE_R];                       // of the lane's requests
+    int pc[LANE_R];
+    int items, parts, joins;             // before them
+    int r0, n;                           // the lane's first request and how many a lane has (the same in every lane)
 };
 template <typename K>
-__device__ __forceinline__ Plan64 plan64(const PlanArgs& a, int lane) {
-    Plan64 p;
-    p.x = request<K>(a, lane);
-    const float units = p.x.tiles ? static_cast<float>(p.x.units) : 0.f;
-    const int per = units_per_piece<K>(a, wave_sum(static_cast<float>(p.x.tiles) * units), wave_top(units));
-    p.pc = pieces_of(p.x, per);
-    const int n = p.x.tiles * p.pc, split = p.pc > 1 ? 1 : 0;
-    p.items = scan_dpp(n) - n;
-    p.parts = scan_dpp(split * n) - split * n;
-    p.joins = scan_dpp(split * p.x.tiles) - split * p.x.tiles;
+__device__ __forceinline__ RegPlan reg_plan(const PlanArgs& a, int lane) {
+    RegPlan p;
+    p.n = a.R <= 64 ? 1 : LANE_R;
+    p.r0 = lane * p.n;
+    float work = 0.f, longest = 0.f;
+#pragma unroll
+    for (int j = 0; j < LANE_R; ++j) {
+        p.x[j] = Req{0, 0, 0, 0, 0};
+        if (j < p.n) p.x[j] = request<K>(a, p.r0 + j);
+    }
+#pragma unroll
+    for (int j = 0; j < LANE_R; ++j) {
+        work += static_cast<float>(p.x[j].tiles) * static_cast<float>(p.x[j].units);
+        if (p.x[j].tiles) longest = fmaxf(longest, static_cast<float>(p.x[j].units));
+    }
+    const int per = units_per_piece<K>(a, wave_sum(work), wave_top(longest));
+    int items = 0, parts = 0, joins = 0;
+#pragma unroll
+    for (int j = 0; j < LANE_R; ++j) {
+        p.pc[j] = 1;
+        if (j < p.n) {
+            p.pc[j] = pieces_of(p.x[j], per);
+            const int n = p.x[j].tiles * p.pc[j], split = p.pc[j] > 1 ? 1 : 0;
+            items += n;
+            parts += split * n;
+            joins += split * p.x[j].tiles;
+        }
+    }
+    p.items = scan_dpp(items) - items;
+    p.parts = scan_dpp(parts) - parts;
+    p.joins = scan_dpp(joins) - joins;
     return p;
 }
-// lane `k`'s request, the same in every lane
-__device__ __forceinline__ Req lane_req(const Req& x, int k) {
-    return Req{__builtin_amdgcn_readlane(x.q0, k), __builtin_amdgcn_readlane(x.qlen, k), __builtin_amdgcn_readlane(x.len, k),
-               __builtin_amdgcn_readlane(x.tiles, k), __builtin_amdgcn_readlane(x.units, k)};
-}
-// the lane whose range [start, start + n) holds i (ranges laid end to end), -1: none
-__device__ __forceinline__ int lane_of(int start, int n, int i) {
-    const uint64_t m = __builtin_amdgcn_ballot_w64(start <= i && i < start + n);
-    return m ? __builtin_ctzll(m) : -1;
-}
 
-// This workgroup's item / join; false: it has none
+// This workgroup's item; false: it has none.  With `head` 0 it also leaves what
+// the join launch reads: a split tile's first piece its join, workgroup 0 how
+// many there are, of requests that fit the limits whole (offsets that do not
+// ascend may name more tiles than the grid has).
 template <typename K>
-__device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int lane, Item& it) {
+__device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int head, int lane, Item& it) {
     if (a.R > INLINE_R) {
         if (i >= a.counts->items) return false;
         it = a.items[i];
         return true;
     }
-    const Plan64 p = plan64<K>(a, lane);
-    const int k = lane_of(p.items, p.x.tiles * p.pc, i);
-    if (k < 0) return false;
-    const int pc = __builtin_amdgcn_readlane(p.pc, k), local = i - __builtin_amdgcn_readlane(p.items, k);
-    const int part = __builtin_amdgcn_readlane(p.parts, k) + local;
+    const RegPlan p = reg_plan<K>(a, lane);
+    // the lane and request that entry i belongs to
+    Req x{};
+    int r = 0, pc = 1, local = 0, part = 0, join = 0;
+    bool any = false;
+    int whole = 0;
+    int at = p.items, parts = p.parts, joins = p.joins;
+#pragma unroll
+    for (int j = 0; j < LANE_R; ++j) {
+        if (j < p.n) {
+            const int n = p.x[j].tiles * p.pc[j];
+            if (at <= i && i < at + n) {
+                x = p.x[j];
+                r = p.r0 + j;
+                pc = p.pc[j];
+                local = i - at;
+                part = parts;
+                join = joins;
+                any = true;
+            }
+            at += n;
+            parts += p.pc[j] > 1 ? n : 0;
+            joins += p.pc[j] > 1 ? p.x[j].tiles : 0;
+            if (at <= a.max_items && parts <= a.max_parts) whole = min(joins, a.max_joins);
+        }
+    }
+    if (i == 0 && head == 0) {
+        const float top = wave_top(static_cast<float>(whole));         // (at most 1024 joins)
+        if (threadIdx.x == 0) a.counts->joins = static_cast<int>(top);
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(any);
+    if (!m) return false;
+    const int k = __builtin_ctzll(m);
+    auto get = [&](int v) { return __builtin_amdgcn_readlane(v, k); };
+    x = Req{get(x.q0), get(x.qlen), get(x.len), get(x.tiles), get(x.units)};
+    pc = get(pc);
+    local = get(local);
     // (a causal request's last tiles have the most keys: they go first)
-    const Req x = lane_req(p.x, k);
-    it = make_item<K>(a, x, k, x.tiles - 1 - local / pc, local % pc, pc, pc > 1 && part < a.max_parts ? part : -1);
+    const int nth = local / pc, piece = local - nth * pc;
+    part = get(part) + local;
+    join = get(join) + nth;
+    const bool split = pc > 1 && part < a.max_parts;
+    it = make_item<K>(a, x, get(r), x.tiles - 1 - nth, piece, pc, split ? part : -1);
+    if (split && piece == 0 && head == 0 && join < a.max_joins && threadIdx.x == 0) a.joins[join] = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
     return true;
-}
-// the joins of a schedule, and join j of them (p: where requests are up to 64)
-template <typename K>
-__device__ __forceinline__ int count_joins(const PlanArgs& a, const Plan64& p) {
-    if (a.R > INLINE_R) return a.counts->joins;
-    return min(__builtin_amdgcn_readlane(p.joins + (p.pc > 1 ? p.x.tiles : 0), 63), a.max_joins);
-}
-template <typename K>
-__device__ __forceinline__ Join find_join(const PlanArgs& a, const Plan64& p, int j) {
-    if (a.R > INLINE_R) return a.joins[j];
-    const int k = lane_of(p.joins, p.pc > 1 ? p.x.tiles : 0, j);
-    const int pc = __builtin_amdgcn_readlane(p.pc, k), nth = j - __builtin_amdgcn_readlane(p.joins, k);
-    const int part = __builtin_amdgcn_readlane(p.parts, k) + nth * pc;
-    const Req x = lane_req(p.x, k);
-    Join jn = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
-    if (part + pc > a.max_parts) jn.rows = 0;
-    return jn;
 }
 
 template <typename K>
@@ -472,6 +509,7 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
     // lengths that make no sense may add up to anything)
     __shared__ int64_t start[3][PLAN_T];
     __shared__ int64_t wsum[3][PLAN_T / 64];
+    __shared__ int whole;                // joins of requests that fit the limits whole
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     __shared__ float fsum[2][PLAN_T / 64];
     float work = 0.f, longest = 0.f;
@@ -483,6 +521,7 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
     work = wave_sum(work);
     longest = wave_top(longest);
     if (lane == 0) { fsum[0][w] = work; fsum[1][w] = longest; }
+    if (tid == 0) whole = 0;
     __syncthreads();
     work = longest = 0.f;
     for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; longest = fmaxf(longest, fsum[1][i]); }
@@ -508,7 +547,10 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
                 total[k] += wsum[k][i];
             }
             start[k][tid] = before + incl[k] - n[k];
+            incl[k] += base[k] + before;
         }
+        if (n[2] && incl[0] <= a.max_items && incl[1] <= a.max_parts)
+            atomicMax(&whole, static_cast<int>(min(incl[2], static_cast<int64_t>(a.max_joins))));
         __syncthreads();
         const int nr = min(PLAN_T, a.R - r0);
         for (int64_t i = tid; i < total[0] && base[0] + i < a.max_items; i += PLAN_T) {
@@ -526,9 +568,7 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
         for (int k = 0; k < 3; ++k) base[k] += total[k];
         __syncthreads();
     }
-    if (tid == 0)
-        *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))),
-                           static_cast<int32_t>(min(base[2], static_cast<int64_t>(a.max_joins))), {0, 0}};
+    if (tid == 0) *a.counts = Counts{static_cast<int32_t>(min(base[0], static_cast<int64_t>(a.max_items))), whole, {0, 0}};
 }
 // block 0: the schedule of the short requests, block 1: the chunks'
 __global__ __launch_bounds__(PLAN_T) void paged_plan_kernel(PlanArgs narrow, PlanArgs wide) {
@@ -625,7 +665,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = blockIdx.y;
     Item it;
-    if (!find_item<Narrow>(a.plan, blockIdx.x, lane, it)) return;
+    if (!find_item<Narrow>(a.plan, blockIdx.x, head, lane, it)) return;
     const int c = lane & 15, kb = lane >> 4;
     const int nrows = min(TILE, it.qlen * a.G - it.row0);
 
@@ -945,7 +985,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = blockIdx.x % a.heads;
     Item it;
-    if (!find_item<Wide>(a.plan, blockIdx.x / a.heads, lane, it)) return;
+    if (!find_item<Wide>(a.plan, blockIdx.x / a.heads, head, lane, it)) return;
     const int r32 = lane & 31, h = lane >> 5;
     const int nrows = min(CHUNK, it.qlen * a.G - it.row0);
 
@@ -1223,35 +1263,33 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     if (it.part >= 0 && h == 0) { a.ml[at * 2] = m_run; a.ml[at * 2 + 1] = l_run; }
 }
 
-// Adds up the pieces of the split tiles.  A workgroup takes JOIN_ROWS rows of a
+// Adds up the pieces of the split tiles, of both kinds in one launch (`blocks`
+// of the grid take the short requests').  A workgroup takes JOIN_ROWS rows of a
 // tile and KV head after the other; a row is 4 channels a lane of D/4, and
 // while rows are fewer than the lane groups, several groups share a row's
 // pieces and meet in LDS.  Four pieces are in flight per group.  By zero_tail
 // it also clears the rows behind the last request.
+template <int D>
+struct JoinLds {
+    static constexpr int LG = JOIN_T / (D / 4);    // lane groups
+    float so[LG][D];
+    float sm[LG], sl[LG];
+};
+
 template <typename K, int D, bool F16>
-__global__ __launch_bounds__(K::JOIN_T) void paged_join_kernel(AttnArgs a) {
-    constexpr int LG = K::JOIN_T / (D / 4);        // lane groups
+__device__ __forceinline__ void join_tiles(const AttnArgs& a, JoinLds<D>& L, int block, int blocks) {
+    constexpr int LG = JoinLds<D>::LG;
     constexpr int PARTS = K::TILE / K::JOIN_ROWS;  // of a tile
-    __shared__ float so[LG][D];
-    __shared__ float sm[LG], sl[LG];
+    auto& so = L.so;
+    auto& sm = L.sm;
+    auto& sl = L.sl;
     const int tid = threadIdx.x;
     const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
-    if (a.zero_tail && a.plan.cu) {
-        const int64_t first = min(max(a.plan.cu[a.plan.R], 0), a.plan.T);
-        const int64_t rows = (a.plan.T - first) * a.G * a.heads;       // (token, query head)
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * LG + g; r < rows; r += static_cast<int64_t>(gridDim.x) * LG) {
-            const int64_t t = r / (a.G * a.heads), h = r - t * (a.G * a.heads);
-            if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (first + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
-            if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(first + t) * a.l_t + h] = -INFINITY;
-        }
-    }
-    Plan64 p{};
-    if (a.plan.R <= INLINE_R) p = plan64<K>(a.plan, tid & 63);
-    const int64_t total = static_cast<int64_t>(count_joins<K>(a.plan, p)) * a.heads * PARTS;
-    for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+    const int64_t total = static_cast<int64_t>(a.plan.counts->joins) * a.heads * PARTS;
+    for (int64_t i = block; i < total; i += blocks) {
         const uint32_t rest = static_cast<uint32_t>(i) / a.heads;
         const int head = static_cast<uint32_t>(i) - rest * a.heads;
-        const Join jn = find_join<K>(a.plan, p, rest / PARTS);
+        const Join jn = a.plan.joins[rest / PARTS];
         const int first = rest % PARTS * K::JOIN_ROWS, rows = min(K::JOIN_ROWS, jn.rows - first);
         const int share = rows <= LG / 8 ? 8 : rows <= LG / 4 ? 4 : rows <= LG / 2 ? 2 : 1;
         const int sub = g % share;
@@ -1300,6 +1338,31 @@ __global__ __launch_bounds__(K::JOIN_T) void paged_join_kernel(AttnArgs a) {
     }
 }
 
+template <int D, bool F16>
+__global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a, PlanArgs wide, float* wide_part, float* wide_ml, int blocks) {
+    __shared__ JoinLds<D> L;
+    constexpr int LG = JoinLds<D>::LG;
+    const int tid = threadIdx.x;
+    const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
+    if (a.zero_tail && a.plan.cu) {
+        const int64_t first = min(max(a.plan.cu[a.plan.R], 0), a.plan.T);
+        const int64_t rows = (a.plan.T - first) * a.G * a.heads;       // (token, query head)
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * LG + g; r < rows; r += static_cast<int64_t>(gridDim.x) * LG) {
+            const int64_t t = r / (a.G * a.heads), h = r - t * (a.G * a.heads);
+            if (a.zero_tail & 1) *reinterpret_cast<u32x2*>(a.out + (first + t) * a.o_t + h * a.o_h + ch) = u32x2{0, 0};
+            if ((a.zero_tail & 2) && a.lse && ch == 0) a.lse[(first + t) * a.l_t + h] = -INFINITY;
+        }
+    }
+    if (static_cast<int>(blockIdx.x) < blocks) {
+        join_tiles<Narrow, D, F16>(a, L, blockIdx.x, blocks);
+    } else {
+        a.plan = wide;
+        a.part = wide_part;
+        a.ml = wide_ml;
+        join_tiles<Wide, D, F16>(a, L, blockIdx.x - blocks, gridDim.x - blocks);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -1313,14 +1376,19 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // Where a kind's schedule and partial results lie, from `at` on.  A request's
 // tiles are cut into ceil(units / per) pieces with per >= total / target: at
 // most target + tiles in all, at most 2 target of them in tiles that are cut
-// (units > per), which are at most target.  `tiles` bounds the tiles.
+// (units > per), which are at most target.  `tiles` bounds the tiles; short
+// tables bound the pieces of one, by per >= MIN_UNITS (one 8K request on 8 key
+// heads: 33 x 8 workgroups instead of 129 x 8, @@A@@ us instead of @@B@@).
 template <typename K>
 Sizes sizes_of(const hyq_paged_params& p, int64_t tiles, size_t at) {
     Sizes s{};
     s.target = std::max<int64_t>(1, K::SLOTS / p.kv_heads);
-    s.items = tiles ? s.target + tiles : 0;
-    s.joins = std::min(tiles, s.target);
-    s.parts = std::min(s.items, 2 * s.target);
+    const int64_t keys = static_cast<int64_t>(p.max_pages) * p.page_size;
+    const int64_t units = (p.window > 0 ? std::min<int64_t>(keys, static_cast<int64_t>(p.window) + K::TILE) : keys) / K::GROUP + 2;
+    const int64_t most = (units + K::MIN_UNITS - 1) / K::MIN_UNITS;       // pieces of a tile
+    s.items = tiles ? std::min(s.target + tiles, tiles * most) : 0;
+    s.joins = most > 1 ? std::min(tiles, s.target) : 0;
+    s.parts = s.joins ? std::min(s.items, 2 * s.target) : 0;
     s.off_counts = at;
     s.off_items = at + 256;
     s.off_joins = up256(s.off_items + s.items * sizeof(Item));
@@ -1401,31 +1469,37 @@ int raise_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
     return HYQ_OK;
 }
 
-// at most a round of the resident workgroups (2048 threads a CU)
+// workgroups of a kind's joins, at most `most`
 template <typename K>
-unsigned join_grid(const Sizes& s, int heads) {
-    return static_cast<unsigned>(std::min<int64_t>(s.joins * heads * (K::TILE / K::JOIN_ROWS), 256 * (2048 / K::JOIN_T)));
+int64_t join_grid(const Sizes& s, int heads, int64_t most) {
+    return std::min<int64_t>(s.joins * heads * (K::TILE / K::JOIN_ROWS), most);
 }
 
 template <int D, bool F16>
-int launch_attention(AttnArgs a, const PlanArgs& wide, const Both& s, char* ws, hipStream_t st) {
-    // (the join launch also clears the rows behind the last request: once)
-    if (s.narrow.items) {
-        a.part = reinterpret_cast<float*>(ws + s.narrow.off_part);
-        a.ml = reinterpret_cast<float*>(ws + s.narrow.off_ml);
-        paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
-        paged_join_kernel<Narrow, D, F16><<<dim3(join_grid<Narrow>(s.narrow, a.heads)), dim3(Narrow::JOIN_T), 0, st>>>(a);
-        a.zero_tail = 0;
-    }
+int launch_attention(AttnArgs a, const PlanArgs& narrow, const PlanArgs& wide, const Both& s, char* ws, hipStream_t st) {
+    auto partials = [&](const Sizes& z) {
+        a.part = reinterpret_cast<float*>(ws + z.off_part);
+        a.ml = reinterpret_cast<float*>(ws + z.off_ml);
+    };
     if (s.wide.items) {
         a.plan = wide;
-        a.part = reinterpret_cast<float*>(ws + s.wide.off_part);
-        a.ml = reinterpret_cast<float*>(ws + s.wide.off_ml);
+        partials(s.wide);
         static std::atomic<uint64_t> raised{0};
         if (int rc = raise_lds(reinterpret_cast<const void*>(paged_chunk_kernel<D, F16>), sizeof(ChunkLds<D>), raised)) return rc;
         paged_chunk_kernel<D, F16><<<dim3(static_cast<unsigned>(s.wide.items * a.heads)), dim3(64 * CHUNK_WAVES), sizeof(ChunkLds<D>), st>>>(a);
-        paged_join_kernel<Wide, D, F16><<<dim3(join_grid<Wide>(s.wide, a.heads)), dim3(Wide::JOIN_T), 0, st>>>(a);
     }
+    a.plan = narrow;
+    partials(s.narrow);
+    if (s.narrow.items) paged_attn_kernel<D, F16><<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
+    // a round of resident workgroups (two a CU) for the kind that there is, half
+    // of one each where both may be
+    const int64_t most = s.narrow.joins && s.wide.joins ? 256 : 512;
+    int64_t jn = join_grid<Narrow>(s.narrow, a.heads, most);
+    const int64_t jw = join_grid<Wide>(s.wide, a.heads, most);
+    if (a.zero_tail && a.plan.cu && jn + jw == 0) jn = 1;
+    if (jn + jw)
+        paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(jn + jw)), dim3(JOIN_T), 0, st>>>(
+            a, wide, reinterpret_cast<float*>(ws + s.wide.off_part), reinterpret_cast<float*>(ws + s.wide.off_ml), static_cast<int>(jn));
     return check_launch("hyq_paged_attention");
 }
 
@@ -1537,6 +1611,6 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
                      p->k_scale, p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, narrow, nullptr, nullptr,
                      p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail,
                      p->sm_scale * 1.44269504f};
-    if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, wide, s, ws, st) : launch_attention<128, false>(a, wide, s, ws, st);
-    return p->dtype_fp16 ? launch_attention<64, true>(a, wide, s, ws, st) : launch_attention<64, false>(a, wide, s, ws, st);
+    if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, narrow, wide, s, ws, st) : launch_attention<128, false>(a, narrow, wide, s, ws, st);
+    return p->dtype_fp16 ? launch_attention<64, true>(a, narrow, wide, s, ws, st) : launch_attention<64, false>(a, narrow, wide, s, ws, st);
 }
