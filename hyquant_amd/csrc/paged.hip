@@ -44,8 +44,9 @@ int log2i(int x) {
 // binary search.  A new page's id comes from the free list, never from the
 // table entry another workgroup writes.  Bound: the chain lengths -> scan ->
 // search -> table -> store, a few microseconds.
-constexpr int BT = 256;                  // threads
-constexpr int BATCH_TOKENS = 1024;       // tokens per workgroup
+constexpr int BT = 512;                  // threads
+constexpr int PER = 2;                   // requests per thread and round of the scan
+constexpr int BATCH_TOKENS = 512;        // tokens per workgroup
 
 struct BatchArgs {
     const int32_t* ctx;
@@ -74,6 +75,17 @@ __device__ __forceinline__ int last_at_most(const T* a, int n, T x) {
     return lo;
 }
 
+// inclusive sums over the wavefront by DPP row shifts and broadcasts
+__device__ __forceinline__ int scan_dpp(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);    // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);    // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_incl_scan(T v, int lane) {
 #pragma unroll
@@ -91,26 +103,35 @@ __global__ __launch_bounds__(BT) void paged_batch_kernel(BatchArgs a) {
     __shared__ int32_t wsum[2][BT / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     int base_t = 0, base_p = 0;
-    for (int r0 = 0; r0 < a.R; r0 += BT) {
-        const int r = r0 + tid;
-        int n = 0, p = 0;
-        if (r < a.R) {
-            const int c = max(a.ctx[r], 0);
-            n = max(a.fresh[r], 0);
-            p = ceil_pages(c + n, a.page_log2) - ceil_pages(c, a.page_log2);
+    for (int r0 = 0; r0 < a.R; r0 += BT * PER) {
+        const int r = r0 + tid * PER;    // this thread's requests: r .. r + PER - 1
+        int n[PER], p[PER], st = 0, sp = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const bool in = r + j < a.R;
+            const int c = in ? max(a.ctx[r + j], 0) : 0;
+            n[j] = in ? max(a.fresh[r + j], 0) : 0;
+            p[j] = ceil_pages(c + n[j], a.page_log2) - ceil_pages(c, a.page_log2);
         }
-        const int in = wave_incl_scan(n, lane), ip = wave_incl_scan(p, lane);
-        if (lane == 63) { wsum[0][w] = in; wsum[1][w] = ip; }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) { st += n[j]; sp += p[j]; }
+        const int it = scan_dpp(st), ip = scan_dpp(sp);
+        if (lane == 63) { wsum[0][w] = it; wsum[1][w] = ip; }
         __syncthreads();
-        int bt = base_t, bp = base_p;
+        int bt = base_t + it - st, bp = base_p + ip - sp;
 #pragma unroll
         for (int i = 0; i < BT / 64; ++i) {
             if (i < w) { bt += wsum[0][i]; bp += wsum[1][i]; }
             base_t += wsum[0][i];
             base_p += wsum[1][i];
         }
-        if (r < a.R) { cu[r] = bt + in - n; first[r] = bp + ip - p; }
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (r + j < a.R) { cu[r + j] = bt; first[r + j] = bp; }
+            bt += n[j];
+            bp += p[j];
+        }
+        if (r0 + BT * PER < a.R) __syncthreads();
     }
     if (tid == 0) { cu[a.R] = base_t; first[a.R] = base_p; }
     __syncthreads();
@@ -168,6 +189,18 @@ struct RowArgs {
     int32_t page_log2, lpt_log2;
 };
 
+// max over each aligned group of 8 lanes, or of 16
+__device__ __forceinline__ float max_lanes(float v, bool sixteen) {
+    auto dpp = [](float x, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    v = fmaxf(v, dpp(v, std::integral_constant<int, 0xb1>{}));    // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4e>{}));    // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp(v, std::integral_constant<int, 0x141>{}));   // row_half_mirror
+    if (sixteen) v = fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));   // row_mirror
+    return v;
+}
+
 // hyq_quant_pack's 4-bit rows (quant_row_codes) into their slots: D/8 lanes
 // of 8 channels own a row, blockIdx.y picks K or V, one launch for both.
 // HBM-bound: 2D bytes read and D/2 + 2 written per row.
@@ -196,8 +229,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    for (int m = 1; m < lpt; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
-    amax = fmaxf(amax, 1e-5f);
+    amax = fmaxf(max_lanes(amax, lpt > 8), 1e-5f);
     _Float16 s16;
     uint32_t c[8];
     quant_row_codes<4>(x, amax, s16, c);
@@ -382,16 +414,6 @@ __device__ __forceinline__ Join make_join(const PlanArgs& a, const Req& x, int t
     return Join{x.q0, tile * K::TILE, min(K::TILE, x.qlen * a.G - tile * K::TILE), part, pc, {0, 0, 0}};
 }
 
-// inclusive sums over the wavefront by DPP row shifts and broadcasts
-__device__ __forceinline__ int scan_dpp(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);    // row_shr:1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);    // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);    // row_bcast:31 into rows 2 and 3
-    return v;
-}
 __device__ __forceinline__ float wave_top(float v) {
     v = col_max(max16_dpp(v));
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
