@@ -317,19 +317,26 @@ constexpr int CHUNK_WAVES = 8;
 constexpr int CHUNK = 32 * CHUNK_WAVES;  // rows of a chunk tile
 struct Narrow {
     static constexpr int TILE = 16, GROUP = 32;   // query rows per tile, keys per step
-    static constexpr int MIN_UNITS = 8;  // steps per piece, at least (two per wavefront)
-    static constexpr int SLOTS = 1024;   // pieces wanted over all KV heads
-    static constexpr float LONGEST = 0.f;         // (see units_per_piece)
+    static constexpr int MIN_UNITS = 12;          // steps per piece, at least: each wavefront's ring of loads full once
+    static constexpr float UNCUT = 1.5f;          // pieces that a tile has to be longer than, to be cut
     static constexpr int JOIN_ROWS = 16;          // rows of a join's workgroup
+    static constexpr int slots(int head_dim) { return head_dim == 64 ? 1024 : 768; }   // resident workgroups
+    static __host__ __device__ bool few(float target, float tiles) { return tiles <= 0.4f * target; }
+    static __host__ __device__ float wanted(float target, float tiles) {
+        return few(target, tiles) ? target - 0.5f * tiles : 1.333f * target;
+    }
+    static __host__ __device__ float uncut(float target, float tiles) { return few(target, tiles) ? UNCUT : 2.1f; }
+    static int64_t most(int64_t target, int64_t tiles) { return few(target, tiles) ? target : target + target / 3 + 1; }
 };
 struct Wide {
     static constexpr int TILE = CHUNK, GROUP = 64;
     static constexpr int MIN_UNITS = 4;
-    // one workgroup a CU, a quarter of them for the pieces that rounding up adds:
-    // a second round costs more than longer pieces
-    static constexpr int SLOTS = 192;
-    static constexpr float LONGEST = 1.15f;
+    static constexpr float UNCUT = 1.15f;
     static constexpr int JOIN_ROWS = 32;
+    static constexpr int slots(int) { return 256; }
+    static __host__ __device__ float wanted(float target, float tiles) { return fmaxf(target - 0.5f * tiles, 0.5f * target); }
+    static __host__ __device__ float uncut(float, float) { return UNCUT; }
+    static int64_t most(int64_t target, int64_t) { return target; }
 };
 
 struct Item {
@@ -382,15 +389,28 @@ __device__ __forceinline__ Req request(const PlanArgs& a, int r) {
     return q;
 }
 
-// GROUP steps per piece: the work of a slot, so that the pieces of all tiles are
-// at most target + tiles (the float sum's rounding is far below 2^-14).  Where
-// no tile is much longer than that, as in a prompt of many tiles, cutting gains
-// nothing and costs the partial results.
+// GROUP steps per piece.  A slot is a resident workgroup (`target` of them per KV
+// head).  Where tiles are few, the pieces are to fill the slots exactly once:
+// rounding up makes half a piece more per tile, so that many slots are kept
+// back.  Where 16-row tiles are many, that would make the pieces long and
+// unequal: a third more pieces than slots are cut, and the last ones fill up.
+// A tile that is hardly longer than a piece is not cut, it would cost the
+// partial results for nothing.  Measured on requests of 128 channels, 8 KV heads:
+//   16 requests of 8K keys    exactly one round 33 us, 1024 pieces and more 39
+//   24 requests of 16K        77, 85
+//   64 requests of 1K to 32K  one round 163, a third more 123, twice as many 120
+//   48 requests of 0.7 to 32K one round 92, a third more 87
+//   64 requests of 1K         cut in two 31, whole 24
+//   one request of 8K         12 steps at least 12.6, 8 steps 14.6, 16 steps 13.8
+//   4 chunks of 100 to 700 tokens at 2K to 9K: wide pieces for one round 206,
+//                             for three quarters of one 253
+// (The float sum's rounding is far below 2^-14.)
 template <typename K>
-__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work, float longest) {
-    const float per = ceilf(work * (1.0f + 0x1p-14f) / static_cast<float>(a.target));
-    if (longest <= per * K::LONGEST) return 1 << 30;
-    return static_cast<int>(fminf(fmaxf(per, static_cast<float>(K::MIN_UNITS)), 0x1p30f));
+__device__ __forceinline__ int units_per_piece(const PlanArgs& a, float work, float tiles, float longest) {
+    const float target = static_cast<float>(a.target);
+    const float per = fmaxf(ceilf(work * (1.0f + 0x1p-14f) / K::wanted(target, tiles)), static_cast<float>(K::MIN_UNITS));
+    if (longest <= per * K::uncut(target, tiles)) return 1 << 30;
+    return static_cast<int>(fminf(per, 0x1p30f));
 }
 __device__ __forceinline__ int pieces_of(const Req& x, int per) {
     return static_cast<int>((static_cast<uint32_t>(x.units) + static_cast<uint32_t>(per) - 1u) / static_cast<uint32_t>(per));
@@ -437,7 +457,7 @@ __device__ __forceinline__ RegPlan reg_plan(const PlanArgs& a, int lane) {
     RegPlan p;
     p.n = a.R <= 64 ? 1 : LANE_R;
     p.r0 = lane * p.n;
-    float work = 0.f, longest = 0.f;
+    float work = 0.f, tiles = 0.f, longest = 0.f;
 #pragma unroll
     for (int j = 0; j < LANE_R; ++j) {
         p.x[j] = Req{0, 0, 0, 0, 0};
@@ -445,10 +465,11 @@ __device__ __forceinline__ RegPlan reg_plan(const PlanArgs& a, int lane) {
     }
 #pragma unroll
     for (int j = 0; j < LANE_R; ++j) {
+        tiles += static_cast<float>(p.x[j].tiles);
         work += static_cast<float>(p.x[j].tiles) * static_cast<float>(p.x[j].units);
         if (p.x[j].tiles) longest = fmaxf(longest, static_cast<float>(p.x[j].units));
     }
-    const int per = units_per_piece<K>(a, wave_sum(work), wave_top(longest));
+    const int per = units_per_piece<K>(a, wave_sum(work), wave_sum(tiles), wave_top(longest));
     int items = 0, parts = 0, joins = 0;
 #pragma unroll
     for (int j = 0; j < LANE_R; ++j) {
@@ -533,22 +554,24 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
     __shared__ int64_t wsum[3][PLAN_T / 64];
     __shared__ int whole;                // joins of requests that fit the limits whole
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    __shared__ float fsum[2][PLAN_T / 64];
-    float work = 0.f, longest = 0.f;
+    __shared__ float fsum[3][PLAN_T / 64];
+    float work = 0.f, tiles = 0.f, longest = 0.f;
     for (int r = tid; r < a.R; r += PLAN_T) {
         const Req q = request<K>(a, r);
+        tiles += static_cast<float>(q.tiles);
         work += static_cast<float>(q.tiles) * static_cast<float>(q.units);
         if (q.tiles) longest = fmaxf(longest, static_cast<float>(q.units));
     }
     work = wave_sum(work);
+    tiles = wave_sum(tiles);
     longest = wave_top(longest);
-    if (lane == 0) { fsum[0][w] = work; fsum[1][w] = longest; }
+    if (lane == 0) { fsum[0][w] = work; fsum[1][w] = longest; fsum[2][w] = tiles; }
     if (tid == 0) whole = 0;
     __syncthreads();
-    work = longest = 0.f;
-    for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; longest = fmaxf(longest, fsum[1][i]); }
+    work = tiles = longest = 0.f;
+    for (int i = 0; i < PLAN_T / 64; ++i) { work += fsum[0][i]; longest = fmaxf(longest, fsum[1][i]); tiles += fsum[2][i]; }
     __syncthreads();
-    const int per = units_per_piece<K>(a, work, longest);
+    const int per = units_per_piece<K>(a, work, tiles, longest);
     int64_t base[3] = {0, 0, 0};
     for (int r0 = 0; r0 < a.R; r0 += PLAN_T) {
         const Req q = request<K>(a, r0 + tid);
@@ -1396,21 +1419,23 @@ struct Sizes {
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Where a kind's schedule and partial results lie, from `at` on.  A request's
-// tiles are cut into ceil(units / per) pieces with per >= total / target: at
-// most target + tiles in all, at most 2 target of them in tiles that are cut
-// (units > per), which are at most target.  `tiles` bounds the tiles; short
+// tiles are cut into ceil(units / per) pieces with per >= total / wanted: at
+// most wanted + tiles in all, at most 2 wanted of them in tiles that are cut
+// (units > per), which are at most wanted.  `tiles` bounds the tiles; short
 // tables bound the pieces of one, by per >= MIN_UNITS (one 8K request on 8 key
-// heads: 33 x 8 workgroups instead of 129 x 8, @@A@@ us instead of @@B@@).
+// heads: 33 x 8 workgroups instead of 129 x 8, 14.6 us instead of 16.9).
 template <typename K>
 Sizes sizes_of(const hyq_paged_params& p, int64_t tiles, size_t at) {
     Sizes s{};
-    s.target = std::max<int64_t>(1, K::SLOTS / p.kv_heads);
+    s.target = std::max<int64_t>(1, K::slots(p.head_dim) / p.kv_heads);
+    const int64_t wanted = K::most(s.target, tiles);
     const int64_t keys = static_cast<int64_t>(p.max_pages) * p.page_size;
     const int64_t units = (p.window > 0 ? std::min<int64_t>(keys, static_cast<int64_t>(p.window) + K::TILE) : keys) / K::GROUP + 2;
-    const int64_t most = (units + K::MIN_UNITS - 1) / K::MIN_UNITS;       // pieces of a tile
-    s.items = tiles ? std::min(s.target + tiles, tiles * most) : 0;
-    s.joins = most > 1 ? std::min(tiles, s.target) : 0;
-    s.parts = s.joins ? std::min(s.items, 2 * s.target) : 0;
+    // pieces of a tile (no piece is shorter than MIN_UNITS, no tile cut that is hardly longer)
+    const int64_t most = units <= K::MIN_UNITS * K::UNCUT ? 1 : (units + K::MIN_UNITS - 1) / K::MIN_UNITS;
+    s.items = tiles ? std::min(wanted + tiles, tiles * most) : 0;
+    s.joins = most > 1 ? std::min(tiles, wanted) : 0;
+    s.parts = s.joins ? std::min(s.items, 2 * wanted) : 0;
     s.off_counts = at;
     s.off_items = at + 256;
     s.off_joins = up256(s.off_items + s.items * sizeof(Item));
