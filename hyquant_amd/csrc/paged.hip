@@ -1330,6 +1330,7 @@ __device__ __forceinline__ void join_tiles(const AttnArgs& a, JoinLds<D>& L, int
     auto& sl = L.sl;
     const int tid = threadIdx.x;
     const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
+    if (a.plan.max_joins == 0) return;   // (nothing can be cut, and where the kind has no tiles nobody wrote the counts)
     const int64_t total = static_cast<int64_t>(a.plan.counts->joins) * a.heads * PARTS;
     for (int64_t i = block; i < total; i += blocks) {
         const uint32_t rest = static_cast<uint32_t>(i) / a.heads;

@@ -109,8 +109,8 @@ def paged_batch(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table:
     R = context_lens.shape[0]
     if new_lens.shape[0] != R or block_table.shape[0] != R:
         raise ValueError(f"context_lens, new_lens and block_table are of {R}, {new_lens.shape[0]} and {block_table.shape[0]} requests")
-    if num_tokens < 0:
-        raise ValueError(f"num_tokens must be >= 0, got {num_tokens}")
+    if not 0 <= num_tokens < 1 << 31:
+        raise ValueError(f"num_tokens must be >= 0 and below 2^31, got {num_tokens}")
     longs = torch.empty(2, num_tokens, dtype=torch.int64, device=dev)
     ints = torch.empty(2 * R + 2, dtype=torch.int32, device=dev)
     cu, lens, used = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
@@ -156,6 +156,14 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1])):
         return t.contiguous() if not t.is_contiguous() else t.clone()
     return t
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether rows of t [T, H, D] (contiguous channels) share memory."""
+    (n0, n1, D), (s0, s1, _) = t.shape, t.stride()
+    if n0 <= 1 or n1 <= 1:
+        return (n0 > 1 and s0 < D) or (n1 > 1 and s1 < D)
+    return min(s0, s1) < D or (s0 < n1 * s1 and s1 < n0 * s0)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -233,7 +241,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns out [T, H_Q, D] of q's dtype, with return_lse also the natural
     log-sum-exp of the scaled scores, fp32 [T, H_Q].  A row that sees no key is
     zero (lse -inf), as are the rows behind the last request of a padded batch
-    (those of an `out` that is handed in are left as they are)."""
+    (those of an `out` that is handed in are left as they are; it shares no
+    memory with the inputs)."""
     fx, stream = _fast(q)
     if fx and out is None:
         try:
@@ -267,11 +276,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise ValueError(f"cu_seqlens must be of {R + 1} entries, got {cu_seqlens.shape[0]}")
     if window < 0:
         raise ValueError(f"window must be >= 0, got {window}")
+    window = window if window < 1 << 30 else 0       # (no table row names as many tokens)
     zero_tail = out is None
     if out is None:
         out = torch.empty(T, HQ, D, dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev or out.stride(2) != 1:
         raise ValueError("out must be of q's shape, dtype and device, with contiguous channels")
+    elif _overlaps_itself(out) or (T and out.data_ptr() == q.data_ptr()):
+        raise ValueError("out must not share memory between its rows, or with q")
     lse = torch.empty(T, HQ, dtype=torch.float32, device=dev) if return_lse else None
     if T and R:
         q = _aligned_rows(q)

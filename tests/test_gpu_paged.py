@@ -584,3 +584,91 @@ def test_refusals():
                        ((lens, lens, table.long(), lens, 16, 4), "block_table")):
         with pytest.raises(ValueError, match=word):
             hq.paged_batch(*args)
+
+
+@pytest.mark.parametrize("R", [65, 200, 256, 257, 400])
+@pytest.mark.parametrize("decode", [True, False])
+def test_attention_batches_of_long_and_short_requests(R, decode):
+    """Schedules on both sides of 64 and 256 requests, with tiles that are cut
+    and tiles that are not, in both kinds of tiles."""
+    g = torch.Generator().manual_seed(R)
+    seq = torch.randint(1, 60, (R,), generator=g).tolist()
+    new = [1] * R
+    seq[3], seq[R // 2], seq[-1], seq[7] = 9000, 5003, 2500, 0
+    if not decode:
+        new = [min(n, s) for n, s in zip(torch.randint(0, 9, (R,), generator=g).tolist(), seq)]
+        new[3], new[R // 2], new[-1] = 300, 2, 70
+    else:
+        new[7] = 1
+    _attend(BF16, 64, 2, 4, 16, seq, new, decode=decode, seed=R, pad=0 if decode else 5)
+
+
+@pytest.mark.parametrize("R", [5, 70, 300])
+@pytest.mark.parametrize("G", [4, 32])
+def test_attention_offsets_that_do_not_ascend(R, G):
+    """More tiles than tokens: rows of such calls are unspecified, memory around the outputs is not touched."""
+    g = _gen(R)
+    seq, page, T = [600] * R, 16, 40
+    table = torch.zeros(R, 40, dtype=torch.int32, device="cuda")
+    pool = U.make_pool(g, 4, 2, page, 64, "cuda")
+    q = torch.randn(T, 2 * G, 64, generator=g, device="cuda").to(BF16)
+    big = torch.full((T + 8, 2 * G, 64), 3.0, dtype=BF16, device="cuda")
+    for cu in ([0, T] * (R // 2 + 1), [T, 0] * (R // 2 + 1), [0, 2 ** 31 - 1, -2 ** 31] * (R // 3 + 1)):
+        hq.paged_attention(q, *pool, table, _i32(seq), _i32(cu[:R + 1]), out=big[4:-4])
+        assert bool((big[:4] == 3.0).all()) and bool((big[-4:] == 3.0).all())
+    # and a call after them is as ever
+    _attend(BF16, 64, 2, G, page, [600, 30], [10, 3])
+
+
+@pytest.mark.parametrize("pad", [0, 9])
+def test_attention_more_heads_than_a_short_tile(pad):
+    """32 query heads on a key head: no tile of 16 rows, and tables too short for any tile to be cut."""
+    for R in (1, 3, 70, 300):
+        _attend(FP16, 128, 2, 32, 32, [33 + r % 7 for r in range(R)], [1 + r % 3 for r in range(R)], pad=pad, seed=R)
+        _attend(BF16, 64, 1, 20, 16, [20] * R, [1] * R, decode=True, seed=R)
+
+
+def test_native_and_checked_calls_agree(monkeypatch):
+    """The C++ form of the calls and the Python form launch the same kernels."""
+    from hyquant_amd import decode_d_stage as dd
+    g = _gen(50)
+    seq, new, page, H, G, D = [700, 65, 0, 130], [1, 65, 0, 9], 16, 2, 4, 64
+    table, pages = U.make_table(g, seq, page, "cuda")
+    T, pad = sum(new), 3
+    ctx = [s - n for s, n in zip(seq, new)]
+    pool = U.make_pool(g, pages, H, page, D, "cuda")
+    q = torch.randn(T + pad, H * G, D, generator=g, device="cuda").to(FP16)
+    kv = torch.randn(2, T + pad, H, D, generator=g, device="cuda").to(FP16)
+    free = torch.arange(pages, dtype=torch.int32, device="cuda")
+
+    def calls():
+        t, p = torch.full_like(table, -1), tuple(x.clone() for x in pool)
+        b = hq.paged_batch(_i32(ctx), _i32(new), t, free, page, T + pad)
+        hq.paged_append(kv[0], kv[1], b.slots, *p)
+        rows = hq.paged_gather(b.slots, *p, dtype=FP16)
+        o = hq.paged_attention(q, *p, table, b.seq_lens, b.cu_seqlens, sm_scale=0.2, window=90, return_lse=True)
+        d = hq.paged_attention(q[:4], *p, table, b.seq_lens)
+        return (t, *p, *b, *rows, *o, d)
+
+    native = calls()
+    assert dd._FX
+    monkeypatch.setattr(dd, "_FX", False)
+    for i, (x, y) in enumerate(zip(native, calls())):
+        assert x.dtype == y.dtype and torch.equal(x, y), i
+
+
+def test_window_past_32_bits_and_shared_outputs():
+    g = _gen(51)
+    table, pages = U.make_table(g, [100, 40], 16, "cuda")
+    pool = U.make_pool(g, pages, 2, 16, 64, "cuda")
+    q = torch.randn(2, 8, 64, generator=g, device="cuda").to(BF16)
+    lens = _i32([100, 40])
+    want = hq.paged_attention(q, *pool, table, lens)
+    for window in (1 << 30, 2 ** 31 - 1, 2 ** 33 + 5):
+        assert torch.equal(hq.paged_attention(q, *pool, table, lens, window=window), want)
+    row = torch.empty(1, 8, 64, dtype=BF16, device="cuda")
+    for out in (q, row.expand(2, 8, 64), row.view(-1).as_strided((2, 8, 64), (64, 32, 1)), row[:, :1].expand(1, 8, 64).expand(2, 8, 64)):
+        with pytest.raises(ValueError, match="share memory"):
+            hq.paged_attention(q, *pool, table, lens, out=out)
+    with pytest.raises(ValueError, match="num_tokens"):
+        hq.paged_batch(lens, lens, table, lens, 16, 1 << 31)
