@@ -164,6 +164,16 @@ bool pool(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks, cons
 template <typename T>
 T* ptr(const at::Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 
+// A contiguous tensor of `type` at element `offset` of base's memory.  A call's
+// outputs are parts of one allocation this way: an allocation costs about 0.6 us
+// of host time, a part about 0.1.
+at::Tensor part(const at::Tensor& base, at::ScalarType type, int64_t offset, at::IntArrayRef sizes) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
 }  // namespace
 
 void set_paged(int64_t batch, int64_t append, int64_t gather, int64_t size, int64_t attention) {
@@ -185,9 +195,11 @@ std::tuple<int64_t, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> 
         !ints(free_pages, at::kInt, 1, dev) || fresh.size(0) != R || table.size(0) != R || free_pages.size(0) > INT32_MAX)
         return {-1, {}, {}, {}, {}, {}};
     const c10::DeviceGuard guard(dev);
-    const auto i32 = ctx.options(), i64 = i32.dtype(at::kLong);
-    const at::Tensor cu = at::empty({R + 1}, i32), lens = at::empty({R}, i32), used = at::empty({1}, i32);
-    const at::Tensor slots = at::empty({tokens}, i64), positions = at::empty({tokens}, i64);
+    // slots, positions, then (in halves of a word) offsets, lengths and the count
+    const at::Tensor all = at::empty({2 * tokens + R + 1}, ctx.options().dtype(at::kLong));
+    const int64_t ints_at = 4 * tokens;
+    const at::Tensor slots = part(all, at::kLong, 0, {tokens}), positions = part(all, at::kLong, tokens, {tokens});
+    const at::Tensor cu = part(all, at::kInt, ints_at, {R + 1}), lens = part(all, at::kInt, ints_at + R + 1, {R}), used = part(all, at::kInt, ints_at + 2 * R + 1, {1});
     const int st = g_paged.batch(ptr<int32_t>(ctx), ptr<int32_t>(fresh), static_cast<int32_t>(R), ptr<int32_t>(table), table.stride(0),
                                  static_cast<int32_t>(table.size(1)), ptr<int32_t>(free_pages),
                                  static_cast<int32_t>(free_pages.size(0)), static_cast<int32_t>(page), static_cast<int32_t>(tokens),
@@ -219,7 +231,9 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_gather(const at::Tensor& slots
         return {-1, {}, {}};
     const c10::DeviceGuard guard(dev);
     const auto opt = slots.options().dtype(fp16 ? at::kHalf : at::kBFloat16);
-    const at::Tensor k = at::empty({slots.size(0), kp.size(1), 2 * kp.size(3)}, opt), v = at::empty(k.sizes(), opt);
+    const at::Tensor kv = at::empty({2, slots.size(0), kp.size(1), 2 * kp.size(3)}, opt);
+    const at::Tensor k = part(kv, kv.scalar_type(), 0, kv.sizes().slice(1));
+    const at::Tensor v = part(kv, kv.scalar_type(), k.numel(), kv.sizes().slice(1));
     const int st = g_paged.gather(ptr<int64_t>(slots), slots.size(0), static_cast<int32_t>(kp.size(1)),
                                   static_cast<int32_t>(2 * kp.size(3)), ptr<int8_t>(kp), ptr<int8_t>(vp), kp.stride(0), kp.stride(1),
                                   ptr<uint16_t>(ks), ptr<uint16_t>(vs), ks.stride(0), ks.stride(1), kp.size(0),

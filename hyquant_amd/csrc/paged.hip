@@ -42,8 +42,12 @@ int log2i(int x) {
 // itself (they stay in the L2) and keeps both prefix arrays in LDS, so the
 // layout is one launch; token and page entries then find their request by a
 // binary search.  A new page's id comes from the free list, never from the
-// table entry another workgroup writes.  Bound: the chain lengths -> scan ->
-// search -> table -> store, a few microseconds.
+// table entry another workgroup writes.  Bound by the chain lengths -> scan ->
+// search -> table -> store, not by bytes: 3.7 us for 24 requests, 5.2 us for
+// 1000 requests and 150000 tokens (2.4 MB), both in a captured graph.  512
+// threads with two requests each and 512 tokens a workgroup are the best of
+// what was measured there: 256 threads and 1024 tokens 7.7 us, 1024 threads
+// 5.9, 2048 tokens 11.0.
 constexpr int BT = 512;                  // threads
 constexpr int PER = 2;                   // requests per thread and round of the scan
 constexpr int BATCH_TOKENS = 512;        // tokens per workgroup
@@ -203,7 +207,11 @@ __device__ __forceinline__ float max_lanes(float v, bool sixteen) {
 
 // hyq_quant_pack's 4-bit rows (quant_row_codes) into their slots: D/8 lanes
 // of 8 channels own a row, blockIdx.y picks K or V, one launch for both.
-// HBM-bound: 2D bytes read and D/2 + 2 written per row.
+// HBM-bound: 2D bytes read and D/2 + 2 written per row.  8192 tokens of 8 heads
+// of 128 (42 MB) take 10.5 us, 4.0 TB/s with the launch's 2.5 us in it; one row
+// per thread, since two or four change nothing there (20.2 us with the read-back
+// for 1 and 2, 20.5 for 4) and cost latency at 16 tokens (4.6 us against 5.0 and
+// 5.9).
 template <bool F16>
 __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
     const int lpt = 1 << a.lpt_log2, sub = threadIdx.x & (lpt - 1);
@@ -245,7 +253,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
 
 // Rows of the cache by slot as bf16 or fp16 values, code * scale rounded once
 // (the product is exact in fp32); slots outside the pool give zero rows.
-// HBM-bound: D/2 + 2 bytes read and 2D written per row.
+// HBM-bound: D/2 + 2 bytes read and 2D written per row; 8192 tokens of 8 heads of
+// 128 (42 MB) take 9.6 us, 4.4 TB/s.
 template <bool F16>
 __global__ __launch_bounds__(256) void paged_gather_kernel(RowArgs a) {
     const int lpt = 1 << a.lpt_log2, sub = threadIdx.x & (lpt - 1);
@@ -690,6 +699,25 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
 }
 
+// A workgroup has one KV head of a tile of 16 rows (a request's tokens times the
+// G query heads) and a range of keys; its four wavefronts take every fourth
+// 32-key step and join through LDS at the end.
+//   QK  S^T[key][row] = K . Q^T with v_mfma_f32_16x16x32_f16.  A K operand is the
+//       code's offset form u = code + 8 as the fp16 subnormal u 2^-24, two bit
+//       operations per pair of codes; the accumulators start at -8 sum(q) 2^-24,
+//       so that the score is exact but for fp32 roundings.
+//   softmax: a row's maximum moves only when a score passes it by SLACK (its own
+//       scores alone move it), sums in fp32.
+//   PV  O^T[channel][row] = V^T . P'^T with v_mfma_f32_16x16x32_bf16, V operands
+//       the bf16 numbers 128 + u, P' = bf16(p v_scale): 136 sum(P') is taken off
+//       at the end, from the same rounded P' by a product with ones.  That
+//       rounding (2^-8 of a weight, random over keys) is the one between scores
+//       and output; an fp16 model's P' is the sum of two bf16 numbers.
+// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 97 us, 5.7
+// TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
+// ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
+// on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
+// chain lengths -> table -> rows -> join: 12.6 us for one request of 8K keys.
 template <int D>
 struct Raw {
     uint32_t k[2][D / 32];               // tile t: row c's channels (D/4) kb .. of token 16t + 4(c & 3) + (c >> 2)
@@ -975,6 +1003,15 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
 //       max(score + log2 of the block's largest V scale), so that P' keeps to
 //       [0, 2^13] whatever the scales are; rounding P' to 11 bits once is the
 //       only rounding between the scores and the output.
+// Bound by the matrix pipe and the VALU work that has to run beside it: 2048
+// tokens at 8192 (309 GFLOP) take 358 us, 0.86 PFLOP/s where a large matrix
+// product reaches 1.35, and the products with their LDS reads alone take 226 us.
+// So the block is worked on in halves of 32 keys: the scores of one half run
+// beside the weights of the half before, and the first four wavefronts have
+// priority, so that the two of a SIMD do not wait for the same pipe (without
+// halves 437 us).  Rows are padded instead of swizzled: operand addresses are
+// constants then (swizzled 437).  256 rows per workgroup, since a block's
+// conversion is paid once per tile (16-row wavefronts, four a SIMD: 421 at best).
 // Output register i of a lane (row l & 31, half h = l >> 5) of a 32-key product
 // is key 8 (i >> 2) + 4 h + (i & 3); registers 8s .. 8s + 7 are the B operand of
 // step s of P.V, without a shuffle.
