@@ -468,15 +468,17 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  *   out = softmax_j(sm_scale q . k_j) v_j,  lse = ln sum_j exp(sm_scale q . k_j)
  * A row that sees no key is 0 (lse -inf).  The codes enter the products as
  * exact operands: the K scale multiplies the fp32 score, the V scale the
- * weight, which is then rounded to bf16 (for an fp16 model to the sum of two
- * bf16 numbers).
+ * weight, which is then rounded once: for requests of at most 16 rows (tokens
+ * times kv_repeat) to bf16, of an fp16 model to the sum of two bf16 numbers,
+ * for larger requests to fp16.
  *   q     bf16 or fp16 [num_tokens, kv_heads * kv_repeat, head_dim] strides (t, h, 1),
  *         16-byte aligned, strides divisible by 8; out the same type, 8-byte aligned,
  *         strides divisible by 4
  *   lse   float [num_tokens, kv_heads * kv_repeat] contiguous, or NULL
  * Lengths beyond max_pages * page_size count as that, negative ones as 0; keys
  * in pages outside [0, num_pages) are left out; cu_seqlens is clamped to
- * [0, num_tokens].  Rows of tokens behind the last request are left as they
+ * [0, num_tokens] (where it does not ascend, out and lse hold anything).  out
+ * and lse share no memory with the inputs.  Rows of tokens behind the last request are left as they
  * are, but with bit 0 of zero_tail out is set to 0 there, with bit 1 lse to -inf.
  * The workspace needs no initialisation; calls that share one must be ordered
  * on one stream.
