@@ -136,8 +136,11 @@ class PagedParams(Structure):
         ("kv_heads", c_int32), ("kv_repeat", c_int32), ("head_dim", c_int32), ("window", c_int32),
         ("sm_scale", c_float),
         ("dtype_fp16", c_int32), ("zero_tail", c_int32),
+        ("counters", c_void_p),
     ]
 
+
+PAGED_COUNTERS = 65536                     # HYQ_PAGED_COUNTERS
 
 _REBUILD = "rebuild it with `python -m hyquant_amd.build`"
 _lib = None

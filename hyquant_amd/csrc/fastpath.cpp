@@ -247,7 +247,7 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q,
                                                             const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table,
                                                             const at::Tensor& lens, const std::optional<at::Tensor>& cu,
                                                             const std::optional<double>& sm_scale, int64_t window,
-                                                            bool want_lse, int64_t stream) {
+                                                            bool want_lse, int64_t stream, int64_t counters) {
     const std::tuple<int64_t, at::Tensor, at::Tensor> skip{-1, {}, {}};
     const auto dev = q.device();
     if (!g_paged.attention || !dev.is_cuda() || !half(q) || !plain(q, q.scalar_type(), 3, dev) || !pool(kp, vp, ks, vs, dev) ||
@@ -296,6 +296,7 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q,
     p.sm_scale = static_cast<float>(sm_scale ? *sm_scale : std::pow(static_cast<double>(D), -0.5));
     p.dtype_fp16 = q.scalar_type() == at::kHalf;
     p.zero_tail = 3;
+    p.counters = reinterpret_cast<uint32_t*>(counters);
     const size_t need = g_paged.size(&p);
     if (need == 0) return skip;
     const at::Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
@@ -306,7 +307,7 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q,
 // the paged parameter block's size and the offsets of two of its fields
 std::tuple<int64_t, int64_t, int64_t> paged_layout() {
     return {static_cast<int64_t>(sizeof(hyq_paged_params)), static_cast<int64_t>(offsetof(hyq_paged_params, num_pages)),
-            static_cast<int64_t>(offsetof(hyq_paged_params, zero_tail))};
+            static_cast<int64_t>(offsetof(hyq_paged_params, counters))};
 }
 
 // the library entry points (addresses from ctypes)
@@ -379,13 +380,13 @@ std::tuple<int64_t, int64_t, int64_t> layout() {
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.def("signatures", [] { return 3; }, "counts up when a function of this module takes other arguments");
+    m.def("signatures", [] { return 4; }, "counts up when a function of this module takes other arguments");
     m.def("layout", &layout, "sizeof(hyq_decode_params), offsetof(seg_n), offsetof(dtype_flags)");
     m.def("set_entry", &set_entry, "the addresses of hyq_decode_hybrid and hyq_append_rows");
     m.def("decode", &decode, "fused_d_stage_decode eager fast path");
     m.def("decode_cache", &decode_cache, "a layer cache's decode step");
     m.def("append", &append, "a layer cache's staging append");
-    m.def("paged_layout", &paged_layout, "sizeof(hyq_paged_params), offsetof(num_pages), offsetof(zero_tail)");
+    m.def("paged_layout", &paged_layout, "sizeof(hyq_paged_params), offsetof(num_pages), offsetof(counters)");
     m.def("set_paged", &set_paged, "the addresses of the five hyq_paged entry points");
     m.def("paged_batch", &paged_batch, "a step's batch layout");
     m.def("paged_append", &paged_append, "new rows into the pages");

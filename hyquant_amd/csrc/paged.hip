@@ -328,7 +328,7 @@ struct Narrow {
     static constexpr int TILE = 16, GROUP = 32;   // query rows per tile, keys per step
     static constexpr int MIN_UNITS = 12;          // steps per piece, at least: each wavefront's ring of loads full once
     static constexpr float UNCUT = 1.5f;          // pieces that a tile has to be longer than, to be cut
-    static constexpr int JOIN_ROWS = 16;          // rows of a join's workgroup
+    static constexpr int join_rows(int lane_groups) { return lane_groups / 4; }   // rows of a join's workgroup
     static constexpr int slots(int head_dim) { return head_dim == 64 ? 1024 : 768; }   // resident workgroups
     static __host__ __device__ bool few(float target, float tiles) { return tiles <= 0.4f * target; }
     static __host__ __device__ float wanted(float target, float tiles) {
@@ -341,7 +341,7 @@ struct Wide {
     static constexpr int TILE = CHUNK, GROUP = 64;
     static constexpr int MIN_UNITS = 4;
     static constexpr float UNCUT = 1.15f;
-    static constexpr int JOIN_ROWS = 32;
+    static constexpr int join_rows(int lane_groups) { return lane_groups; }
     static constexpr int slots(int) { return 256; }
     static __host__ __device__ float wanted(float target, float tiles) { return fmaxf(target - 0.5f * tiles, 0.5f * target); }
     static __host__ __device__ float uncut(float, float) { return UNCUT; }
@@ -353,6 +353,8 @@ struct Item {
     int32_t row0;                        // first row of the tile within the request
     int32_t key0, key1;                  // keys of this piece
     int32_t part;                        // partial slot, -1: the tile is whole
+    int32_t join, part0, pieces;         // of a cut tile: its join, its first partial slot, its pieces
+    int32_t pad;
 };
 struct Join {
     int32_t q0, row0, rows, part, pieces, pad[3];
@@ -428,12 +430,12 @@ __device__ __forceinline__ int pieces_of(const Req& x, int per) {
 // Piece `piece` of pc of tile `tile` of a request
 template <typename K>
 __device__ __forceinline__ Item make_item(const PlanArgs& a, const Req& x, int r, int tile, int piece, int pc,
-                                          int part) {
+                                          int part0, int join) {
     const int row0 = tile * K::TILE, row1 = min(row0 + K::TILE, x.qlen * a.G);
     const int p0 = x.len - x.qlen + row0 / a.G, p1 = x.len - x.qlen + (row1 - 1) / a.G;   // first and last position
     const int lo = first_key(p0, a.window) / K::GROUP, hi = (max(p1, -1) + K::GROUP) / K::GROUP;   // GROUP steps
     const int steps = max(hi - lo, 0), each = static_cast<int>((static_cast<uint32_t>(steps) + pc - 1u) / pc);
-    Item it{r, x.q0, x.qlen, x.len, row0, 0, 0, part};
+    Item it{r, x.q0, x.qlen, x.len, row0, 0, 0, part0 >= 0 ? part0 + piece : -1, join, part0, pc, 0};
     it.key0 = (lo + min(steps, piece * each)) * K::GROUP;
     it.key1 = min(p1 + 1, (lo + min(steps, (piece + 1) * each)) * K::GROUP);
     return it;
@@ -547,11 +549,11 @@ __device__ __forceinline__ bool find_item(const PlanArgs& a, int i, int head, in
     local = get(local);
     // (a causal request's last tiles have the most keys: they go first)
     const int nth = local / pc, piece = local - nth * pc;
-    part = get(part) + local;
+    part = get(part) + nth * pc;
     join = get(join) + nth;
-    const bool split = pc > 1 && part < a.max_parts;
-    it = make_item<K>(a, x, get(r), x.tiles - 1 - nth, piece, pc, split ? part : -1);
-    if (split && piece == 0 && head == 0 && join < a.max_joins && threadIdx.x == 0) a.joins[join] = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
+    const bool split = pc > 1 && part + pc <= a.max_parts && join < a.max_joins;
+    it = make_item<K>(a, x, get(r), x.tiles - 1 - nth, piece, pc, split ? part : -1, join);
+    if (split && piece == 0 && head == 0 && threadIdx.x == 0) a.joins[join] = make_join<K>(a, x, x.tiles - 1 - nth, pc, part);
     return true;
 }
 
@@ -612,11 +614,10 @@ __device__ __forceinline__ void plan(const PlanArgs& a) {
             const Req x = request<K>(a, r0 + k);
             const int pc = pieces_of(x, per), local = static_cast<int>(i - start[0][k]), nth = local / pc, piece = local - nth * pc;
             const int tile = x.tiles - 1 - nth;
-            const int64_t part = base[1] + start[1][k] + local;
-            const bool split = pc > 1 && part < a.max_parts;
-            a.items[base[0] + i] = make_item<K>(a, x, r0 + k, tile, piece, pc, split ? static_cast<int>(part) : -1);
-            const int64_t j = base[2] + start[2][k] + nth;
-            if (split && piece == 0 && j < a.max_joins) a.joins[j] = make_join<K>(a, x, tile, pc, static_cast<int>(part));
+            const int64_t part = base[1] + start[1][k] + local - piece, j = base[2] + start[2][k] + nth;
+            const bool split = pc > 1 && part + pc <= a.max_parts && j < a.max_joins;
+            a.items[base[0] + i] = make_item<K>(a, x, r0 + k, tile, piece, pc, split ? static_cast<int>(part) : -1, static_cast<int>(j));
+            if (split && piece == 0) a.joins[j] = make_join<K>(a, x, tile, pc, static_cast<int>(part));
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k) base[k] += total[k];
@@ -649,6 +650,7 @@ struct AttnArgs {
     PlanArgs plan;
     float* part;                         // [slot][key head][TILE][D] sums; ml: [slot][key head][TILE][2] (m, l)
     float* ml;
+    uint32_t* counters;                  // arrivals per join and KV head (the last workgroup joins), or null: a launch joins
     int32_t G, heads, page_log2, num_pages, window, zero_tail;
     float scale;                         // sm_scale * log2(e)
 };
@@ -693,6 +695,20 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int q0, int rr, int
     if (a.lse && ch == 0) a.lse[t * a.l_t + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+// ---- adding up pieces ----
+// The pieces of a row of a 16-row tile are eight interleaved streams, each added
+// in order, and the streams a binary tree: the same sums whichever kernel adds
+// them and however many threads share a row.  A 256-row tile's few pieces are
+// added in order.
+struct Sum {
+    float m, l;
+    f32x4 o;
+};
+__device__ __forceinline__ Sum add(const Sum& x, const Sum& y) {
+    const float m = fmaxf(x.m, y.m), fx = fast_exp2(x.m - m), fy = fast_exp2(y.m - m);
+    return Sum{m, x.l * fx + y.l * fy, x.o * fx + y.o * fy};
+}
+
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int NT = 2;                    // cache policy bit: non-temporal (codes are read once)
 __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
@@ -717,7 +733,45 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 // TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
 // ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
 // on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
-// chain lengths -> table -> rows -> join: 12.6 us for one request of 8K keys.
+// chain lengths -> table -> rows -> pieces: 11.7 us for one request of 8K keys.
+constexpr int COUNTER_PAD = 32;          // a counter has a 128-byte line: arrivals at one line queue up
+constexpr int SC1 = 16;                  // cache policy bit: device scope
+
+// Streams s0 .. s0 + VS - 1 of a row's pieces at this lane's 4 channels: `o` and
+// `ml` describe the pieces' sums and (m, l), the lane's own at byte offsets
+// oat and mat, the next piece's ostep and mstep further (past the last one the
+// loads are out of range: zeros, no access).  `DEEP` pieces in flight.
+template <int VS, int DEEP, int POLICY, int STREAMS = 8>
+__device__ __forceinline__ Sum add_streams(Rsrc o, Rsrc ml, uint32_t oat, uint32_t mat, uint32_t ostep, uint32_t mstep,
+                                           int pieces, int s0) {
+    constexpr int RD = DEEP / VS;
+    Sum s[VS];
+#pragma unroll
+    for (int v = 0; v < VS; ++v) s[v] = Sum{M_INIT, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    for (int i0 = s0; i0 < pieces; i0 += STREAMS * RD) {
+        Sum x[RD][VS];
+#pragma unroll
+        for (int r = 0; r < RD; ++r)
+#pragma unroll
+            for (int v = 0; v < VS; ++v) {
+                const uint32_t p = static_cast<uint32_t>(i0 + STREAMS * r + v);
+                const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, mat + p * mstep, 0, POLICY));
+                x[r][v] = Sum{__uint_as_float(t[0]), __uint_as_float(t[1]),
+                              __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(o, oat + p * ostep, 0, POLICY))};
+            }
+#pragma unroll
+        for (int r = 0; r < RD; ++r)
+#pragma unroll
+            for (int v = 0; v < VS; ++v)
+                if (i0 + STREAMS * r + v < pieces) s[v] = add(s[v], x[r][v]);
+    }
+#pragma unroll
+    for (int d = 1; d < VS; d *= 2)
+#pragma unroll
+        for (int v = 0; v < VS; v += 2 * d) s[v] = add(s[v], s[v + d]);
+    return s[0];
+}
+
 template <int D>
 struct Raw {
     uint32_t k[2][D / 32];               // tile t: row c's channels (D/4) kb .. of token 16t + 4(c & 3) + (c >> 2)
@@ -728,7 +782,7 @@ struct Raw {
 };
 
 template <int D, bool F16>
-__global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel(AttnArgs a) {
     constexpr int TILE = Narrow::TILE, GROUP = Narrow::GROUP;
     constexpr int NB = D / 16;           // PV products per group
     constexpr int KW = D / 32;           // QK products (and K dwords) per tile
@@ -979,12 +1033,56 @@ __global__ __launch_bounds__(64 * WAVES, 3) void paged_attn_kernel(AttnArgs a) {
             l += f * redl[i][rw];
             o += f * *reinterpret_cast<const f32x4*>(&red[i][rw][ch]);
         }
-        if (it.part >= 0) {
+        if (it.part >= 0) {              // (device scope: another XCD's workgroup may read them in this launch)
             const int64_t slot = static_cast<int64_t>(it.part) * a.heads + head;
-            *reinterpret_cast<f32x4*>(a.part + (slot * TILE + rw) * D + ch) = o;
-            if (ch == 0) { a.ml[(slot * TILE + rw) * 2] = m; a.ml[(slot * TILE + rw) * 2 + 1] = l; }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), make_rsrc(a.part + slot * TILE * D, TILE * D * 4),
+                                                   (rw * D + ch) * 4, 0, SC1);
+            if (ch == 0) {
+                __hip_atomic_store(a.ml + (slot * TILE + rw) * 2, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(a.ml + (slot * TILE + rw) * 2 + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         } else {
             store_row<F16>(a, it.q0, it.row0 + rw, head, ch, m, l, o);
+        }
+    }
+    if (!a.counters || it.part < 0) return;
+
+    // ---- the tile's last workgroup adds up its pieces ----
+    // every store of this workgroup is acknowledged before its arrival is counted
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    __shared__ int last;
+    uint32_t* const counter = a.counters + (static_cast<int64_t>(it.join) * a.heads + head) * COUNTER_PAD;
+    if (tid == 0) {
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(it.pieces - 1);
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    constexpr int LG = 64 * WAVES / (D / 4);       // lane groups of a row
+    const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
+    const uint32_t pieces = it.pieces, ostep = a.heads * (TILE * D * 4), mstep = a.heads * (TILE * 2 * 4);
+    const int64_t slot0 = static_cast<int64_t>(it.part0) * a.heads + head;
+    const Rsrc ro = make_rsrc(a.part + slot0 * TILE * D, (pieces - 1) * ostep + TILE * D * 4);
+    const Rsrc rm = make_rsrc(a.ml + slot0 * TILE * 2, (pieces - 1) * mstep + TILE * 2 * 4);
+    if (nrows <= LG / 2) {               // two lane groups share a row
+        const int rw = g >> 1;
+        Sum s{M_INIT, 0.f, {0.f, 0.f, 0.f, 0.f}};
+        if (rw < nrows) s = add_streams<4, 8, SC1>(ro, rm, (rw * D + ch) * 4, rw * 8, ostep, mstep, it.pieces, 4 * (g & 1));
+        float* const other = &red[0][0][0] + rw * (D + 4) + ch;
+        if (g & 1) {
+            *reinterpret_cast<f32x4*>(other) = s.o;
+            if (ch == 0) { redm[0][rw] = s.m; redl[0][rw] = s.l; }
+        }
+        __syncthreads();
+        if (!(g & 1) && rw < nrows) {
+            s = add(s, Sum{redm[0][rw], redl[0][rw], *reinterpret_cast<const f32x4*>(other)});
+            store_row<F16>(a, it.q0, it.row0 + rw, head, ch, s.m, s.l, s.o);
+        }
+    } else {
+        for (int rw = g; rw < nrows; rw += LG) {
+            const Sum s = add_streams<8, 8, SC1>(ro, rm, (rw * D + ch) * 4, rw * 8, ostep, mstep, it.pieces, 0);
+            store_row<F16>(a, it.q0, it.row0 + rw, head, ch, s.m, s.l, s.o);
         }
     }
 }
@@ -1346,10 +1444,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 }
 
 // Adds up the pieces of the split tiles, of both kinds in one launch (`blocks`
-// of the grid take the short requests').  A workgroup takes JOIN_ROWS rows of a
-// tile and KV head after the other; a row is 4 channels a lane of D/4, and
-// while rows are fewer than the lane groups, several groups share a row's
-// pieces and meet in LDS.  Four pieces are in flight per group.  By zero_tail
+// of the grid take the short requests').  A workgroup takes some rows of a tile
+// and KV head after the other; a row is 4 channels a lane of D/4, and 4 or 8 lane
+// groups share the pieces of a short request's row and meet in LDS.  Four pieces are in flight per lane (with eight one
+// workgroup a CU is resident instead of two: 15 us instead of 7 beside chunks).  By zero_tail
 // it also clears the rows behind the last request.
 template <int D>
 struct JoinLds {
@@ -1361,10 +1459,8 @@ struct JoinLds {
 template <typename K, int D, bool F16>
 __device__ __forceinline__ void join_tiles(const AttnArgs& a, JoinLds<D>& L, int block, int blocks) {
     constexpr int LG = JoinLds<D>::LG;
-    constexpr int PARTS = K::TILE / K::JOIN_ROWS;  // of a tile
-    auto& so = L.so;
-    auto& sm = L.sm;
-    auto& sl = L.sl;
+    constexpr int ROWS = K::join_rows(LG), PARTS = K::TILE / ROWS;     // of a tile
+    constexpr bool NARROW = K::TILE == Narrow::TILE;
     const int tid = threadIdx.x;
     const int g = tid / (D / 4), ch = 4 * (tid - g * (D / 4));
     if (a.plan.max_joins == 0) return;   // (nothing can be cut, and where the kind has no tiles nobody wrote the counts)
@@ -1373,56 +1469,35 @@ __device__ __forceinline__ void join_tiles(const AttnArgs& a, JoinLds<D>& L, int
         const uint32_t rest = static_cast<uint32_t>(i) / a.heads;
         const int head = static_cast<uint32_t>(i) - rest * a.heads;
         const Join jn = a.plan.joins[rest / PARTS];
-        const int first = rest % PARTS * K::JOIN_ROWS, rows = min(K::JOIN_ROWS, jn.rows - first);
-        const int share = rows <= LG / 8 ? 8 : rows <= LG / 4 ? 4 : rows <= LG / 2 ? 2 : 1;
-        const int sub = g % share;
-        for (int r0 = 0; r0 < rows; r0 += LG / share) {
-            const int rw = r0 + g / share;
-            float m = M_INIT, l = 0.f;
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            if (rw < rows) {
-                constexpr int DEEP = 4;
-                for (int i0 = sub; i0 < jn.pieces; i0 += DEEP * share) {
-                    float mi[DEEP], li[DEEP];
-                    f32x4 oi[DEEP];
-#pragma unroll
-                    for (int j = 0; j < DEEP; ++j) {
-                        const int64_t at = ((static_cast<int64_t>(jn.part) + min(i0 + j * share, jn.pieces - 1)) * a.heads + head) * K::TILE + first + rw;
-                        mi[j] = a.ml[at * 2];
-                        li[j] = a.ml[at * 2 + 1];
-                        oi[j] = *reinterpret_cast<const f32x4*>(a.part + at * D + ch);
-                    }
-#pragma unroll
-                    for (int j = 0; j < DEEP; ++j) {
-                        if (i0 + j * share >= jn.pieces) break;
-                        const float mn = fmaxf(m, mi[j]), f = fast_exp2(m - mn), fi = fast_exp2(mi[j] - mn);
-                        o = o * f + oi[j] * fi;
-                        l = l * f + li[j] * fi;
-                        m = mn;
-                    }
-                }
-            }
-            if (share > 1) {             // (one round of this loop: rows <= LG / share)
-                *reinterpret_cast<f32x4*>(&so[g][ch]) = o;
-                if (ch == 0) { sm[g] = m; sl[g] = l; }
-                __syncthreads();
-                if (sub == 0) {
-                    for (int k = 1; k < share; ++k) {
-                        const float mn = fmaxf(m, sm[g + k]), f = fast_exp2(m - mn), fi = fast_exp2(sm[g + k] - mn);
-                        o = o * f + *reinterpret_cast<const f32x4*>(&so[g + k][ch]) * fi;
-                        l = l * f + sl[g + k] * fi;
-                        m = mn;
-                    }
-                }
-                __syncthreads();
-            }
-            if (sub == 0 && rw < rows) store_row<F16>(a, jn.q0, jn.row0 + first + rw, head, ch, m, l, o);
+        const int first = rest % PARTS * ROWS, rows = min(ROWS, jn.rows - first);
+        const int share = NARROW ? rows <= LG / 8 ? 8 : 4 : 1;         // lane groups of a row
+        const int sub = g % share, rw = g / share;
+        const uint32_t ostep = a.heads * (K::TILE * D * 4), mstep = a.heads * (K::TILE * 2 * 4);
+        const int64_t slot0 = static_cast<int64_t>(jn.part) * a.heads + head;
+        Sum s{M_INIT, 0.f, {0.f, 0.f, 0.f, 0.f}};
+        if (rw < rows) {
+            const Rsrc ro = make_rsrc(a.part + slot0 * K::TILE * D, (jn.pieces - 1) * ostep + K::TILE * D * 4);
+            const Rsrc rm = make_rsrc(a.ml + slot0 * K::TILE * 2, (jn.pieces - 1) * mstep + K::TILE * 2 * 4);
+            const uint32_t oat = ((first + rw) * D + ch) * 4, mat = (first + rw) * 8;
+            if (!NARROW) s = add_streams<1, 4, 0, 1>(ro, rm, oat, mat, ostep, mstep, jn.pieces, 0);
+            else if (share == 8) s = add_streams<1, 4, 0>(ro, rm, oat, mat, ostep, mstep, jn.pieces, sub);
+            else s = add_streams<2, 4, 0>(ro, rm, oat, mat, ostep, mstep, jn.pieces, 2 * sub);
         }
+        for (int d = 1; d < share; d *= 2) {
+            if (sub & d) {
+                *reinterpret_cast<f32x4*>(&L.so[g][ch]) = s.o;
+                if (ch == 0) { L.sm[g] = s.m; L.sl[g] = s.l; }
+            }
+            __syncthreads();
+            if (!(sub & (2 * d - 1))) s = add(s, Sum{L.sm[g + d], L.sl[g + d], *reinterpret_cast<const f32x4*>(&L.so[g + d][ch])});
+            __syncthreads();
+        }
+        if (sub == 0 && rw < rows) store_row<F16>(a, jn.q0, jn.row0 + first + rw, head, ch, s.m, s.l, s.o);
     }
 }
 
 template <int D, bool F16>
-__global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a, PlanArgs wide, float* wide_part, float* wide_ml, int blocks) {
+__global__ __launch_bounds__(JOIN_T, 8) void paged_join_kernel(AttnArgs a, PlanArgs wide, float* wide_part, float* wide_ml, int blocks) {
     __shared__ JoinLds<D> L;
     constexpr int LG = JoinLds<D>::LG;
     const int tid = threadIdx.x;
@@ -1450,7 +1525,7 @@ __global__ __launch_bounds__(JOIN_T) void paged_join_kernel(AttnArgs a, PlanArgs
 // host side
 // ---------------------------------------------------------------------------
 struct Sizes {
-    int64_t target, items, joins, parts;
+    int64_t target, wanted, most, items, joins, parts;   // most: pieces of a tile
     size_t off_counts, off_items, off_joins, off_part, off_ml, end;
 };
 
@@ -1466,14 +1541,14 @@ template <typename K>
 Sizes sizes_of(const hyq_paged_params& p, int64_t tiles, size_t at) {
     Sizes s{};
     s.target = std::max<int64_t>(1, K::slots(p.head_dim) / p.kv_heads);
-    const int64_t wanted = K::most(s.target, tiles);
+    s.wanted = K::most(s.target, tiles);
     const int64_t keys = static_cast<int64_t>(p.max_pages) * p.page_size;
     const int64_t units = (p.window > 0 ? std::min<int64_t>(keys, static_cast<int64_t>(p.window) + K::TILE) : keys) / K::GROUP + 2;
     // pieces of a tile (no piece is shorter than MIN_UNITS, no tile cut that is hardly longer)
-    const int64_t most = units <= K::MIN_UNITS * K::UNCUT ? 1 : (units + K::MIN_UNITS - 1) / K::MIN_UNITS;
-    s.items = tiles ? std::min(wanted + tiles, tiles * most) : 0;
-    s.joins = most > 1 ? std::min(tiles, wanted) : 0;
-    s.parts = s.joins ? std::min(s.items, 2 * wanted) : 0;
+    s.most = units <= K::MIN_UNITS * K::UNCUT ? 1 : (units + K::MIN_UNITS - 1) / K::MIN_UNITS;
+    s.items = tiles ? std::min(s.wanted + tiles, tiles * s.most) : 0;
+    s.joins = s.most > 1 ? std::min(tiles, s.wanted) : 0;
+    s.parts = s.joins ? std::min(s.items, 2 * s.wanted) : 0;
     s.off_counts = at;
     s.off_items = at + 256;
     s.off_joins = up256(s.off_items + s.items * sizeof(Item));
@@ -1518,6 +1593,7 @@ int check_attention(const hyq_paged_params* p) {
     if (int st = check_pool(w, p->head_dim, p->page_size, p->num_pages, p->kv_heads, p->k_pages, p->v_pages, p->k_scale, p->v_scale,
                             p->p_stride_page, p->p_stride_head, p->s_stride_page, p->s_stride_head))
         return st;
+    if (p->kv_heads > 1024) return fail(HYQ_ENOTSUP, s + "more than 1024 key heads");   // (32-bit offsets between a row's pieces)
     if (p->kv_repeat < 1 || p->kv_repeat > 1024) return fail(HYQ_ENOTSUP, s + "kv_repeat must be 1 to 1024");
     if (p->num_requests < 0 || p->num_tokens < 0 || p->max_pages < 0 || p->window < 0)
         return fail(HYQ_EINVAL, s + "negative size");
@@ -1537,8 +1613,8 @@ int check_attention(const hyq_paged_params* p) {
         return fail(HYQ_EINVAL, s + "q must be 16-byte aligned with strides divisible by 8");
     if (!aligned(p->out, 8) || p->o_stride_t % 4 || p->o_stride_h % 4)
         return fail(HYQ_EINVAL, s + "out must be 8-byte aligned with strides divisible by 4");
-    if (!aligned(p->seq_lens, 4) || !aligned(p->cu_seqlens, 4) || !aligned(p->block_table, 4) || !aligned(p->lse, 4))
-        return fail(HYQ_EINVAL, s + "lengths, table and lse must be 4-byte aligned");
+    if (!aligned(p->seq_lens, 4) || !aligned(p->cu_seqlens, 4) || !aligned(p->block_table, 4) || !aligned(p->lse, 4) || !aligned(p->counters, 4))
+        return fail(HYQ_EINVAL, s + "lengths, table, lse and counters must be 4-byte aligned");
     return HYQ_OK;
 }
 
@@ -1555,9 +1631,9 @@ int raise_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
 }
 
 // workgroups of a kind's joins, at most `most`
-template <typename K>
+template <typename K, int D>
 int64_t join_grid(const Sizes& s, int heads, int64_t most) {
-    return std::min<int64_t>(s.joins * heads * (K::TILE / K::JOIN_ROWS), most);
+    return std::min<int64_t>(s.joins * heads * (K::TILE / K::join_rows(JOIN_T / (D / 4))), most);
 }
 
 template <int D, bool F16>
@@ -1579,13 +1655,30 @@ int launch_attention(AttnArgs a, const PlanArgs& narrow, const PlanArgs& wide, c
     // a round of resident workgroups (two a CU) for the kind that there is, half
     // of one each where both may be
     const int64_t most = s.narrow.joins && s.wide.joins ? 256 : 512;
-    int64_t jn = join_grid<Narrow>(s.narrow, a.heads, most);
-    const int64_t jw = join_grid<Wide>(s.wide, a.heads, most);
+    int64_t jn = a.counters ? 0 : join_grid<Narrow, D>(s.narrow, a.heads, most);
+    const int64_t jw = join_grid<Wide, D>(s.wide, a.heads, most);
     if (a.zero_tail && a.plan.cu && jn + jw == 0) jn = 1;
     if (jn + jw)
         paged_join_kernel<D, F16><<<dim3(static_cast<unsigned>(jn + jw)), dim3(JOIN_T), 0, st>>>(
             a, wide, reinterpret_cast<float*>(ws + s.wide.off_part), reinterpret_cast<float*>(ws + s.wide.off_ml), static_cast<int>(jn));
     return check_launch("hyq_paged_attention");
+}
+
+// Whether the attention launch joins the pieces itself: a decode step (a ragged
+// call's join launch also clears rows) with counters, in no captured graph, whose
+// replays on another stream would share them.  One 8K sequence takes 11.6 us
+// instead of 13.8, 200 requests 28.7 instead of 30.8, one of 1K 10.0 instead of
+// 12.7; but where a request may be cut into more than 48 pieces, one workgroup
+// takes longer than the launch does (one 32K sequence 22.9, 20.5).
+bool join_here(const hyq_paged_params& p, const Both& s, hipStream_t st) {
+    if (!p.counters || p.cu_seqlens || s.wide.items || s.narrow.joins * p.kv_heads * COUNTER_PAD > HYQ_PAGED_COUNTERS) return false;
+    if (s.narrow.most > 48 && s.narrow.wanted > 48 * static_cast<int64_t>(p.num_requests)) return false;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return status == hipStreamCaptureStatusNone;
 }
 
 }  // namespace
@@ -1694,7 +1787,7 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
     const AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
                      p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head,
                      p->k_scale, p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, narrow, nullptr, nullptr,
-                     p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail,
+                     join_here(*p, s, st) ? p->counters : nullptr, p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail,
                      p->sm_scale * 1.44269504f};
     if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, narrow, wide, s, ws, st) : launch_attention<128, false>(a, narrow, wide, s, ws, st);
     return p->dtype_fp16 ? launch_attention<64, true>(a, narrow, wide, s, ws, st) : launch_attention<64, false>(a, narrow, wide, s, ws, st);

@@ -311,8 +311,8 @@ def _load_fast_ext():
             return False
         P, G = _lib.DecodeParams, _lib.PagedParams
         # (a build of earlier sources has no signatures())
-        if (getattr(m, "signatures", lambda: 0)() == 3 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset)
-                and m.paged_layout() == (ctypes.sizeof(G), G.num_pages.offset, G.zero_tail.offset)):
+        if (getattr(m, "signatures", lambda: 0)() == 4 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset)
+                and m.paged_layout() == (ctypes.sizeof(G), G.num_pages.offset, G.counters.offset)):
             L = _lib.lib()
             at = lambda *fs: (ctypes.cast(f, ctypes.c_void_p).value for f in fs)  # noqa: E731
             m.set_entry(*at(L.hyq_decode_hybrid, L.hyq_append_rows))

@@ -23,7 +23,8 @@ A step of a serving program:
 
 Nothing is read back to the host, so a captured graph of a step follows the
 lengths it is replayed with.  Every call allocates its own outputs and
-workspace on the current stream.  Inference only: no gradients.
+workspace on the current stream; 256 KiB of arrival counters are kept
+per stream.  Inference only: no gradients.
 """
 
 from __future__ import annotations
@@ -58,6 +59,23 @@ def _fast(t: torch.Tensor):
     if fx and isinstance(t, torch.Tensor) and t.is_cuda:
         return fx, _stream(t.device)
     return None, 0
+
+
+_counts = {}                               # (device, stream) -> arrival counters of the calls on that stream
+
+
+def _counters(device: torch.device, stream: int) -> int:
+    """The address of the arrival counters of eager calls on `stream`, zero
+    between calls; 0 while the stream is being captured and has none yet (the
+    library uses them in no captured call: a graph may be replayed beside
+    eager calls)."""
+    c = _counts.get((device.index, stream))
+    if c is None:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return 0
+            c = _counts.setdefault((device.index, stream), torch.zeros(_lib.PAGED_COUNTERS, dtype=torch.int32, device=device))
+    return c.data_ptr()
 
 
 def _ints(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: torch.device) -> None:
@@ -247,7 +265,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if fx and out is None:
         try:
             st, o, lse = fx.paged_attention(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens,
-                                            sm_scale, window, return_lse, stream)
+                                            sm_scale, window, return_lse, stream, 0 if cu_seqlens is not None else _counters(q.device, stream))
             if st == 0:
                 return (o, lse) if return_lse else o
         except TypeError:
@@ -299,6 +317,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         p.kv_heads, p.kv_repeat, p.head_dim, p.window = H, HQ // H, D, window
         p.sm_scale = D ** -0.5 if sm_scale is None else sm_scale
         p.dtype_fp16, p.zero_tail = int(q.dtype == torch.float16), 3 if zero_tail else 2
+        if cu_seqlens is None:
+            p.counters = _counters(dev, _stream(dev)) or None
         L = _lib.lib()
         ref = ctypes.byref(p)
         need = L.hyq_paged_attention_workspace_size(ref)

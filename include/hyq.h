@@ -482,7 +482,13 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  * are, but with bit 0 of zero_tail out is set to 0 there, with bit 1 lse to -inf.
  * The workspace needs no initialisation; calls that share one must be ordered
  * on one stream.
+ *   counters  NULL, or uint32 [HYQ_PAGED_COUNTERS] that are zero before the first call; every
+ *             completed call leaves them at zero, and calls that share them must be ordered
+ *             on one stream.  A call without cu_seqlens on a stream that is not being
+ *             captured then needs no launch of its own for the pieces of cut requests; other
+ *             calls leave them alone.  The results are the same bit for bit.
  */
+#define HYQ_PAGED_COUNTERS 65536
 typedef struct hyq_paged_params {
     const void* q; int64_t q_stride_t, q_stride_h;
     void* out; int64_t o_stride_t, o_stride_h;
@@ -497,6 +503,7 @@ typedef struct hyq_paged_params {
     int32_t kv_heads, kv_repeat, head_dim, window;
     float sm_scale;
     int32_t dtype_fp16, zero_tail;
+    uint32_t* counters;
 } hyq_paged_params;
 
 size_t hyq_paged_attention_workspace_size(const hyq_paged_params* p);

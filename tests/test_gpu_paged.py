@@ -672,3 +672,28 @@ def test_window_past_32_bits_and_shared_outputs():
             hq.paged_attention(q, *pool, table, lens, out=out)
     with pytest.raises(ValueError, match="num_tokens"):
         hq.paged_batch(lens, lens, table, lens, 16, 1 << 31)
+
+
+@pytest.mark.parametrize("dtype,D,H,G,seq,window", [(BF16, 128, 8, 4, [8192], 0), (FP16, 64, 2, 16, [9000, 3, 700, 0, 5001], 0),
+                                                    (BF16, 128, 1, 1, [20000], 0), (FP16, 128, 3, 7, [4000] * 70, 1500),
+                                                    (BF16, 64, 4, 9, [100 + 90 * i for i in range(300)], 0),
+                                                    (BF16, 128, 2, 13, [6000, 11, 2000], 0)])
+def test_pieces_joined_by_either_launch(dtype, D, H, G, seq, window, monkeypatch):
+    """A cut request's pieces are added up by its last workgroup, or by a launch
+    of their own where a call has no counters: the same bits, also lse, and
+    the counters are zero again."""
+    from hyquant_amd import paged
+    g = _gen(60)
+    table, pages = U.make_table(g, seq, 16, "cuda")
+    pool = U.make_pool(g, pages, H, 16, D, "cuda")
+    q = torch.randn(len(seq), H * G, D, generator=g, device="cuda").to(dtype)
+    lens = _i32(seq)
+    got = [hq.paged_attention(q, *pool, table, lens, window=window, return_lse=True) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert paged._counts and all(bool((c == 0).all()) for c in paged._counts.values())
+    monkeypatch.setattr(paged, "_counters", lambda *_: 0)
+    out, lse = hq.paged_attention(q, *pool, table, lens, window=window, return_lse=True)
+    for o, x in got:
+        assert torch.equal(o, out) and torch.equal(x, lse)
+    ref, ref_lse, tol = U.reference(q, pool, table, seq, [1] * len(seq), window)
+    U.check(out, ref, tol)

@@ -106,3 +106,11 @@ def test_pool_checks():
     with pytest.raises(ValueError, match="GPU"):
         paged.paged_attention(torch.zeros(1, 2, 64, dtype=torch.bfloat16), *pool, torch.zeros(1, 1, dtype=torch.int32),
                               torch.ones(1, dtype=torch.int32))
+
+
+def test_attention_limits_of_heads_and_counters():
+    _lib, L = _L()
+    assert L.hyq_paged_attention_workspace_size(_params(_lib, kv_heads=1024)) > 0
+    for bad, code in ((dict(kv_heads=1025), _lib.HYQ_ENOTSUP), (dict(counters=4097), _lib.HYQ_EINVAL)):
+        assert L.hyq_paged_attention_workspace_size(_params(_lib, **bad)) == 0, bad
+        assert L.hyq_paged_attention(_params(_lib, **bad), 4096, 1 << 40, None) == code, bad
