@@ -697,3 +697,36 @@ def test_pieces_joined_by_either_launch(dtype, D, H, G, seq, window, monkeypatch
         assert torch.equal(o, out) and torch.equal(x, lse)
     ref, ref_lse, tol = U.reference(q, pool, table, seq, [1] * len(seq), window)
     U.check(out, ref, tol)
+
+
+def test_captured_decode_replayed_beside_eager_calls():
+    """A graph captured on a stream that has arrival counters leaves them alone:
+    its replays on another stream run beside eager calls on that one."""
+    from hyquant_amd import paged
+    g = _gen(70)
+    seq, H, G, D = [9000, 5000, 3001], 2, 8, 128
+    table, pages = U.make_table(g, seq, 16, "cuda")
+    pool = U.make_pool(g, pages, H, 16, D, "cuda")
+    lens = _i32(seq)
+    qa, qb = (torch.randn(3, H * G, D, generator=g, device="cuda").to(BF16) for _ in range(2))
+    want_a, want_b = (hq.paged_attention(x, *pool, table, lens).clone() for x in (qa, qb))
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        hq.paged_attention(qa, *pool, table, lens)
+    torch.cuda.synchronize()
+    assert (0, s.cuda_stream) in paged._counts
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        captured = [hq.paged_attention(qa, *pool, table, lens) for _ in range(4)]
+    for _ in range(5):
+        for x in captured:
+            x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(t):
+            graph.replay()
+        with torch.cuda.stream(s):
+            eager = [hq.paged_attention(qb, *pool, table, lens) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want_a) for x in captured) and all(torch.equal(x, want_b) for x in eager)
+    assert all(bool((c == 0).all()) for c in paged._counts.values())
