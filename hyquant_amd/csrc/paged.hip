@@ -725,11 +725,16 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 //   softmax: a row's maximum moves only when a score passes it by SLACK (its own
 //       scores alone move it), sums in fp32.
 //   PV  O^T[channel][row] = V^T . P'^T with v_mfma_f32_16x16x32_bf16, V operands
-//       the bf16 numbers 128 + u, P' = bf16(p v_scale): 136 sum(P') is taken off
-//       at the end, from the same rounded P' by a product with ones.  That
-//       rounding (2^-8 of a weight, random over keys) is the one between scores
-//       and output; an fp16 model's P' is the sum of two bf16 numbers.
-// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 97 us, 5.7
+//       the bf16 numbers 128 + u, P' = bf16(p v_scale): 136 sum(P') is taken
+//       off every 96 keys of a wavefront, from the same rounded P' by a product
+//       with ones.  The running sum carries up to 140 times those keys' weights,
+//       and its fp32 roundings stay in the result: taken off at the end alone
+//       they made a relative error of 2.4e-3 over 32K keys in one piece, where an
+//       fp16 output's own rounding is 2.1e-4 (and so is the error now, for 1% of
+//       the time).  The rounding of P' (2^-8 of a weight, random over keys) is
+//       the one between scores and output; an fp16 model's P' is the sum of two
+//       bf16 numbers.
+// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 99 us, 5.6
 // TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
 // ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
 // on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
@@ -1006,6 +1011,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         if (i + 1 < mine) compute(ring[1]);
         load(ring[1], i + 4);
         if (i + 2 < mine) compute(ring[2]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)  // the codes' offset
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[nb][j] = __builtin_fmaf(-136.0f, ones[j], acc[nb][j]);
+        ones = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     // ---- the four wavefronts' results, joined through LDS ----
@@ -1017,7 +1027,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         for (int i = 0; i < 4; ++i) {
             const int j = 4 * kb + i;
             const int ch = D == 128 ? 8 * j + nb : 8 * (j & 7) + 4 * (j >> 3) + nb;
-            red[w][c][ch] = acc[nb][i] - 136.0f * ones[i];
+            red[w][c][ch] = acc[nb][i];
         }
     __syncthreads();
     for (int e = tid; e < nrows * (D / 4); e += 64 * WAVES) {
