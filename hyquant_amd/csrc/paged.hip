@@ -725,16 +725,16 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 //   softmax: a row's maximum moves only when a score passes it by SLACK (its own
 //       scores alone move it), sums in fp32.
 //   PV  O^T[channel][row] = V^T . P'^T with v_mfma_f32_16x16x32_bf16, V operands
-//       the bf16 numbers 128 + u, P' = bf16(p v_scale): 136 sum(P') is taken
-//       off every 96 keys of a wavefront, from the same rounded P' by a product
-//       with ones.  The running sum carries up to 140 times those keys' weights,
-//       and its fp32 roundings stay in the result: taken off at the end alone
-//       they made a relative error of 2.4e-3 over 32K keys in one piece, where an
-//       fp16 output's own rounding is 2.1e-4 (and so is the error now, for 1% of
-//       the time).  The rounding of P' (2^-8 of a weight, random over keys) is
-//       the one between scores and output; an fp16 model's P' is the sum of two
-//       bf16 numbers.
-// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 99 us, 5.6
+//       the bf16 numbers 128 + u, P' = p v_scale as the sum of two bf16 numbers
+//       (2^-16 of a weight is lost; one bf16 number, 2^-8, made a bf16 output's
+//       error 2.4e-3 where its own rounding is 1.7e-3, and was 4% faster):
+//       136 sum(P') is taken off every 96 keys of a wavefront, from the same
+//       rounded P' by products with ones.  The running sum carries up to 140
+//       times those keys' weights, and its fp32 roundings stay in the result:
+//       taken off at the end alone they made a relative error of 2.4e-3 over 32K
+//       keys in one piece, where an fp16 output's own rounding is 2.1e-4 (1% of
+//       the time).  Outputs of either type are then as good as their type.
+// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 103 us, 5.4
 // TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
 // ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
 // on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
@@ -974,13 +974,10 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         }
         const u32x4 pw = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
         const bf16x8 pop = __builtin_bit_cast(bf16x8, pw);
-        bf16x8 plo;
-        if constexpr (F16) {             // an fp16 model's output keeps 11 bits: P' as the sum of two bf16 numbers
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] -= half_at<false>(pw[i >> 1], i & 1);
-            const u32x4 pl = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
-            plo = __builtin_bit_cast(bf16x8, pl);
-        }
+        for (int i = 0; i < 8; ++i) p[i] -= half_at<false>(pw[i >> 1], i & 1);
+        const u32x4 pl = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+        const bf16x8 plo = __builtin_bit_cast(bf16x8, pl);
         uint32_t vlo[4], vhi[4];
 #pragma unroll
         for (int pr = 0; pr < 4; ++pr) {
@@ -998,11 +995,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
             const int sh = 4 * (nb & 3);
             const u32x4 o = {nib2(src[0], sh, 0x43084308u), nib2(src[1], sh, 0x43084308u), nib2(src[2], sh, 0x43084308u), nib2(src[3], sh, 0x43084308u)};
             acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), pop, acc[nb], 0, 0, 0);
-            if constexpr (F16) acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), plo, acc[nb], 0, 0, 0);
+            acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), plo, acc[nb], 0, 0, 0);
         }
         const u32x4 onesw = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
         ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), pop, ones, 0, 0, 0);
-        if constexpr (F16) ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), plo, ones, 0, 0, 0);
+        ones = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, onesw), plo, ones, 0, 0, 0);
     };
     for (int i = 0; i < mine; i += 3) {
         load(ring[2], i + 2);

@@ -469,8 +469,8 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  * A row that sees no key is 0 (lse -inf).  The codes enter the products as
  * exact operands: the K scale multiplies the fp32 score, the V scale the
  * weight, which is then rounded once: for requests of at most 16 rows (tokens
- * times kv_repeat) to bf16, of an fp16 model to the sum of two bf16 numbers,
- * for larger requests to fp16.
+ * times kv_repeat) to the sum of two bf16 numbers (2^-16), for larger requests
+ * to fp16 (2^-11).
  *   q     bf16 or fp16 [num_tokens, kv_heads * kv_repeat, head_dim] strides (t, h, 1),
  *         16-byte aligned, strides divisible by 8; out the same type, 8-byte aligned,
  *         strides divisible by 4
