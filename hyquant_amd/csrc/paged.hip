@@ -1783,8 +1783,11 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
     if (!aligned(workspace, 256)) return fail(HYQ_EINVAL, "hyq_paged_attention: workspace must be 256-byte aligned");
     char* ws = static_cast<char*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
+    // no table row names 2^30 tokens: such a window hides nothing, and position -
+    // window stays within 32 bits also for tokens before position 0
+    const int32_t window = p->window < (1 << 30) ? p->window : 0;
     auto plan_of = [&](const Sizes& z) {
-        return PlanArgs{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, p->window, p->max_pages * p->page_size,
+        return PlanArgs{p->seq_lens, p->cu_seqlens, p->num_requests, p->num_tokens, p->kv_repeat, window, p->max_pages * p->page_size,
                         static_cast<int32_t>(z.target), static_cast<int32_t>(z.items),
                         static_cast<int32_t>(z.parts), static_cast<int32_t>(z.joins), reinterpret_cast<Counts*>(ws + z.off_counts),
                         reinterpret_cast<Item*>(ws + z.off_items), reinterpret_cast<Join*>(ws + z.off_joins)};
@@ -1794,7 +1797,7 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
     const AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
                      p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head,
                      p->k_scale, p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, narrow, nullptr, nullptr,
-                     join_here(*p, s, st) ? p->counters : nullptr, p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), p->window, p->zero_tail,
+                     join_here(*p, s, st) ? p->counters : nullptr, p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), window, p->zero_tail,
                      p->sm_scale * 1.44269504f};
     if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, narrow, wide, s, ws, st) : launch_attention<128, false>(a, narrow, wide, s, ws, st);
     return p->dtype_fp16 ? launch_attention<64, true>(a, narrow, wide, s, ws, st) : launch_attention<64, false>(a, narrow, wide, s, ws, st);

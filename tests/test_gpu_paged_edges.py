@@ -1,0 +1,44 @@
+"""Calls of the paged operators at the edges of what they allow."""
+
+import math
+
+import pytest
+import torch
+
+import hyquant_amd as hq
+from hyquant_amd import decode_d_stage as dd
+from tests import paged_util as U
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _cu(new):
+    return _i32([0] + torch.tensor(new, dtype=torch.int64).cumsum(0).tolist())
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("G,R", [(1, 2), (4, 2), (4, 300)])
+def test_largest_windows_and_rows_before_position_0(native, G, R, monkeypatch):
+    """More new tokens than cached ones under windows that hide nothing: the same
+    as without a window, in short tiles and long ones and by both forms of the call."""
+    if not native:
+        monkeypatch.setattr(dd, "_FX", False)
+    g, page = _gen(1), 16
+    seq, new = [5, 40] + [7] * (R - 2), [10, 300] + [12] * (R - 2)
+    table, pages = U.make_table(g, seq, page, "cuda")
+    pool = U.make_pool(g, pages, 2, page, 64, "cuda")
+    q = torch.randn(sum(new), 2 * G, 64, generator=g, device="cuda").to(BF16)
+    want, want_lse = hq.paged_attention(q, *pool, table, _i32(seq), _cu(new), return_lse=True)
+    assert bool((want[5:10] != 0).any(-1).all()) and bool(torch.isfinite(want_lse[5:10]).all())
+    for window in (1 << 20, (1 << 30) - 1, 1 << 30, (1 << 31) - 257, (1 << 31) - 2, (1 << 31) - 1, 1 << 40):
+        out, lse = hq.paged_attention(q, *pool, table, _i32(seq), _cu(new), window=window, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), window
