@@ -147,15 +147,19 @@ __global__ __launch_bounds__(BT) void paged_batch_kernel(BatchArgs a) {
         if (tid == 0) a.used[0] = base_p;
     }
     // the pages taken: entry i of the free list goes to request r at table
-    // column ceil(ctx / page) + i - first[r]
-    for (int i = blockIdx.x * BT + tid; i < base_p; i += gridDim.x * BT) {
+    // column ceil(ctx / page) + i - first[r].  (Both loops count without a sign:
+    // a step past a count below 2^31 does not wrap.)
+    const uint32_t start = blockIdx.x * BT + tid, stride = gridDim.x * BT;
+    for (uint32_t u = start; u < static_cast<uint32_t>(max(base_p, 0)); u += stride) {
+        const int i = static_cast<int>(u);
         const int r = last_at_most(first, a.R - 1, i);
         const int col = ceil_pages(max(a.ctx[r], 0), a.page_log2) + i - first[r];
         if (static_cast<uint32_t>(col) < static_cast<uint32_t>(a.max_pages))
             a.table[r * a.bt_stride + col] = i < a.num_free ? a.free_pages[i] : -1;
     }
     const int page = 1 << a.page_log2;
-    for (int t = blockIdx.x * BT + tid; t < a.tokens; t += gridDim.x * BT) {
+    for (uint32_t u = start; u < static_cast<uint32_t>(a.tokens); u += stride) {
+        const int t = static_cast<int>(u);
         int64_t slot = -1, pos = -1;
         if (t < base_t) {
             const int r = last_at_most(cu, a.R - 1, t);

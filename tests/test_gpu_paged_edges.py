@@ -42,3 +42,16 @@ def test_largest_windows_and_rows_before_position_0(native, G, R, monkeypatch):
     for window in (1 << 20, (1 << 30) - 1, 1 << 30, (1 << 31) - 257, (1 << 31) - 2, (1 << 31) - 1, 1 << 40):
         out, lse = hq.paged_attention(q, *pool, table, _i32(seq), _cu(new), window=window, return_lse=True)
         assert torch.equal(out, want) and torch.equal(lse, want_lse), window
+
+
+def test_batch_layout_of_most_tokens():
+    """Token tensors of 2^31 - 1 entries, nearly all of them padding."""
+    T = 2 ** 31 - 1
+    table = _i32([[3, -1], [7, -1]])
+    b = hq.paged_batch(_i32([14, 0]), _i32([4, 2]), table, _i32([5, 9]), 16, T)
+    assert b.slots.shape == b.positions.shape == (T,)
+    assert b.slots[:8].tolist() == [62, 63, 80, 81, 144, 145, -1, -1] and b.positions[:8].tolist() == [14, 15, 16, 17, 0, 1, -1, -1]
+    for x in (b.slots, b.positions):
+        for part in x[6:].split(1 << 28):
+            assert bool((part == -1).all())
+    assert table.tolist() == [[3, 5], [9, -1]] and b.cu_seqlens.tolist() == [0, 4, 6] and b.pages_used.tolist() == [2]
