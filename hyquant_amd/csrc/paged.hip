@@ -1712,6 +1712,9 @@ extern "C" int hyq_paged_batch(const int32_t* context_lens, const int32_t* new_l
     if (!aligned(context_lens, 4) || !aligned(new_lens, 4) || !aligned(block_table, 4) || !aligned(free_pages, 4) ||
         !aligned(cu_seqlens, 4) || !aligned(seq_lens, 4) || !aligned(pages_used, 4) || !aligned(slots, 8) || !aligned(positions, 8))
         return fail(HYQ_EINVAL, "hyq_paged_batch: misaligned pointer");
+    // (a request's new entries would be written over another's)
+    if (num_requests > 1 && bt_stride < max_pages && bt_stride > -static_cast<int64_t>(max_pages))
+        return fail(HYQ_EINVAL, "hyq_paged_batch: rows of block_table share memory");
     BatchArgs a{context_lens, new_lens, block_table, bt_stride, free_pages, cu_seqlens, seq_lens, pages_used, slots, positions,
                 num_requests, max_pages, num_free, log2i(page_size), num_tokens};
     const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(512, 1 + (static_cast<int64_t>(num_tokens) - 1) / BATCH_TOKENS));

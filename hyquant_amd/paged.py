@@ -104,7 +104,8 @@ def paged_batch(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table:
 
     block_table (int32 [R, max_pages]) is extended in place: the entries of
     the pages that a request newly needs are taken from free_pages (int32),
-    in order, request by request; the others are left as they are.  num_tokens
+    in order, request by request; the others are left as they are (its rows
+    must not share memory).  num_tokens
     is the length of the token tensors of the step, at least the new tokens'
     sum; the slots and positions behind that sum are -1.  Where free_pages or
     max_pages do not suffice, the missing entries and their tokens' slots are

@@ -417,7 +417,7 @@ int hyq_prefill_unified(const hyq_prefill_params* params, void* workspace, size_
  *                           tokens that this step adds (0 allowed); negative counts as 0
  *   block_table  int32 [num_requests, max_pages] stride bt_stride: entries of the pages that a
  *                request holds are read; the entries [ceil(ctx / page), ceil((ctx + new) /
- *                page)) are written, the others left as they are
+ *                page)) are written, the others left as they are; its rows share no memory
  *   free_pages   int32 [num_free]: page ids, taken in order, request by request
  * writes
  *   cu_seqlens   int32 [num_requests + 1]  prefix sums of new_lens

@@ -55,3 +55,19 @@ def test_batch_layout_of_most_tokens():
         for part in x[6:].split(1 << 28):
             assert bool((part == -1).all())
     assert table.tolist() == [[3, 5], [9, -1]] and b.cu_seqlens.tolist() == [0, 4, 6] and b.pages_used.tolist() == [2]
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_batch_tables_whose_rows_share_memory(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(dd, "_FX", False)
+    lens, free = _i32([3, 3]), _i32([5, 6, 7, 8])
+    flat = torch.full((8,), -1, dtype=torch.int32, device="cuda")
+    for table in (flat[:4].expand(2, 4), flat.as_strided((2, 4), (3, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            hq.paged_batch(lens, lens, table, free, 16, 6)
+    assert bool((flat == -1).all())
+    b = hq.paged_batch(lens[:1], lens[:1], flat[:4].expand(1, 4), free, 16, 3)      # one row shares it with none
+    assert b.slots.tolist() == [-1] * 3                                               # (its held page is entry -1)
+    b = hq.paged_batch(lens, lens, flat.as_strided((2, 1), (1, 1)), free, 16, 6)
+    assert b.cu_seqlens.tolist() == [0, 3, 6]
