@@ -1341,8 +1341,9 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         if (j0 + 31 > all_hi || j0 < all_lo || __builtin_amdgcn_readfirstlane(__float_as_int(ve)) >= __float_as_int(BAD / 2)) {
             // the row's bound is over the V scales that it sees, so that what
             // is hidden from a row does not touch its bits; a row that sees a
-            // scale that is not finite is NaN
+            // scale that is not finite is NaN (its lse is not: l stays)
             float vx = 0.f;
+            bool nan = false;
             mx = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -1357,10 +1358,16 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                     t[4 * g + i] = seen ? t[4 * g + i] : -INFINITY;
                     mx = fmaxf(mx, t[4 * g + i]);
                     vx = fmaxf(vx, seen ? fabsf(v4[i]) : 0.f);
-                    if (seen && ((bad >> i) & 1)) l_run = __builtin_nanf("");
+                    nan |= seen && ((bad >> i) & 1);
                 }
             }
             ve = scale_bound(xmax32(vx));
+            if (__builtin_amdgcn_ballot_w64(nan)) {
+                const auto both = __builtin_amdgcn_permlane32_swap(nan, nan, false, false);      // (a row's two lanes)
+                const float z = both[0] | both[1] ? __builtin_nanf("") : 0.f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] += z;
+            }
         }
         mx += ve;
         // (a row's own scores alone decide whether its reference moves)

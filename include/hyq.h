@@ -466,7 +466,8 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  * is at position p = seq_lens[r] - (its tokens) + i and sees the keys j <= p,
  * with window > 0 only those with j > p - window:
  *   out = softmax_j(sm_scale q . k_j) v_j,  lse = ln sum_j exp(sm_scale q . k_j)
- * A row that sees no key is 0 (lse -inf).  The codes enter the products as
+ * A row that sees no key is 0 (lse -inf); one that sees a V scale that is not
+ * finite is NaN in every channel, its lse as ever.  The codes enter the products as
  * exact operands: the K scale multiplies the fp32 score, the V scale the
  * weight, which is then rounded once: for requests of at most 16 rows (tokens
  * times kv_repeat) to the sum of two bf16 numbers (2^-16), for larger requests

@@ -71,3 +71,28 @@ def test_batch_tables_whose_rows_share_memory(native, monkeypatch):
     assert b.slots.tolist() == [-1] * 3                                               # (its held page is entry -1)
     b = hq.paged_batch(lens, lens, flat.as_strided((2, 1), (1, 1)), free, 16, 6)
     assert b.cu_seqlens.tolist() == [0, 3, 6]
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,seq,new,window", [(128, [700, 90], [1, 1], 0), (128, [700, 90], [65, 40], 0), (64, [9000, 300], [80, 80], 0),
+                                              (64, [9000, 300], [1, 1], 500), (128, [30, 200], [40, 200], 64)])
+def test_v_scales_that_are_not_finite(bad, D, seq, new, window):
+    """A row that sees one is NaN, in short requests, long ones and cut ones; its lse
+    does not depend on V, and other rows and heads are left alone."""
+    g, page, H, G = _gen(3), 16, 2, 4
+    table, pages = U.make_table(g, seq, page, "cuda")
+    pool = U.make_pool(g, pages, H, page, D, "cuda")
+    q = torch.randn(sum(new), H * G, D, generator=g, device="cuda").to(BF16)
+    want, want_lse = hq.paged_attention(q, *pool, table, _i32(seq), _cu(new), window=window, return_lse=True)
+    at = max(seq[0] - new[0] // 2 - 5, 0)                # request 0's key of head 1
+    vs = pool[3].clone()
+    vs[table[0, at // page], 1, at % page] = bad
+    out, lse = hq.paged_attention(q, *pool[:3], vs, table, _i32(seq), _cu(new), window=window, return_lse=True)
+    pos = seq[0] - new[0] + torch.arange(new[0], device="cuda")
+    sees = (pos >= at) & ((pos < at + window) if window else True)
+    assert bool(sees.any())
+    hit = torch.zeros(sum(new), H * G, dtype=torch.bool, device="cuda")
+    hit[:new[0], G:] = sees[:, None]
+    assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
+    # (the rows' references differ: fp32 roundings of m and log2 l)
+    assert bool(((lse - want_lse)[hit].abs() <= 2.0 ** -20 * (1 + want_lse[hit].abs())).all())
