@@ -1109,9 +1109,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
 //       score in the fma that subtracts the reference: t = S k_scale - M.
 //   PV  O^T[channel][row] = V^T . P'^T, P' = fp16(2^t v_scale) against the exact
 //       codes, V^T by transposing LDS reads.  The reference M of a row follows
-//       max(score + log2 of the block's largest V scale), so that P' keeps to
-//       [0, 2^13] whatever the scales are; rounding P' to 11 bits once is the
-//       only rounding between the scores and the output.
+//       max(score) + log2 of the largest V scale of 16 keys, so that P' keeps to
+//       [0, 2^13]; rounding P' to 11 bits once is the only rounding between the
+//       scores and the output.  Where the 16 scales do not lie within a factor of
+//       2^9, the largest may be another key's than the largest score's, and M so
+//       high that P' sinks below fp16's 2^-14: there M follows max(score + log2 V
+//       scale), key by key.
 // Bound by the matrix pipe and the VALU work that has to run beside it: 2048
 // tokens at 8192 (309 GFLOP) take 358 us, 0.86 PFLOP/s where a large matrix
 // product reaches 1.35, and the products with their LDS reads alone take 226 us.
@@ -1131,6 +1134,7 @@ constexpr float SLACK_W = 6.0f;
 constexpr int BLK = 64;                  // keys per block
 constexpr int BUFS = 3;                  // blocks in LDS
 constexpr float BAD = 4096.0f;
+constexpr float FAR = 8.0f;              // binary orders that the V scales of 16 keys may span
 
 __device__ __forceinline__ uint32_t pk_sub1032(uint32_t x) {
     const f16x2 b = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
@@ -1156,14 +1160,16 @@ struct ChunkLds {
     uint8_t v[BUFS][BLK * VROW<D>];
     float ks[BUFS][BLK];                 // K scale * qk
     float vs[BUFS][BLK];                 // V scale, 0 where it is not finite or not to be looked at
-    float ve[BUFS][4];                   // per 16-key tile: log2 bound of vs, BAD more if a key needs care
+    float ve[BUFS][4];                   // per 16-key tile: log2 bound of vs, BAD more if the keys need care
     uint32_t care[BUFS][4];              // bits 0..15: keys whose V scale is not finite; bit 16: the page is in the pool
     float red[CHUNK_WAVES];
 };
 
-// e with x < 2^e, x >= 0 finite
+// e with x < 2^e, x >= 0 finite (an fp16 value: at least 2^-24, or 0, which takes
+// a bound so low that it does not count beside others, and that 2^30 weights of
+// 2^(12 + 79) do not overflow)
 __device__ __forceinline__ float scale_bound(float x) {
-    return static_cast<float>(static_cast<int>(__float_as_uint(fmaxf(x, 0x1p-24f)) >> 23) - 126);
+    return static_cast<float>(__builtin_amdgcn_frexp_expf(fmaxf(x, 0x1p-80f)));
 }
 
 template <int D, bool F16>
@@ -1266,10 +1272,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             const bool bad = live && !(fabsf(f) < INFINITY);
             const float x = live && !bad ? f : 0.f;
             const uint32_t mask = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(bad));
-            const float most = max16_dpp(fabsf(x));
+            const float e = scale_bound(fabsf(x)), most = max16_dpp(e), least = -max16_dpp(-e);
             if (lane < 16) L.vs[b][16 * tile + lane] = x;
             if (lane == 0) {
-                L.ve[b][tile] = scale_bound(most) + (mask || !sok ? BAD : 0.f);
+                L.ve[b][tile] = most + (mask || !sok || most - least > FAR ? BAD : 0.f);
                 L.care[b][tile] = mask | (sok ? 1u << 16 : 0u);
             }
         } else if (lane < 16) {
@@ -1320,7 +1326,8 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                                                                 acc[d], 0, 0, 0);
         }
     };
-    // t = scale * S - reference (0 while the row has seen no key); the lane's largest
+    // t = scale * S - reference (0 while the row has seen no key); the lane's
+    // largest + log2 of the largest V scale, 16-key tile by tile (t[0..7], t[8..15])
     auto scores = [&](int b, int x, float m_use) __attribute__((always_inline)) -> float {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -1328,40 +1335,41 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 #pragma unroll
             for (int i = 0; i < 4; ++i) t[4 * g + i] = __builtin_fmaf(sc[4 * g + i], k4[i], -m_use);
         }
-        float mx = vmax3(t[0], t[1], t[2]);
+        float mx[2];
 #pragma unroll
-        for (int i = 3; i < 15; i += 2) mx = vmax3(mx, t[i], t[i + 1]);
-        return vmax2(mx, t[15]);
+        for (int i = 0; i < 2; ++i) {
+            const float* u = t + 8 * i;
+            mx[i] = vmax3(vmax3(u[0], u[1], u[2]), u[3], u[4]);
+            mx[i] = vmax2(vmax3(mx[i], u[5], u[6]), u[7]) + L.ve[b][2 * x + i];
+        }
+        return vmax2(mx[0], mx[1]);
     };
     // hides what the rows do not see, and raises their reference where a
     // score passes it
     auto settle = [&](int b, int x, int blk, float mx, float m_use, bool unset) __attribute__((always_inline)) {
         const int j0 = it.key0 + BLK * blk + 32 * x;
-        float ve = fmaxf(L.ve[b][2 * x], L.ve[b][2 * x + 1]);
+        const float ve = fmaxf(L.ve[b][2 * x], L.ve[b][2 * x + 1]);
         if (j0 + 31 > all_hi || j0 < all_lo || __builtin_amdgcn_readfirstlane(__float_as_int(ve)) >= __float_as_int(BAD / 2)) {
             // the row's bound is over the V scales that it sees, so that what
             // is hidden from a row does not touch its bits; a row that sees a
             // scale that is not finite is NaN (its lse is not: l stays)
-            float vx = 0.f;
             bool nan = false;
             mx = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 v4 = *reinterpret_cast<const f32x4*>(&L.vs[b][32 * x + 8 * g + 4 * h]);
-                const uint32_t care = L.care[b][2 * x + (g >> 1)];
-                const uint32_t bad = care >> (8 * (g & 1) + 4 * h);
-                const bool in_pool = care >> 16;
+                const uint32_t keys = L.care[b][2 * x + (g >> 1)];
+                const uint32_t bad = keys >> (8 * (g & 1) + 4 * h);
+                const bool in_pool = keys >> 16;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = j0 + 8 * g + 4 * h + i;
                     const bool seen = j <= top && j >= lo && in_pool;
                     t[4 * g + i] = seen ? t[4 * g + i] : -INFINITY;
-                    mx = fmaxf(mx, t[4 * g + i]);
-                    vx = fmaxf(vx, seen ? fabsf(v4[i]) : 0.f);
+                    mx = fmaxf(mx, t[4 * g + i] + scale_bound(fabsf(v4[i])));
                     nan |= seen && ((bad >> i) & 1);
                 }
             }
-            ve = scale_bound(xmax32(vx));
             if (__builtin_amdgcn_ballot_w64(nan)) {
                 const auto both = __builtin_amdgcn_permlane32_swap(nan, nan, false, false);      // (a row's two lanes)
                 const float z = both[0] | both[1] ? __builtin_nanf("") : 0.f;
@@ -1369,7 +1377,6 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 for (int d = 0; d < DT; ++d) acc[d] += z;
             }
         }
-        mx += ve;
         // (a row's own scores alone decide whether its reference moves)
         if (__builtin_amdgcn_ballot_w64(unset || mx > P_SHIFT + SLACK_W)) {      // rare after the first keys
             mx = xmax32(mx);

@@ -5,7 +5,7 @@ number of keys while a mean over many keys shrinks.  Here rounding errors of
 different keys count as independent, as they are: an output's error before its
 own rounding is at most a few standard deviations,
 
-    E_i = 3 sqrt(sum_j (eps_j w_j v_ij)^2 + acc^2)
+    E_i = 3 sqrt(sum_j (eps_j w_j v_ij)^2 + sum_j (floor max W code_ij)^2 + acc^2)
 
   eps_j   relative error of a weight: half a step of what holds it (`weight`),
           and its score's error: a score is a sum of products exact in fp32 of
@@ -16,7 +16,11 @@ own rounding is at most a few standard deviations,
           weights W of the 96 keys whose offset has not been taken off; each
           product over 32 keys rounds it 4 times.  Over all steps
           143 2^-24 sqrt(4 sum (g_1 + g_2 + g_3)^2) <= 143 2^-24 6 sqrt(sum g^2),
-          g the sums of W over 32 keys.
+          g the sums of W = w_j v_scale_j over 32 keys.
+  floor   (256-row tiles) a weight times its V scale is an fp16 number, the row's
+          largest at least 2^5: below 2^-14 the step is 2^-24, so that half of it
+          is 2^-30 of the largest; 2^-21 where the row's scale follows 16 keys whose
+          V scales lie within a factor of 2^9 and so may be that much too high.
 
 and the output is the correctly rounded value wherever that error does not reach
 over the middle between two values: it does in a share E_i / step_i of cases.
@@ -27,7 +31,7 @@ import torch
 from tests import paged_util as U
 
 
-def rows(q, pool, table_row, n, window=0, sm_scale=None, weight=2.0 ** -16):
+def rows(q, pool, table_row, n, window=0, sm_scale=None, weight=2.0 ** -16, floor=0.0):
     """(out, E) of one request's new tokens q [m, HQ, D], the last of its n tokens."""
     kp, vp, ks, vs = pool
     m, HQ, D = q.shape
@@ -50,9 +54,10 @@ def rows(q, pool, table_row, n, window=0, sm_scale=None, weight=2.0 ** -16):
         w = torch.softmax(s, -1)
         size = 15 * abs(sm) * x.abs().sum(-1, keepdim=True) * sk.double()
         eps = weight ** 2 + (4 * 2.0 ** -24 * size) ** 2
-        var = (eps * w * w) @ (v * v)
-        g = (w * sv.double().abs())
-        g = torch.nn.functional.pad(g, (0, -n % 32)).reshape(m * G, -1, 32).sum(-1)
+        W = w * sv.double().abs()
+        code = U.values(vp[ids, h, j % P], torch.ones_like(sv))
+        var = (eps * w * w) @ (v * v) + (floor * W.amax(-1, keepdim=True)) ** 2 * ((~hide).double() @ (code * code))
+        g = torch.nn.functional.pad(W, (0, -n % 32)).reshape(m * G, -1, 32).sum(-1)
         acc = 143 * 6 * 2.0 ** -24 * g.square().sum(-1, keepdim=True).sqrt()
         out[:, h * G:(h + 1) * G] = (w @ v).reshape(m, G, D)
         E[:, h * G:(h + 1) * G] = (3 * (var + acc * acc).sqrt()).reshape(m, G, D)

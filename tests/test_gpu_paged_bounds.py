@@ -49,3 +49,69 @@ def test_short_requests_round_their_outputs_alone(dtype, D, H, G, seq, window):
         some = sorted({0, len(seq) // 2, len(seq) - 1})
         refs = [B.rows(q[r:r + 1], pool, table[r], seq[r], window) for r in some]
         B.check(out[some], torch.cat([x for x, _ in refs]), torch.cat([x for _, x in refs]), f"requests {some}, queries of {amp}")
+
+
+LONG = dict(weight=2.0 ** -11, floor=2.0 ** -21)         # requests of more than 16 rows
+
+
+def _v_scales(kind, shape, g):
+    """Factors of the V rows' magnitudes [pages, heads, page]."""
+    u = torch.rand(shape, generator=g, device="cuda")
+    if kind == "some":                                   # 2^-6 to 2^6
+        return torch.exp2(12 * u - 6)
+    if kind == "all":                                    # what fp16 scales hold
+        return torch.exp2(30 * u - 16)
+    if kind == "spikes":                                 # few tokens are far larger
+        return torch.where(u < 0.02, 2.0 ** 14, 2.0 ** -10)
+    if kind == "holes":                                  # few tokens are far smaller
+        return torch.where(u < 0.02, 2.0 ** -16, 2.0 ** 12)
+    if kind == "zeros":                                  # some tokens count for nothing, whatever their weight
+        return torch.ones_like(u)
+    ramp = torch.arange(shape[0] * shape[2], device="cuda").reshape(shape[0], 1, shape[2]) / (shape[0] * shape[2])
+    return torch.exp2(28 * (ramp if kind == "rising" else 1 - ramp) - 15).expand(shape)
+
+
+@pytest.mark.parametrize("kind", ["some", "all", "spikes", "holes", "rising", "falling", "zeros"])
+@pytest.mark.parametrize("dtype,D,H,G,seq,new,window", [
+    (BF16, 128, 2, 4, [1000, 40], [300, 20], 0), (FP16, 64, 2, 8, [700, 33], [40, 33], 0), (BF16, 64, 1, 4, [6000], [60], 0),
+    (BF16, 128, 2, 4, [900], [100], 90), (BF16, 128, 2, 4, [3000, 50], [1, 1], 0), (BF16, 64, 2, 4, [3000, 50], [4, 3], 200)])
+def test_v_rows_of_different_magnitudes(kind, dtype, D, H, G, seq, new, window):
+    """V scales that differ between tokens, up to all that fp16 holds; queries that
+    pick single keys out, whatever their scale, among them."""
+    g, page = _gen(5), 16
+    pages = sum(-(-n // page) for n in seq)
+    table = torch.full((len(seq), max(-(-n // page) for n in seq)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(seq):                          # pages in order: the ramps run along the sequences
+        table[r, :-(-n // page)] = torch.arange(at, at - (-n // page), dtype=torch.int32, device="cuda")
+        at += -(-n // page)
+    k, v = (torch.randn(pages, H, page, D, generator=g, device="cuda") for _ in range(2))
+    kc, ks = U.quantise(k)
+    vc, vs = U.quantise(v * _v_scales(kind, (pages, H, page), g)[..., None])
+    assert bool(torch.isfinite(vs.float()).all())
+    if kind == "zeros":
+        vs[torch.rand(vs.shape, generator=g, device="cuda") < 0.3] = 0.0
+    pool = (kc, vc, ks, vs)
+    q = torch.randn(sum(new), H, G, D, generator=g, device="cuda")
+    first = 0
+    for r, (n, m) in enumerate(zip(seq, new)):           # every second token looks for one key that it sees
+        for i in range(0, m, 2):
+            pos = n - m + i
+            lo = max(0, pos - window + 1) if window else 0
+            j = lo + int(torch.randint(0, pos - lo + 1, (1,), generator=g, device="cuda"))
+            q[first + i] = 4 * k[table[r, j // page].long(), :, j % page][:, None]
+        first += m
+    q = q.reshape(-1, H * G, D).to(dtype)
+    out = hq.paged_attention(q, *pool, table, _i32(seq), _i32([0] + torch.tensor(new).cumsum(0).tolist()), window=window)
+    first = 0
+    for r, (n, m) in enumerate(zip(seq, new)):
+        short = m * G <= 16
+        ref, E = B.rows(q[first:first + m], pool, table[r], n, window, **({} if short else LONG))
+        got = out[first:first + m]
+        B.check(got, ref, E, f"{kind}, request {r}")
+        # row by row: rows of small values do not hide behind rows of large ones
+        lim = 1.2 * (ref.to(dtype).double() - ref).norm(dim=-1) + E.norm(dim=-1) + 2.0 ** -60
+        worst = ((got.double() - ref).norm(dim=-1) / lim).max()
+        print(f"{kind}, request {r}: rows at most {float(worst):.3g} of their limit")
+        assert worst <= 1, (kind, r, float(worst))
+        first += m
