@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <mutex>
 #include <string>
 
 namespace hyq {
@@ -654,7 +655,8 @@ struct AttnArgs {
     PlanArgs plan;
     float* part;                         // [slot][key head][TILE][D] sums; ml: [slot][key head][TILE][2] (m, l)
     float* ml;
-    uint32_t* counters;                  // arrivals per join and KV head (the last workgroup joins), or null: a launch joins
+    uint64_t* counters;                  // arrivals per join and KV head (the last workgroup joins), or null: a launch joins
+    uint64_t call;                       // this call's number << CALL_SHIFT
     int32_t G, heads, page_log2, num_pages, window, zero_tail;
     float scale;                         // sm_scale * log2(e)
 };
@@ -743,7 +745,8 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 // ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
 // on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
 // chain lengths -> table -> rows -> pieces: 11.7 us for one request of 8K keys.
-constexpr int COUNTER_PAD = 32;          // a counter has a 128-byte line: arrivals at one line queue up
+constexpr int COUNTER_PAD = 16;          // a counter has a 128-byte line: arrivals at one line queue up
+constexpr int CALL_SHIFT = 16;           // a counter is the call's number and its arrivals (at most 1366 pieces)
 constexpr int SC1 = 16;                  // cache policy bit: device scope
 
 // Streams s0 .. s0 + VS - 1 of a row's pieces at this lane's 4 channels: `o` and
@@ -1063,10 +1066,13 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     __shared__ int last;
-    uint32_t* const counter = a.counters + (static_cast<int64_t>(it.join) * a.heads + head) * COUNTER_PAD;
+    // (arrivals that an earlier call left behind, because its lengths were changed
+    // while it ran, are below this call's number: the maximum takes them away)
+    uint64_t* const counter = a.counters + (static_cast<int64_t>(it.join) * a.heads + head) * COUNTER_PAD;
     if (tid == 0) {
-        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(it.pieces - 1);
-        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        (void)__hip_atomic_fetch_max(counter, a.call, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(counter, uint64_t{1}, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.call + it.pieces - 1;
+        if (last) __hip_atomic_store(counter, uint64_t{0}, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!last) return;
@@ -1696,7 +1702,8 @@ int launch_attention(AttnArgs a, const PlanArgs& narrow, const PlanArgs& wide, c
 // 12.7; but where a request may be cut into more than 48 pieces, one workgroup
 // takes longer than the launch does (one 32K sequence 22.9, 20.5).
 bool join_here(const hyq_paged_params& p, const Both& s, hipStream_t st) {
-    if (!p.counters || p.cu_seqlens || s.wide.items || s.narrow.joins * p.kv_heads * COUNTER_PAD > HYQ_PAGED_COUNTERS) return false;
+    if (!p.counters || p.cu_seqlens || s.wide.items || s.narrow.joins * p.kv_heads * COUNTER_PAD * 2 > HYQ_PAGED_COUNTERS) return false;
+    if (!aligned(p.counters, 8)) return false;
     if (s.narrow.most > 48 && s.narrow.wanted > 48 * static_cast<int64_t>(p.num_requests)) return false;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(st, &status) != hipSuccess) {
@@ -1815,10 +1822,17 @@ extern "C" int hyq_paged_attention(const hyq_paged_params* p, void* workspace, s
     };
     const PlanArgs narrow = plan_of(s.narrow), wide = plan_of(s.wide);
     if (p->num_requests > INLINE_R) paged_plan_kernel<<<dim3(s.wide.items ? 2 : 1), dim3(PLAN_T), 0, st>>>(narrow, wide);
+    // calls with counters are numbered in the order of their launches
+    static std::mutex order;
+    static uint64_t calls = 0;
+    const bool here = join_here(*p, s, st);
+    std::unique_lock<std::mutex> lock(order, std::defer_lock);
+    if (here) lock.lock();
+    const uint64_t call = here ? ++calls : 0;
     const AttnArgs a{static_cast<const uint16_t*>(p->q), p->q_stride_t, p->q_stride_h, static_cast<uint16_t*>(p->out), p->o_stride_t, p->o_stride_h,
                      p->lse, static_cast<int64_t>(p->kv_heads) * p->kv_repeat, p->k_pages, p->v_pages, p->p_stride_page, p->p_stride_head,
                      p->k_scale, p->v_scale, p->s_stride_page, p->s_stride_head, p->block_table, p->bt_stride, narrow, nullptr, nullptr,
-                     join_here(*p, s, st) ? p->counters : nullptr, p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), window, p->zero_tail,
+                     here ? reinterpret_cast<uint64_t*>(p->counters) : nullptr, call << CALL_SHIFT, p->kv_repeat, p->kv_heads, log2i(p->page_size), static_cast<int32_t>(p->num_pages), window, p->zero_tail,
                      p->sm_scale * 1.44269504f};
     if (p->head_dim == 128) return p->dtype_fp16 ? launch_attention<128, true>(a, narrow, wide, s, ws, st) : launch_attention<128, false>(a, narrow, wide, s, ws, st);
     return p->dtype_fp16 ? launch_attention<64, true>(a, narrow, wide, s, ws, st) : launch_attention<64, false>(a, narrow, wide, s, ws, st);

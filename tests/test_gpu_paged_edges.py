@@ -96,3 +96,32 @@ def test_v_scales_that_are_not_finite(bad, D, seq, new, window):
     assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
     # (the rows' references differ: fp32 roundings of m and log2 l)
     assert bool(((lse - want_lse)[hit].abs() <= 2.0 ** -20 * (1 + want_lse[hit].abs())).all())
+
+
+def _decode_setup(seed=4):
+    g, seq, page, H, G, D = _gen(seed), [9000, 5000, 3001], 16, 2, 8, 128
+    table, pages = U.make_table(g, seq, page, "cuda")
+    pool = U.make_pool(g, pages, H, page, D, "cuda")
+    q = torch.randn(3, H * G, D, generator=g, device="cuda").to(BF16)
+    return q, pool, table, _i32(seq)
+
+
+def test_arrivals_left_behind_do_not_count(monkeypatch):
+    """What a call leaves in the counters whose lengths were changed while it ran
+    (arrivals, but not the last one) does no harm to the calls after it."""
+    from hyquant_amd import paged
+    q, pool, table, lens = _decode_setup()
+    qs = [q, 3 * q, -q]                                  # (other memory and other values from call to call)
+    with monkeypatch.context() as m:
+        m.setattr(paged, "_counters", lambda *_: 0)
+        want = [hq.paged_attention(x, *pool, table, lens) for x in qs]
+    assert torch.equal(hq.paged_attention(q, *pool, table, lens), want[0])
+    stream = torch.cuda.current_stream().cuda_stream
+    words = paged._counts[(0, stream)].view(torch.int64)
+    for left in (1, 2, 5, 30, 200):
+        words.fill_(left)                                # (of the call before the first)
+        got = [hq.paged_attention(x, *pool, table, lens) for x in qs]
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), left
+        for x in got:
+            x.fill_(7.0)                                 # (the next calls get this memory)
+    words.zero_()
