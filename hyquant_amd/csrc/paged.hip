@@ -1703,7 +1703,7 @@ int launch_attention(AttnArgs a, const PlanArgs& narrow, const PlanArgs& wide, c
 // takes longer than the launch does (one 32K sequence 22.9, 20.5).
 bool join_here(const hyq_paged_params& p, const Both& s, hipStream_t st) {
     if (!p.counters || p.cu_seqlens || s.wide.items || s.narrow.joins * p.kv_heads * COUNTER_PAD * 2 > HYQ_PAGED_COUNTERS) return false;
-    if (!aligned(p.counters, 8)) return false;
+    if (!aligned(p.counters, 8) || st == hipStreamPerThread) return false;     // (that handle names a stream of every thread)
     if (s.narrow.most > 48 && s.narrow.wanted > 48 * static_cast<int64_t>(p.num_requests)) return false;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(st, &status) != hipSuccess) {

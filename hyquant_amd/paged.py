@@ -24,7 +24,7 @@ A step of a serving program:
 Nothing is read back to the host, so a captured graph of a step follows the
 lengths it is replayed with.  Every call allocates its own outputs and
 workspace on the current stream; 256 KiB of arrival counters are kept
-per stream.  Inference only: no gradients.
+per stream of torch's.  Inference only: no gradients.
 """
 
 from __future__ import annotations
@@ -62,17 +62,25 @@ def _fast(t: torch.Tensor):
 
 
 _counts = {}                               # (device, stream) -> arrival counters of the calls on that stream
+_foreign = set()                           # (device, stream) of streams that are not torch's
 
 
 def _counters(device: torch.device, stream: int) -> int:
     """The address of the arrival counters of eager calls on `stream`, zero
     between calls; 0 while the stream is being captured and has none yet (the
     library uses them in no captured call: a graph may be replayed beside
-    eager calls)."""
+    eager calls), and for streams that torch does not own: their handles may
+    come back for another stream, or name several."""
     c = _counts.get((device.index, stream))
     if c is None:
+        if (device.index, stream) in _foreign:
+            return 0
         with torch.cuda.device(device):
             if torch.cuda.is_current_stream_capturing():
+                return 0
+            # (a stream handed to torch has its handle for an id, torch's own have small ones)
+            if stream and torch.cuda.current_stream(device).stream_id == stream:
+                _foreign.add((device.index, stream))
                 return 0
             c = _counts.setdefault((device.index, stream), torch.zeros(_lib.PAGED_COUNTERS, dtype=torch.int32, device=device))
     return c.data_ptr()

@@ -487,7 +487,8 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  *             completed call leaves them at zero, and calls that share them must be ordered
  *             on one stream.  A call without cu_seqlens on a stream that is not being
  *             captured then needs no launch of its own for the pieces of cut requests; other
- *             calls leave them alone, as do all where they are not 8-byte aligned.  The results are the same bit for bit.  A call whose
+ *             calls leave them alone, as do calls on hipStreamPerThread and all where they
+ *             are not 8-byte aligned.  The results are the same bit for bit.  A call whose
  *             lengths are written while it runs gives anything, and leaves later calls alone.
  */
 #define HYQ_PAGED_COUNTERS 65536

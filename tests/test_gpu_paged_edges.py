@@ -125,3 +125,20 @@ def test_arrivals_left_behind_do_not_count(monkeypatch):
         for x in got:
             x.fill_(7.0)                                 # (the next calls get this memory)
     words.zero_()
+
+
+def test_streams_of_others_have_no_counters():
+    """A handle that torch does not own may come back for another stream: its calls
+    take the form without state."""
+    from hyquant_amd import paged
+    q, pool, table, lens = _decode_setup()
+    want = hq.paged_attention(q, *pool, table, lens)
+    torch.cuda.synchronize()
+    own = torch.cuda.Stream()
+    other = torch.cuda.ExternalStream(own.cuda_stream)
+    known = (0, own.cuda_stream) in paged._counts        # (torch hands its streams out in turn)
+    with torch.cuda.stream(other):
+        got = [hq.paged_attention(q, *pool, table, lens) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert ((0, own.cuda_stream) in paged._counts) == known
+    assert all(torch.equal(x, want) for x in got)
