@@ -1617,6 +1617,10 @@ int check_pool(const char* what, int32_t head_dim, int32_t page_size, int64_t nu
     return HYQ_OK;
 }
 
+// a launch has fewer than 2^32 threads along a dimension
+constexpr int64_t MOST_THREADS = (int64_t{1} << 32) - 1024;
+int64_t most_rows(int head_dim) { return MOST_THREADS / (head_dim / 8); }
+
 int check_attention(const hyq_paged_params* p) {
     const char* w = "hyq_paged_attention";
     if (!p) return fail(HYQ_EINVAL, std::string(w) + ": null parameters");
@@ -1646,6 +1650,9 @@ int check_attention(const hyq_paged_params* p) {
         return fail(HYQ_EINVAL, s + "out must be 8-byte aligned with strides divisible by 4");
     if (!aligned(p->seq_lens, 4) || !aligned(p->cu_seqlens, 4) || !aligned(p->block_table, 4) || !aligned(p->lse, 4) || !aligned(p->counters, 4))
         return fail(HYQ_EINVAL, s + "lengths, table, lse and counters must be 4-byte aligned");
+    const Both z = sizes_of(*p);
+    if (z.wide.items * p->kv_heads > MOST_THREADS / (64 * CHUNK_WAVES))
+        return fail(HYQ_ENOTSUP, s + std::to_string(z.wide.items) + " tiles of " + std::to_string(p->kv_heads) + " key heads are more than a launch holds");
     return HYQ_OK;
 }
 
@@ -1761,8 +1768,9 @@ extern "C" int hyq_paged_append(const uint16_t* k, int64_t k_stride_t, int64_t k
     if (!k || !v || !slots) return fail(HYQ_EINVAL, "hyq_paged_append: null pointer");
     if (!aligned(k, 16) || !aligned(v, 16) || (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 || !aligned(slots, 8))
         return fail(HYQ_EINVAL, "hyq_paged_append: rows must be 16-byte aligned with strides divisible by 8");
+    if (num_tokens > most_rows(head_dim) / kv_heads)
+        return fail(HYQ_ENOTSUP, "hyq_paged_append: more than " + std::to_string(most_rows(head_dim)) + " rows");
     const int64_t rows = num_tokens * kv_heads;
-    if (num_tokens > (int64_t{1} << 30) || rows > (int64_t{1} << 30)) return fail(HYQ_ENOTSUP, "hyq_paged_append: more than 2^30 rows");
     RowArgs a{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, nullptr, nullptr, slots, k_pages, v_pages, p_stride_page, p_stride_head,
               k_scale, v_scale, s_stride_page, s_stride_head, num_pages * page_size, static_cast<uint32_t>(rows),
               static_cast<uint32_t>(kv_heads), log2i(page_size), log2i(head_dim / 8)};
@@ -1785,8 +1793,9 @@ extern "C" int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_
     if (num_tokens == 0) return HYQ_OK;
     if (!k_out || !v_out || !slots) return fail(HYQ_EINVAL, "hyq_paged_gather: null pointer");
     if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(slots, 8)) return fail(HYQ_EINVAL, "hyq_paged_gather: misaligned pointer");
+    if (num_tokens > most_rows(head_dim) / kv_heads)
+        return fail(HYQ_ENOTSUP, "hyq_paged_gather: more than " + std::to_string(most_rows(head_dim)) + " rows");
     const int64_t rows = num_tokens * kv_heads;
-    if (num_tokens > (int64_t{1} << 30) || rows > (int64_t{1} << 30)) return fail(HYQ_ENOTSUP, "hyq_paged_gather: more than 2^30 rows");
     RowArgs a{nullptr, nullptr, 0, 0, 0, 0, k_out, v_out, slots, const_cast<int8_t*>(k_pages), const_cast<int8_t*>(v_pages), p_stride_page,
               p_stride_head, const_cast<uint16_t*>(k_scale), const_cast<uint16_t*>(v_scale), s_stride_page, s_stride_head,
               num_pages * page_size, static_cast<uint32_t>(rows), static_cast<uint32_t>(kv_heads), log2i(page_size), log2i(head_dim / 8)};
