@@ -115,3 +115,76 @@ def test_v_rows_of_different_magnitudes(kind, dtype, D, H, G, seq, new, window):
         print(f"{kind}, request {r}: rows at most {float(worst):.3g} of their limit")
         assert worst <= 1, (kind, r, float(worst))
         first += m
+
+
+def _check_rows(out, pool, table, seq, new, q, window, G, what):
+    """Every request's outputs together and row by row (rows of small values do not
+    hide behind rows of large ones)."""
+    first = 0
+    for r, (n, m) in enumerate(zip(seq, new)):
+        x = q[first:first + m]
+        ref, E = B.rows(x, pool, table[r], n, window, **({} if m * G <= 16 else LONG))
+        got = out[first:first + m]
+        B.check(got, ref, E, f"{what}, request {r}")
+        lim = 1.2 * (ref.to(out.dtype).double() - ref).norm(dim=-1) + E.norm(dim=-1) + 2.0 ** -60
+        worst = ((got.double() - ref).norm(dim=-1) / lim).max()
+        assert worst <= 1, (what, r, float(worst))
+        first += m
+
+
+@pytest.mark.parametrize("dtype,D,H,G,page,seq,new,window", [
+    (FP16, 128, 8, 4, 16, [32768, 3], [1, 1], 0), (BF16, 128, 8, 4, 64, [8192], [1], 0), (BF16, 128, 2, 8, 128, [20001, 7, 12345], [1] * 3, 0),
+    (FP16, 64, 8, 4, 256, [30011], [1], 0), (BF16, 128, 8, 4, 64, [9000] * 48, [1] * 48, 0), (FP16, 128, 8, 4, 32, [20001], [1], 5000),
+    (BF16, 64, 2, 4, 16, [700] * 300, [1] * 300, 0), (BF16, 128, 8, 8, 256, [20000], [40], 0), (FP16, 128, 2, 8, 16, [9000, 4000], [30, 77], 0),
+    (BF16, 64, 4, 4, 64, [12000, 300], [64, 200], 3000), (FP16, 64, 2, 32, 32, [5000] * 3, [1] * 3, 0)])
+def test_each_row_finds_its_key(dtype, D, H, G, page, seq, new, window):
+    """Every second row looks for one key, at the edges of tiles, pages and steps and
+    at random places of long contexts: reading another key's codes, scales or page in
+    its place would be the whole of such a row's output."""
+    g = _gen(7)
+    table, pages = U.make_table(g, seq, page, "cuda")
+    k, v = (torch.randn(pages, H, page, D, generator=g, device="cuda") for _ in range(2))
+    (kc, ks), (vc, vs) = U.quantise(k), U.quantise(v)
+    pool = (kc, vc, ks, vs)
+    q = torch.randn(sum(new), H, G, D, generator=g, device="cuda")
+    rnd = torch.randint(0, 1 << 30, (sum(new), H, G), generator=g, device="cuda").tolist()
+    first = 0
+    for r, (n, m) in enumerate(zip(seq, new)):
+        at, who = [], []
+        for i in range(m):
+            pos = n - m + i
+            lo = max(0, pos - window + 1) if window else 0
+            edges = sorted({min(max(e, lo), pos) for b in (0, 16, 32, 64, page, 128, 256, 384, 1024, 4096, n // 2 // 32 * 32, n // page * page, lo, pos)
+                            for e in (b - 1, b, b + 1)})
+            for h in range(H):
+                for a in range(G):
+                    x = rnd[first + i][h][a]
+                    if (i + h + a) % 2 == 0:
+                        at.append(edges[x % len(edges)] if x & 1 << 20 else lo + x % (pos - lo + 1))
+                        who.append((first + i, h, a))
+        at, who = torch.tensor(at, device="cuda"), torch.tensor(who, device="cuda")
+        q[who[:, 0], who[:, 1], who[:, 2]] = (6 if D == 64 else 4) * k[table[r, at // page].long(), who[:, 1], at % page]
+        first += m
+    q = q.reshape(-1, H * G, D).to(dtype)
+    out = hq.paged_attention(q, *pool, table, _i32(seq), None if max(new) == 1 else _i32([0] + torch.tensor(new).cumsum(0).tolist()), window=window)
+    some = range(len(seq)) if len(seq) < 10 else (0, len(seq) // 2, len(seq) - 1)
+    if max(new) == 1:
+        for r in some:
+            _check_rows(out[r:r + 1], pool, table[r:r + 1], seq[r:r + 1], [1], q[r:r + 1], window, G, f"row {r}")
+    else:
+        _check_rows(out, pool, table, seq, new, q, window, G, "rows")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D,H,G,page,seq,new,window", [
+    (128, 8, 4, 64, [2500], [700], 0), (128, 2, 8, 16, [1300, 4000], [1300, 77], 0), (64, 8, 4, 16, [6000, 700], [600, 700], 1024),
+    (128, 8, 8, 256, [20000], [40], 0), (64, 2, 32, 32, [3000] * 4, [1] * 4, 0), (128, 2, 4, 32, [17, 9000], [17, 5], 0)])
+def test_longer_requests_round_weights_to_11_bits(dtype, D, H, G, page, seq, new, window):
+    """Requests of more than 16 rows: half a step of fp16 for a weight, no more."""
+    g = _gen(8)
+    table, pages = U.make_table(g, seq, page, "cuda")
+    pool = U.make_pool(g, pages, H, page, D, "cuda")
+    for amp in (1.0, 3.0):
+        q = (amp * torch.randn(sum(new), H * G, D, generator=g, device="cuda")).to(dtype)
+        out = hq.paged_attention(q, *pool, table, _i32(seq), _i32([0] + torch.tensor(new).cumsum(0).tolist()), window=window)
+        _check_rows(out, pool, table, seq, new, q, window, G, f"queries of {amp}")

@@ -142,3 +142,21 @@ def test_streams_of_others_have_no_counters():
     torch.cuda.synchronize()
     assert ((0, own.cuda_stream) in paged._counts) == known
     assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_rows_that_are_not_finite(dtype, D):
+    """Rows with NaN and infinities among their channels: quantize_per_token's codes and scales all the same."""
+    g, H, page = _gen(6), 2, 16
+    x = torch.randn(40, H, D, generator=g, device="cuda")
+    x[0, 0, 3], x[1, 1, D - 1], x[2, 0, 0], x[3] = math.nan, math.inf, -math.inf, math.nan
+    x[4, 1, 5], x[4, 1, 6], x[5, 0, 7], x[5, 0, 8] = math.nan, math.inf, math.inf, -math.inf
+    x = x.to(dtype)
+    pool = tuple(t.clone() for t in U.make_pool(g, 4, H, page, D, "cuda"))
+    slots = torch.randperm(4 * page, generator=g, device="cuda")[:40]
+    hq.paged_append(x, x, slots, *pool)
+    c, s = hq.quantize_per_token(x.reshape(-1, 1, D).contiguous(), 4)
+    for i in (0, 1):
+        assert torch.equal(pool[i][slots // page, :, slots % page], c.reshape(40, H, D // 2))
+        assert torch.equal(pool[2 + i][slots // page, :, slots % page].view(torch.int16), s.reshape(40, H).view(torch.int16))
