@@ -661,7 +661,7 @@ struct AttnArgs {
     float scale;                         // sm_scale * log2(e)
 };
 
-constexpr float M_INIT = -1.0e30f;
+constexpr float M_INIT = -3.0e38f;       // below any score
 constexpr float SLACK = 8.0f;            // the running maximum moves when a score passes it by this (log2 units)
 constexpr int WAVES = 4;                 // of the 16-row kernel
 constexpr float LN2 = 0.69314718055994531f;
@@ -673,12 +673,12 @@ __device__ __forceinline__ float half_at(uint32_t w, int hi) {
     else return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
 }
 
-// The power of two that brings the largest finite row maximum of a tile to
-// [2^14, 2^15), so that fp16 holds the queries exactly down to 2^-38 of it;
-// returned as the exponent to subtract, in [-100, 100].
+// The power of two that brings a row's largest magnitude (or that of many rows)
+// to [2^14, 2^15), so that fp16 holds the queries exactly down to 2^-38 of it;
+// returned as the exponent to subtract, in [-114, 113].
 __device__ __forceinline__ int q_exponent(float amax) {
     const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127;
-    return min(max(e, -100), 100) - 14;
+    return max(e, -100) - 14;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
@@ -879,11 +879,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
     for (int m = 0; m < KW; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(half_at<F16>(qr[m][i], 0)), fabsf(half_at<F16>(qr[m][i], 1))));
+    // (a power of two of each row's own: rows of any magnitude stand side by side)
     amax = col_max(amax);
     if (!(amax < INFINITY)) amax = 0.f;
-    amax = max16_dpp(amax);
     const int qe = q_exponent(amax);
-    const float qs = pow2(-qe);
+    const float qs = pow2(-qe), row_scale = pow2(qe);
     f16x8 qop[KW];
 #pragma unroll
     for (int m = 0; m < KW; ++m) {
@@ -893,7 +893,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         qop[m] = f16x8{static_cast<_Float16>(f[0]), static_cast<_Float16>(f[4]), static_cast<_Float16>(f[1]), static_cast<_Float16>(f[5]),
                        static_cast<_Float16>(f[2]), static_cast<_Float16>(f[6]), static_cast<_Float16>(f[3]), static_cast<_Float16>(f[7])};
     }
-    const float qk = a.scale * pow2(qe) * 16777216.0f;     // K operands are codes * 2^-24
+    const float qk = a.scale * 16777216.0f;                // K operands are codes * 2^-24
     f32x4 kbias = {0.f, 0.f, 0.f, 0.f};
     {
         const u32x4 half = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};
@@ -951,7 +951,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         float mx = vmax3(s[0], s[1], s[2]);
         mx = vmax3(mx, s[3], s[4]);
         mx = vmax3(mx, s[5], s[6]);
-        mx = vmax2(mx, s[7]);
+        mx = vmax2(mx, s[7]) * row_scale;
         if (__builtin_amdgcn_ballot_w64(mx > m_run + SLACK)) {
             mx = col_max(mx);
             const float mnew = mx > m_run + SLACK ? mx : m_run;        // (a row's own scores alone move its maximum)
@@ -964,7 +964,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            s[e] = fast_exp2(s[e] - m_run);
+            s[e] = fast_exp2(__builtin_fmaf(s[e], row_scale, -m_run));
             l_run += s[e];
         }
         float p[8];

@@ -51,7 +51,7 @@ def rows(q, pool, table_row, n, window=0, sm_scale=None, weight=2.0 ** -16, floo
         k, v = U.values(kp[ids, h, j % P], sk), U.values(vp[ids, h, j % P], sv)
         x = q[:, h * G:(h + 1) * G].double().reshape(m * G, D)
         s = (x @ k.t() * sm).masked_fill(hide, float("-inf"))
-        w = torch.softmax(s, -1)
+        w = torch.softmax(s, -1).masked_fill(hide.all(-1, keepdim=True), 0.0)      # (a row without keys is zero)
         size = 15 * abs(sm) * x.abs().sum(-1, keepdim=True) * sk.double()
         eps = weight ** 2 + (4 * 2.0 ** -24 * size) ** 2
         W = w * sv.double().abs()

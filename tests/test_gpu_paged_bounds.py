@@ -188,3 +188,23 @@ def test_longer_requests_round_weights_to_11_bits(dtype, D, H, G, page, seq, new
         q = (amp * torch.randn(sum(new), H * G, D, generator=g, device="cuda")).to(dtype)
         out = hq.paged_attention(q, *pool, table, _i32(seq), _i32([0] + torch.tensor(new).cumsum(0).tolist()), window=window)
         _check_rows(out, pool, table, seq, new, q, window, G, f"queries of {amp}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D,H,G,page,seq,new,spread", [(128, 2, 8, 16, [900, 77], [1, 1], 60), (64, 2, 3, 32, [300], [5], 60), (64, 1, 1, 16, [7], [9], 60),
+                                                       (128, 2, 4, 16, [700, 90], [70, 20], 11), (64, 1, 16, 64, [9000], [40], 11)])
+def test_query_rows_of_very_different_magnitude(dtype, D, H, G, page, seq, new, spread):
+    """Rows of one request, tokens or heads, that are 2^120 times others (2^28 in
+    fp16, 2^22 in requests of more than 16 rows): each row's output is its own."""
+    spread = spread if dtype == BF16 else min(spread, 14)
+    g = _gen(9)
+    table, pages = U.make_table(g, seq, page, "cuda")
+    pool = U.make_pool(g, pages, H, page, D, "cuda")
+    q = torch.randn(sum(new), H * G, D, generator=g, device="cuda").clamp(-3.9, 3.9)
+    e = torch.randint(-spread, spread + 1, q.shape[:2], generator=g, device="cuda")
+    e = torch.where(torch.rand(e.shape, generator=g, device="cuda") < 0.6, 0, e)
+    q = (q * torch.exp2(e.float())[..., None]).to(dtype)
+    assert bool(torch.isfinite(q.float()).all())
+    cu = None if max(new) == 1 else _i32([0] + torch.tensor(new).cumsum(0).tolist())
+    out = hq.paged_attention(q, *pool, table, _i32(seq), cu)
+    _check_rows(out, pool, table, seq, new, q, 0, G, "rows")
