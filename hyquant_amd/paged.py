@@ -178,10 +178,15 @@ def _pool_args(kp, vp, ks, vs):
             ks.stride(1))
 
 
+def _row_strides(t: torch.Tensor) -> Tuple[int, int]:
+    """The strides (token, head) of t [T, H, D]; 0 where there is one alone, whatever t says."""
+    return t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+
+
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous channels and 16-byte aligned rows (a copy if it has others)."""
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1])):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
+    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in _row_strides(t))):
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -220,7 +225,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages:
     k, v = _aligned_rows(k), _aligned_rows(v)
     with _on(k.device):
         st = _lib.lib().hyq_paged_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), int(k.dtype == torch.float16),
+            k.data_ptr(), *_row_strides(k), v.data_ptr(), *_row_strides(v), int(k.dtype == torch.float16),
             slots.data_ptr(), k.shape[0], H, D, *_pool_args(k_pages, v_pages, k_scale, v_scale), N, P, _stream(k.device))
     _lib.check(st, "paged_append")
 
@@ -319,8 +324,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if T and R:
         q = _aligned_rows(q)
         p = _lib.PagedParams()
-        p.q, p.q_stride_t, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-        p.out, p.o_stride_t, p.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+        p.q, (p.q_stride_t, p.q_stride_h) = q.data_ptr(), _row_strides(q)
+        p.out, (p.o_stride_t, p.o_stride_h) = out.data_ptr(), _row_strides(out)
         p.lse = lse.data_ptr() if return_lse else None
         (p.k_pages, p.v_pages, p.p_stride_page, p.p_stride_head, p.k_scale, p.v_scale, p.s_stride_page,
          p.s_stride_head) = _pool_args(k_pages, v_pages, k_scale, v_scale)

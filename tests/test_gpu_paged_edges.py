@@ -160,3 +160,29 @@ def test_append_rows_that_are_not_finite(dtype, D):
     for i in (0, 1):
         assert torch.equal(pool[i][slots // page, :, slots % page], c.reshape(40, H, D // 2))
         assert torch.equal(pool[2 + i][slots // page, :, slots % page].view(torch.int16), s.reshape(40, H).view(torch.int16))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_one_token_of_a_buffer_of_odd_pitch(native, monkeypatch):
+    """The stride of a dimension of one is no stride: one token's rows of a buffer
+    whose rows are no multiple of 16 bytes, as inputs and as out."""
+    if not native:
+        monkeypatch.setattr(dd, "_FX", False)
+    g, H, G, D, page = _gen(8), 2, 4, 64, 16
+    pool = U.make_pool(g, 3, H, page, D, "cuda")
+    buf = torch.randn(6, 2 * H * D + H * G * D + 6, generator=g, device="cuda").to(BF16)
+    at = 4                                               # (a row at a 16-byte address: 4 * 774 * 2 bytes)
+    assert buf[at].data_ptr() % 16 == 0 and buf.stride(0) % 8
+    k, v, q = (x.view(6, -1, D)[at:at + 1] for x in buf[:, :-6].split([H * D, H * D, H * G * D], 1))
+    assert q.stride(0) % 8 and q.is_contiguous()
+    slots = torch.tensor([20], device="cuda")
+    hq.paged_append(k, v, slots, *pool)
+    c, s = U.quantise(k.clone())
+    assert torch.equal(pool[0][1, :, 4], c[0]) and torch.equal(pool[2][1, :, 4], s[0])
+    table, lens = _i32([[2, 1]]), _i32([21])
+    want = hq.paged_attention(q.clone(memory_format=torch.contiguous_format) + 0, *pool, table, lens)
+    assert torch.equal(hq.paged_attention(q, *pool, table, lens), want)
+    wide = torch.zeros(6, H * G * D + 2, dtype=BF16, device="cuda")
+    out = wide[:, :-2].view(6, H * G, D)[at:at + 1]
+    assert out.stride(0) % 4 and hq.paged_attention(q, *pool, table, lens, out=out) is out and torch.equal(out, want)
+    assert bool((wide[:at] == 0).all()) and bool((wide[at + 1:] == 0).all())
