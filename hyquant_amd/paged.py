@@ -91,7 +91,7 @@ def _ints(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: torc
         raise ValueError(f"{name} must be a {dim}-d {dtype} tensor")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.stride(-1) != 1 and t.numel() > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
 
 

@@ -186,3 +186,15 @@ def test_one_token_of_a_buffer_of_odd_pitch(native, monkeypatch):
     out = wide[:, :-2].view(6, H * G, D)[at:at + 1]
     assert out.stride(0) % 4 and hq.paged_attention(q, *pool, table, lens, out=out) is out and torch.equal(out, want)
     assert bool((wide[:at] == 0).all()) and bool((wide[at + 1:] == 0).all())
+
+
+def test_tables_of_one_column():
+    """Whatever the stride of a table's only column says."""
+    g = _gen(10)
+    pool = U.make_pool(g, 4, 2, 16, 64, "cuda")
+    q = torch.randn(3, 4, 64, generator=g, device="cuda").to(BF16)
+    lens, flat = _i32([5, 16, 9]), _i32([3, 0, 2])
+    want = hq.paged_attention(q, *pool, flat[:, None].contiguous(), lens)
+    column = flat[None].t()
+    assert column.stride() == (1, 3) and torch.equal(hq.paged_attention(q, *pool, column, lens), want)
+    assert hq.paged_batch(lens - 1, torch.ones_like(lens), column, flat, 16, 3).slots.tolist() == [52, 15, 40]
