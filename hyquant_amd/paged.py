@@ -62,7 +62,15 @@ def _fast(t: torch.Tensor):
 
 
 _counts = {}                               # (device, stream) -> arrival counters of the calls on that stream
-_foreign = set()                           # (device, stream) of streams that are not torch's
+_stream_data = getattr(torch._C, "_cuda_getCurrentStream", None)      # (id, device, type)
+
+
+def _is_torchs(device: torch.device, stream: int) -> bool:
+    """Whether the current stream, of handle `stream`, is one of torch's own: one
+    that was handed to torch has its handle for an id, torch's have small ones."""
+    if _stream_data is not None and device.index is not None:
+        return stream == 0 or _stream_data(device.index)[0] != stream
+    return stream == 0 or torch.cuda.current_stream(device).stream_id != stream
 
 
 def _counters(device: torch.device, stream: int) -> int:
@@ -73,14 +81,10 @@ def _counters(device: torch.device, stream: int) -> int:
     come back for another stream, or name several."""
     c = _counts.get((device.index, stream))
     if c is None:
-        if (device.index, stream) in _foreign:
+        if not _is_torchs(device, stream):
             return 0
         with torch.cuda.device(device):
             if torch.cuda.is_current_stream_capturing():
-                return 0
-            # (a stream handed to torch has its handle for an id, torch's own have small ones)
-            if stream and torch.cuda.current_stream(device).stream_id == stream:
-                _foreign.add((device.index, stream))
                 return 0
             c = _counts.setdefault((device.index, stream), torch.zeros(_lib.PAGED_COUNTERS, dtype=torch.int32, device=device))
     return c.data_ptr()

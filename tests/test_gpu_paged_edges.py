@@ -142,6 +142,10 @@ def test_streams_of_others_have_no_counters():
     torch.cuda.synchronize()
     assert ((0, own.cuda_stream) in paged._counts) == known
     assert all(torch.equal(x, want) for x in got)
+    with torch.cuda.stream(own):                         # and torch's stream has them after all
+        got = [hq.paged_attention(q, *pool, table, lens) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert (0, own.cuda_stream) in paged._counts and all(torch.equal(x, want) for x in got)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
