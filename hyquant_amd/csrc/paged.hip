@@ -411,7 +411,8 @@ __device__ __forceinline__ Req request(const PlanArgs& a, int r) {
 // back.  Where 16-row tiles are many, that would make the pieces long and
 // unequal: a third more pieces than slots are cut, and the last ones fill up.
 // A tile that is hardly longer than a piece is not cut, it would cost the
-// partial results for nothing.  Measured on requests of 128 channels, 8 KV heads:
+// partial results for nothing.  Measured on requests of 128 channels, 8 KV heads
+// (decode steps with a weight in one bf16 number; in two they take 3 to 6% more):
 //   16 requests of 8K keys    exactly one round 33 us, 1024 pieces and more 39
 //   24 requests of 16K        77, 85
 //   64 requests of 1K to 32K  one round 163, a third more 123, twice as many 120
@@ -733,18 +734,18 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 //   PV  O^T[channel][row] = V^T . P'^T with v_mfma_f32_16x16x32_bf16, V operands
 //       the bf16 numbers 128 + u, P' = p v_scale as the sum of two bf16 numbers
 //       (2^-16 of a weight is lost; one bf16 number, 2^-8, made a bf16 output's
-//       error 2.4e-3 where its own rounding is 1.7e-3, and was 4% faster):
+//       error 2.4e-3 where its own rounding is 1.7e-3, and was 3 to 6% faster):
 //       136 sum(P') is taken off every 96 keys of a wavefront, from the same
 //       rounded P' by products with ones.  The running sum carries up to 140
 //       times those keys' weights, and its fp32 roundings stay in the result:
 //       taken off at the end alone they made a relative error of 2.4e-3 over 32K
 //       keys in one piece, where an fp16 output's own rounding is 2.1e-4 (1% of
 //       the time).  Outputs of either type are then as good as their type.
-// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 103 us, 5.4
-// TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
+// Bound by the cache's bytes: 16 requests of 32K keys (554 MB) take 103 to 106
+// us, 5.3 TB/s where a copy reaches 5.1 and a stream of reads 6.8.  What feeds it is the
 // ring of three groups' loads in registers per wavefront (two: 121 us), no LDS
 // on the way in, and 3 resident workgroups a CU.  Short calls are bound by the
-// chain lengths -> table -> rows -> pieces: 11.7 us for one request of 8K keys.
+// chain lengths -> table -> rows -> pieces: 12.0 us for one request of 8K keys.
 constexpr int COUNTER_PAD = 16;          // a counter has a 128-byte line: arrivals at one line queue up
 constexpr int CALL_SHIFT = 16;           // a counter is the call's number and its arrivals (at most 1366 pieces)
 constexpr int SC1 = 16;                  // cache policy bit: device scope
@@ -1122,7 +1123,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
 //       high that P' sinks below fp16's 2^-14: there M follows max(score + log2 V
 //       scale), key by key.
 // Bound by the matrix pipe and the VALU work that has to run beside it: 2048
-// tokens at 8192 (309 GFLOP) take 358 us, 0.86 PFLOP/s where a large matrix
+// tokens at 8192 (309 GFLOP) take 354 to 362 us, 0.87 PFLOP/s where a large matrix
 // product reaches 1.35, and the products with their LDS reads alone take 226 us.
 // So the block is worked on in halves of 32 keys: the scores of one half run
 // beside the weights of the half before, and the first four wavefronts have
@@ -1704,9 +1705,9 @@ int launch_attention(AttnArgs a, const PlanArgs& narrow, const PlanArgs& wide, c
 
 // Whether the attention launch joins the pieces itself: a decode step (a ragged
 // call's join launch also clears rows) with counters, in no captured graph, whose
-// replays on another stream would share them.  One 8K sequence takes 11.6 us
-// instead of 13.8, 200 requests 28.7 instead of 30.8, one of 1K 10.0 instead of
-// 12.7; but where a request may be cut into more than 48 pieces, one workgroup
+// replays on another stream would share them.  One 8K sequence takes 12.0 us
+// instead of 14.1, 200 requests 29.0 instead of 31.2, one of 1K 10.5 instead of
+// 13.1; but where a request may be cut into more than 48 pieces, one workgroup
 // takes longer than the launch does (one 32K sequence 22.9, 20.5).
 bool join_here(const hyq_paged_params& p, const Both& s, hipStream_t st) {
     if (!p.counters || p.cu_seqlens || s.wide.items || s.narrow.joins * p.kv_heads * COUNTER_PAD * 2 > HYQ_PAGED_COUNTERS) return false;

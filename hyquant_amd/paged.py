@@ -42,7 +42,8 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
 class PagedBatch(NamedTuple):
-    """The layout of one step's batch (paged_batch)."""
+    """The layout of one step's batch (paged_batch): parts of one allocation (clone
+    one to keep it alone, or to torch.save them together)."""
     cu_seqlens: torch.Tensor      # int32 [R + 1], prefix sums of the new lengths
     seq_lens: torch.Tensor        # int32 [R], context + new
     slots: torch.Tensor           # int64 [num_tokens], -1 past the last new token

@@ -427,7 +427,8 @@ int hyq_prefill_unified(const hyq_prefill_params* params, void* workspace, size_
  *                                          than num_free: the entries of those that there are
  *                                          not become -1, and so do their tokens' slots, as
  *                                          where a row would need more than max_pages)
- * Tokens past num_tokens are left out.  At most 16384 requests; the new
+ * Tokens past num_tokens are left out (of slots and positions; cu_seqlens and
+ * seq_lens count them).  At most 16384 requests; the new
  * lengths' sum below 2^31.
  */
 int hyq_paged_batch(const int32_t* context_lens, const int32_t* new_lens, int32_t num_requests,
