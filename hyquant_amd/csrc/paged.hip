@@ -1169,7 +1169,7 @@ struct ChunkLds {
     float vs[BUFS][BLK];                 // V scale, 0 where it is not finite or not to be looked at
     float ve[BUFS][4];                   // per 16-key tile: log2 bound of vs, BAD more if the keys need care
     uint32_t care[BUFS][4];              // bits 0..15: keys whose V scale is not finite; bit 16: the page is in the pool
-    float red[CHUNK_WAVES];
+    float red[2][CHUNK_WAVES];
 };
 
 // e with x < 2^e, x >= 0 finite (an fp16 value: at least 2^-24, or 0, which takes
@@ -1208,13 +1208,22 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     }
     amax = xmax32(amax);
     if (!(amax < INFINITY)) amax = 0.f;
-    amax = xmax16(max16_dpp(amax));
-    if (lane == 0) L.red[w] = amax;
+    const float most = xmax16(max16_dpp(amax)), least = -xmax16(max16_dpp(amax > 0.f ? -amax : -INFINITY));
+    if (lane == 0) { L.red[0][w] = most; L.red[1][w] = least; }
     __syncthreads();
+    float all_most = 0.f, all_least = INFINITY;
 #pragma unroll
-    for (int i = 0; i < CHUNK_WAVES; ++i) amax = fmaxf(amax, L.red[i]);
-    const int qe = q_exponent(amax);
-    const float qs = pow2(-qe), qk = a.scale * pow2(qe);
+    for (int i = 0; i < CHUNK_WAVES; ++i) {
+        all_most = fmaxf(all_most, L.red[0][i]);
+        all_least = fminf(all_least, L.red[1][i]);
+    }
+    // One power of two for all rows.  Where some are below 2^-16 of the largest
+    // (rare), they would lose bits of 2^-23 to it: then each row has its own, which the
+    // careful path of `settle` applies to the scores (a product more per score in
+    // the other path would cost 3%; so it is 1%, for the scores that live longer).
+    const bool apart = __builtin_amdgcn_readfirstlane(all_least < all_most * 0x1p-16f);
+    const int qe = q_exponent(apart ? amax : all_most);
+    const float qs = pow2(-qe), row_scale = pow2(qe), qk = apart ? a.scale : a.scale * row_scale;
     f16x8 qop[KM];
 #pragma unroll
     for (int m = 0; m < KM; ++m) {
@@ -1228,7 +1237,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     const int lo = first_key(pos, a.window), top = min(pos, it.key1 - 1);
     // every row of this wavefront sees [all_lo, all_hi]
     const int t0 = (it.row0 + min(32 * w, nrows - 1)) / a.G, t1 = (it.row0 + min(32 * w + 31, nrows - 1)) / a.G;
-    const int all_hi = min(it.len - it.qlen + t0, it.key1 - 1), all_lo = first_key(it.len - it.qlen + t1, a.window);
+    const int all_hi = apart ? -1 : min(it.len - it.qlen + t0, it.key1 - 1), all_lo = first_key(it.len - it.qlen + t1, a.window);
 
     // ---- conversion ----
     // Wavefronts 0..3 have the V codes and scales of the 16-key tiles 0..3 of a
@@ -1368,6 +1377,11 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 const uint32_t keys = L.care[b][2 * x + (g >> 1)];
                 const uint32_t bad = keys >> (8 * (g & 1) + 4 * h);
                 const bool in_pool = keys >> 16;
+                if (apart) {             // (again, with the row's own power of two)
+                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(&L.ks[b][32 * x + 8 * g + 4 * h]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[4 * g + i] = __builtin_fmaf(sc[4 * g + i] * row_scale, k4[i], -m_use);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = j0 + 8 * g + 4 * h + i;

@@ -275,10 +275,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     are the last of its seq_lens[r] (int32 [R]) tokens: a token at position p
     sees the keys j <= p, with window > 0 only the last `window` of those.
 
-    Query rows of any magnitude stand side by side in requests of at most 16
-    rows (tokens * H_Q / key heads); in larger ones they should lie within 2^24
-    of each other (smaller rows lose bits).
-
     Returns out [T, H_Q, D] of q's dtype, with return_lse also the natural
     log-sum-exp of the scaled scores, fp32 [T, H_Q].  A row that sees no key is
     zero (lse -inf), as are the rows behind the last request of a padded batch

@@ -472,10 +472,8 @@ int hyq_paged_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads,
  * exact operands: the K scale multiplies the fp32 score, the V scale the
  * weight, which is then rounded once: for requests of at most 16 rows (tokens
  * times kv_repeat) to the sum of two bf16 numbers (2^-16), for larger requests
- * to fp16 (2^-11).  Queries enter as fp16 numbers under a power of two, exactly
- * but for values below 2^-38 of the largest it is chosen for: the row's in
- * requests of at most 16 rows, that of up to 256 rows in larger ones.  There,
- * rows of less than 2^-24 of the largest finite value among those rows lose bits.
+ * to fp16 (2^-11).  Queries enter as fp16 numbers under a power of two, to
+ * within 2^-23 of their row's largest.
  *   q     bf16 or fp16 [num_tokens, kv_heads * kv_repeat, head_dim] strides (t, h, 1),
  *         16-byte aligned, strides divisible by 8; out the same type, 8-byte aligned,
  *         strides divisible by 4

@@ -192,10 +192,11 @@ def test_longer_requests_round_weights_to_11_bits(dtype, D, H, G, page, seq, new
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("D,H,G,page,seq,new,spread", [(128, 2, 8, 16, [900, 77], [1, 1], 60), (64, 2, 3, 32, [300], [5], 60), (64, 1, 1, 16, [7], [9], 60),
-                                                       (128, 2, 4, 16, [700, 90], [70, 20], 11), (64, 1, 16, 64, [9000], [40], 11)])
+                                                       (128, 2, 4, 16, [700, 90], [70, 20], 60), (64, 1, 16, 64, [9000], [40], 60),
+                                                       (64, 2, 4, 32, [400, 60], [90, 70], 11), (128, 2, 4, 32, [400], [90], 5), (128, 1, 32, 16, [1000], [1], 40)])
 def test_query_rows_of_very_different_magnitude(dtype, D, H, G, page, seq, new, spread):
     """Rows of one request, tokens or heads, that are 2^120 times others (2^28 in
-    fp16, 2^22 in requests of more than 16 rows): each row's output is its own."""
+    fp16): each row's output is its own."""
     spread = spread if dtype == BF16 else min(spread, 14)
     g = _gen(9)
     table, pages = U.make_table(g, seq, page, "cuda")
