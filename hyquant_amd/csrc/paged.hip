@@ -1123,7 +1123,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged_attn_kernel
 //       high that P' sinks below fp16's 2^-14: there M follows max(score + log2 V
 //       scale), key by key.
 // Bound by the matrix pipe and the VALU work that has to run beside it: 2048
-// tokens at 8192 (309 GFLOP) take 354 to 362 us, 0.87 PFLOP/s where a large matrix
+// tokens at 8192 (309 GFLOP) take 353 to 377 us by box, 0.82 to 0.87 PFLOP/s where a large matrix
 // product reaches 1.35, and the products with their LDS reads alone take 226 us.
 // So the block is worked on in halves of 32 keys: the scores of one half run
 // beside the weights of the half before, and the first four wavefronts have
