@@ -34,6 +34,12 @@ from .paged import (  # noqa: F401
     paged_batch,
     paged_gather,
 )
+from .paged8 import (  # noqa: F401
+    SCALE_BLOCK,
+    paged8_append,
+    paged8_gather,
+)
+from .rope import paged_rope_append, qk_norm_rope  # noqa: F401
 from .cache_io import load_cache, save_cache  # noqa: F401
 
 __all__ = [
@@ -60,4 +66,9 @@ __all__ = [
     "paged_append",
     "paged_gather",
     "paged_attention",
+    "SCALE_BLOCK",
+    "paged8_append",
+    "paged8_gather",
+    "qk_norm_rope",
+    "paged_rope_append",
 ]

@@ -60,6 +60,10 @@ EXPORTS = (
     "hyq_paged_gather",
     "hyq_paged_attention_workspace_size",
     "hyq_paged_attention",
+    "hyq_qk_norm_rope",
+    "hyq_paged8_append",
+    "hyq_paged_rope_append",
+    "hyq_paged8_gather",
 )
 
 
@@ -137,6 +141,32 @@ class PagedParams(Structure):
         ("sm_scale", c_float),
         ("dtype_fp16", c_int32), ("zero_tail", c_int32),
         ("counters", c_void_p),
+    ]
+
+
+class RopeParams(Structure):
+    """Mirror of `hyq_rope_params` (include/hyq.h)."""
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_n", c_int64), ("q_stride_h", c_int64),
+        ("k", c_void_p), ("k_stride_b", c_int64), ("k_stride_n", c_int64), ("k_stride_h", c_int64),
+        ("q_out", c_void_p), ("k_out", c_void_p),
+        ("cos", c_void_p), ("sin", c_void_p), ("table_stride_b", c_int64), ("table_stride_m", c_int64), ("table_rows", c_int64),
+        ("positions", c_void_p),
+        ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("eps", c_double),
+        ("batch", c_int64), ("n", c_int64),
+        ("q_heads", c_int32), ("k_heads", c_int32), ("head_dim", c_int32), ("rotary", c_int32),
+        ("interleaved", c_int32), ("dtype_fp16", c_int32), ("table_type", c_int32), ("weight_fp32", c_int32),
+    ]
+
+
+class PagedPool(Structure):
+    """Mirror of `hyq_paged_pool` (include/hyq.h)."""
+    _fields_ = [
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("p_stride_page", c_int64), ("p_stride_head", c_int64),
+        ("k_scale", c_void_p), ("v_scale", c_void_p), ("s_stride_page", c_int64), ("s_stride_head", c_int64),
+        ("num_pages", c_int64),
+        ("page_size", c_int32), ("bits", c_int32),
     ]
 
 
@@ -226,6 +256,15 @@ def _declare(lib):
     lib.hyq_paged_attention_workspace_size.argtypes = [POINTER(PagedParams)]
     lib.hyq_paged_attention.restype = c_int
     lib.hyq_paged_attention.argtypes = [POINTER(PagedParams), c_void_p, c_size_t, c_void_p]
+    lib.hyq_qk_norm_rope.restype = c_int
+    lib.hyq_qk_norm_rope.argtypes = [POINTER(RopeParams), c_void_p]
+    lib.hyq_paged8_append.restype = c_int
+    lib.hyq_paged8_append.argtypes = ([c_void_p, c_int64, c_int64] * 2 + [c_int32, c_void_p, c_int64, c_int32, c_int32]
+                                      + [POINTER(PagedPool), c_void_p])
+    lib.hyq_paged_rope_append.restype = c_int
+    lib.hyq_paged_rope_append.argtypes = [POINTER(RopeParams), c_void_p, c_int64, c_int64, c_void_p, POINTER(PagedPool), c_void_p]
+    lib.hyq_paged8_gather.restype = c_int
+    lib.hyq_paged8_gather.argtypes = [c_void_p, c_int64, c_int32, c_int32, POINTER(PagedPool), c_int32, c_void_p, c_void_p, c_void_p]
 
 
 def lib():

@@ -514,6 +514,95 @@ typedef struct hyq_paged_params {
 size_t hyq_paged_attention_workspace_size(const hyq_paged_params* p);
 int hyq_paged_attention(const hyq_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Rotation of queries and keys by position, with the norms of their heads where
+ * there are weights (the reference's attention modules make both with the
+ * model's own torch operations, src/patch/patch_llama.py:27-110,
+ * src/patch/patch_qwen.py).  A row x of head_dim channels becomes
+ *   y = x / sqrt(mean(x^2) + eps) * w                          (w not NULL)
+ *   (y_a, y_b) <- (y_a cos - y_b sin, y_b cos + y_a sin)
+ * for the rotary / 2 channel pairs (a, b) = (i, i + rotary / 2) or, interleaved,
+ * (2i, 2i + 1), with cos and sin [rotary / 2] of its position's table row; the
+ * channels from rotary on are not rotated.  In fp32, rounded once.
+ *   q, k    bf16 (dtype_fp16 = 0) or fp16 [batch, n, heads, head_dim], strides (b, n, h, 1),
+ *           16-byte aligned, strides divisible by 8; q_out, k_out the same, contiguous,
+ *           sharing no memory with the inputs
+ *   cos, sin  fp32 (table_type 0), bf16 (1) or fp16 (2) [batch or 1, table_rows, rotary / 2],
+ *           strides (table_stride_b, table_stride_m, 1) divisible by 8, 16-byte aligned
+ *   positions int64 [batch * n], rows of the table (table_stride_b unused); a token whose position
+ *           is outside [0, table_rows) gives rows of zeros.  NULL: token i of batch entry b has row i
+ *           of table b.
+ *   q_weight, k_weight  [head_dim], fp32 (weight_fp32 = 1) or the rows' type, 16-byte aligned, or NULL
+ * head_dim 64 or 128, rotary a multiple of 16 up to head_dim.
+ */
+typedef struct hyq_rope_params {
+    const void* q; int64_t q_stride_b, q_stride_n, q_stride_h;
+    const void* k; int64_t k_stride_b, k_stride_n, k_stride_h;
+    void* q_out; void* k_out;
+    const void* cos; const void* sin; int64_t table_stride_b, table_stride_m, table_rows;
+    const int64_t* positions;
+    const void* q_weight; const void* k_weight;
+    double eps;
+    int64_t batch, n;
+    int32_t q_heads, k_heads, head_dim, rotary;
+    int32_t interleaved, dtype_fp16, table_type, weight_fp32;
+} hyq_rope_params;
+
+int hyq_qk_norm_rope(const hyq_rope_params* p, void* stream);
+
+/*
+ * A paged cache: of 4 bits as above (k_scale, v_scale fp16 [num_pages, kv_heads,
+ * page_size]), or of 8 bits with a scale for each block of 16 tokens and head:
+ *   k_pages, v_pages  int8 [num_pages, kv_heads, page_size, head_dim], strides (p_stride_page,
+ *                     p_stride_head, head_dim), the same for K and V; 16-byte aligned, strides
+ *                     divisible by 16
+ *   k_scale, v_scale  fp32 [num_pages, kv_heads, page_size / 16], strides (s_stride_page,
+ *                     s_stride_head, 1), the same for K and V; value = code * scale
+ * page_size: a power of two from 16 to 256; head_dim 64 or 128.
+ */
+typedef struct hyq_paged_pool {
+    int8_t* k_pages; int8_t* v_pages; int64_t p_stride_page, p_stride_head;
+    void* k_scale; void* v_scale; int64_t s_stride_page, s_stride_head;
+    int64_t num_pages;
+    int32_t page_size, bits;
+} hyq_paged_pool;
+
+/*
+ * New rows of k and v [n, k_heads, head_dim] (strides t, h; 16-byte aligned, divisible
+ * by 8) into their slots of an 8-bit pool.  A block's scale is 2^e, the smallest with
+ * max(|x|, 1e-5) <= 127 2^e over the block's new rows; the rows before the first of
+ * them stay, and where their scale was larger it stays too, where it was smaller
+ * their codes become RNE(code * old / new).  code = RNE(x / scale).  Rows behind the
+ * new ones of a block hold anything.  A block with a value that is not finite, or
+ * past 127 2^40, has the scale NaN.
+ *   slots  int64 [n]; one outside [0, num_pages * page_size) writes nothing.
+ *          Precondition: no slot is named twice, the slots of one block are neighbours and
+ *          ascend (as hyq_paged_batch gives them), and the rows of a block before the first
+ *          have been appended.
+ */
+int hyq_paged8_append(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v,
+                      int64_t v_stride_t, int64_t v_stride_h, int32_t is_fp16, const int64_t* slots,
+                      int64_t num_tokens, int32_t kv_heads, int32_t head_dim, const hyq_paged_pool* pool, void* stream);
+
+/*
+ * q rotated as hyq_qk_norm_rope's, k rotated the same and put into the cache with v,
+ * in one launch: hyq_paged_append's or hyq_paged8_append's codes and scales of v, and
+ * of k's rows before any rounding to 16 bits (rotated in 64 bits: scale =
+ * fp16(fp32(max(amax, 1e-5) / 7)), code = RNE(k / scale) in a 4-bit pool).  batch = 1,
+ * n tokens; k_out is not used.  A token whose position is outside the table or whose
+ * slot is outside the pool writes nothing into the cache.
+ */
+int hyq_paged_rope_append(const hyq_rope_params* p, const uint16_t* v, int64_t v_stride_t, int64_t v_stride_h,
+                          const int64_t* slots, const hyq_paged_pool* pool, void* stream);
+
+/*
+ * Rows of an 8-bit pool by slot: k_out, v_out bf16 (out_fp16 = 0) or fp16
+ * [num_tokens, kv_heads, head_dim] contiguous = RNE(code * scale); zero rows
+ * for slots outside the pool.
+ */
+int hyq_paged8_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads, int32_t head_dim,
+                      const hyq_paged_pool* pool, int32_t out_fp16, uint16_t* k_out, uint16_t* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
