@@ -37,6 +37,7 @@ from .paged import (  # noqa: F401
 from .paged8 import (  # noqa: F401
     SCALE_BLOCK,
     paged8_append,
+    paged8_attention,
     paged8_gather,
 )
 from .rope import paged_rope_append, qk_norm_rope  # noqa: F401
@@ -69,6 +70,7 @@ __all__ = [
     "SCALE_BLOCK",
     "paged8_append",
     "paged8_gather",
+    "paged8_attention",
     "qk_norm_rope",
     "paged_rope_append",
 ]

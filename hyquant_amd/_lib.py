@@ -64,6 +64,8 @@ EXPORTS = (
     "hyq_paged8_append",
     "hyq_paged_rope_append",
     "hyq_paged8_gather",
+    "hyq_paged8_attention_workspace_size",
+    "hyq_paged8_attention",
 )
 
 
@@ -263,6 +265,10 @@ def _declare(lib):
                                       + [POINTER(PagedPool), c_void_p])
     lib.hyq_paged_rope_append.restype = c_int
     lib.hyq_paged_rope_append.argtypes = [POINTER(RopeParams), c_void_p, c_int64, c_int64, c_void_p, POINTER(PagedPool), c_void_p]
+    lib.hyq_paged8_attention_workspace_size.restype = c_size_t
+    lib.hyq_paged8_attention_workspace_size.argtypes = [POINTER(PagedParams)]
+    lib.hyq_paged8_attention.restype = c_int
+    lib.hyq_paged8_attention.argtypes = [POINTER(PagedParams), c_void_p, c_size_t, c_void_p]
     lib.hyq_paged8_gather.restype = c_int
     lib.hyq_paged8_gather.argtypes = [c_void_p, c_int64, c_int32, c_int32, POINTER(PagedPool), c_int32, c_void_p, c_void_p, c_void_p]
 

@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhyq.so")
 
-SOURCES = ["status.hip", "quant.hip", "decode.hip", "select.hip", "prefill.hip", "paged.hip", "rope.hip"]
+SOURCES = ["status.hip", "quant.hip", "decode.hip", "select.hip", "prefill.hip", "paged.hip", "paged8.hip", "rope.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -289,11 +289,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                 return (o, lse) if return_lse else o
         except TypeError:
             pass
+    return _attention("paged_attention", _check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
+                      window, return_lse, out)
+
+
+def _attention(name, check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale, window, return_lse, out):
+    """The checked form of an attention call over the pages of either cache (`name` its entry point's)."""
     _require_gpu(q, "q")
     dev = q.device
-    N, H, P, D = _check_pool(k_pages, v_pages, k_scale, v_scale, dev)
+    N, H, P, D = check_pool(k_pages, v_pages, k_scale, v_scale, dev)
     if q.dtype not in _HALF:
-        raise ValueError(f"paged_attention expects bf16 or fp16 queries, got {q.dtype}")
+        raise ValueError(f"{name} expects bf16 or fp16 queries, got {q.dtype}")
     if q.dim() != 3 or q.shape[2] != D:
         raise ValueError(f"q must be [T, H_Q, {D}], got {tuple(q.shape)}")
     T, HQ, _ = q.shape
@@ -340,12 +346,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             p.counters = _counters(dev, _stream(dev)) or None
         L = _lib.lib()
         ref = ctypes.byref(p)
-        need = L.hyq_paged_attention_workspace_size(ref)
+        need = getattr(L, f"hyq_{name}_workspace_size")(ref)
         # a workspace of its own for every call: two streams or captured graphs never share one
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         with _on(dev):
-            st = L.hyq_paged_attention(ref, ws.data_ptr(), need, _stream(dev))
-        _lib.check(st, "paged_attention")
+            st = getattr(L, f"hyq_{name}")(ref, ws.data_ptr(), need, _stream(dev))
+        _lib.check(st, name)
     elif T:                                # no request: every row is behind the last
         if zero_tail:
             out.zero_()

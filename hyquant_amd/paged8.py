@@ -20,13 +20,13 @@ the block's last scale.  Inference only: no gradients.
 from __future__ import annotations
 
 import ctypes
-from typing import Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
 from .decode_d_stage import _HALF, _require_gpu, _stream
-from .paged import _aligned_rows, _check_page_size, _ints, _on, _row_strides
+from .paged import _aligned_rows, _attention, _check_page_size, _ints, _on, _row_strides
 
 SCALE_BLOCK = 16                           # tokens of a scale
 
@@ -104,3 +104,15 @@ def paged8_gather(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
                                           v.data_ptr(), _stream(slots.device))
     _lib.check(st, "paged8_gather")
     return k, v
+
+
+def paged8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                     sm_scale: Optional[float] = None, window: int = 0, return_lse: bool = False,
+                     out: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """paged_attention over an 8-bit pool: causal attention of the new tokens of R
+    requests over their cached tokens (their own among them: append first), the
+    same arguments, masks and results.  A row that sees a key of a block whose K
+    or V scale is NaN, or not within [2^-40, 2^48], is NaN."""
+    return _attention("paged8_attention", _check_pool8, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
+                      window, return_lse, out)

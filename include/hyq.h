@@ -499,7 +499,7 @@ typedef struct hyq_paged_params {
     void* out; int64_t o_stride_t, o_stride_h;
     float* lse;
     const int8_t* k_pages; const int8_t* v_pages; int64_t p_stride_page, p_stride_head;
-    const uint16_t* k_scale; const uint16_t* v_scale; int64_t s_stride_page, s_stride_head;
+    const void* k_scale; const void* v_scale; int64_t s_stride_page, s_stride_head;    /* fp16 */
     const int32_t* block_table; int64_t bt_stride;
     const int32_t* seq_lens;
     const int32_t* cu_seqlens;
@@ -602,6 +602,18 @@ int hyq_paged_rope_append(const hyq_rope_params* p, const uint16_t* v, int64_t v
  */
 int hyq_paged8_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads, int32_t head_dim,
                       const hyq_paged_pool* pool, int32_t out_fp16, uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/*
+ * hyq_paged_attention over an 8-bit pool: the same parameters, but k_scale and
+ * v_scale are fp32 [num_pages, kv_heads, page_size / 16] (strides s_stride_page,
+ * s_stride_head, 1).  The codes enter the products as exact operands, a block's
+ * scales as constants of the fp32 scores; a weight times its V scale is then
+ * rounded once: for requests of at most 16 rows to the sum of two fp16 numbers
+ * (2^-21), for larger requests to fp16 (2^-11).  A row that sees a key
+ * whose block's K or V scale is not within [2^-40, 2^48] is NaN, its lse too.
+ */
+size_t hyq_paged8_attention_workspace_size(const hyq_paged_params* p);
+int hyq_paged8_attention(const hyq_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
