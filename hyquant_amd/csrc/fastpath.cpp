@@ -6,7 +6,8 @@
 // output and calls hyq_decode_hybrid through the pointer the Python side
 // hands over at set-up (the library ctypes loaded, whichever file that is).
 //
-// The paged cache's calls (hyquant_amd/paged.py) take the same way: each makes
+// The paged caches' calls (hyquant_amd/paged.py, paged8.py) and the rotation's
+// (rope.py) take the same way: each makes
 // the checks of its Python form and declines (status -1) whatever fails one,
 // so that the Python form copies, or raises.
 //
@@ -136,6 +137,12 @@ struct {
     GatherFn gather = nullptr;
     AttentionSizeFn size = nullptr;
     AttentionFn attention = nullptr;
+    AttentionSizeFn size8 = nullptr;
+    AttentionFn attention8 = nullptr;
+    decltype(&hyq_paged8_append) append8 = nullptr;
+    decltype(&hyq_paged8_gather) gather8 = nullptr;
+    decltype(&hyq_qk_norm_rope) rope = nullptr;
+    decltype(&hyq_paged_rope_append) rope_append = nullptr;
 } g_paged;
 
 bool plain(const at::Tensor& t, at::ScalarType type, int64_t dim, const at::Device& device) {
@@ -151,18 +158,24 @@ bool rows16(const at::Tensor& t) {
     return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
-// a pool as _check_pool wants it (sizes and alignment are the library's to check)
-bool pool(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks, const at::Tensor& vs, const at::Device& device) {
-    if (!plain(kp, at::kChar, 4, device) || !plain(vp, at::kChar, 4, device) || !plain(ks, at::kHalf, 3, device) ||
-        !plain(vs, at::kHalf, 3, device))
+// a pool as _check_pool (4 bits) or _check_pool8 wants it (sizes and alignment are the library's to check)
+bool pool(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks, const at::Tensor& vs, const at::Device& device, int bits = 4) {
+    const auto type = bits == 4 ? at::kHalf : at::kFloat;
+    if (!plain(kp, at::kChar, 4, device) || !plain(vp, at::kChar, 4, device) || !plain(ks, type, 3, device) || !plain(vs, type, 3, device))
         return false;
     if (kp.sizes() != vp.sizes() || kp.strides() != vp.strides() || ks.sizes() != vs.sizes() || ks.strides() != vs.strides())
         return false;
-    if (ks.size(0) != kp.size(0) || ks.size(1) != kp.size(1) || ks.size(2) != kp.size(2)) return false;
-    return kp.numel() > 0 && kp.stride(3) == 1 && kp.stride(2) == kp.size(3) && ks.stride(2) == 1;
+    const int64_t scales = bits == 4 ? kp.size(2) : kp.size(2) / 16;
+    if (ks.size(0) != kp.size(0) || ks.size(1) != kp.size(1) || ks.size(2) != scales) return false;
+    return kp.numel() > 0 && kp.stride(3) == 1 && kp.stride(2) == kp.size(3) && (ks.stride(2) == 1 || scales == 1);
 }
 template <typename T>
 T* ptr(const at::Tensor& t) { return static_cast<T*>(t.data_ptr()); }
+
+hyq_paged_pool pool_of(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks, const at::Tensor& vs, int bits) {
+    return {ptr<int8_t>(kp), ptr<int8_t>(vp), kp.stride(0), kp.stride(1), ks.data_ptr(), vs.data_ptr(), ks.stride(0), ks.stride(1),
+            kp.size(0), static_cast<int32_t>(kp.size(2)), bits};
+}
 
 // A contiguous tensor of `type` at element `offset` of base's memory.  A call's
 // outputs are parts of one allocation this way: an allocation costs about 0.6 us
@@ -242,19 +255,20 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_gather(const at::Tensor& slots
     return {st, k, v};
 }
 
-// (status, out, lse)
-std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
+// (status, out, lse) over the pages of the cache of `bits` bits
+std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(int64_t bits, const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
                                                             const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table,
                                                             const at::Tensor& lens, const std::optional<at::Tensor>& cu,
                                                             const std::optional<double>& sm_scale, int64_t window,
                                                             bool want_lse, int64_t stream, int64_t counters) {
     const std::tuple<int64_t, at::Tensor, at::Tensor> skip{-1, {}, {}};
     const auto dev = q.device();
-    if (!g_paged.attention || !dev.is_cuda() || !half(q) || !plain(q, q.scalar_type(), 3, dev) || !pool(kp, vp, ks, vs, dev) ||
+    const bool four = bits == 4;
+    if (!g_paged.attention || !dev.is_cuda() || !half(q) || !plain(q, q.scalar_type(), 3, dev) || !pool(kp, vp, ks, vs, dev, four ? 4 : 8) ||
         !ints(table, at::kInt, 2, dev) || !ints(lens, at::kInt, 1, dev))
         return skip;
     const int64_t T = q.size(0), HQ = q.size(1), D = q.size(2), R = lens.size(0), H = kp.size(1);
-    if (T == 0 || R == 0 || T > INT32_MAX || HQ == 0 || HQ % H || D != 2 * kp.size(3) || table.size(0) != R || !rows16(q) || window < 0 ||
+    if (T == 0 || R == 0 || T > INT32_MAX || HQ == 0 || HQ % H || D != (four ? 2 : 1) * kp.size(3) || table.size(0) != R || !rows16(q) || window < 0 ||
         window > INT32_MAX)
         return skip;
     if (cu ? !ints(*cu, at::kInt, 1, dev) || cu->size(0) != R + 1 : T != R) return skip;
@@ -276,8 +290,8 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q,
     p.v_pages = ptr<int8_t>(vp);
     p.p_stride_page = kp.stride(0);
     p.p_stride_head = kp.stride(1);
-    p.k_scale = ptr<uint16_t>(ks);
-    p.v_scale = ptr<uint16_t>(vs);
+    p.k_scale = ks.data_ptr();
+    p.v_scale = vs.data_ptr();
     p.s_stride_page = ks.stride(0);
     p.s_stride_head = ks.stride(1);
     p.block_table = ptr<int32_t>(table);
@@ -297,11 +311,160 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_attention(const at::Tensor& q,
     p.dtype_fp16 = q.scalar_type() == at::kHalf;
     p.zero_tail = 3;
     p.counters = reinterpret_cast<uint32_t*>(counters);
-    const size_t need = g_paged.size(&p);
+    const size_t need = (four ? g_paged.size : g_paged.size8)(&p);
     if (need == 0) return skip;
     const at::Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
-    const int st = g_paged.attention(&p, ws.data_ptr(), need, reinterpret_cast<void*>(stream));
+    const int st = (four ? g_paged.attention : g_paged.attention8)(&p, ws.data_ptr(), need, reinterpret_cast<void*>(stream));
     return {st, out, lse};
+}
+
+int64_t paged8_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, const at::Tensor& kp, const at::Tensor& vp,
+                      const at::Tensor& ks, const at::Tensor& vs, int64_t stream) {
+    const auto dev = k.device();
+    if (!g_paged.append8 || !dev.is_cuda() || !half(k) || !plain(k, k.scalar_type(), 3, dev) || !plain(v, k.scalar_type(), 3, dev) ||
+        k.sizes() != v.sizes() || !pool(kp, vp, ks, vs, dev, 8) || k.size(1) != kp.size(1) || k.size(2) != kp.size(3) ||
+        !ints(slots, at::kLong, 1, dev) || slots.size(0) != k.size(0) || k.size(0) == 0 || !rows16(k) || !rows16(v))
+        return -1;
+    const c10::DeviceGuard guard(dev);
+    const hyq_paged_pool p = pool_of(kp, vp, ks, vs, 8);
+    return g_paged.append8(ptr<uint16_t>(k), k.stride(0), k.stride(1), ptr<uint16_t>(v), v.stride(0), v.stride(1), k.scalar_type() == at::kHalf,
+                           ptr<int64_t>(slots), k.size(0), static_cast<int32_t>(kp.size(1)), static_cast<int32_t>(k.size(2)), &p,
+                           reinterpret_cast<void*>(stream));
+}
+
+// (status, k, v)
+std::tuple<int64_t, at::Tensor, at::Tensor> paged8_gather(const at::Tensor& slots, const at::Tensor& kp, const at::Tensor& vp,
+                                                          const at::Tensor& ks, const at::Tensor& vs, bool fp16, int64_t stream) {
+    const auto dev = slots.device();
+    if (!g_paged.gather8 || !dev.is_cuda() || !ints(slots, at::kLong, 1, dev) || slots.size(0) == 0 || !pool(kp, vp, ks, vs, dev, 8))
+        return {-1, {}, {}};
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor kv = at::empty({2, slots.size(0), kp.size(1), kp.size(3)}, slots.options().dtype(fp16 ? at::kHalf : at::kBFloat16));
+    const at::Tensor k = part(kv, kv.scalar_type(), 0, kv.sizes().slice(1));
+    const at::Tensor v = part(kv, kv.scalar_type(), k.numel(), kv.sizes().slice(1));
+    const hyq_paged_pool p = pool_of(kp, vp, ks, vs, 8);
+    const int st = g_paged.gather8(ptr<int64_t>(slots), slots.size(0), static_cast<int32_t>(kp.size(1)), static_cast<int32_t>(kp.size(3)), &p,
+                                   fp16, ptr<uint16_t>(k), ptr<uint16_t>(v), reinterpret_cast<void*>(stream));
+    return {st, k, v};
+}
+
+// ---- rotation ----
+
+using Maybe = std::optional<at::Tensor>;
+
+// The parameter block of rows q, k ([T, heads, D], or [B, N, heads, D]); false: the checked form takes the call
+bool rope_params(hyq_rope_params& p, const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& sin,
+                 const Maybe& positions, const Maybe& qw, const Maybe& kw, double eps, bool interleaved) {
+    const auto dev = q.device();
+    const auto type = q.scalar_type();
+    const int64_t d = q.dim();
+    if (!dev.is_cuda() || !half(q) || (d != 3 && d != 4) || !plain(q, type, d, dev) || !plain(k, type, d, dev)) return false;
+    const auto table = cos.scalar_type();
+    const int64_t td = cos.dim();
+    if ((table != at::kFloat && table != at::kBFloat16 && table != at::kHalf) || td < 2 || td > 3 || !plain(cos, table, td, dev) ||
+        !plain(sin, table, td, dev) || cos.sizes() != sin.sizes() || cos.strides() != sin.strides() || cos.stride(td - 1) != 1)
+        return false;
+    const int64_t B = d == 4 ? q.size(0) : 1, N = q.size(d - 3), D = q.size(d - 1), rows = cos.size(td - 2), halfr = cos.size(td - 1);
+    if ((d == 4 && k.size(0) != B) || k.size(d - 3) != N || k.size(d - 1) != D || q.stride(d - 1) != 1 || k.stride(d - 1) != 1) return false;
+    if (halfr < 1 || halfr > 512 || N > INT32_MAX || q.size(d - 2) > INT32_MAX || k.size(d - 2) > INT32_MAX || D > 1024) return false;
+    if (positions) {
+        const int64_t pd = positions->dim();
+        if (td != 2 || pd < 1 || pd > 2 || !plain(*positions, at::kLong, pd, dev) || !positions->is_contiguous()) return false;
+        if (pd == 1 ? positions->size(0) != B * N : positions->size(0) != B || positions->size(1) != N) return false;
+        p.positions = ptr<int64_t>(*positions);
+    } else if (rows < N || (td == 3 && cos.size(0) != 1 && cos.size(0) != B)) {
+        return false;
+    }
+    const Maybe* ws[2] = {&qw, &kw};
+    const void** to[2] = {&p.q_weight, &p.k_weight};
+    int fp32 = -1;
+    for (int i = 0; i < 2; ++i) {
+        if (!*ws[i]) continue;
+        const at::Tensor& w = **ws[i];
+        const bool f = w.scalar_type() == at::kFloat;
+        if ((!f && w.scalar_type() != type) || !plain(w, w.scalar_type(), 1, dev) || w.size(0) != D || w.stride(0) != 1) return false;
+        if (fp32 >= 0 && fp32 != f) return false;
+        fp32 = f;
+        *to[i] = w.data_ptr();
+    }
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || cos.requires_grad() || sin.requires_grad() ||
+                                       (qw && qw->requires_grad()) || (kw && kw->requires_grad())))
+        return false;
+    auto stride = [](const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+    p.q = q.data_ptr();
+    p.q_stride_b = d == 4 ? stride(q, 0) : 0;
+    p.q_stride_n = stride(q, d - 3);
+    p.q_stride_h = stride(q, d - 2);
+    p.k = k.data_ptr();
+    p.k_stride_b = d == 4 ? stride(k, 0) : 0;
+    p.k_stride_n = stride(k, d - 3);
+    p.k_stride_h = stride(k, d - 2);
+    p.cos = cos.data_ptr();
+    p.sin = sin.data_ptr();
+    p.table_rows = rows;
+    p.table_stride_m = stride(cos, td - 2);
+    p.table_stride_b = td == 3 ? stride(cos, 0) : 0;
+    p.eps = eps;
+    p.batch = B;
+    p.n = N;
+    p.q_heads = static_cast<int32_t>(q.size(d - 2));
+    p.k_heads = static_cast<int32_t>(k.size(d - 2));
+    p.head_dim = static_cast<int32_t>(D);
+    p.rotary = static_cast<int32_t>(2 * halfr);
+    p.interleaved = interleaved;
+    p.dtype_fp16 = type == at::kHalf;
+    p.table_type = table == at::kFloat ? 0 : table == at::kBFloat16 ? 1 : 2;
+    p.weight_fp32 = fp32 == 1;
+    return true;
+}
+
+// (status, q, k)
+std::tuple<int64_t, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& sin,
+                                                         const Maybe& positions, const Maybe& qw, const Maybe& kw, double eps,
+                                                         bool interleaved, int64_t stream) {
+    hyq_rope_params p{};
+    if (!g_paged.rope || q.numel() == 0 || k.numel() == 0 || !rope_params(p, q, k, cos, sin, positions, qw, kw, eps, interleaved)) return {-1, {}, {}};
+    const c10::DeviceGuard guard(q.device());
+    // (two allocations: a cache that keeps the keys does not keep the queries)
+    const at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    p.q_out = qo.data_ptr();
+    p.k_out = ko.data_ptr();
+    return {g_paged.rope(&p, reinterpret_cast<void*>(stream)), qo, ko};
+}
+
+// (status, q)
+Result rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos, const at::Tensor& sin,
+                   const at::Tensor& positions, const at::Tensor& slots, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& ks,
+                   const at::Tensor& vs, const Maybe& qw, const Maybe& kw, double eps, bool interleaved, int64_t stream) {
+    const Result skip{-1, at::Tensor()};
+    hyq_rope_params p{};
+    const auto dev = q.device();
+    const int bits = ks.scalar_type() == at::kFloat ? 8 : 4;
+    if (!g_paged.rope_append || q.dim() != 3 || q.numel() == 0 || !ints(positions, at::kLong, 1, dev) ||
+        !rope_params(p, q, k, cos, sin, positions, qw, kw, eps, interleaved) || !plain(v, q.scalar_type(), 3, dev) || v.sizes() != k.sizes() ||
+        (at::GradMode::is_enabled() && v.requires_grad()) || !pool(kp, vp, ks, vs, dev, bits) || k.size(1) != kp.size(1) ||
+        k.size(2) != (bits == 4 ? 2 : 1) * kp.size(3) || !ints(slots, at::kLong, 1, dev) || slots.size(0) != k.size(0) || !rows16(v))
+        return skip;
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor qo = at::empty(q.sizes(), q.options());
+    p.q_out = qo.data_ptr();
+    const hyq_paged_pool to = pool_of(kp, vp, ks, vs, bits);
+    return {g_paged.rope_append(&p, ptr<uint16_t>(v), v.stride(0), v.stride(1), ptr<int64_t>(slots), &to, reinterpret_cast<void*>(stream)), qo};
+}
+
+void set_rope(int64_t size8, int64_t attention8, int64_t append8, int64_t gather8, int64_t rope, int64_t rope_append) {
+    g_paged.size8 = reinterpret_cast<AttentionSizeFn>(size8);
+    g_paged.attention8 = reinterpret_cast<AttentionFn>(attention8);
+    g_paged.append8 = reinterpret_cast<decltype(&hyq_paged8_append)>(append8);
+    g_paged.gather8 = reinterpret_cast<decltype(&hyq_paged8_gather)>(gather8);
+    g_paged.rope = reinterpret_cast<decltype(&hyq_qk_norm_rope)>(rope);
+    g_paged.rope_append = reinterpret_cast<decltype(&hyq_paged_rope_append)>(rope_append);
+}
+
+// sizeof(hyq_rope_params), offsetof(positions), sizeof(hyq_paged_pool)
+std::tuple<int64_t, int64_t, int64_t> rope_layout() {
+    return {static_cast<int64_t>(sizeof(hyq_rope_params)), static_cast<int64_t>(offsetof(hyq_rope_params, positions)),
+            static_cast<int64_t>(sizeof(hyq_paged_pool))};
 }
 
 // the paged parameter block's size and the offsets of two of its fields
@@ -380,7 +543,7 @@ std::tuple<int64_t, int64_t, int64_t> layout() {
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.def("signatures", [] { return 4; }, "counts up when a function of this module takes other arguments");
+    m.def("signatures", [] { return 5; }, "counts up when a function of this module takes other arguments");
     m.def("layout", &layout, "sizeof(hyq_decode_params), offsetof(seg_n), offsetof(dtype_flags)");
     m.def("set_entry", &set_entry, "the addresses of hyq_decode_hybrid and hyq_append_rows");
     m.def("decode", &decode, "fused_d_stage_decode eager fast path");
@@ -392,4 +555,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("paged_append", &paged_append, "new rows into the pages");
     m.def("paged_gather", &paged_gather, "rows of the pages");
     m.def("paged_attention", &paged_attention, "attention over the pages");
+    m.def("rope_layout", &rope_layout, "sizeof(hyq_rope_params), offsetof(positions), sizeof(hyq_paged_pool)");
+    m.def("set_rope", &set_rope, "the addresses of the 8-bit cache's and the rotation's entry points");
+    m.def("paged8_append", &paged8_append, "new rows into the 8-bit pages");
+    m.def("paged8_gather", &paged8_gather, "rows of the 8-bit pages");
+    m.def("qk_norm_rope", &qk_norm_rope, "rotation of queries and keys");
+    m.def("rope_append", &rope_append, "rotation on the way into the pages");
 }

@@ -309,15 +309,18 @@ def _load_fast_ext():
             # built against another torch: the Python paths take every call
             _FX = False
             return False
-        P, G = _lib.DecodeParams, _lib.PagedParams
+        P, G, R = _lib.DecodeParams, _lib.PagedParams, _lib.RopeParams
         # (a build of earlier sources has no signatures())
-        if (getattr(m, "signatures", lambda: 0)() == 4 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset)
-                and m.paged_layout() == (ctypes.sizeof(G), G.num_pages.offset, G.counters.offset)):
+        if (getattr(m, "signatures", lambda: 0)() == 5 and m.layout() == (ctypes.sizeof(P), P.seg_n.offset, P.dtype_flags.offset)
+                and m.paged_layout() == (ctypes.sizeof(G), G.num_pages.offset, G.counters.offset)
+                and m.rope_layout() == (ctypes.sizeof(R), R.positions.offset, ctypes.sizeof(_lib.PagedPool))):
             L = _lib.lib()
             at = lambda *fs: (ctypes.cast(f, ctypes.c_void_p).value for f in fs)  # noqa: E731
             m.set_entry(*at(L.hyq_decode_hybrid, L.hyq_append_rows))
             m.set_paged(*at(L.hyq_paged_batch, L.hyq_paged_append, L.hyq_paged_gather, L.hyq_paged_attention_workspace_size,
                             L.hyq_paged_attention))
+            m.set_rope(*at(L.hyq_paged8_attention_workspace_size, L.hyq_paged8_attention, L.hyq_paged8_append, L.hyq_paged8_gather,
+                           L.hyq_qk_norm_rope, L.hyq_paged_rope_append))
             mod = m
     _FX = mod
     return mod

@@ -280,17 +280,22 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     zero (lse -inf), as are the rows behind the last request of a padded batch
     (those of an `out` that is handed in are left as they are; it shares no
     memory with the inputs)."""
+    return _attend("paged_attention", 4, _check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
+                   window, return_lse, out)
+
+
+def _attend(name, bits, check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale, window, return_lse, out):
+    """An attention call over the pages of either cache: its C++ form, or the checked one."""
     fx, stream = _fast(q)
     if fx and out is None:
         try:
-            st, o, lse = fx.paged_attention(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens,
+            st, o, lse = fx.paged_attention(bits, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens,
                                             sm_scale, window, return_lse, stream, 0 if cu_seqlens is not None else _counters(q.device, stream))
             if st == 0:
                 return (o, lse) if return_lse else o
         except TypeError:
             pass
-    return _attention("paged_attention", _check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
-                      window, return_lse, out)
+    return _attention(name, check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale, window, return_lse, out)
 
 
 def _attention(name, check_pool, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale, window, return_lse, out):

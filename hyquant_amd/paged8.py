@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from .decode_d_stage import _HALF, _require_gpu, _stream
-from .paged import _aligned_rows, _attention, _check_page_size, _ints, _on, _row_strides
+from .paged import _aligned_rows, _attend, _check_page_size, _fast, _ints, _on, _row_strides
 
 SCALE_BLOCK = 16                           # tokens of a scale
 
@@ -68,6 +68,13 @@ def paged8_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages
     were appended by earlier calls; rows behind its last new one hold anything
     after the call.  A block with a value that is not finite, or past 127 * 2^40,
     has the scale NaN."""
+    fx, stream = _fast(k)
+    if fx:
+        try:
+            if fx.paged8_append(k, v, slots, k_pages, v_pages, k_scale, v_scale, stream) == 0:
+                return
+        except TypeError:
+            pass
     _require_gpu(k, "k")
     N, H, P, D = _check_pool8(k_pages, v_pages, k_scale, v_scale, k.device)
     if k.dtype not in _HALF or v.dtype != k.dtype:
@@ -91,6 +98,14 @@ def paged8_gather(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
                   dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The K and V rows [T, H, D] of slots (int64 [T]) as bf16 (exact) or fp16:
     code * scale rounded once; zeros for slots outside the pool."""
+    fx, stream = _fast(slots)
+    if fx and dtype in _HALF:
+        try:
+            st, k, v = fx.paged8_gather(slots, k_pages, v_pages, k_scale, v_scale, dtype == torch.float16, stream)
+            if st == 0:
+                return k, v
+        except TypeError:
+            pass
     _require_gpu(slots, "slots")
     _ints(slots, "slots", torch.int64, 1, slots.device)
     N, H, P, D = _check_pool8(k_pages, v_pages, k_scale, v_scale, slots.device)
@@ -114,5 +129,5 @@ def paged8_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     requests over their cached tokens (their own among them: append first), the
     same arguments, masks and results.  A row that sees a key of a block whose K
     or V scale is NaN, or not within [2^-40, 2^48], is NaN."""
-    return _attention("paged8_attention", _check_pool8, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
-                      window, return_lse, out)
+    return _attend("paged8_attention", 8, _check_pool8, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens, sm_scale,
+                   window, return_lse, out)

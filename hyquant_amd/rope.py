@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from .decode_d_stage import _HALF, _require_gpu, _stream
-from .paged import _aligned_rows, _check_pool, _ints, _on, _row_strides
+from .paged import _aligned_rows, _check_pool, _fast, _ints, _on, _row_strides
 from .paged8 import _check_pool8, _pool_struct
 
 _TABLE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -138,6 +138,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     [D]: RMS norm of each head, in fp32 or q's dtype.
 
     Returns (q, k) of the inputs' shapes and dtype, contiguous."""
+    fx, stream = _fast(q)
+    if fx:
+        try:
+            st, qo, ko = fx.qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved, stream)
+            if st == 0:
+                return qo, ko
+        except TypeError:
+            pass
     _require_gpu(q, "q")
     _no_grad(q, k, cos, sin, q_weight, k_weight)
     if q.dtype not in _HALF or q.dim() not in (3, 4):
@@ -168,6 +176,15 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: to
     of the rotated keys before any rounding to 16 bits.  A token whose position is
     outside the table or whose slot is outside the pool writes nothing; q's rows
     are zero where the position is.  Returns q rotated, contiguous."""
+    fx, stream = _fast(q)
+    if fx:
+        try:
+            st, qo = fx.rope_append(q, k, v, cos, sin, positions, slots, k_pages, v_pages, k_scale, v_scale, q_weight, k_weight, eps,
+                                    interleaved, stream)
+            if st == 0:
+                return qo
+        except TypeError:
+            pass
     _require_gpu(q, "q")
     _no_grad(q, k, v, cos, sin, q_weight, k_weight)
     if q.dtype not in _HALF or q.dim() != 3:

@@ -352,3 +352,37 @@ def test_gradients_are_refused():
         hq.paged_rope_append(x, x.clone().requires_grad_(), x, cos, sin, as_long([0, 1]), as_long([0, 1]), *pool)
     with torch.no_grad():
         hq.qk_norm_rope(x.clone().requires_grad_(), x, cos, sin)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_native_and_checked_calls_agree(bits, monkeypatch):
+    """The C++ form of the calls and the Python form launch the same kernels."""
+    from hyquant_amd import decode_d_stage as dd
+    from tests import paged8_util, paged_util
+    g = gen(50)
+    T, HQ, H, D, page, pages = 41, 8, 2, 64, 32, 6
+    x = randn(g, T, HQ + 2 * H, D, dtype=HF)
+    q, k, v = x[:, :HQ], x[:, HQ:HQ + H], x[:, HQ + H:]
+    w = randn(g, D, dtype=HF)
+    cos, sin = U.tables(T, 32, device=DEV)
+    dev_gen = torch.Generator(device="cuda").manual_seed(1)
+    pool = (paged_util if bits == 4 else paged8_util).make_pool(dev_gen, pages, H, page, D, "cuda")
+    slots, pos = as_long(list(range(30, 30 + T))), as_long(list(range(T)))
+    table, lens = torch.arange(4, dtype=torch.int32, device=DEV)[None], torch.tensor([71], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+
+    def calls():
+        p = tuple(t.clone() for t in pool)
+        out = hq.qk_norm_rope(q, k, cos, sin, q_weight=w, interleaved=True) + hq.qk_norm_rope(q[None], k[None], cos[None], sin[None], k_weight=w.float())
+        out += (hq.paged_rope_append(q, k, v, cos, sin, pos, slots, *p, q_weight=w, k_weight=w, eps=1e-5),)
+        out += tuple(t.clone() for t in p)
+        (hq.paged_append if bits == 4 else hq.paged8_append)(v, k, slots, *p)
+        out += p + (hq.paged_gather if bits == 4 else hq.paged8_gather)(slots, *p, dtype=HF)
+        attend = hq.paged_attention if bits == 4 else hq.paged8_attention
+        return out + attend(q, *p, table, lens, cu, sm_scale=0.2, window=90, return_lse=True) + (attend(q[:1], *p, table, lens),)
+
+    native = calls()
+    assert dd._FX
+    monkeypatch.setattr(dd, "_FX", False)
+    for i, (a, b) in enumerate(zip(native, calls())):
+        assert a.dtype == b.dtype and torch.equal(a, b), i
