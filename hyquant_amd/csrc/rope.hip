@@ -53,60 +53,64 @@ __device__ __forceinline__ float half_at(uint32_t w, int hi) {
     if constexpr (F16) return f16_bits_to_f32(static_cast<uint16_t>(hi ? w >> 16 : w));
     else return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
 }
-template <bool F16, typename T>
-__device__ __forceinline__ void unpack8(const uint4& raw, T (&x)[8]) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<T>(half_at<F16>(w[i >> 1], i & 1));
-}
-// `count` table or weight values (fp32: type 0, bf16: 1, fp16: 2), 4 * size aligned
-template <int COUNT, typename T>
-__device__ __forceinline__ void load_values(const void* p, int64_t at, int type, T (&f)[8]) {
+// four values (fp32: type 0, bf16: 1, fp16: 2), aligned to their size
+__device__ __forceinline__ void load4(const void* p, int64_t at, int type, float (&f)[4]) {
     if (type == 0) {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-#pragma unroll
-        for (int i = 0; i < COUNT / 4; ++i) {
-            const float4 v = s[i];
-            f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
-        }
+        const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
     } else {
-        const uint2* s = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
 #pragma unroll
-        for (int i = 0; i < COUNT / 4; ++i) {
-            const uint2 v = s[i];
-            const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                f[4 * i + j] = type == 1 ? half_at<false>(w[j >> 1], j & 1) : half_at<true>(w[j >> 1], j & 1);
-        }
+        for (int j = 0; j < 4; ++j) f[j] = type == 1 ? half_at<false>(j < 2 ? v.x : v.y, j & 1) : half_at<true>(j < 2 ? v.x : v.y, j & 1);
     }
 }
 
-template <int LPT, typename T>
-__device__ __forceinline__ T lanes_sum(T v) {
-#pragma unroll
-    for (int d = 1; d < LPT; d <<= 1) v += __shfl_xor(v, d, 64);
+// ---- over the D/8 lanes of a row (8 or 16), by DPP row operations ----
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false); }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = dpp<CTRL>(static_cast<int>(b)), hi = dpp<CTRL>(static_cast<int>(b >> 32));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <int LPT, typename T, typename OP>
+__device__ __forceinline__ T over_lanes(T v, OP op) {
+    v = op(v, dpp<0xb1>(v));             // quad_perm [1,0,3,2]
+    v = op(v, dpp<0x4e>(v));             // quad_perm [2,3,0,1]
+    v = op(v, dpp<0x141>(v));            // row_half_mirror
+    if (LPT == 16) v = op(v, dpp<0x140>(v));       // row_mirror
     return v;
 }
 template <int LPT, typename T>
-__device__ __forceinline__ T lanes_max(T v) {
-#pragma unroll
-    for (int d = 1; d < LPT; d <<= 1) {
-        const T o = __shfl_xor(v, d, 64);
-        v = o > v ? o : v;
-    }
-    return v;
-}
+__device__ __forceinline__ T lanes_sum(T v) { return over_lanes<LPT>(v, [](T a, T b) { return a + b; }); }
+template <int LPT, typename T>
+__device__ __forceinline__ T lanes_max(T v) { return over_lanes<LPT>(v, [](T a, T b) { return b > a ? b : a; }); }
 
-__device__ __forceinline__ float inv_root(float x) { return 1.0f / sqrtf(x); }
-__device__ __forceinline__ double inv_root(double x) { return 1.0 / sqrt(x); }
+// 1 / sqrt(x): the hardware's estimate (a unit in the last place of fp32; 2^-24,
+// and two Newton steps, in 64 bits), the division where that has no range
+__device__ __forceinline__ float inv_root(float x) {
+    return x >= 0x1p-126f && x < INFINITY ? __builtin_amdgcn_rsqf(x) : 1.0f / sqrtf(x);
+}
+__device__ __forceinline__ double inv_root(double x) {
+    if (!(x >= 0x1p-1000 && x < static_cast<double>(INFINITY))) return 1.0 / sqrt(x);
+    double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r = __builtin_fma(0.5 * r, __builtin_fma(-x * r, r, 1.0), r);
+    return r;
+}
 
 // The row of the table for token t; false: its position is outside of it
 __device__ __forceinline__ bool table_row(const RopeArgs& a, uint32_t t, int64_t& at) {
     if (a.positions) {
         const int64_t m = a.positions[t];
-        at = m * a.cs_m;
-        return static_cast<uint64_t>(m) < static_cast<uint64_t>(a.table_rows);
+        const bool ok = static_cast<uint64_t>(m) < static_cast<uint64_t>(a.table_rows);
+        at = ok ? m * a.cs_m : 0;
+        return ok;
     }
     const uint32_t b = t / a.n;
     at = b * a.cs_b + (t - b * a.n) * a.cs_m;
@@ -117,89 +121,155 @@ __device__ __forceinline__ const uint16_t* row_of(const RopeArgs& a, const Rows&
     return r.p + b * r.sb + (t - b * a.n) * r.sn + h * r.sh;
 }
 
-// Channels 8 sub .. of a row, normalised and rotated, in T.  All lanes of the
-// row take part.
-template <int D, bool F16, typename T>
-__device__ __forceinline__ void turn(const RopeArgs& a, const uint16_t* row, const void* w, int64_t at, int sub, T (&y)[8]) {
-    constexpr int LPT = D / 8;
-    const int lo = a.half >> 3;          // 8-channel chunks of a half
-    const bool apart = !a.interleaved;
-    const int other = !apart || sub >= 2 * lo ? sub : sub < lo ? sub + lo : sub - lo;     // the partners' chunk
-    T x[8], p[8];
-    unpack8<F16>(reinterpret_cast<const uint4*>(row)[sub], x);
-    unpack8<F16>(reinterpret_cast<const uint4*>(row)[other], p);
+// A lane's channels of a row: a .. a + 3 and b .. b + 3.  Each rotated pair is in
+// one lane: no value is read or computed twice.
+struct Lane {
+    int a, b;
+    bool turns;                          // they are rotated, by the table's columns j .. j + 3
+    int j;
+};
+__device__ __forceinline__ Lane lane_of(const RopeArgs& args, int sub) {
+    if (args.interleaved) return Lane{8 * sub, 8 * sub + 4, 4 * sub < args.half, 4 * sub};
+    const int left = 4 * sub - args.half;          // (half is a multiple of 8)
+    if (left < 0) return Lane{4 * sub, args.half + 4 * sub, true, 4 * sub};
+    return Lane{2 * args.half + 2 * left, 2 * args.half + 2 * left + 4, false, 0};
+}
+// A token's angles at the lane's channels, and the weights there
+struct Angles {
+    float c[4], s[4];
+};
+__device__ __forceinline__ Angles load_angles(const RopeArgs& a, const Lane& l, int64_t at) {
+    Angles k{};
+    if (l.turns) {
+        load4(a.cos, at + l.j, a.table_type, k.c);
+        load4(a.sin, at + l.j, a.table_type, k.s);
+    }
+    return k;
+}
+struct Weights {
+    float w[8];
+    bool norm;
+};
+template <bool F16>
+__device__ __forceinline__ Weights load_weights(const RopeArgs& a, const Lane& l, const void* w) {
+    Weights k{};
+    k.norm = w != nullptr;
     if (w) {
-        T sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
-        const T inv = inv_root(lanes_sum<LPT>(sum) * static_cast<T>(1.0 / D) + static_cast<T>(a.eps));
         const int type = a.weight_fp32 ? 0 : F16 ? 2 : 1;
-        T wx[8], wp[8];
-        load_values<8>(w, 8 * sub, type, wx);
-        load_values<8>(w, 8 * other, type, wp);
+        float lo[4], hi[4];
+        load4(w, l.a, type, lo);
+        load4(w, l.b, type, hi);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] * inv * wx[i];
-            p[i] = p[i] * inv * wp[i];
+        for (int i = 0; i < 4; ++i) { k.w[i] = lo[i]; k.w[4 + i] = hi[i]; }
+    }
+    return k;
+}
+struct Raw {
+    uint2 a, b;
+};
+__device__ __forceinline__ Raw load_raw(const uint16_t* row, const Lane& l) {
+    return Raw{*reinterpret_cast<const uint2*>(row + l.a), *reinterpret_cast<const uint2*>(row + l.b)};
+}
+template <bool F16>
+__device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = half_at<F16>(w[i >> 1], i & 1);
+}
+
+// A lane's channels normalised and rotated, in T; the norm's sum in SUM.  `most`: where it is
+// asked for, the sum of the magnitudes that each value is the sum of.
+template <int D, typename SUM, typename T, bool MOST = false>
+__device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Angles& k, const Weights& w, const float (&x)[8], T (&y)[8],
+                                     T (*most)[8] = nullptr) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
+    if (w.norm) {
+        SUM sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += static_cast<SUM>(x[i]) * static_cast<SUM>(x[i]);
+        const T inv = static_cast<T>(inv_root(lanes_sum<D / 8>(sum) * static_cast<SUM>(1.0 / D) + static_cast<SUM>(a.eps)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * static_cast<T>(w.w[i]);
+    }
+    auto mag = [](T z) { return z < 0 ? -z : z; };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = v[i];
+        if constexpr (MOST) (*most)[i] = mag(v[i]);
+    }
+    if (!l.turns) return;
+    auto pair = [&](int p, int q, T c, T s) {
+        const T f = v[p], g = v[q];
+        y[p] = f * c - g * s;
+        y[q] = g * c + f * s;
+        if constexpr (MOST) {
+            (*most)[p] = mag(f * c) + mag(g * s);
+            (*most)[q] = mag(g * c) + mag(f * s);
         }
-    }
-    if (sub >= 2 * lo) {
+    };
+    if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i];
-        return;
-    }
-    T c[8], s[8];
-    if (apart) {
-        const int j = 8 * (sub < lo ? sub : sub - lo);
-        load_values<8>(a.cos, at + j, a.table_type, c);
-        load_values<8>(a.sin, at + j, a.table_type, s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i] * c[i] + (sub < lo ? -p[i] : p[i]) * s[i];
+        for (int i = 0; i < 4; ++i) pair(2 * i, 2 * i + 1, k.c[i], k.s[i]);
     } else {
-        load_values<4>(a.cos, at + 4 * sub, a.table_type, c);
-        load_values<4>(a.sin, at + 4 * sub, a.table_type, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-            y[2 * i + 1] = x[2 * i + 1] * c[i] + x[2 * i] * s[i];
-        }
+        for (int i = 0; i < 4; ++i) pair(i, i + 4, k.c[i], k.s[i]);
     }
 }
 
 template <bool F16>
-__device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        o[i] = F16 ? f32_to_f16_bits(y[2 * i]) | (static_cast<uint32_t>(f32_to_f16_bits(y[2 * i + 1])) << 16)
-                   : pack_bf16x2(y[2 * i], y[2 * i + 1]);
-    return make_uint4(o[0], o[1], o[2], o[3]);
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    if constexpr (F16)
+        return make_uint2(f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16,
+                          f32_to_f16_bits(c) | static_cast<uint32_t>(f32_to_f16_bits(d)) << 16);
+    else return make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
 }
 
-// Row `row` of `heads` heads a token into contiguous rows; a position outside the
-// table gives zeros.
-template <int D, bool F16>
-__device__ __forceinline__ void rotate_row(const RopeArgs& a, const Rows& src, uint16_t* dst, const void* w, uint32_t row,
-                                           uint32_t rows, uint32_t heads, int sub) {
-    const uint32_t rr = row < rows ? row : rows - 1;
-    const uint32_t t = rr / heads, h = rr - t * heads;
+// HP heads of a token into contiguous rows: their loads in flight together, the
+// table's row and the weights loaded once.  A position outside the table gives zeros.
+template <int D, bool F16, int HP>
+__device__ __forceinline__ void rotate_heads(const RopeArgs& a, const Rows& src, uint16_t* dst, const void* w, uint32_t unit, uint32_t heads,
+                                             int sub) {
+    const uint32_t per = (heads + HP - 1) / HP, t = unit / per, h0 = (unit - t * per) * HP;
+    if (t >= a.tokens) return;
+    const Lane l = lane_of(a, sub);
+    Raw raw[HP];
+#pragma unroll
+    for (int i = 0; i < HP; ++i) raw[i] = load_raw(row_of(a, src, t, min(h0 + i, heads - 1)), l);
     int64_t at;
     const bool ok = table_row(a, t, at);
-    float y[8];
-    turn<D, F16, float>(a, row_of(a, src, t, h), w, ok ? at : 0, sub, y);
-    if (row >= rows) return;
-    const uint4 o = pack8<F16>(y);
-    reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row) * D)[sub] = ok ? o : make_uint4(0, 0, 0, 0);
+    const Angles k = load_angles(a, l, at);
+    const Weights wt = load_weights<F16>(a, l, w);
+    uint16_t* out = dst + (static_cast<int64_t>(t) * heads + h0) * D;
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+        float x[8], y[8];
+        unpack<F16>(raw[i], x);
+        turn<D, float>(a, l, k, wt, x, y);
+        if (h0 + i < heads) {
+            *reinterpret_cast<uint2*>(out + i * D + l.a) = ok ? pack4<F16>(y[0], y[1], y[2], y[3]) : make_uint2(0, 0);
+            *reinterpret_cast<uint2*>(out + i * D + l.b) = ok ? pack4<F16>(y[4], y[5], y[6], y[7]) : make_uint2(0, 0);
+        }
+    }
 }
 
-template <int D, bool F16>
+template <int D, bool F16, int HP>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
     const int sub = threadIdx.x & (LPT - 1);
     const uint32_t at = threadIdx.x / LPT;
-    if (blockIdx.x < a.q_blocks) rotate_row<D, F16>(a, a.q, a.qo, a.qw, blockIdx.x * (256 / LPT) + at, a.tokens * a.hq, a.hq, sub);
-    else rotate_row<D, F16>(a, a.k, a.ko, a.kw, (blockIdx.x - a.q_blocks) * (256 / LPT) + at, a.tokens * a.hk, a.hk, sub);
+    if (blockIdx.x < a.q_blocks) rotate_heads<D, F16, HP>(a, a.q, a.qo, a.qw, blockIdx.x * (256 / LPT) + at, a.hq, sub);
+    else rotate_heads<D, F16, HP>(a, a.k, a.ko, a.kw, (blockIdx.x - a.q_blocks) * (256 / LPT) + at, a.hk, sub);
 }
+
+// ---- codes of rotated keys ----
+// They are those of the formula: a key is rotated in 32 bits (the norm's sum in 64),
+// and again in 64 bits where 32 bits' error may reach over a code's or a scale's
+// border (a wavefront decides for its rows; one of 50 to 100 does).  The error of
+// a value is at most 5 2^-24 of the magnitudes that it is the sum of: the inverse
+// root's rounding, two products, and the rotation's product and sum.
+constexpr float TURN_ERROR = 6.0f * 0x1p-24f;
 
 // The correctly rounded quotient x / s (s > 0 finite) from inv = RN(1 / s)
 __device__ __forceinline__ double quot_rn(double x, double s, double inv) {
@@ -207,59 +277,101 @@ __device__ __forceinline__ double quot_rn(double x, double s, double inv) {
     return __builtin_fma(__builtin_fma(-q, s, x), inv, q);
 }
 
-// A row of 4-bit codes: scale = fp16(fp32(max(amax, 1e-5) / 7)), code =
-// RNE(x / scale).  Keys are rotated in 64 bits, so that the codes are those of
-// the formula (a key next to a code's border by less than 32 bits' error would
-// else fall on the wrong side).
+// 4 bits: scale = fp16(fp32(max(amax, 1e-5) / 7)), code = RNE(x / scale)
 template <int D, bool F16>
+__device__ __forceinline__ void key_codes4(const RopeArgs& a, const Lane& l, const Angles& k, const Weights& wt, const Raw& raw, _Float16& s16, int (&c)[8]) {
+    float x[8], y[8], err[8];
+    unpack<F16>(raw, x);
+    turn<D, double, float, true>(a, l, k, wt, x, y, &err);
+    float amax = 0.f, off = 0.f;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        err[i] *= TURN_ERROR;
+        amax = fmaxf(amax, fabsf(y[i]));
+        off = fmaxf(off, err[i]);
+        fine = fine && y[i] == y[i];
+    }
+    amax = lanes_max<D / 8>(amax);
+    off = lanes_max<D / 8>(off) + amax * 0x1p-22f;
+    s16 = static_cast<_Float16>(fmaxf(amax, 1e-5f) * (1.0f / 7.0f));
+    const float sf = static_cast<float>(s16), inv = 1.0f / sf;
+    fine = fine && sf <= 65504.0f && static_cast<_Float16>(fmaxf(amax - off, 1e-5f) * (1.0f / 7.0f)) == s16 &&
+           static_cast<_Float16>(fmaxf(amax + off, 1e-5f) * (1.0f / 7.0f)) == s16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = y[i] * inv, z = rintf(q);
+        // (2^-19: the quotient's own error, at most 8 of three roundings)
+        fine = fine && fabsf(q - z) + err[i] * inv < 0.5f - 0x1p-19f;
+        c[i] = static_cast<int>(fminf(fmaxf(z, -8.0f), 7.0f));
+    }
+    if (__builtin_amdgcn_ballot_w64(!fine)) {
+        double v[8], top = 0.0;
+        turn<D, double>(a, l, k, wt, x, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmax(top, fabs(v[i]));
+        top = fmax(lanes_max<D / 8>(top), 1e-5);
+        s16 = static_cast<_Float16>(static_cast<float>(top / 7.0));
+        const double sd = static_cast<double>(s16), invd = 1.0 / sd;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double q = sd <= 65504.0 ? quot_rn(v[i], sd, invd) : v[i] / sd;
+            c[i] = static_cast<int>(fmin(fmax(rint(q), -8.0), 7.0));
+        }
+    }
+}
+
+// q's heads, and a K and a V row of a token and head each
+template <int D, bool F16, int HP>
 __global__ __launch_bounds__(256) void paged_rope_append_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
     const int sub = threadIdx.x & (LPT - 1);
-    const uint32_t at = threadIdx.x / LPT;
+    const uint32_t unit = threadIdx.x / LPT;
     if (blockIdx.x < a.q_blocks) {
-        rotate_row<D, F16>(a, a.q, a.qo, a.qw, blockIdx.x * (256 / LPT) + at, a.tokens * a.hq, a.hq, sub);
+        rotate_heads<D, F16, HP>(a, a.q, a.qo, a.qw, blockIdx.x * (256 / LPT) + unit, a.hq, sub);
         return;
     }
-    // (K and V rows of a token follow each other)
-    const uint32_t row = (blockIdx.x - a.q_blocks) * (256 / LPT) + at, rows = a.tokens * a.hk * 2;
-    const uint32_t rr = row < rows ? row : rows - 1;
-    const uint32_t t = rr / (2 * a.hk), hh = rr - t * (2 * a.hk);
-    const bool is_v = hh >= a.hk;
-    const uint32_t h = is_v ? hh - a.hk : hh;
+    const uint32_t row = (blockIdx.x - a.q_blocks) * (256 / LPT) + unit, t = row / a.hk, h = row - t * a.hk;
+    if (t >= a.tokens) return;
+    const Lane l = lane_of(a, sub);
+    const Raw kr = load_raw(row_of(a, a.k, t, h), l);
+    const uint4 vr = reinterpret_cast<const uint4*>(row_of(a, a.v, t, h))[sub];
     const int64_t slot = a.pool.slots[t];
-    int64_t tab;
-    const bool ok = table_row(a, t, tab);
-    _Float16 s16;
-    uint32_t c[8];
-    if (is_v) {
-        float x[8], amax = 0.f;
-        unpack8<F16>(reinterpret_cast<const uint4*>(row_of(a, a.v, t, h))[sub], x);
+    int64_t at;
+    const bool ok = table_row(a, t, at);
+    const Angles k = load_angles(a, l, at);
+    const Weights wt = load_weights<F16>(a, l, a.kw);
+    float x[8], amax = 0.f;
+    const uint32_t w[4] = {vr.x, vr.y, vr.z, vr.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-        quant_row_codes<4>(x, fmaxf(lanes_max<LPT>(amax), 1e-5f), s16, c);
-    } else {
-        double x[8], amax = 0.0;
-        turn<D, F16, double>(a, row_of(a, a.k, t, h), a.kw, ok ? tab : 0, sub, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmax(amax, fabs(x[i]));
-        amax = fmax(lanes_max<LPT>(amax), 1e-5);
-        s16 = static_cast<_Float16>(static_cast<float>(amax / 7.0));
-        const double sf = static_cast<double>(s16), inv = 1.0 / sf;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double q = sf <= 65504.0 ? quot_rn(x[i], sf, inv) : x[i] / sf;
-            c[i] = static_cast<uint32_t>(static_cast<int>(fmin(fmax(rint(q), -8.0), 7.0)));
-        }
+    for (int i = 0; i < 8; ++i) {
+        x[i] = half_at<F16>(w[i >> 1], i & 1);
+        amax = fmaxf(amax, fabsf(x[i]));
     }
-    if (row >= rows || !ok || slot < 0 || slot >= a.pool.num_slots) return;
-    uint32_t word = 0;
+    _Float16 ks, vs;
+    uint32_t cv[8];
+    int ck[8];
+    quant_row_codes<4>(x, fmaxf(lanes_max<LPT>(amax), 1e-5f), vs, cv);
+    key_codes4<D, F16>(a, l, k, wt, kr, ks, ck);
+    if (!ok || slot < 0 || slot >= a.pool.num_slots) return;
+    uint32_t vw = 0, ka = 0, kb = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) word |= (c[i] & 15u) << (4 * i);
+    for (int i = 0; i < 8; ++i) vw |= (cv[i] & 15u) << (4 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ka |= (static_cast<uint32_t>(ck[i]) & 15u) << (4 * i);
+        kb |= (static_cast<uint32_t>(ck[4 + i]) & 15u) << (4 * i);
+    }
     const int64_t page = slot >> a.pool.page_log2, off = slot & ((1 << a.pool.page_log2) - 1);
-    int8_t* dst = (is_v ? a.pool.vp : a.pool.kp) + page * a.pool.ps_page + h * a.pool.ps_head + off * (D / 2);
-    reinterpret_cast<uint32_t*>(dst)[sub] = word;
-    if (sub == 0)
-        static_cast<uint16_t*>(is_v ? a.pool.vs : a.pool.ks)[page * a.pool.ss_page + h * a.pool.ss_head + off] = __builtin_bit_cast(uint16_t, s16);
+    const int64_t to = page * a.pool.ps_page + h * a.pool.ps_head + off * (D / 2);
+    reinterpret_cast<uint32_t*>(a.pool.vp + to)[sub] = vw;
+    *reinterpret_cast<uint16_t*>(a.pool.kp + to + l.a / 2) = static_cast<uint16_t>(ka);
+    *reinterpret_cast<uint16_t*>(a.pool.kp + to + l.b / 2) = static_cast<uint16_t>(kb);
+    if (sub == 0) {
+        const int64_t so = page * a.pool.ss_page + h * a.pool.ss_head + off;
+        static_cast<uint16_t*>(a.pool.ks)[so] = __builtin_bit_cast(uint16_t, ks);
+        static_cast<uint16_t*>(a.pool.vs)[so] = __builtin_bit_cast(uint16_t, vs);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -278,119 +390,230 @@ __device__ __forceinline__ int exponent(double amax) {
 __device__ __forceinline__ int exponent(float amax) { return exponent(static_cast<double>(amax)); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-// 16 tokens' new rows of one K or V head.  A run of tokens whose slots lie in one
-// block is worked on by the workgroup that has its first token (31 rows at
-// most): the block's scale is the largest that its new rows, and the rows before
-// them, need; rows before the run's first live one (a token whose position is
-// outside the table is not) stay, and are rounded again where the scale has
-// grown.
-template <int D, bool F16, bool ROPE>
-__global__ __launch_bounds__(32 * (D / 8)) void paged8_append_kernel(RopeArgs a) {
-    constexpr int LPT = D / 8, ROWS = 32;
-    const int sub = threadIdx.x & (LPT - 1), r = threadIdx.x / LPT;
+// A run of tokens whose slots lie in one block is worked on by the workgroup that
+// has its first token among its 16, K and V of one head: the block's scale is the
+// largest that its new rows, and the rows before them, need; rows before the
+// run's first live one (a token whose position is outside the table is not) stay,
+// and are rounded again where the scale has grown.  The rows of a long run that
+// starts at the window's token f are the tokens f .. f + 15: the lanes of the first f
+// rows take those behind the window.  Only where more runs start in it may a second pass
+// be left.
+template <int D, bool F16, bool ROPE, int HP>
+__global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
+    constexpr int LPT = D / 8;
+    const int sub = threadIdx.x & (LPT - 1), r0 = threadIdx.x / LPT, lane = threadIdx.x & 63;
     if constexpr (ROPE) {
         if (blockIdx.x < a.q_blocks) {
-            rotate_row<D, F16>(a, a.q, a.qo, a.qw, blockIdx.x * ROWS + r, a.tokens * a.hq, a.hq, sub);
+            rotate_heads<D, F16, HP>(a, a.q, a.qo, a.qw, blockIdx.x * 16 + r0, a.hq, sub);
             return;
         }
     }
-    __shared__ int64_t slot_of[ROWS];
-    __shared__ uint32_t starts, live;
-    __shared__ int need[ROWS];
-    const uint32_t i = blockIdx.x - a.q_blocks, win = i / (2 * a.hk), hh = i - win * (2 * a.hk);
-    const bool is_v = hh >= a.hk;
-    const uint32_t h = is_v ? hh - a.hk : hh, t0 = win * 16;
-    if (threadIdx.x < 64) {              // tokens t0 - 1 .. t0 + 31
-        const int64_t t = static_cast<int64_t>(t0) + threadIdx.x - 1;
-        int64_t slot = -1;
-        bool ok = true;
-        if (threadIdx.x <= ROWS && t >= 0 && t < a.tokens) {
+    __shared__ int need[2][32];
+    const uint32_t i = blockIdx.x - a.q_blocks, win = i / a.hk, h = i - win * a.hk, t0 = win * 16;
+
+    // ---- the runs: lane l of each wavefront looks at token t0 - 1 + l, up to t0 + 31 ----
+    int64_t slot = -1;
+    bool ok = true;
+    {
+        const int64_t t = static_cast<int64_t>(t0) + lane - 1;
+        if (lane <= 32 && t >= 0 && t < a.tokens) {
             slot = a.pool.slots[t];
             if (slot >= a.pool.num_slots || slot < 0) slot = -1;
             int64_t unused;
             if constexpr (ROPE) ok = table_row(a, static_cast<uint32_t>(t), unused);
         }
-        const int64_t block = slot >> 4, before = __shfl_up(block, 1, 64);
-        const uint64_t m = __builtin_amdgcn_ballot_w64(block != before), l = __builtin_amdgcn_ballot_w64(ok && slot >= 0);
-        if (threadIdx.x == 0) { starts = static_cast<uint32_t>(m >> 1); live = static_cast<uint32_t>(l >> 1); }
-        if (threadIdx.x >= 1 && threadIdx.x <= ROWS) slot_of[threadIdx.x - 1] = slot;
     }
-    __syncthreads();
-    const uint32_t upto = starts & (0xffffffffu >> (31 - r));
-    const int run = upto ? 31 - __builtin_clz(upto) : -1;        // the run's first token, its live ones and the first of them
-    const uint32_t more = run >= 0 && run < 31 ? starts & (0xfffffffeu << run) : 0;
-    const uint32_t mine = run >= 0 ? live & (0xffffffffu << run) & (more ? (1u << __builtin_ctz(more)) - 1u : 0xffffffffu) : 0;
-    const bool active = run < 16 && (mine >> r) & 1;
-    const int first = mine ? __builtin_ctz(mine) : 0;
-    const int64_t block = slot_of[r] >> 4;
-    using T = std::conditional_t<ROPE, double, float>;
-    T x[8];
-    int e = NO_E;
-    const uint32_t t = t0 + r;
-    if (active) {
-        if (is_v) unpack8<F16>(reinterpret_cast<const uint4*>(row_of(a, a.v, t, h))[sub], x);
-        else if constexpr (!ROPE) unpack8<F16>(reinterpret_cast<const uint4*>(row_of(a, a.k, t, h))[sub], x);
-        else {
-            int64_t tab;
-            table_row(a, t, tab);
-            turn<D, F16, T>(a, row_of(a, a.k, t, h), a.kw, tab, sub, x);
+    const int64_t block = slot >> 4, before = __shfl_up(block, 1, 64);
+    const uint32_t starts = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(block != before) >> 1);
+    const uint32_t live = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok && slot >= 0) >> 1);
+    if (!(starts & 0xffffu)) return;                                     // (all tokens belong to a run that started before)
+    const int f = __builtin_ctz(starts), end = starts >> 16 ? 16 + __builtin_ctz(starts >> 16) : 32;
+    const bool twice = end > 16 + f;
+
+    struct Row {
+        int r;                           // the token's place behind t0
+        bool active;
+        uint32_t mine;                   // its run's live tokens
+        int64_t slot;
+    };
+    auto row_at = [&](int p) {
+        Row w;
+        w.r = r0 + 16 * (p ? r0 >= f : r0 < f);
+        const bool out = w.r >= end || w.r < f || (p && r0 < f);
+        const uint32_t upto = starts & (0xffffffffu >> (31 - w.r));
+        const int run = upto ? 31 - __builtin_clz(upto) : 0;
+        const uint32_t more = run < 31 ? starts & (0xfffffffeu << run) : 0;
+        w.mine = live & (0xffffffffu << run) & (more ? (1u << __builtin_ctz(more)) - 1u : 0xffffffffu);
+        w.active = !out && (w.mine >> w.r) & 1;
+        w.slot = __shfl(slot, w.r + 1, 64);
+        return w;
+    };
+    const Lane plain{8 * sub, 8 * sub + 4, false, 0}, l = ROPE ? lane_of(a, sub) : plain;
+    const Weights wt = load_weights<F16>(a, l, ROPE ? a.kw : nullptr);
+    Raw kr, vr;
+    Angles k{};
+    auto load = [&](const Row& w) {
+        const uint32_t t = min(t0 + w.r, a.tokens - 1);
+        kr = load_raw(row_of(a, a.k, t, h), l);
+        vr = load_raw(row_of(a, a.v, t, h), plain);
+        if constexpr (ROPE) {
+            int64_t at;
+            table_row(a, t, at);
+            k = load_angles(a, l, at);
         }
-        T amax = 0;
-        bool bad = false;
+    };
+    // a K row's values, and how far off they may be (formed anew for the codes: kept
+    // they would take 16 registers more)
+    auto keys = [&](float (&x)[8], float (&y)[8], float (&err)[8]) {
+        unpack<F16>(kr, x);
+        if constexpr (ROPE) {
+            turn<D, double, float, true>(a, l, k, wt, x, y, &err);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) err[j] *= TURN_ERROR;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { y[j] = x[j]; err[j] = 0.f; }
+        }
+    };
+    auto largest = [&](const float (&y)[8], float& amax) {               // the row's exponent; the lane's largest magnitude
+        bool fine = true;
+        amax = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const T y = x[j] < 0 ? -x[j] : x[j];
-            bad |= !(y <= static_cast<T>(127.0 * 0x1p40));
-            amax = y > amax ? y : amax;
+            fine = fine && fabsf(y[j]) <= 127.0f * 0x1p40f;              // (a NaN is not)
+            amax = fmaxf(amax, fabsf(y[j]));
         }
-        e = lanes_max<LPT>(bad ? BAD_E : exponent(amax));
-    }
-    const int64_t page = block * BLOCK >> a.pool.page_log2;      // (an inactive row's address is not used)
-    const int32_t off = static_cast<int32_t>(block * BLOCK & ((1 << a.pool.page_log2) - 1));
-    int8_t* const rows = (is_v ? a.pool.vp : a.pool.kp) + page * a.pool.ps_page + h * a.pool.ps_head + off * D;
-    float* const scale = static_cast<float*>(is_v ? a.pool.vs : a.pool.ks) + page * a.pool.ss_page + h * a.pool.ss_head + off / BLOCK;
-    const int kept = active ? static_cast<int>(slot_of[first] & (BLOCK - 1)) : 0;
-    const float old = kept ? *scale : 0.f;       // (read by all before the run's first row writes it)
-    if (sub == 0) need[r] = e;
-    __syncthreads();
-    if (!active) return;
-    for (uint32_t left = mine; left; left &= left - 1) e = max(e, need[__builtin_ctz(left)]);
-    if (kept) {
-        if (!(old >= 0.f && old <= pow2(MOST_E + 1))) e = BAD_E;
-        else if (old > 0.f) {            // the smallest power of two from it on
-            const uint32_t b = __float_as_uint(old);
-            e = max(e, static_cast<int>(b >> 23) - 127 + (b & 0x7fffffu ? 1 : 0));
-        }
-    }
-    const bool bad = e > MOST_E + 1;
-    const float now = bad ? __builtin_nanf("") : pow2(e), inv = bad ? 0.f : pow2(-e);
-    uint32_t c[8];
+        return lanes_max<LPT>(fine ? exponent(amax) : BAD_E);
+    };
+    auto measure = [&](const Row& w) {
+        float x[8], y[8], err[8], amax, off = 0.f;
+        keys(x, y, err);
+        int e = largest(y, amax);
+        if constexpr (ROPE) {            // the row's largest may be another value's than the formula's, but not its exponent
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if constexpr (ROPE) c[j] = static_cast<uint32_t>(static_cast<int>(rint(x[j] * static_cast<double>(inv)))) & 255u;
-        else c[j] = static_cast<uint32_t>(static_cast<int>(rintf(x[j] * inv))) & 255u;
-    }
-    const uint2 word = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-    const int row = static_cast<int>(slot_of[r] & (BLOCK - 1));
-    reinterpret_cast<uint2*>(rows + row * D)[sub] = word;
-    if (r != first) return;
-    if (kept && now != old) {
-        const float by = old * inv;
-        for (int j = 0; j < kept; ++j) {
-            uint2* const p = reinterpret_cast<uint2*>(rows + j * D) + sub;
-            const uint2 w = *p;
-            const uint32_t in[2] = {w.x, w.y};
-            uint32_t out[2] = {0, 0};
+            for (int j = 0; j < 8; ++j) off = fmaxf(off, err[j]);
+            amax = lanes_max<LPT>(amax);
+            off = lanes_max<LPT>(off) + amax * 0x1p-22f;
+            const bool sure = exponent(amax + off) == e && exponent(amax - off) == e;
+            if (__builtin_amdgcn_ballot_w64(w.active && !sure)) {
+                double v[8], top = 0.0;
+                bool good = true;
+                turn<D, double>(a, l, k, wt, x, v);
 #pragma unroll
-            for (int i8 = 0; i8 < 8; ++i8) {
-                const int code = static_cast<int8_t>(in[i8 >> 2] >> (8 * (i8 & 3)));
-                const int again = static_cast<int>(rintf(static_cast<float>(code) * by));
-                out[i8 >> 2] |= (static_cast<uint32_t>(again) & 255u) << (8 * (i8 & 3));
+                for (int j = 0; j < 8; ++j) {
+                    good = good && fabs(v[j]) <= 127.0 * 0x1p40;
+                    top = fmax(top, fabs(v[j]));
+                }
+                e = lanes_max<LPT>(good ? exponent(top) : BAD_E);
             }
-            *p = make_uint2(out[0], out[1]);
         }
+        unpack<F16>(vr, y);
+        const int ev = largest(y, amax);
+        if (sub == 0 && w.active) { need[0][w.r] = e; need[1][w.r] = ev; }
+    };
+
+    const int64_t hp = h * a.pool.ps_head, hs = h * a.pool.ss_head;
+    struct Place {
+        int64_t rows, scale;             // of the block, from the pools' first
+        int first, kept;
+        float old[2];
+    };
+    auto place = [&](const Row& w) {
+        Place q;
+        const int64_t s = w.active ? w.slot : 0, page = s >> a.pool.page_log2;
+        const int32_t off = static_cast<int32_t>(s & ((1 << a.pool.page_log2) - 1)) & ~(BLOCK - 1);
+        q.first = w.active ? __builtin_ctz(w.mine) : 0;
+        q.rows = page * a.pool.ps_page + hp + off * D;
+        q.scale = page * a.pool.ss_page + hs + off / BLOCK;
+        const int kept = static_cast<int>(__shfl(slot, q.first + 1, 64)) & (BLOCK - 1);
+        q.kept = w.active ? kept : 0;
+        q.old[0] = q.kept ? static_cast<const float*>(a.pool.ks)[q.scale] : 0.f;
+        q.old[1] = q.kept ? static_cast<const float*>(a.pool.vs)[q.scale] : 0.f;
+        return q;
+    };
+    auto write = [&](const Row& w, const Place& q) {
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+            const float old = q.old[kind];
+            int e = NO_E;
+            for (uint32_t left = w.active ? w.mine : 0; left; left &= left - 1) e = max(e, need[kind][__builtin_ctz(left)]);
+            if (q.kept) {
+                if (!(old >= 0.f && old <= pow2(MOST_E + 1))) e = BAD_E;
+                else if (old > 0.f) {    // the smallest power of two from it on
+                    const uint32_t b = __float_as_uint(old);
+                    e = max(e, static_cast<int>(b >> 23) - 127 + (b & 0x7fffffu ? 1 : 0));
+                }
+            }
+            const bool bad = e > MOST_E + 1;
+            e = max(e, -126);            // (an inactive row's)
+            const float now = bad ? __builtin_nanf("") : pow2(e), inv = bad ? 0.f : pow2(-e);
+            float x[8], y[8], err[8];
+            bool fine = true;
+            if (kind == 0) keys(x, y, err);
+            else unpack<F16>(vr, y);
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float z = y[j] * inv, n = rintf(z);
+                if (ROPE && kind == 0) fine = fine && fabsf(z - n) + err[j] * inv < 0.5f - 0x1p-23f;
+                c[j] = static_cast<int>(n);
+            }
+            if (ROPE && kind == 0) {
+                if (__builtin_amdgcn_ballot_w64(w.active && !bad && !fine)) {
+                    double v[8];
+                    turn<D, double>(a, l, k, wt, x, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) c[j] = static_cast<int>(rint(v[j] * static_cast<double>(inv)));
+                }
+            }
+            if (!w.active) continue;
+            auto word = [&](int j) {
+                return (static_cast<uint32_t>(c[j]) & 255u) | (static_cast<uint32_t>(c[j + 1]) & 255u) << 8 |
+                       (static_cast<uint32_t>(c[j + 2]) & 255u) << 16 | static_cast<uint32_t>(c[j + 3]) << 24;
+            };
+            int8_t* const rows = (kind ? a.pool.vp : a.pool.kp) + q.rows;
+            int8_t* const row = rows + (w.slot & (BLOCK - 1)) * D;
+            *reinterpret_cast<uint32_t*>(row + (kind ? plain.a : l.a)) = word(0);
+            *reinterpret_cast<uint32_t*>(row + (kind ? plain.b : l.b)) = word(4);
+            if (w.r != q.first) continue;
+            if (q.kept && now != old) {
+                const float by = old * inv;
+                for (int j = 0; j < q.kept; ++j) {
+                    uint2* const to = reinterpret_cast<uint2*>(rows + j * D) + sub;
+                    const uint2 v = *to;
+                    const uint32_t in[2] = {v.x, v.y};
+                    uint32_t out[2] = {0, 0};
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const int code = static_cast<int8_t>(in[n >> 2] >> (8 * (n & 3)));
+                        out[n >> 2] |= (static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(code) * by))) & 255u) << (8 * (n & 3));
+                    }
+                    *to = make_uint2(out[0], out[1]);
+                }
+            }
+            if (sub == 0) static_cast<float*>(kind ? a.pool.vs : a.pool.ks)[q.scale] = now;
+        }
+    };
+
+    Row w = row_at(0);
+    load(w);
+    Place q = place(w);
+    measure(w);
+    if (twice) {                         // (the same in all lanes)
+        const Place q0 = q;
+        w = row_at(1);
+        load(w);
+        q = place(w);
+        measure(w);
+        __syncthreads();
+        write(w, q);
+        w = row_at(0);
+        load(w);
+        write(w, q0);
+    } else {
+        __syncthreads();
+        write(w, q);
     }
-    if (sub == 0) *scale = now;
 }
 
 // Rows of the cache by slot as bf16 or fp16 values, code * scale rounded once
@@ -414,7 +637,8 @@ __global__ __launch_bounds__(256) void paged8_gather_kernel(Pool pool, uint16_t*
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(static_cast<int8_t>(in[i >> 2] >> (8 * (i & 3)))) * s;
     }
-    reinterpret_cast<uint4*>((is_v ? ov : ok) + static_cast<int64_t>(row) * D)[sub] = pack8<F16>(y);
+    const uint2 lo = pack4<F16>(y[0], y[1], y[2], y[3]), hi = pack4<F16>(y[4], y[5], y[6], y[7]);
+    reinterpret_cast<uint4*>((is_v ? ov : ok) + static_cast<int64_t>(row) * D)[sub] = make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
 // ---------------------------------------------------------------------------
@@ -506,18 +730,49 @@ Pool pool_of(const hyq_paged_pool& p, const int64_t* slots) {
 
 unsigned blocks_of(uint64_t rows, unsigned per) { return static_cast<unsigned>((rows + per - 1) / per); }
 
-template <bool ROPE>
-int launch_append8(RopeArgs a, int head_dim, bool fp16, hipStream_t st) {
-    a.q_blocks = ROPE ? blocks_of(static_cast<uint64_t>(a.tokens) * a.hq, 32) : 0;
-    const dim3 grid(a.q_blocks + blocks_of(a.tokens, 16) * a.hk * 2);
+// Heads that a lane group takes after the other: with more the table's row and the
+// weights are loaded less often and more loads are in flight, with one the
+// rows of a small step spread over more of the chip.
+constexpr int MANY = 4;
+bool many_heads(uint64_t rows, int head_dim) { return rows * (head_dim / 8) >= (1 << 20); }
+
+template <bool ROPE, int HP>
+void append8(RopeArgs a, int head_dim, bool fp16, hipStream_t st) {
+    a.q_blocks = ROPE ? blocks_of(static_cast<uint64_t>(a.tokens) * ((a.hq + HP - 1) / HP), 16) : 0;
+    const dim3 grid(a.q_blocks + blocks_of(a.tokens, 16) * a.hk);
     if (head_dim == 128) {
-        if (fp16) paged8_append_kernel<128, true, ROPE><<<grid, dim3(512), 0, st>>>(a);
-        else paged8_append_kernel<128, false, ROPE><<<grid, dim3(512), 0, st>>>(a);
+        if (fp16) paged8_append_kernel<128, true, ROPE, HP><<<grid, dim3(256), 0, st>>>(a);
+        else paged8_append_kernel<128, false, ROPE, HP><<<grid, dim3(256), 0, st>>>(a);
     } else {
-        if (fp16) paged8_append_kernel<64, true, ROPE><<<grid, dim3(256), 0, st>>>(a);
-        else paged8_append_kernel<64, false, ROPE><<<grid, dim3(256), 0, st>>>(a);
+        if (fp16) paged8_append_kernel<64, true, ROPE, HP><<<grid, dim3(128), 0, st>>>(a);
+        else paged8_append_kernel<64, false, ROPE, HP><<<grid, dim3(128), 0, st>>>(a);
     }
-    return check_launch("hyq_paged8_append");
+}
+template <int HP>
+void append4(RopeArgs a, int head_dim, bool fp16, hipStream_t st) {
+    const unsigned per = 256 / (head_dim / 8);
+    a.q_blocks = blocks_of(static_cast<uint64_t>(a.tokens) * ((a.hq + HP - 1) / HP), per);
+    const dim3 grid(a.q_blocks + blocks_of(static_cast<uint64_t>(a.tokens) * a.hk, per));
+    if (head_dim == 128) {
+        if (fp16) paged_rope_append_kernel<128, true, HP><<<grid, dim3(256), 0, st>>>(a);
+        else paged_rope_append_kernel<128, false, HP><<<grid, dim3(256), 0, st>>>(a);
+    } else {
+        if (fp16) paged_rope_append_kernel<64, true, HP><<<grid, dim3(256), 0, st>>>(a);
+        else paged_rope_append_kernel<64, false, HP><<<grid, dim3(256), 0, st>>>(a);
+    }
+}
+template <int HP>
+void rotate(RopeArgs a, int head_dim, bool fp16, hipStream_t st) {
+    const unsigned per = 256 / (head_dim / 8);
+    a.q_blocks = blocks_of(static_cast<uint64_t>(a.tokens) * ((a.hq + HP - 1) / HP), per);
+    const dim3 grid(a.q_blocks + blocks_of(static_cast<uint64_t>(a.tokens) * ((a.hk + HP - 1) / HP), per));
+    if (head_dim == 128) {
+        if (fp16) qk_norm_rope_kernel<128, true, HP><<<grid, dim3(256), 0, st>>>(a);
+        else qk_norm_rope_kernel<128, false, HP><<<grid, dim3(256), 0, st>>>(a);
+    } else {
+        if (fp16) qk_norm_rope_kernel<64, true, HP><<<grid, dim3(256), 0, st>>>(a);
+        else qk_norm_rope_kernel<64, false, HP><<<grid, dim3(256), 0, st>>>(a);
+    }
 }
 
 int check_rows(const std::string& w, const hyq_rope_params* p, const uint16_t* v, int64_t vt, int64_t vh, const int64_t* slots) {
@@ -536,19 +791,10 @@ using namespace hyq;
 
 extern "C" int hyq_qk_norm_rope(const hyq_rope_params* p, void* stream) {
     if (int st = check_rope("hyq_qk_norm_rope: ", p, false)) return st;
-    RopeArgs a = args_of(*p);
-    const unsigned per = 256 / (p->head_dim / 8);
-    a.q_blocks = blocks_of(static_cast<uint64_t>(a.tokens) * a.hq, per);
-    const unsigned grid = a.q_blocks + blocks_of(static_cast<uint64_t>(a.tokens) * a.hk, per);
-    if (a.tokens == 0 || grid == 0) return HYQ_OK;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    if (p->head_dim == 128) {
-        if (p->dtype_fp16) qk_norm_rope_kernel<128, true><<<dim3(grid), dim3(256), 0, st>>>(a);
-        else qk_norm_rope_kernel<128, false><<<dim3(grid), dim3(256), 0, st>>>(a);
-    } else {
-        if (p->dtype_fp16) qk_norm_rope_kernel<64, true><<<dim3(grid), dim3(256), 0, st>>>(a);
-        else qk_norm_rope_kernel<64, false><<<dim3(grid), dim3(256), 0, st>>>(a);
-    }
+    const RopeArgs a = args_of(*p);
+    if (a.tokens == 0 || a.hq + a.hk == 0) return HYQ_OK;
+    if (many_heads(static_cast<uint64_t>(a.tokens) * (a.hq + a.hk), p->head_dim)) rotate<MANY>(a, p->head_dim, p->dtype_fp16, static_cast<hipStream_t>(stream));
+    else rotate<1>(a, p->head_dim, p->dtype_fp16, static_cast<hipStream_t>(stream));
     return check_launch("hyq_qk_norm_rope");
 }
 
@@ -564,16 +810,13 @@ extern "C" int hyq_paged_rope_append(const hyq_rope_params* p, const uint16_t* v
     a.v = Rows{v, 0, v_stride_t, v_stride_h};
     a.pool = pool_of(*pool, slots);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (pool->bits == 8) return launch_append8<true>(a, p->head_dim, p->dtype_fp16, st);
-    const unsigned per = 256 / (p->head_dim / 8);
-    a.q_blocks = blocks_of(static_cast<uint64_t>(a.tokens) * a.hq, per);
-    const dim3 grid(a.q_blocks + blocks_of(static_cast<uint64_t>(a.tokens) * a.hk * 2, per));
-    if (p->head_dim == 128) {
-        if (p->dtype_fp16) paged_rope_append_kernel<128, true><<<grid, dim3(256), 0, st>>>(a);
-        else paged_rope_append_kernel<128, false><<<grid, dim3(256), 0, st>>>(a);
+    const bool many = many_heads(static_cast<uint64_t>(a.tokens) * (a.hq + 2 * a.hk), p->head_dim);
+    if (pool->bits == 8) {
+        if (many) append8<true, MANY>(a, p->head_dim, p->dtype_fp16, st);
+        else append8<true, 1>(a, p->head_dim, p->dtype_fp16, st);
     } else {
-        if (p->dtype_fp16) paged_rope_append_kernel<64, true><<<grid, dim3(256), 0, st>>>(a);
-        else paged_rope_append_kernel<64, false><<<grid, dim3(256), 0, st>>>(a);
+        if (many) append4<MANY>(a, p->head_dim, p->dtype_fp16, st);
+        else append4<1>(a, p->head_dim, p->dtype_fp16, st);
     }
     return check_launch("hyq_paged_rope_append");
 }
@@ -599,7 +842,8 @@ extern "C" int hyq_paged8_append(const uint16_t* k, int64_t k_stride_t, int64_t 
     a.tokens = a.n = static_cast<uint32_t>(num_tokens);
     a.hk = static_cast<uint32_t>(kv_heads);
     a.pool = pool_of(*pool, slots);
-    return launch_append8<false>(a, head_dim, is_fp16, static_cast<hipStream_t>(stream));
+    append8<false, 1>(a, head_dim, is_fp16, static_cast<hipStream_t>(stream));
+    return check_launch("hyq_paged8_append");
 }
 
 extern "C" int hyq_paged8_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads, int32_t head_dim,
