@@ -104,6 +104,8 @@ __device__ __forceinline__ double inv_root(double x) {
     return r;
 }
 
+__device__ __forceinline__ uint32_t batch_of(const RopeArgs& a, uint32_t t) { return a.tokens == a.n ? 0 : t / a.n; }
+
 // The row of the table for token t; false: its position is outside of it
 __device__ __forceinline__ bool table_row(const RopeArgs& a, uint32_t t, int64_t& at) {
     if (a.positions) {
@@ -112,12 +114,12 @@ __device__ __forceinline__ bool table_row(const RopeArgs& a, uint32_t t, int64_t
         at = ok ? m * a.cs_m : 0;
         return ok;
     }
-    const uint32_t b = t / a.n;
+    const uint32_t b = batch_of(a, t);
     at = b * a.cs_b + (t - b * a.n) * a.cs_m;
     return true;
 }
 __device__ __forceinline__ const uint16_t* row_of(const RopeArgs& a, const Rows& r, uint32_t t, uint32_t h) {
-    const uint32_t b = t / a.n;
+    const uint32_t b = batch_of(a, t);
     return r.p + b * r.sb + (t - b * a.n) * r.sn + h * r.sh;
 }
 
@@ -381,13 +383,18 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(RopeArgs a) {
 // 2^e, so that x 2^-e and its rounding are exact and so are codes that are
 // rounded again for a larger e.  Values past 127 2^MOST_E (and what is not
 // finite) make the block's scale NaN.
+constexpr int AGAIN = 5;                 // kept rows that are rounded again at a time
 constexpr int MOST_E = 40, BAD_E = 1 << 20, NO_E = -(1 << 20);
 __device__ __forceinline__ int exponent(double amax) {
     if (!(amax <= 127.0 * 0x1p40)) return BAD_E;
     const uint64_t b = __builtin_bit_cast(uint64_t, fmax(amax, 1e-5));
     return static_cast<int>((b >> 52) & 2047) - 1022 - 7 + ((b & 0xfffffffffffffull) > 0xfc00000000000ull ? 1 : 0);
 }
-__device__ __forceinline__ int exponent(float amax) { return exponent(static_cast<double>(amax)); }
+__device__ __forceinline__ int exponent(float amax) {                    // (1e-5 and its fp32 neighbour have the same)
+    if (!(amax <= 127.0f * 0x1p40f)) return BAD_E;
+    const uint32_t b = __float_as_uint(fmaxf(amax, 1e-5f));
+    return static_cast<int>(b >> 23) - 126 - 7 + ((b & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // A run of tokens whose slots lie in one block is worked on by the workgroup that
@@ -399,7 +406,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // rows take those behind the window.  Only where more runs start in it may a second pass
 // be left.
 template <int D, bool F16, bool ROPE, int HP>
-__global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
+__global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
     const int sub = threadIdx.x & (LPT - 1), r0 = threadIdx.x / LPT, lane = threadIdx.x & 63;
     if constexpr (ROPE) {
@@ -411,6 +418,7 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
     __shared__ int need[2][32];
     const uint32_t i = blockIdx.x - a.q_blocks, win = i / a.hk, h = i - win * a.hk, t0 = win * 16;
 
+    for (int j = threadIdx.x; j < 64; j += 2 * D) need[j >> 5][j & 31] = NO_E;
     // ---- the runs: lane l of each wavefront looks at token t0 - 1 + l, up to t0 + 31 ----
     int64_t slot = -1;
     bool ok = true;
@@ -462,19 +470,6 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
             k = load_angles(a, l, at);
         }
     };
-    // a K row's values, and how far off they may be (formed anew for the codes: kept
-    // they would take 16 registers more)
-    auto keys = [&](float (&x)[8], float (&y)[8], float (&err)[8]) {
-        unpack<F16>(kr, x);
-        if constexpr (ROPE) {
-            turn<D, double, float, true>(a, l, k, wt, x, y, &err);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) err[j] *= TURN_ERROR;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { y[j] = x[j]; err[j] = 0.f; }
-        }
-    };
     auto largest = [&](const float (&y)[8], float& amax) {               // the row's exponent; the lane's largest magnitude
         bool fine = true;
         amax = 0.f;
@@ -485,16 +480,23 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
         }
         return lanes_max<LPT>(fine ? exponent(amax) : BAD_E);
     };
+    float y[8], off = 0.f;               // K's values, and how far off they may be
     auto measure = [&](const Row& w) {
-        float x[8], y[8], err[8], amax, off = 0.f;
-        keys(x, y, err);
+        float x[8], amax;
+        unpack<F16>(kr, x);
+        if constexpr (ROPE) {
+            float most[8];
+            turn<D, double, float, true>(a, l, k, wt, x, y, &most);
+            off = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7]))) * TURN_ERROR;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j];
+        }
         int e = largest(y, amax);
         if constexpr (ROPE) {            // the row's largest may be another value's than the formula's, but not its exponent
-#pragma unroll
-            for (int j = 0; j < 8; ++j) off = fmaxf(off, err[j]);
             amax = lanes_max<LPT>(amax);
-            off = lanes_max<LPT>(off) + amax * 0x1p-22f;
-            const bool sure = exponent(amax + off) == e && exponent(amax - off) == e;
+            const float far = lanes_max<LPT>(off) + amax * 0x1p-22f;
+            const bool sure = exponent(amax + far) == e && exponent(amax - far) == e;
             if (__builtin_amdgcn_ballot_w64(w.active && !sure)) {
                 double v[8], top = 0.0;
                 bool good = true;
@@ -507,9 +509,12 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
                 e = lanes_max<LPT>(good ? exponent(top) : BAD_E);
             }
         }
-        unpack<F16>(vr, y);
-        const int ev = largest(y, amax);
-        if (sub == 0 && w.active) { need[0][w.r] = e; need[1][w.r] = ev; }
+        unpack<F16>(vr, x);
+        const int ev = largest(x, amax);
+        if (sub == 0 && w.active) {      // (the order does not matter)
+            atomicMax(&need[0][__builtin_ctz(w.mine)], e);
+            atomicMax(&need[1][__builtin_ctz(w.mine)], ev);
+        }
     };
 
     const int64_t hp = h * a.pool.ps_head, hs = h * a.pool.ss_head;
@@ -535,8 +540,7 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind) {
             const float old = q.old[kind];
-            int e = NO_E;
-            for (uint32_t left = w.active ? w.mine : 0; left; left &= left - 1) e = max(e, need[kind][__builtin_ctz(left)]);
+            int e = need[kind][q.first];
             if (q.kept) {
                 if (!(old >= 0.f && old <= pow2(MOST_E + 1))) e = BAD_E;
                 else if (old > 0.f) {    // the smallest power of two from it on
@@ -547,20 +551,20 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
             const bool bad = e > MOST_E + 1;
             e = max(e, -126);            // (an inactive row's)
             const float now = bad ? __builtin_nanf("") : pow2(e), inv = bad ? 0.f : pow2(-e);
-            float x[8], y[8], err[8];
-            bool fine = true;
-            if (kind == 0) keys(x, y, err);
-            else unpack<F16>(vr, y);
+            float x[8];
+            if (kind == 1) unpack<F16>(vr, x);
             int c[8];
+            float edge = 0.f;            // the nearest to a code's border
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float z = y[j] * inv, n = rintf(z);
-                if (ROPE && kind == 0) fine = fine && fabsf(z - n) + err[j] * inv < 0.5f - 0x1p-23f;
+                const float z = (kind ? x[j] : y[j]) * inv, n = rintf(z);
+                edge = fmaxf(edge, fabsf(z - n));
                 c[j] = static_cast<int>(n);
             }
             if (ROPE && kind == 0) {
-                if (__builtin_amdgcn_ballot_w64(w.active && !bad && !fine)) {
+                if (__builtin_amdgcn_ballot_w64(w.active && !bad && !(edge + off * inv < 0.5f - 0x1p-23f))) {
                     double v[8];
+                    unpack<F16>(kr, x);
                     turn<D, double>(a, l, k, wt, x, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) c[j] = static_cast<int>(rint(v[j] * static_cast<double>(inv)));
@@ -578,17 +582,22 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
             if (w.r != q.first) continue;
             if (q.kept && now != old) {
                 const float by = old * inv;
-                for (int j = 0; j < q.kept; ++j) {
-                    uint2* const to = reinterpret_cast<uint2*>(rows + j * D) + sub;
-                    const uint2 v = *to;
-                    const uint32_t in[2] = {v.x, v.y};
-                    uint32_t out[2] = {0, 0};
+                uint2* const to = reinterpret_cast<uint2*>(rows) + sub;
+                for (int j0 = 0; j0 < q.kept; j0 += AGAIN) {             // (AGAIN rows' loads in flight)
+                    uint2 v[AGAIN];
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const int code = static_cast<int8_t>(in[n >> 2] >> (8 * (n & 3)));
-                        out[n >> 2] |= (static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(code) * by))) & 255u) << (8 * (n & 3));
+                    for (int j = 0; j < AGAIN; ++j) v[j] = to[min(j0 + j, q.kept - 1) * LPT];
+#pragma unroll
+                    for (int j = 0; j < AGAIN; ++j) {
+                        const uint32_t in[2] = {v[j].x, v[j].y};
+                        uint32_t out[2] = {0, 0};
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const int code = static_cast<int8_t>(in[n >> 2] >> (8 * (n & 3)));
+                            out[n >> 2] |= (static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(code) * by))) & 255u) << (8 * (n & 3));
+                        }
+                        if (j0 + j < q.kept) to[(j0 + j) * LPT] = make_uint2(out[0], out[1]);
                     }
-                    *to = make_uint2(out[0], out[1]);
                 }
             }
             if (sub == 0) static_cast<float*>(kind ? a.pool.vs : a.pool.ks)[q.scale] = now;
@@ -598,6 +607,7 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
     Row w = row_at(0);
     load(w);
     Place q = place(w);
+    __syncthreads();                     // (need is set)
     measure(w);
     if (twice) {                         // (the same in all lanes)
         const Place q0 = q;
@@ -609,6 +619,7 @@ __global__ __launch_bounds__(2 * D) void paged8_append_kernel(RopeArgs a) {
         write(w, q);
         w = row_at(0);
         load(w);
+        measure(w);                      // (its values again: the exponents are the same)
         write(w, q0);
     } else {
         __syncthreads();
