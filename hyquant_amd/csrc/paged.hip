@@ -892,7 +892,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 
 template <int D, bool F16>
 struct Kernels {
-    static constexpr auto narrow = paged_attn_kernel<D, F16>;
+    static auto narrow(const AttnArgs&) { return paged_attn_kernel<D, F16>; }
     static constexpr auto chunk = paged_chunk_kernel<D, F16>;
     static constexpr size_t chunk_lds = sizeof(ChunkLds<D>);
 };

@@ -852,7 +852,7 @@ int launch_attention(const char* what, AttnArgs a, const PlanArgs& narrow, const
     }
     a.plan = narrow;
     partials(s.narrow);
-    if (s.narrow.items) KERNELS::narrow<<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
+    if (s.narrow.items) KERNELS::narrow(a)<<<dim3(static_cast<unsigned>(s.narrow.items), a.heads), dim3(64 * WAVES), 0, st>>>(a);
     // a round of resident workgroups (two a CU) for the kind that there is, half
     // of one each where both may be
     const int64_t most = s.narrow.joins && s.wide.joins ? 256 : 512;
