@@ -9,7 +9,8 @@ and the helpers of src/patch/_common.py (mode table, argument validation,
 the D-stage cache hand-off of :198-228).
 
 Each patched attention module keeps its projections, rotary embedding and
-output projection and routes the attention itself by mode:
+output projection (with fused_rope=True the head norms and the rotation are one
+launch of qk_norm_rope) and routes the attention itself by mode:
   dense                the model's own attention (cache updated as usual);
   D-stage modes        (d_k4v4 ... hybrid_k2v4, the mode table below) with a
                        DStageKVCache attached: prefill keeps the bf16 KV and
@@ -42,7 +43,8 @@ from typing import Any, Optional, Tuple
 import torch
 
 from .d_stage_kv_cache import DStageKVCache
-from .decode_d_stage import _dequantize_by_bits, _quantize_by_bits
+from .decode_d_stage import _HALF, _dequantize_by_bits, _quantize_by_bits
+from .rope import qk_norm_rope
 from .sage_unified import sage_vertical_attention_v2
 from .vertical import compute_vertical_indices
 
@@ -192,9 +194,23 @@ def _quant_roundtrip_decode(q, k, v, mode: str, window_size: int, top_ratio: flo
     return torch.softmax(scores.float(), dim=-1).to(vd.dtype) @ vd
 
 
-def build_attention_forward(family: str, *, mode: str, window_size: int, top_ratio: float):
+def _takes_fused_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *weights: torch.Tensor) -> bool:
+    """Whether qk_norm_rope takes a module's rows [B, N, heads, D], its embedding [B or 1, N, R] and its norms'
+    weights, with no gradient of any to record."""
+    if not q.is_cuda or q.dtype not in _HALF or q.shape[-1] not in (64, 128) or cos.dim() != 3 or cos.shape != sin.shape:
+        return False
+    r = cos.shape[-1]
+    if r % 16 or not 0 < r <= q.shape[-1] or cos.shape[0] not in (1, q.shape[0]) or cos.shape[1] != q.shape[1]:
+        return False
+    return not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin, *weights)))
+
+
+def build_attention_forward(family: str, *, mode: str, window_size: int, top_ratio: float, fused_rope: bool = False):
     """Patched forward of a Llama-3 ("llama") or Qwen3 ("qwen", q/k RMS norms)
-    attention module (src/patch/patch_llama.py:27-259, src/patch/patch_qwen.py)."""
+    attention module (src/patch/patch_llama.py:27-259, src/patch/patch_qwen.py).
+    fused_rope: the head norms and the rotation in one launch (qk_norm_rope, rounded
+    once) instead of the module's own torch operations, which round after each;
+    where a gradient is recorded, or on the CPU, the module's own are used."""
     if family == "llama":
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb, eager_attention_forward
     elif family == "qwen":
@@ -219,12 +235,22 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
         hidden_shape = (*input_shape, -1, self.head_dim)
         q = self.q_proj(hidden_states).view(hidden_shape)
         k = self.k_proj(hidden_states).view(hidden_shape)
-        if family == "qwen":
-            q, k = self.q_norm(q), self.k_norm(k)
-        q, k = q.transpose(1, 2), k.transpose(1, 2)
-        v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         cos, sin = position_embeddings
-        q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        norms = {}
+        if fused_rope and family == "qwen":
+            norms = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight)
+        if fused_rope and _takes_fused_rope(q, k, cos, sin, *norms.values()):
+            half = cos.shape[-1] // 2
+            if norms:
+                norms["eps"] = self.q_norm.variance_epsilon
+            q, k = qk_norm_rope(q, k, cos[..., :half], sin[..., :half], **norms)
+            q, k = q.transpose(1, 2), k.transpose(1, 2)
+        else:
+            if family == "qwen":
+                q, k = self.q_norm(q), self.k_norm(k)
+            q, k = q.transpose(1, 2), k.transpose(1, 2)
+            q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         q_len = int(q.shape[2])
         kv_repeat = infer_kv_repeat(self)
 
@@ -271,12 +297,12 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
 
 
 def _patch(model: torch.nn.Module, family: str, cls, mode: str, window_size: int, top_ratio: float,
-           k_bits: Optional[int], v_bits: Optional[int]) -> torch.nn.Module:
+           k_bits: Optional[int], v_bits: Optional[int], fused_rope: bool) -> torch.nn.Module:
     mode = validate_patch_args(mode, window_size, top_ratio, k_bits, v_bits)
     if mode in _NOT_BUILT:
         raise NotImplementedError(f"mode '{mode}' (sparse baseline) is not part of this build; the attention "
                                   "modes are dense, full_attention, sage_w, sage_w0, vquant_vert, hybrid_* and d_*")
-    fwd = build_attention_forward(family, mode=mode, window_size=window_size, top_ratio=top_ratio)
+    fwd = build_attention_forward(family, mode=mode, window_size=window_size, top_ratio=top_ratio, fused_rope=fused_rope)
     patched = 0
     for module in model.modules():
         if isinstance(module, cls):
@@ -292,21 +318,21 @@ def _patch(model: torch.nn.Module, family: str, cls, mode: str, window_size: int
 def patch_llama3_attention_forward_model(model: torch.nn.Module, *, mode: str = "sage_w", window_size: int = 256,
                                          top_ratio: float = 0.05, k_bits: Optional[int] = None,
                                          v_bits: Optional[int] = None, report_stats: bool = False,
-                                         use_vertical_indices: bool = True) -> torch.nn.Module:
+                                         use_vertical_indices: bool = True, fused_rope: bool = False) -> torch.nn.Module:
     """Patch every LlamaAttention module in place (src/patch/patch_llama.py:265-298)."""
     del report_stats, use_vertical_indices
     from transformers.models.llama.modeling_llama import LlamaAttention
-    return _patch(model, "llama", LlamaAttention, mode, window_size, top_ratio, k_bits, v_bits)
+    return _patch(model, "llama", LlamaAttention, mode, window_size, top_ratio, k_bits, v_bits, fused_rope)
 
 
 def patch_qwen3_attention_forward_model(model: torch.nn.Module, *, mode: str = "sage_w", window_size: int = 256,
                                         top_ratio: float = 0.05, k_bits: Optional[int] = None,
                                         v_bits: Optional[int] = None, report_stats: bool = False,
-                                        use_vertical_indices: bool = True) -> torch.nn.Module:
+                                        use_vertical_indices: bool = True, fused_rope: bool = False) -> torch.nn.Module:
     """Patch every Qwen3Attention module in place (src/patch/patch_qwen.py)."""
     del report_stats, use_vertical_indices
     from transformers.models.qwen3.modeling_qwen3 import Qwen3Attention
-    return _patch(model, "qwen", Qwen3Attention, mode, window_size, top_ratio, k_bits, v_bits)
+    return _patch(model, "qwen", Qwen3Attention, mode, window_size, top_ratio, k_bits, v_bits, fused_rope)
 
 
 def _infer_patch_target(model) -> str:
@@ -323,14 +349,15 @@ def _infer_patch_target(model) -> str:
 
 def patch_attention_forward_model(model, *, mode: str = "sage_w", window_size: int = 256, top_ratio: float = 0.05,
                                   report_stats: bool = False, use_vertical_indices: bool = True,
-                                  patch_target: str = "auto"):
-    """Patch qwen / llama attention with optional auto detection (src/patch/__init__.py:29-71)."""
+                                  patch_target: str = "auto", fused_rope: bool = False):
+    """Patch qwen / llama attention with optional auto detection (src/patch/__init__.py:29-71).
+    fused_rope=True normalises and rotates queries and keys in one launch (qk_norm_rope)."""
     if patch_target == "auto":
         patch_target = _infer_patch_target(model)
     if patch_target == "qwen":
-        return patch_qwen3_attention_forward_model(model, mode=mode, window_size=window_size, top_ratio=top_ratio)
+        return patch_qwen3_attention_forward_model(model, mode=mode, window_size=window_size, top_ratio=top_ratio, fused_rope=fused_rope)
     if patch_target == "llama":
-        return patch_llama3_attention_forward_model(model, mode=mode, window_size=window_size, top_ratio=top_ratio)
+        return patch_llama3_attention_forward_model(model, mode=mode, window_size=window_size, top_ratio=top_ratio, fused_rope=fused_rope)
     if patch_target == "glm4":
         raise NotImplementedError("the GLM-4 patch never reaches the hybrid kernels and is not part of this build")
     raise ValueError("Unsupported patch_target. Expected one of: auto, qwen, llama, glm4.")

@@ -141,3 +141,20 @@ def test_python_checks():
                  lambda: hq.paged8_gather(torch.zeros(3, dtype=torch.int64), *pool)):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+@pytest.mark.parametrize("family", ["llama", "qwen"])
+def test_fused_rope_on_the_cpu_is_the_models_own(family):
+    transformers = pytest.importorskip("transformers")
+    from hyquant_amd.patch import patch_attention_forward_model
+    torch.manual_seed(0)
+    common = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+                  vocab_size=128, max_position_embeddings=512, attn_implementation="sdpa")
+    make = (lambda: transformers.LlamaForCausalLM(transformers.LlamaConfig(**common))) if family == "llama" else (
+        lambda: transformers.Qwen3ForCausalLM(transformers.Qwen3Config(**common)))
+    ref, pat = make().eval(), make().eval()
+    pat.load_state_dict(ref.state_dict())
+    patch_attention_forward_model(pat, mode="dense", fused_rope=True)
+    ids = torch.randint(0, 128, (1, 40), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        assert torch.equal(ref(ids).logits, pat(ids).logits)
