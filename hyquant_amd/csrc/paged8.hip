@@ -295,10 +295,10 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged8_attn_kerne
 // A wavefront owns 32 rows.  The codes of 64 keys at a time are turned into
 // fp16 operands once for all rows of the workgroup and laid in LDS, two blocks
 // ahead of the products.
-//   QK  S^T[key][row] = K . Q^T  with v_mfma_f32_32x32x16_f16; codes and queries
-//       (each row's scaled by a power of two of its own) are exact.
-//   t = S k_scale + log2(V scale) - M: a tile's scales, times the row's power of
-//       two, are one fma's constants.
+//   QK  S^T[key][row] = K . Q^T  with v_mfma_f32_32x32x16_f16, K operands u 2^-24
+//       as above, queries (each row's scaled by a power of two of its own) exact.
+//   t = (S - 128 2^-24 sum(q)) k_scale + log2(V scale) - M: a tile's scales, times
+//       the row's power of two, and the offset are one fma's constants.
 //   PV  O^T[channel][row] = V^T . P'^T, P' = fp16(2^t) against the exact codes,
 //       V^T by transposing LDS reads.  M follows the row's own largest t, so that
 //       P' keeps to [0, 2^13]; rounding P' to 11 bits once is the only rounding
@@ -310,12 +310,12 @@ template <int D>
 struct ChunkLds8 {
     uint8_t k[BUFS][BLK * KROW<D>];
     uint8_t v[BUFS][BLK * VROW<D>];
-    float ks[BUFS][4];                   // per 16-key tile: K scale * scale, or NaN
+    float ks[BUFS][4];                   // per 16-key tile: K scale * scale * 2^24, or NaN
     float lv[BUFS][4], vi[BUFS][4];      // log2 of the V scale, or NaN; its inverse, or 0
     uint32_t in[BUFS][4];                // the page is in the pool
 };
 
-// bytes b and b + 1 of u = code + 128 as fp16 codes: 1024 + u is exact, so is minus 1152
+// bytes b and b + 1 of u = code + 128 as fp16 codes (V's): 1024 + u is exact, so is minus 1152
 template <int B> __device__ __forceinline__ uint32_t codes2(uint32_t u) {
     const f16x2 x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04000400u | (B + 1) << 16 | B));
     const f16x2 b = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
@@ -357,6 +357,14 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged8_chunk_kernel(AttnA
     for (int m = 0; m < KM; ++m)
 #pragma unroll
         for (int i = 0; i < 8; ++i) qop[m][i] = static_cast<_Float16>(half_at<F16>(qr[m][i >> 1], i & 1) * qs);
+    // -128 2^-24 sum(q): what the K codes' offset adds to a score, less it
+    float qsum = 0.f;
+#pragma unroll
+    for (int m = 0; m < KM; ++m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qsum += static_cast<float>(qop[m][i]);
+    const auto qh = __builtin_amdgcn_permlane32_swap(__float_as_uint(qsum), __float_as_uint(qsum), false, false);
+    const float qbias = -0x1p-17f * (__uint_as_float(qh[0]) + __uint_as_float(qh[1]));
     const int pos = it.len - it.qlen + tok;
     const int lo = first_key(pos, a.window), top = min(pos, it.key1 - 1);
     // every row of this wavefront sees [all_lo, all_hi]
@@ -364,57 +372,64 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged8_chunk_kernel(AttnA
     const int all_hi = min(it.len - it.qlen + t0, it.key1 - 1), all_lo = first_key(it.len - it.qlen + t1, a.window);
 
     // ---- conversion ----
-    // Wavefronts 0..3 have the V codes and scales of the 16-key tiles 0..3 of a
-    // block, wavefronts 4..7 the K codes and scales: one page id and one
-    // descriptor each, of range 0 (zeros, no access) where the page is not in
-    // the pool.
-    const bool is_v = w < 4;
-    const int tile = w & 3;
-    const int64_t hk = head * a.ps_head, hs = head * a.ss_head;
+    // A wavefront has the K and V codes of 8 keys of a block's 64, half a tile: one
+    // page id, and descriptors of range 0 (zeros, no access) where the page is not
+    // in the pool.
+    const int tile = w >> 1;
+    const int64_t hk = head * a.ps_head + 8 * (w & 1) * D, hs = head * a.ss_head;
     const int page_mask = (1 << a.page_log2) - 1;
     const int32_t* trow = a.table + it.req * a.bt_stride;
     const int nblk = a.num_pages > 0 ? (max(it.key1 - it.key0, 0) + BLK - 1) / BLK : 0;
-    // lane = key of the tile * KL + 32-channel part kq (D = 64: the upper 32
-    // lanes store what the lower ones store)
-    constexpr int KL = D / 32;
-    const int cl = D == 128 ? lane : lane & 31;
-    const int kkey = cl / KL, kq = cl % KL;
-    const int8_t* const codes = is_v ? a.vp : a.kp;
-    const float* const scales = static_cast<const float*>(is_v ? a.vs : a.ks);
-    uint8_t* const mine = (is_v ? L.v[0] + (16 * tile + kkey) * VROW<D> : L.k[0] + (16 * tile + kkey) * KROW<D>) + 64 * kq;
+    // lane = key * 8 + part: D / 8 codes of K and of V
+    constexpr int CODES = D / 32;        // words of them
+    const int ckey = lane >> 3, part = lane & 7;
+    uint8_t* const kst = L.k[0] + (8 * w + ckey) * KROW<D> + (D / 4) * part;
+    uint8_t* const vst = L.v[0] + (8 * w + ckey) * VROW<D> + (D / 4) * part;
+    const float *const kscale = static_cast<const float*>(a.ks), *const vscale = static_cast<const float*>(a.vs);
     auto tile_key = [&](int blk) { return it.key0 + BLK * blk + 16 * tile; };
     auto page_id = [&](int blk) -> int { return trow[min(tile_key(blk), it.key1 - 1) >> a.page_log2]; };
-    u32x4 raw[2] = {};                   // 32 codes
-    uint32_t sraw = 0;                   // scale bits
+    uint32_t kraw[CODES] = {}, vraw[CODES] = {};
+    uint32_t ksraw = 0, vsraw = 0;       // scale bits
     bool sok = false;                    // the page is in the pool
     auto fetch = [&](int blk, int id) __attribute__((always_inline)) {
         id = __builtin_amdgcn_readfirstlane(id);
         sok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages);
         const int64_t pg = sok ? id : 0;
         const int o = (min(tile_key(blk), it.key1 - 1) & page_mask) & ~15;
-        const Rsrc rc = make_rsrc(codes + pg * a.ps_page + hk + o * D, sok ? 16 * D : 0);
-        const Rsrc rs = make_rsrc(scales + pg * a.ss_page + hs + (o >> 4), sok ? 4 : 0);
-        raw[0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, 32 * cl, 0, 0));
-        raw[1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, 32 * cl + 16, 0, 0));
-        sraw = __builtin_amdgcn_raw_buffer_load_b32(rs, 0, 0, 0);
-    };
-    // the fetched block into buffer b
-    auto store = [&](int b) __attribute__((always_inline)) {
-        uint8_t* const dst = mine + b * (is_v ? sizeof(L.v[0]) : sizeof(L.k[0]));
+        const int64_t co = pg * a.ps_page + hk + o * D, so = pg * a.ss_page + hs + (o >> 4);
+        const Rsrc rk = make_rsrc(a.kp + co, sok ? 8 * D : 0), rv = make_rsrc(a.vp + co, sok ? 8 * D : 0);
+        if constexpr (D == 128) {
+            const u32x4 k = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, 16 * lane, 0, 0));
+            const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * lane, 0, 0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t x = raw[i >> 1][2 * (i & 1)] ^ FLIP, y = raw[i >> 1][2 * (i & 1) + 1] ^ FLIP;
-            *reinterpret_cast<u32x4*>(dst + 16 * i) = u32x4{codes2<0>(x), codes2<2>(x), codes2<0>(y), codes2<2>(y)};
+            for (int i = 0; i < 4; ++i) { kraw[i] = k[i]; vraw[i] = v[i]; }
+        } else {
+            const u32x2 k = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, 8 * lane, 0, 0));
+            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, 8 * lane, 0, 0));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { kraw[i] = k[i]; vraw[i] = v[i]; }
         }
-        if (lane == 0) {
-            const float f = checked(__uint_as_float(sraw));
-            if (is_v) {
-                L.lv[b][tile] = __builtin_amdgcn_logf(f);
-                L.vi[b][tile] = f == f ? __builtin_amdgcn_rcpf(f) : 0.f;
-                L.in[b][tile] = sok;
-            } else {
-                L.ks[b][tile] = f * a.scale;
-            }
+        ksraw = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(kscale + so, sok ? 4 : 0), 0, 0, 0);
+        vsraw = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(vscale + so, sok ? 4 : 0), 0, 0, 0);
+    };
+    // the fetched block into buffer b: K as u 2^-24, V as exact codes
+    auto store = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < CODES; i += 2) {
+            const uint32_t x = kraw[i] ^ FLIP, y = kraw[i + 1] ^ FLIP;
+            *reinterpret_cast<u32x4*>(kst + b * static_cast<int>(sizeof(L.k[0])) + 8 * i) = u32x4{bytes2<0>(x), bytes2<2>(x), bytes2<0>(y), bytes2<2>(y)};
+        }
+#pragma unroll
+        for (int i = 0; i < CODES; i += 2) {
+            const uint32_t x = vraw[i] ^ FLIP, y = vraw[i + 1] ^ FLIP;
+            *reinterpret_cast<u32x4*>(vst + b * static_cast<int>(sizeof(L.v[0])) + 8 * i) = u32x4{codes2<0>(x), codes2<2>(x), codes2<0>(y), codes2<2>(y)};
+        }
+        if (lane == 0) {                 // (both wavefronts of a tile store the same)
+            const float f = checked(__uint_as_float(vsraw));
+            L.lv[b][tile] = __builtin_amdgcn_logf(f);
+            L.vi[b][tile] = f == f ? __builtin_amdgcn_rcpf(f) : 0.f;
+            L.in[b][tile] = sok;
+            L.ks[b][tile] = checked(__uint_as_float(ksraw)) * a.scale * 16777216.0f;
         }
     };
 
@@ -465,7 +480,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged8_chunk_kernel(AttnA
     auto scores = [&](int b, int x, float m_use) __attribute__((always_inline)) -> float {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float k = L.ks[b][2 * x + i] * row_scale, o = L.lv[b][2 * x + i] - m_use;
+            const float k = L.ks[b][2 * x + i] * row_scale, o = __builtin_fmaf(qbias, k, L.lv[b][2 * x + i] - m_use);
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[8 * i + j] = __builtin_fmaf(sc[8 * i + j], k, o);
         }
