@@ -384,6 +384,7 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(RopeArgs a) {
 // rounded again for a larger e.  Values past 127 2^MOST_E (and what is not
 // finite) make the block's scale NaN.
 constexpr int AGAIN = 5;                 // kept rows that are rounded again at a time
+constexpr int LEAST_E = -23;             // of 1e-5
 constexpr int MOST_E = 40, BAD_E = 1 << 20, NO_E = -(1 << 20);
 __device__ __forceinline__ int exponent(double amax) {
     if (!(amax <= 127.0 * 0x1p40)) return BAD_E;
@@ -470,34 +471,26 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
             k = load_angles(a, l, at);
         }
     };
-    auto largest = [&](const float (&y)[8], float& amax) {               // the row's exponent; the lane's largest magnitude
-        bool fine = true;
-        amax = 0.f;
+    // the row's largest magnitude's bits (those of what is not finite are above all others)
+    auto largest = [&](const float (&y)[8]) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            fine = fine && fabsf(y[j]) <= 127.0f * 0x1p40f;              // (a NaN is not)
-            amax = fmaxf(amax, fabsf(y[j]));
-        }
-        return lanes_max<LPT>(fine ? exponent(amax) : BAD_E);
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(y[j])));
+        return static_cast<uint32_t>(lanes_max<LPT>(static_cast<int>(m)));
     };
     float y[8], off = 0.f;               // K's values, and how far off they may be
     auto measure = [&](const Row& w) {
-        float x[8], amax;
+        float x[8];
         unpack<F16>(kr, x);
+        int e;
         if constexpr (ROPE) {
             float most[8];
             turn<D, double, float, true>(a, l, k, wt, x, y, &most);
             off = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7]))) * TURN_ERROR;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = x[j];
-        }
-        int e = largest(y, amax);
-        if constexpr (ROPE) {            // the row's largest may be another value's than the formula's, but not its exponent
-            amax = lanes_max<LPT>(amax);
-            const float far = lanes_max<LPT>(off) + amax * 0x1p-22f;
-            const bool sure = exponent(amax + far) == e && exponent(amax - far) == e;
-            if (__builtin_amdgcn_ballot_w64(w.active && !sure)) {
+            // the row's largest may be another value's than the formula's, but not its exponent
+            const float amax = __uint_as_float(largest(y)), far = lanes_max<LPT>(off) + amax * 0x1p-22f;
+            e = exponent(amax + far);
+            if (__builtin_amdgcn_ballot_w64(w.active && !(e == LEAST_E || amax - far > 63.5f * pow2(min(e, 0x60))))) {
                 double v[8], top = 0.0;
                 bool good = true;
                 turn<D, double>(a, l, k, wt, x, v);
@@ -508,9 +501,13 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
                 }
                 e = lanes_max<LPT>(good ? exponent(top) : BAD_E);
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j];
+            e = exponent(__uint_as_float(largest(y)));
         }
         unpack<F16>(vr, x);
-        const int ev = largest(x, amax);
+        const int ev = exponent(__uint_as_float(largest(x)));
         if (sub == 0 && w.active) {      // (the order does not matter)
             atomicMax(&need[0][__builtin_ctz(w.mine)], e);
             atomicMax(&need[1][__builtin_ctz(w.mine)], ev);
@@ -553,13 +550,14 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
             const float now = bad ? __builtin_nanf("") : pow2(e), inv = bad ? 0.f : pow2(-e);
             float x[8];
             if (kind == 1) unpack<F16>(vr, x);
-            int c[8];
+            // x / scale + 1.5 2^23, rounded once: the code is its low byte
+            uint32_t c[8];
             float edge = 0.f;            // the nearest to a code's border
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float z = (kind ? x[j] : y[j]) * inv, n = rintf(z);
-                edge = fmaxf(edge, fabsf(z - n));
-                c[j] = static_cast<int>(n);
+                const float v = kind ? x[j] : y[j], z = __builtin_fmaf(v, inv, 12582912.0f);
+                if (ROPE && kind == 0) edge = fmaxf(edge, fabsf(__builtin_fmaf(v, inv, 12582912.0f - z)));
+                c[j] = __float_as_uint(z);
             }
             if (ROPE && kind == 0) {
                 if (__builtin_amdgcn_ballot_w64(w.active && !bad && !(edge + off * inv < 0.5f - 0x1p-23f))) {
@@ -567,13 +565,12 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
                     unpack<F16>(kr, x);
                     turn<D, double>(a, l, k, wt, x, v);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) c[j] = static_cast<int>(rint(v[j] * static_cast<double>(inv)));
+                    for (int j = 0; j < 8; ++j) c[j] = static_cast<uint32_t>(static_cast<int>(rint(v[j] * static_cast<double>(inv))));
                 }
             }
             if (!w.active) continue;
-            auto word = [&](int j) {
-                return (static_cast<uint32_t>(c[j]) & 255u) | (static_cast<uint32_t>(c[j + 1]) & 255u) << 8 |
-                       (static_cast<uint32_t>(c[j + 2]) & 255u) << 16 | static_cast<uint32_t>(c[j + 3]) << 24;
+            auto word = [&](int j) {     // the low bytes of four
+                return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[j + 3], c[j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(c[j + 1], c[j], 0x0c0c0400u), 0x05040100u);
             };
             int8_t* const rows = (kind ? a.pool.vp : a.pool.kp) + q.rows;
             int8_t* const row = rows + (w.slot & (BLOCK - 1)) * D;
