@@ -91,17 +91,26 @@ __device__ __forceinline__ T lanes_sum(T v) { return over_lanes<LPT>(v, [](T a, 
 template <int LPT, typename T>
 __device__ __forceinline__ T lanes_max(T v) { return over_lanes<LPT>(v, [](T a, T b) { return b > a ? b : a; }); }
 
-// 1 / sqrt(x): the hardware's estimate (a unit in the last place of fp32; 2^-24,
-// and two Newton steps, in 64 bits), the division where that has no range
-__device__ __forceinline__ float inv_root(float x) {
-    return x >= 0x1p-126f && x < INFINITY ? __builtin_amdgcn_rsqf(x) : 1.0f / sqrtf(x);
-}
+// 1 / sqrt(x): the hardware's estimate (2^-24) and two Newton steps, the division
+// where that has no range
 __device__ __forceinline__ double inv_root(double x) {
     if (!(x >= 0x1p-1000 && x < static_cast<double>(INFINITY))) return 1.0 / sqrt(x);
     double r = __builtin_amdgcn_rsq(x);
 #pragma unroll
     for (int i = 0; i < 2; ++i) r = __builtin_fma(0.5 * r, __builtin_fma(-x * r, r, 1.0), r);
     return r;
+}
+// The inverse root mean square of a row, its squares summed in SUM; in 32 bits (and
+// by the hardware's estimate, a unit in the last place) only where they hold it.
+// (64 bits for every row of a rotation: 232 us where this takes 222.)
+template <int D, typename SUM>
+__device__ __forceinline__ SUM inv_rms(const float (&x)[8], double eps) {
+    SUM sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += static_cast<SUM>(x[i]) * static_cast<SUM>(x[i]);
+    sum = lanes_sum<D / 8>(sum) * static_cast<SUM>(1.0 / D) + static_cast<SUM>(eps);
+    if constexpr (std::is_same_v<SUM, double>) return inv_root(sum);
+    else return sum >= 0x1p-90f && sum <= 0x1p120f ? __builtin_amdgcn_rsqf(sum) : static_cast<float>(inv_rms<D, double>(x, eps));
 }
 
 __device__ __forceinline__ uint32_t batch_of(const RopeArgs& a, uint32_t t) { return a.tokens == a.n ? 0 : t / a.n; }
@@ -188,10 +197,7 @@ __device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Ang
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
     if (w.norm) {
-        SUM sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += static_cast<SUM>(x[i]) * static_cast<SUM>(x[i]);
-        const T inv = static_cast<T>(inv_root(lanes_sum<D / 8>(sum) * static_cast<SUM>(1.0 / D) + static_cast<SUM>(a.eps)));
+        const T inv = static_cast<T>(inv_rms<D, SUM>(x, a.eps));
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * static_cast<T>(w.w[i]);
     }

@@ -108,6 +108,24 @@ def test_rotation_of_values_that_are_not_finite_stays_in_their_rows():
     assert not q.any()
 
 
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_norms_of_rows_of_any_magnitude(eps):
+    """bf16 rows from 1e-30 to 1e37: their squares are no 32-bit numbers."""
+    g = gen(7)
+    scale = torch.logspace(-30, 37, 24).reshape(24, 1, 1)
+    x = (torch.randn(24, 3, 64, generator=g) * scale).clamp(-3e38, 3e38).to(BF).to(DEV)
+    w = randn(g, 64, dtype=FL)
+    cos, sin = U.tables(24, 64, device=DEV)
+    q, k = hq.qk_norm_rope(x, x, cos, sin, q_weight=w, k_weight=w, eps=eps)
+    check(q, *U.turn(x, cos, sin, w, eps))
+    assert torch.equal(q, k)
+    pool = U.pool8(g, 2, 3, 16, 64, DEV)
+    want = pool[0].cpu().clone(), pool[2].cpu().clone()
+    hq.paged_rope_append(x, x, x.clamp(-1, 1), cos, sin, as_long(list(range(24))), as_long(list(range(24))), *pool, q_weight=w, k_weight=w, eps=eps)
+    U.append8(*want, U.turn(x, cos, sin, w, eps)[0].cpu(), list(range(24)))
+    assert torch.equal(pool[0].cpu(), want[0]) and torch.equal(pool[2].cpu(), want[1])
+
+
 def test_rotation_by_far_rows_of_a_table():
     """A table past 2^31 values."""
     rows = (1 << 28) + 5
@@ -292,6 +310,36 @@ def test_rope_append_at_position_zero_is_the_plain_append(bits):
     q = hq.paged_rope_append(x, k, v, cos, sin, as_long([0] * T), as_long(slots), *a)
     (hq.paged_append if bits == 4 else hq.paged8_append)(k, v, as_long(slots), *b)
     assert torch.equal(q, x) and all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_keys_next_to_the_borders_of_their_codes(bits, interleaved):
+    """Keys rotated by 2^-32: values on the border between two codes move by less
+    than 32 bits hold, and fall on their own side of it; the largest values of a row
+    that lie on the border between two scales, too."""
+    D, H, page, T = 64, 2, 16, 48
+    g = gen(13)
+    cos, sin = torch.ones(1, D // 2, device=DEV), torch.full((1, D // 2), 2.0 ** -32, device=DEV)
+    most = 7 if bits == 4 else 127
+    x = torch.randint(-most, most, (T, H, D), generator=g).float() + 0.5                 # borders of a scale of one
+    x[..., 5] = most
+    x[T // 2:, :, 40] = -most
+    x = x.to(BF).to(DEV)                 # (at most 8 bits: exact)
+    pool = U.pool8(g, T // 16, H, page, D, DEV) if bits == 8 else (
+        tuple(torch.zeros(T // 16, H, page, D // 2, dtype=torch.int8, device=DEV) for _ in range(2)) +
+        tuple(torch.zeros(T // 16, H, page, dtype=HF, device=DEV) for _ in range(2)))
+    want = [t.cpu().clone() for t in pool]
+    at, slots = as_long([0] * T), list(range(T))
+    hq.paged_rope_append(x, x, x, cos, sin, at, as_long(slots), *pool, interleaved=interleaved)
+    y = U.turn(x, cos[at], sin[at], None, 1e-6, interleaved)[0].cpu()
+    if bits == 8:
+        U.append8(want[0], want[2], y, slots)
+    else:
+        c, sc = U.codes4(y)
+        for t in slots:
+            want[0][t // page, :, t % page], want[2][t // page, :, t % page] = c[t], sc[t]
+    assert torch.equal(pool[0].cpu(), want[0]) and torch.equal(pool[2].cpu(), want[2])
 
 
 def test_rope_append_of_nothing_and_into_nothing():
