@@ -1,9 +1,9 @@
 """MI355X-native (gfx950) implementation of HyQuant's hybrid-precision
 attention hot path: per-token KV quantisation (2/4/8 bits), the fused
 four-segment split-K decode, the vertical-line selector, the freeze / flush
-of the decode cache, the hybrid INT8-QK prefill and a paged 4-bit cache with
-the attention that reads it, exposed through the C ABI
-of libhyq.so (include/hyq.h)."""
+of the decode cache, the hybrid INT8-QK prefill, paged caches of 4 and 8 bits with
+the attention that reads them, and the rotation of queries and keys, exposed
+through the C ABI of libhyq.so (include/hyq.h)."""
 
 from .decode_d_stage import (  # noqa: F401
     GROUP_SIZE,

@@ -42,8 +42,14 @@ __device__ __forceinline__ float f16_at(uint32_t w, int hi) { return f16_bits_to
 //       row's own largest t, and l sums P' / v_scale.
 //   PV  O^T[channel][row] = V^T . P'^T with the same instruction, V operands
 //       u 2^-24 again, P' as the sum of two fp16 numbers (2^-21 of a weight is
-//       lost); 128 sum(P') is taken off every RING steps of a wavefront, by products
-//       with a constant.
+//       lost; one fp16 number would be 2^-12 of it, as much as an fp16 output's own
+//       rounding); 128 sum(P') is taken off every RING steps of a wavefront, by
+//       products with a constant, before its fp32 roundings add up.
+// Bound by the cache's bytes: 16 requests of 32K keys (1.08 GB) take 172 to 174 us, 6.2
+// TB/s, where a copy reaches 5.05 and a stream of reads alone 6.8.  48 requests of 700 to
+// 32000 keys in pages of 16 149 us (5.15 TB/s; in pages of 64 146): pieces of unequal
+// length.  Short calls are bound by the chain lengths -> table -> rows -> pieces: 12.7
+// us for one request of 8K keys.
 template <int D>
 struct Raw8 {
     uint32_t k[2][D / 16];               // tile t: channels 16 kb .. and 64 + 16 kb .. of token 16t + 4(c & 3) + (c >> 2)
@@ -303,6 +309,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged8_attn_kerne
 //       V^T by transposing LDS reads.  M follows the row's own largest t, so that
 //       P' keeps to [0, 2^13]; rounding P' to 11 bits once is the only rounding
 //       between the scores and the output.  l sums 2^t / v_scale.
+// Bound by the matrix pipe, the LDS reads that feed it and the VALU work beside it:
+// 2048 tokens at 8192 (309 GFLOP) take 334 to 339 us, 0.92 PFLOP/s where a large matrix
+// product reaches 1.33; of 347 us on another box the products with their LDS reads alone
+// took 224, with the conversion 267, with the softmax 311.  Both halves of a block are pipelined against
+// each other, and the first four wavefronts have priority, as in the 4-bit kernel.
+// Four wavefronts of 64 rows, one a SIMD, read LDS half as often but leave the pipes
+// to one instruction stream: 542 us.  K and V converted by different wavefronts, K's
+// offset taken off there: 342.
 // Output register i of a lane (row l & 31, half h = l >> 5) of a 32-key product
 // is key 8 (i >> 2) + 4 h + (i & 3); registers 8s .. 8s + 7 are the B operand of
 // step s of P.V, without a shuffle.

@@ -189,15 +189,17 @@ __device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
 }
 
 // A lane's channels normalised and rotated, in T; the norm's sum in SUM.  `most`: where it is
-// asked for, the sum of the magnitudes that each value is the sum of.
+// asked for, the sum of the magnitudes that each value is the sum of, 0 where it is not computed.
 template <int D, typename SUM, typename T, bool MOST = false>
 __device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Angles& k, const Weights& w, const float (&x)[8], T (&y)[8],
                                      T (*most)[8] = nullptr) {
     T v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
+    bool rough = false;                  // the inverse root is no normal 32-bit number: the bound does not hold
     if (w.norm) {
         const T inv = static_cast<T>(inv_rms<D, SUM>(x, a.eps));
+        if constexpr (MOST) rough = !(inv >= static_cast<T>(0x1p-120) && inv <= static_cast<T>(0x1p120));
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * static_cast<T>(w.w[i]);
     }
@@ -205,9 +207,8 @@ __device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Ang
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         y[i] = v[i];
-        if constexpr (MOST) (*most)[i] = mag(v[i]);
+        if constexpr (MOST) (*most)[i] = w.norm ? mag(v[i]) : static_cast<T>(0);       // (a value that passes is exact)
     }
-    if (!l.turns) return;
     auto pair = [&](int p, int q, T c, T s) {
         const T f = v[p], g = v[q];
         y[p] = f * c - g * s;
@@ -217,12 +218,17 @@ __device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Ang
             (*most)[q] = mag(g * c) + mag(f * s);
         }
     };
-    if (a.interleaved) {
+    if (l.turns) {
+        if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pair(2 * i, 2 * i + 1, k.c[i], k.s[i]);
-    } else {
+            for (int i = 0; i < 4; ++i) pair(2 * i, 2 * i + 1, k.c[i], k.s[i]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pair(i, i + 4, k.c[i], k.s[i]);
+            for (int i = 0; i < 4; ++i) pair(i, i + 4, k.c[i], k.s[i]);
+        }
+    }
+    if constexpr (MOST) {
+        if (rough) (*most)[0] = static_cast<T>(INFINITY);
     }
 }
 
@@ -236,6 +242,10 @@ __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
 
 // HP heads of a token into contiguous rows: their loads in flight together, the
 // table's row and the weights loaded once.  A position outside the table gives zeros.
+// Bound by bytes, 2 D in and 2 D out of a row, where there are many: four prompts of 8191
+// tokens, 64 + 8 heads of 128 (1.21 GB), take 221 us, 5.5 TB/s, where a copy of
+// 1 GiB reaches 5.05.  A pair in two lanes, each reading and normalising both
+// values of it, took 306.  Few rows are bound by the launch: 16 tokens 3.2 us.
 template <int D, bool F16, int HP>
 __device__ __forceinline__ void rotate_heads(const RopeArgs& a, const Rows& src, uint16_t* dst, const void* w, uint32_t unit, uint32_t heads,
                                              int sub) {
@@ -274,7 +284,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
 // ---- codes of rotated keys ----
 // They are those of the formula: a key is rotated in 32 bits (the norm's sum in 64),
 // and again in 64 bits where 32 bits' error may reach over a code's or a scale's
-// border (a wavefront decides for its rows; one of 50 to 100 does).  The error of
+// border (a wavefront decides for its rows; one of 55 to 95 does, of Gaussian keys).  The error of
 // a value is at most 5 2^-24 of the magnitudes that it is the sum of: the inverse
 // root's rounding, two products, and the rotation's product and sum.
 constexpr float TURN_ERROR = 6.0f * 0x1p-24f;
@@ -316,9 +326,13 @@ __device__ __forceinline__ void key_codes4(const RopeArgs& a, const Lane& l, con
     if (__builtin_amdgcn_ballot_w64(!fine)) {
         double v[8], top = 0.0;
         turn<D, double>(a, l, k, wt, x, v);
+        int nan = 0;                     // (a maximum passes them over)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmax(top, fabs(v[i]));
-        top = fmax(lanes_max<D / 8>(top), 1e-5);
+        for (int i = 0; i < 8; ++i) {
+            top = fmax(top, fabs(v[i]));
+            nan |= v[i] != v[i];
+        }
+        top = lanes_max<D / 8>(nan) ? __builtin_nan("") : fmax(lanes_max<D / 8>(top), 1e-5);
         s16 = static_cast<_Float16>(static_cast<float>(top / 7.0));
         const double sd = static_cast<double>(s16), invd = 1.0 / sd;
 #pragma unroll
@@ -329,7 +343,10 @@ __device__ __forceinline__ void key_codes4(const RopeArgs& a, const Lane& l, con
     }
 }
 
-// q's heads, and a K and a V row of a token and head each
+// q's heads, and a K and a V row of a token and head each, in one launch.  Bound by
+// bytes for many rows: 8191 tokens of 64 + 2 x 8 heads of 128 (311 MB) take 69 us,
+// 4.5 TB/s (with every key in 64 bits 127); 48 decode steps 4.3 us, the
+// launch and slot -> page -> row.
 template <int D, bool F16, int HP>
 __global__ __launch_bounds__(256) void paged_rope_append_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
@@ -411,7 +428,11 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // and are rounded again where the scale has grown.  The rows of a long run that
 // starts at the window's token f are the tokens f .. f + 15: the lanes of the first f
 // rows take those behind the window.  Only where more runs start in it may a second pass
-// be left.
+// be left.  60 chunks of 33 to 1501 tokens, 32 + 2 x 8 heads of 64 (284 MB with q), take
+// 73 us, 3.9 TB/s: q's rows alone 45; VALU issue is half of it, a workgroup's chain
+// slots -> rows and scales -> exponents -> codes the rest.  Windows that are worked on
+// row by row twice (16 tokens and the 16 behind them), K and V apart: 146.  200 decode
+// steps 8 us, the chain, and codes again where a scale grows.
 template <int D, bool F16, bool ROPE, int HP>
 __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
@@ -494,7 +515,9 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
             turn<D, double, float, true>(a, l, k, wt, x, y, &most);
             off = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7]))) * TURN_ERROR;
             // the row's largest may be another value's than the formula's, but not its exponent
-            const float amax = __uint_as_float(largest(y)), far = lanes_max<LPT>(off) + amax * 0x1p-22f;
+            const float amax = __uint_as_float(largest(y));
+            if (!(amax < INFINITY)) off = INFINITY;        // (32 bits do not hold them)
+            const float far = lanes_max<LPT>(off) + amax * 0x1p-22f;
             e = exponent(amax + far);
             if (__builtin_amdgcn_ballot_w64(w.active && !(e == LEAST_E || amax - far > 63.5f * pow2(min(e, 0x60))))) {
                 double v[8], top = 0.0;
@@ -566,7 +589,7 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
                 c[j] = __float_as_uint(z);
             }
             if (ROPE && kind == 0) {
-                if (__builtin_amdgcn_ballot_w64(w.active && !bad && !(edge + off * inv < 0.5f - 0x1p-23f))) {
+                if (__builtin_amdgcn_ballot_w64(w.active && !bad && off != 0.f && !(edge + off * inv < 0.5f - 0x1p-23f))) {
                     double v[8];
                     unpack<F16>(kr, x);
                     turn<D, double>(a, l, k, wt, x, v);
@@ -631,7 +654,8 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
 }
 
 // Rows of the cache by slot as bf16 or fp16 values, code * scale rounded once
-// (exact for bf16); slots outside the pool give zero rows.
+// (exact for bf16); slots outside the pool give zero rows.  HBM-bound: 25000 tokens of 2 x 8
+// heads of 64 (78 MB) take 15 us, 5.2 TB/s.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged8_gather_kernel(Pool pool, uint16_t* ok, uint16_t* ov, uint32_t rows, uint32_t heads) {
     constexpr int LPT = D / 8;
@@ -744,11 +768,14 @@ Pool pool_of(const hyq_paged_pool& p, const int64_t* slots) {
 
 unsigned blocks_of(uint64_t rows, unsigned per) { return static_cast<unsigned>((rows + per - 1) / per); }
 
-// Heads that a lane group takes after the other: with more the table's row and the
-// weights are loaded less often and more loads are in flight, with one the
-// rows of a small step spread over more of the chip.
+// Heads that a lane group takes after the other.  With one the rows of a small step
+// spread over more of the chip, with four the table's row and the weights are
+// loaded less often and more loads are in flight; four from one round of resident
+// wavefronts (8192) on.  Rows of 40 heads of 128 in a captured graph, one and
+// four (us): 64 tokens 2.8 and 4.1, 512 tokens 4.3 and 4.9, 1024 7.4 and 7.1, 4096 21.1
+// and 18.3, 16384 87.4 and 71.0 (eight: 5.5, 6.3, 8.2, 16.6 and 70.8).
 constexpr int MANY = 4;
-bool many_heads(uint64_t rows, int head_dim) { return rows * (head_dim / 8) >= (1 << 20); }
+bool many_heads(uint64_t rows, int head_dim) { return rows * (head_dim / 8) >= 8192 * 64; }
 
 template <bool ROPE, int HP>
 void append8(RopeArgs a, int head_dim, bool fp16, hipStream_t st) {

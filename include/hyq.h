@@ -523,7 +523,8 @@ int hyq_paged_attention(const hyq_paged_params* p, void* workspace, size_t works
  *   (y_a, y_b) <- (y_a cos - y_b sin, y_b cos + y_a sin)
  * for the rotary / 2 channel pairs (a, b) = (i, i + rotary / 2) or, interleaved,
  * (2i, 2i + 1), with cos and sin [rotary / 2] of its position's table row; the
- * channels from rotary on are not rotated.  In fp32, rounded once.
+ * channels from rotary on are not rotated.  In fp32 (squares that it does not hold in
+ * 64 bits), rounded once.
  *   q, k    bf16 (dtype_fp16 = 0) or fp16 [batch, n, heads, head_dim], strides (b, n, h, 1),
  *           16-byte aligned, strides divisible by 8; q_out, k_out the same, contiguous,
  *           sharing no memory with the inputs
@@ -590,7 +591,8 @@ int hyq_paged8_append(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h,
  * of k's rows before any rounding to 16 bits (rotated in 64 bits: scale =
  * fp16(fp32(max(amax, 1e-5) / 7)), code = RNE(k / scale) in a 4-bit pool).  batch = 1,
  * n tokens; k_out is not used.  A token whose position is outside the table or whose
- * slot is outside the pool writes nothing into the cache.
+ * slot is outside the pool writes nothing into the cache.  A row of k that is not finite
+ * has a scale that is not.
  */
 int hyq_paged_rope_append(const hyq_rope_params* p, const uint16_t* v, int64_t v_stride_t, int64_t v_stride_h,
                           const int64_t* slots, const hyq_paged_pool* pool, void* stream);

@@ -126,6 +126,45 @@ def test_norms_of_rows_of_any_magnitude(eps):
     assert torch.equal(pool[0].cpu(), want[0]) and torch.equal(pool[2].cpu(), want[1])
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("norm", [False, True])
+def test_appended_keys_that_are_not_finite_or_hardly(bits, norm):
+    """Rows with an infinity or NaN have scales that are not finite, in their own
+    block alone; rows next to fp32's largest number, and products past it, have
+    their codes."""
+    g = gen(17)
+    T, H, D, page = 64, 2, 64, 16
+    x = randn(g, T, H, D)
+    x[3, 0, 7], x[20, 1, 40] = math.inf, math.nan
+    if norm:
+        x[36] = (x[36].float() * 1e38).clamp(-3e38, 3e38).to(BF)          # the inverse root is no normal fp32 number
+    w = (1 + 0.1 * torch.randn(D, generator=g)).to(DEV) if norm else None
+    cos, sin = U.tables(T, D, device=DEV)
+    if norm:
+        cos[50], sin[50] = 3e38, -3e38   # sums of products past fp32, small in the cache no more than there
+    pool = U.pool8(g, T // 16, H, page, D, DEV) if bits == 8 else (
+        tuple(torch.zeros(T // 16, H, page, D // 2, dtype=torch.int8, device=DEV) for _ in range(2)) +
+        tuple(torch.zeros(T // 16, H, page, dtype=HF, device=DEV) for _ in range(2)))
+    want = [t.cpu().clone() for t in pool]
+    at, v = as_long(list(range(T))), randn(g, T, H, D)
+    hq.paged_rope_append(x, x, v, cos, sin, at, at, *pool, q_weight=w, k_weight=w)
+    y = U.turn(x, cos, sin, w)[0].cpu()
+    if bits == 8:
+        U.append8(want[0], want[2], y, list(range(T)))
+        bad = want[2].isnan()
+        good = ~bad.repeat_interleave(16, -1)
+        assert torch.equal(pool[2].cpu().isnan(), bad) and int(bad.sum()) == (4 if norm else 2)
+    else:
+        for t in range(T):
+            c, sc = U.codes4(y[t])
+            want[0][t // page, :, t % page], want[2][t // page, :, t % page] = c, sc
+        bad = ~want[2].isfinite()
+        good = ~bad
+        assert torch.equal(~pool[2].cpu().isfinite(), bad) and int(bad.sum()) == (4 if norm else 2)
+    assert torch.equal(pool[0].cpu()[good], want[0][good])
+    assert torch.equal(pool[2].cpu()[~bad], want[2][~bad])
+
+
 def test_rotation_by_far_rows_of_a_table():
     """A table past 2^31 values."""
     rows = (1 << 28) + 5
