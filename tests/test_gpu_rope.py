@@ -52,6 +52,18 @@ def test_rotation(dtype, dim, rotary, interleaved, norm, table, shape):
     assert torch.equal(qp, qo.flatten(0, 1)[at]) and torch.equal(kp, ko.flatten(0, 1)[at])
 
 
+def test_rotation_of_rows_past_32_bits():
+    """More than 2^31 values in and out."""
+    T, HQ, HK, D = 240000, 64, 8, 128
+    x = torch.empty(T, HQ + HK, D, dtype=BF, device=DEV)
+    some = torch.tensor([0, 1, T // 2, T - 17, T - 1], device=DEV)
+    x[some] = randn(gen(8), len(some), HQ + HK, D)
+    cos, sin = U.tables(T, D, device=DEV)
+    q, k = hq.qk_norm_rope(x[:, :HQ], x[:, HQ:], cos, sin)
+    check(q[some], *U.turn(x[some, :HQ], cos[some], sin[some]))
+    check(k[some], *U.turn(x[some, HQ:], cos[some], sin[some]))
+
+
 def test_rotation_takes_strides_and_tables_of_each_sequence():
     g = gen(1)
     B, N, HQ, HK, D = 2, 11, 6, 2, 128
@@ -264,6 +276,32 @@ def test_append8_holes_strange_scales_and_values():
     assert torch.equal(pool[0].cpu()[good], want[0][good]) and torch.equal(pool[2].cpu()[good], want[2][good])
     k, _ = hq.paged8_gather(as_long([64 + 2, 96]), *pool)
     assert k[0].isnan().all() and not k[1].any()
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_append8_slots_out_of_order_touch_their_own_blocks_alone(rope):
+    """Slots of a block that are not neighbours, or descend, leave anything in that
+    block; the others are as ever."""
+    g = gen(10)
+    H, D, page, pages = 2, 128, 32, 6
+    pool = U.pool8(g, pages, H, page, D, DEV)
+    want = [t.cpu().clone() for t in pool]
+    wild = [5, 40, 6, 41, 3, 42, 4] + list(range(79, 63, -1)) + [7, 8, 9] * 7            # blocks 0, 2 and 4
+    fine = list(range(96, 130)) + list(range(145, 160))
+    slots = wild + fine
+    x = randn(g, len(slots), H, D)
+    if rope:
+        cos, sin = torch.ones(1, D // 2, device=DEV), torch.zeros(1, D // 2, device=DEV)
+        hq.paged_rope_append(x, x, x, cos, sin, as_long([0] * len(slots)), as_long(slots), *pool)
+    else:
+        hq.paged8_append(x, x, as_long(slots), *pool)
+    U.append8(want[0], want[2], x[len(wild):].double().cpu(), fine)
+    blocks = lambda t: t.cpu().reshape(pages, H, page // 16, -1)  # noqa: E731
+    for a, b in ((pool[0], want[0]), (pool[2], want[2])):
+        a, b = blocks(a).transpose(1, 2).reshape(pages * 2, H, -1), blocks(b).transpose(1, 2).reshape(pages * 2, H, -1)
+        for i in range(pages * 2):
+            if i not in (0, 2, 4):
+                assert torch.equal(a[i], b[i]), i
 
 
 def test_append8_pool_inside_a_larger_allocation_past_32_bits():
