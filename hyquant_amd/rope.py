@@ -14,8 +14,8 @@ half of Hugging Face's rotary embedding: cos[..., :R // 2]).  paged_rope_append
 rotates the queries, and the keys on their way into the pages of a 4-bit
 (hyquant_amd.paged) or 8-bit (hyquant_amd.paged8) cache.
 
-Arithmetic is in 32 bits and rounded once; keys that become codes are rotated in
-64 bits.  Inference only: inputs that record gradients are refused.
+Arithmetic is in 32 bits and rounded once; keys that become codes have those of a
+rotation in 64 bits.  Inference only: inputs that record gradients are refused.
 """
 
 from __future__ import annotations
