@@ -407,6 +407,7 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(RopeArgs a) {
 // rounded again for a larger e.  Values past 127 2^MOST_E (and what is not
 // finite) make the block's scale NaN.
 constexpr int AGAIN = 8;                 // kept rows that are rounded again at a time (5: 8.3 us instead of 8.1 for 200 decode steps)
+constexpr int SKIP = 8;                  // slots a lane looks at together in a stretch without any
 constexpr int LEAST_E = -23;             // of 1e-5
 constexpr int MOST_E = 40, BAD_E = 1 << 20, NO_E = -(1 << 20);
 __device__ __forceinline__ int exponent(double amax) {
@@ -428,11 +429,13 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // and are rounded again where the scale has grown.  The rows of a long run that
 // starts at the window's token f are the tokens f .. f + 15: the lanes of the first f
 // rows take those behind the window.  Only where more runs start in it may a second pass
-// be left.  60 chunks of 33 to 1501 tokens, 32 + 2 x 8 heads of 64 (284 MB with q), take
-// 73 us, 3.9 TB/s: q's rows alone 45; VALU issue is half of it, a workgroup's chain
-// slots -> rows and scales -> exponents -> codes the rest.  Windows that are worked on
-// row by row twice (16 tokens and the 16 behind them), K and V apart: 146.  200 decode
-// steps 8 us, the chain, and codes again where a scale grows.
+// be left.  Tokens whose slot is outside the pool belong to no run and part none:
+// runs that they parted would be two workgroups' on one block.  60 chunks of 33 to
+// 1501 tokens, 32 + 2 x 8 heads of 64 (284 MB with q), take 73 us, 3.9 TB/s: q's rows
+// alone 45; VALU issue is half of it, a workgroup's chain slots -> rows and scales ->
+// exponents -> codes the rest.  Windows that are worked on row by row twice (16 tokens
+// and the 16 behind them), K and V apart: 146.  200 decode steps 8 us, the chain, and
+// codes again where a scale grows.
 template <int D, bool F16, bool ROPE, int HP>
 __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
     constexpr int LPT = D / 8;
@@ -448,26 +451,84 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
 
     for (int j = threadIdx.x; j < 64; j += 2 * D) need[j >> 5][j & 31] = NO_E;
     // ---- the runs: lane l of each wavefront looks at token t0 - 1 + l, up to t0 + 31 ----
+    uint32_t tok = min(max(t0 + lane, 1u) - 1, a.tokens - 1);
+    auto slot_of = [&](uint32_t t) -> int64_t {
+        const int64_t s = a.pool.slots[t];
+        return s >= 0 && s < a.pool.num_slots ? s : -1;
+    };
+    int own = 16;                        // places of the window's own tokens
     int64_t slot = -1;
-    bool ok = true;
-    {
-        const int64_t t = static_cast<int64_t>(t0) + lane - 1;
-        if (lane <= 32 && t >= 0 && t < a.tokens) {
-            slot = a.pool.slots[t];
-            if (slot >= a.pool.num_slots || slot < 0) slot = -1;
-            int64_t unused;
-            if constexpr (ROPE) ok = table_row(a, static_cast<uint32_t>(t), unused);
+    const bool in = lane <= 32 && t0 + lane >= 1 && t0 + lane <= a.tokens;
+    if (in) slot = slot_of(tok);
+    const bool gaps = __builtin_amdgcn_ballot_w64(in && slot < 0);       // (the same in all wavefronts)
+    if (gaps) {
+        // Tokens without a slot do not part a run: the lanes take the tokens that have
+        // one instead, the last before t0 and 32 from it on, however far apart.
+        uint64_t m = __builtin_amdgcn_ballot_w64(slot >= 0) & 0x1fffeu;
+        if (!m) return;
+        own = __builtin_popcountll(m);
+        int64_t before = -1;
+        const int64_t first = __shfl(slot, __builtin_ctzll(m), 64), last = __shfl(slot, 63 - __builtin_clzll(m), 64);
+        if (first & (BLOCK - 1)) {       // (a block's first row starts a run)
+            for (int64_t t = static_cast<int64_t>(t0) - 1 - lane; t + lane >= 0 && before < 0; t -= 64 * SKIP) {
+                int64_t s[SKIP];
+#pragma unroll
+                for (int j = 0; j < SKIP; ++j) s[j] = t - 64 * j >= 0 ? slot_of(static_cast<uint32_t>(t - 64 * j)) : -1;
+#pragma unroll
+                for (int j = 0; j < SKIP; ++j) {
+                    m = __builtin_amdgcn_ballot_w64(s[j] >= 0);
+                    if (m && before < 0) before = __shfl(s[j], __builtin_ctzll(m), 64);
+                }
+            }
+        }
+        slot = lane == 0 ? before : -1;
+        tok = t0;
+        int n = 0;                       // places taken
+        bool more = true;                // the last of the window's own runs may go on
+        for (int64_t t = t0; more && n < 32 && t < a.tokens; t += 64) {
+            if (n >= own) {              // what is between may be long
+                while (t < a.tokens) {
+                    int64_t any = -1;    // (not negative where one of them has a slot)
+#pragma unroll
+                    for (int j = 0; j < SKIP; ++j) {
+                        const int64_t at = t + 64 * j + lane;
+                        any &= at < a.tokens ? slot_of(static_cast<uint32_t>(at)) : -1;
+                    }
+                    if (__builtin_amdgcn_ballot_w64(any >= 0)) break;
+                    t += 64 * SKIP;
+                }
+            }
+            const int64_t at = t + lane, s = at < a.tokens ? slot_of(static_cast<uint32_t>(at)) : -1;
+            m = __builtin_amdgcn_ballot_w64(s >= 0);
+            const int place = 1 + n + __builtin_popcountll(m & ((uint64_t{1} << lane) - 1));
+            const int to = 4 * (s >= 0 && place <= 32 ? place : 63);     // (lane 63 takes no part)
+            const uint32_t lo = __builtin_amdgcn_ds_permute(to, static_cast<int>(s)), hi = __builtin_amdgcn_ds_permute(to, static_cast<int>(s >> 32));
+            const uint32_t who = __builtin_amdgcn_ds_permute(to, static_cast<int>(at));
+            const int until = min(n + __builtin_popcountll(m), 32);
+            if (lane > n && lane <= until) {
+                slot = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+                tok = who;
+            }
+            n = until;
+            const bool other = s >= 0 && at >= t0 + 16u && (s >> 4) != (last >> 4);
+            more = !__builtin_amdgcn_ballot_w64(other || (s >= 0 && (s >> 4) == (last >> 4) && (s & (BLOCK - 1)) == BLOCK - 1));
         }
     }
-    const int64_t block = slot >> 4, before = __shfl_up(block, 1, 64);
-    const uint32_t starts = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(block != before) >> 1);
+    bool ok = true;
+    if constexpr (ROPE) {
+        int64_t unused;
+        if (slot >= 0) ok = table_row(a, tok, unused);
+    }
+    const int64_t block = slot >> 4, ahead = __shfl_up(block, 1, 64);
+    const uint32_t starts = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(block != ahead) >> 1);
     const uint32_t live = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok && slot >= 0) >> 1);
-    if (!(starts & 0xffffu)) return;                                     // (all tokens belong to a run that started before)
-    const int f = __builtin_ctz(starts), end = starts >> 16 ? 16 + __builtin_ctz(starts >> 16) : 32;
+    if (!(starts & ((1u << own) - 1))) return;                           // (all tokens belong to a run that started before)
+    const int f = __builtin_ctz(starts), end = starts >> own ? own + __builtin_ctz(starts >> own) : 32;
     const bool twice = end > 16 + f;
 
     struct Row {
-        int r;                           // the token's place behind t0
+        int r;                           // its place (where no token is without a slot, the token behind t0)
+        uint32_t t;                      // its token
         bool active;
         uint32_t mine;                   // its run's live tokens
         int64_t slot;
@@ -482,6 +543,7 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
         w.mine = live & (0xffffffffu << run) & (more ? (1u << __builtin_ctz(more)) - 1u : 0xffffffffu);
         w.active = !out && (w.mine >> w.r) & 1;
         w.slot = __shfl(slot, w.r + 1, 64);
+        w.t = gaps ? __shfl(tok, w.r + 1, 64) : min(t0 + w.r, a.tokens - 1);
         return w;
     };
     const Lane plain{8 * sub, 8 * sub + 4, false, 0}, l = ROPE ? lane_of(a, sub) : plain;
@@ -489,12 +551,11 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
     Raw kr, vr;
     Angles k{};
     auto load = [&](const Row& w) {
-        const uint32_t t = min(t0 + w.r, a.tokens - 1);
-        kr = load_raw(row_of(a, a.k, t, h), l);
-        vr = load_raw(row_of(a, a.v, t, h), plain);
+        kr = load_raw(row_of(a, a.k, w.t, h), l);
+        vr = load_raw(row_of(a, a.v, w.t, h), plain);
         if constexpr (ROPE) {
             int64_t at;
-            table_row(a, t, at);
+            table_row(a, w.t, at);
             k = load_angles(a, l, at);
         }
     };

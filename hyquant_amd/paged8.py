@@ -62,11 +62,11 @@ def _pool_struct(kp, vp, ks, vs, bits: int) -> "_lib.PagedPool":
 def paged8_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                   k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
     """Put the rows k, v [T, H, D] (bf16 or fp16, any strides) into their slots
-    (int64 [T]).  A slot outside the pool writes nothing.  The slots of one call
-    are distinct, those of one block of 16 are neighbours and ascend (as
-    paged_batch gives them), and the rows of a block before its first new one
-    were appended by earlier calls; rows behind its last new one hold anything
-    after the call.  A block with a value that is not finite, or past 127 * 2^40,
+    (int64 [T]).  A slot outside the pool writes nothing, wherever it stands.  The
+    slots of one call are distinct, those of one block of 16 are neighbours (but for
+    slots outside the pool) and ascend, as paged_batch gives them, and the rows of a
+    block before its first new one were appended by earlier calls; rows behind its
+    last new one hold anything after the call.  A block with a value that is not finite, or past 127 * 2^40,
     has the scale NaN."""
     fx, stream = _fast(k)
     if fx:

@@ -577,9 +577,10 @@ typedef struct hyq_paged_pool {
  * new ones of a block hold anything.  A block with a value that is not finite, or
  * past 127 2^40, has the scale NaN.
  *   slots  int64 [n]; one outside [0, num_pages * page_size) writes nothing.
- *          Precondition: no slot is named twice, the slots of one block are neighbours and
- *          ascend (as hyq_paged_batch gives them), and the rows of a block before the first
- *          have been appended.
+ *          Precondition: no slot is named twice, the slots of one block are neighbours (tokens
+ *          whose slot is outside the pool may stand between them) and ascend (as
+ *          hyq_paged_batch gives them), and the rows of a block before the first have been
+ *          appended.
  */
 int hyq_paged8_append(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v,
                       int64_t v_stride_t, int64_t v_stride_h, int32_t is_fp16, const int64_t* slots,
