@@ -667,7 +667,7 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
             *reinterpret_cast<uint32_t*>(row + (kind ? plain.a : l.a)) = word(0);
             *reinterpret_cast<uint32_t*>(row + (kind ? plain.b : l.b)) = word(4);
             if (w.r != q.first) continue;
-            if (q.kept && now != old) {
+            if (q.kept && !bad && now != old) {              // (a block whose scale is NaN keeps its codes: the old scale brings them back)
                 const float by = old * inv;
                 uint2* const to = reinterpret_cast<uint2*>(rows) + sub;
                 for (int j0 = 0; j0 < q.kept; j0 += AGAIN) {             // (AGAIN rows' loads in flight)

@@ -66,8 +66,14 @@ def paged8_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages
     slots of one call are distinct, those of one block of 16 are neighbours (but for
     slots outside the pool) and ascend, as paged_batch gives them, and the rows of a
     block before its first new one were appended by earlier calls; rows behind its
-    last new one hold anything after the call.  A block with a value that is not finite, or past 127 * 2^40,
-    has the scale NaN."""
+    last new one hold anything after the call.  A block with a value that is not
+    finite, or past 127 * 2^40, has the scale NaN for as long as earlier rows of it
+    stay; their codes are untouched.
+
+    A scale does not fall by itself.  Tokens that are taken back (a rejected draft)
+    have coarsened the block that they share with accepted ones, or made its scale
+    NaN: put its codes and scales back as they were before, or append its tokens
+    again from its first slot on."""
     fx, stream = _fast(k)
     if fx:
         try:

@@ -575,7 +575,8 @@ typedef struct hyq_paged_pool {
  * them stay, and where their scale was larger it stays too, where it was smaller
  * their codes become RNE(code * old / new).  code = RNE(x / scale).  Rows behind the
  * new ones of a block hold anything.  A block with a value that is not finite, or
- * past 127 2^40, has the scale NaN.
+ * past 127 2^40, has the scale NaN, for as long as rows before a call's first stay; the
+ * codes of the rows before the first are untouched then.
  *   slots  int64 [n]; one outside [0, num_pages * page_size) writes nothing.
  *          Precondition: no slot is named twice, the slots of one block are neighbours (tokens
  *          whose slot is outside the pool may stand between them) and ascend (as
