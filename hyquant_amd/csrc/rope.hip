@@ -100,17 +100,27 @@ __device__ __forceinline__ double inv_root(double x) {
     for (int i = 0; i < 2; ++i) r = __builtin_fma(0.5 * r, __builtin_fma(-x * r, r, 1.0), r);
     return r;
 }
-// The inverse root mean square of a row, its squares summed in SUM; in 32 bits (and
-// by the hardware's estimate, a unit in the last place) only where they hold it.
-// (64 bits for every row of a rotation: 232 us where this takes 222.)
+// The mean of a row's squares and eps, in SUM
 template <int D, typename SUM>
-__device__ __forceinline__ SUM inv_rms(const float (&x)[8], double eps) {
+__device__ __forceinline__ SUM mean_square(const float (&x)[8], double eps) {
     SUM sum = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += static_cast<SUM>(x[i]) * static_cast<SUM>(x[i]);
-    sum = lanes_sum<D / 8>(sum) * static_cast<SUM>(1.0 / D) + static_cast<SUM>(eps);
-    if constexpr (std::is_same_v<SUM, double>) return inv_root(sum);
-    else return sum >= 0x1p-90f && sum <= 0x1p120f ? __builtin_amdgcn_rsqf(sum) : static_cast<float>(inv_rms<D, double>(x, eps));
+    return lanes_sum<D / 8>(sum) * static_cast<SUM>(1.0 / D) + static_cast<SUM>(eps);
+}
+// The inverse root mean square of a row, by the hardware's estimate (a unit in the last place) where
+// 32 bits hold the mean, from 64 bits else.  (64 bits for every row of a rotation: 232 us where this
+// takes 222.)  Rows whose inverse is no normal 32-bit number are scaled on the way by a power of two
+// that the inverse makes up for: subnormal rows have inverses up to 2^137.
+template <int D>
+__device__ __forceinline__ float inv_rms(float (&x)[8], double eps) {
+    const float mean = mean_square<D, float>(x, eps);
+    if (mean >= 0x1p-90f && mean <= 0x1p120f) return __builtin_amdgcn_rsqf(mean);
+    const double inv = inv_root(mean_square<D, double>(x, eps));
+    const float by = inv > 0x1p100 ? 0x1p32f : inv < 0x1p-100 ? 0x1p-8f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= by;
+    return static_cast<float>(inv * (1.0f / by));
 }
 
 __device__ __forceinline__ uint32_t batch_of(const RopeArgs& a, uint32_t t) { return a.tokens == a.n ? 0 : t / a.n; }
@@ -198,7 +208,9 @@ __device__ __forceinline__ void turn(const RopeArgs& a, const Lane& l, const Ang
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
     bool rough = false;                  // the inverse root is no normal 32-bit number: the bound does not hold
     if (w.norm) {
-        const T inv = static_cast<T>(inv_rms<D, SUM>(x, a.eps));
+        T inv;
+        if constexpr (std::is_same_v<SUM, float>) inv = inv_rms<D>(v, a.eps);
+        else inv = static_cast<T>(inv_root(mean_square<D, SUM>(x, a.eps)));
         if constexpr (MOST) rough = !(inv >= static_cast<T>(0x1p-120) && inv <= static_cast<T>(0x1p120));
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * static_cast<T>(w.w[i]);
