@@ -352,6 +352,11 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged8_gather(const at::Tensor& slot
 
 using Maybe = std::optional<at::Tensor>;
 
+// Autograd records a gradient of t or carries its tangent (forward mode), or a function transform wraps t
+bool differentiated(const at::Tensor& t) {
+    return !t.has_storage() || (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+}
+
 // The parameter block of rows q, k ([T, heads, D], or [B, N, heads, D]); false: the checked form takes the call
 bool rope_params(hyq_rope_params& p, const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& sin,
                  const Maybe& positions, const Maybe& qw, const Maybe& kw, double eps, bool interleaved) {
@@ -366,6 +371,9 @@ bool rope_params(hyq_rope_params& p, const at::Tensor& q, const at::Tensor& k, c
         return false;
     const int64_t B = d == 4 ? q.size(0) : 1, N = q.size(d - 3), D = q.size(d - 1), rows = cos.size(td - 2), halfr = cos.size(td - 1);
     if ((d == 4 && k.size(0) != B) || k.size(d - 3) != N || k.size(d - 1) != D || q.stride(d - 1) != 1 || k.stride(d - 1) != 1) return false;
+    if (differentiated(q) || differentiated(k) || differentiated(cos) || differentiated(sin) || (qw && differentiated(*qw)) ||
+        (kw && differentiated(*kw)))
+        return false;
     if (halfr < 1 || halfr > 512 || N > INT32_MAX || q.size(d - 2) > INT32_MAX || k.size(d - 2) > INT32_MAX || D > 1024) return false;
     if (positions) {
         const int64_t pd = positions->dim();
@@ -387,9 +395,6 @@ bool rope_params(hyq_rope_params& p, const at::Tensor& q, const at::Tensor& k, c
         fp32 = f;
         *to[i] = w.data_ptr();
     }
-    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || cos.requires_grad() || sin.requires_grad() ||
-                                       (qw && qw->requires_grad()) || (kw && kw->requires_grad())))
-        return false;
     auto stride = [](const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };
     p.q = q.data_ptr();
     p.q_stride_b = d == 4 ? stride(q, 0) : 0;
@@ -442,7 +447,7 @@ Result rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
     const int bits = ks.scalar_type() == at::kFloat ? 8 : 4;
     if (!g_paged.rope_append || q.dim() != 3 || q.numel() == 0 || !ints(positions, at::kLong, 1, dev) ||
         !rope_params(p, q, k, cos, sin, positions, qw, kw, eps, interleaved) || !plain(v, q.scalar_type(), 3, dev) || v.sizes() != k.sizes() ||
-        (at::GradMode::is_enabled() && v.requires_grad()) || !pool(kp, vp, ks, vs, dev, bits) || k.size(1) != kp.size(1) ||
+        differentiated(v) || !pool(kp, vp, ks, vs, dev, bits) || k.size(1) != kp.size(1) ||
         k.size(2) != (bits == 4 ? 2 : 1) * kp.size(3) || !ints(slots, at::kLong, 1, dev) || slots.size(0) != k.size(0) || !rows16(v))
         return skip;
     const c10::DeviceGuard guard(dev);

@@ -15,7 +15,8 @@ rotates the queries, and the keys on their way into the pages of a 4-bit
 (hyquant_amd.paged) or 8-bit (hyquant_amd.paged8) cache.
 
 Arithmetic is in 32 bits and rounded once; keys that become codes have those of a
-rotation in 64 bits.  Inference only: inputs that record gradients are refused.
+rotation in 64 bits.  Inference only: inputs that record gradients or carry
+forward-mode tangents are refused.
 """
 
 from __future__ import annotations
@@ -24,6 +25,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .decode_d_stage import _HALF, _require_gpu, _stream
@@ -33,9 +35,18 @@ from .paged8 import _check_pool8, _pool_struct
 _TABLE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records a gradient of one of the tensors, or carries its tangent (forward mode, which no_grad
+    does not stop), or a function transform wraps it."""
+    grad = torch.is_grad_enabled()
+    return any(t is not None and ((grad and t.requires_grad) or torch._C._functorch.is_functorch_wrapped_tensor(t)
+                                  or forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
+
+
 def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("inputs that record gradients are not supported: call it under torch.no_grad()")
+    if _differentiated(*tensors):
+        raise ValueError("inputs that record gradients or carry tangents are not supported: detach them, or call it under "
+                         "torch.no_grad() (which forward mode ignores)")
 
 
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
