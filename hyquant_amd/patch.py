@@ -205,16 +205,25 @@ def _takes_fused_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: 
     return not _differentiated(q, k, cos, sin, *weights)
 
 
+def _only_norms(cls, *modules: torch.nn.Module) -> bool:
+    """Whether calling the modules is cls's own forward and nothing else: no hook (which may observe, change or
+    bring in what the module works on) and no forward put in its place."""
+    hooks = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+    return not any(type(m) is not cls or "forward" in m.__dict__ or any(getattr(m, h) for h in hooks) for m in modules) and not any(
+        getattr(torch.nn.modules.module, "_global" + h) for h in hooks)
+
+
 def build_attention_forward(family: str, *, mode: str, window_size: int, top_ratio: float, fused_rope: bool = False):
     """Patched forward of a Llama-3 ("llama") or Qwen3 ("qwen", q/k RMS norms)
     attention module (src/patch/patch_llama.py:27-259, src/patch/patch_qwen.py).
     fused_rope: the head norms and the rotation in one launch (qk_norm_rope, rounded
     once) instead of the module's own torch operations, which round after each;
-    where a gradient is recorded or a tangent carried, or on the CPU, the module's own are used."""
+    where a gradient is recorded or a tangent carried, on the CPU, or where q_norm or
+    k_norm has hooks or another forward, the module's own are used."""
     if family == "llama":
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb, eager_attention_forward
     elif family == "qwen":
-        from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb, eager_attention_forward
+        from transformers.models.qwen3.modeling_qwen3 import Qwen3RMSNorm, apply_rotary_pos_emb, eager_attention_forward
     else:
         raise ValueError(f"unknown model family '{family}'")
     d_mode = is_d_stage_mode(mode)
@@ -237,9 +246,11 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
         k = self.k_proj(hidden_states).view(hidden_shape)
         cos, sin = position_embeddings
         norms = {}
-        if fused_rope and family == "qwen":
-            norms = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight)
-        if fused_rope and _takes_fused_rope(q, k, cos, sin, *norms.values()):
+        fused = fused_rope
+        if fused and family == "qwen":
+            fused = _only_norms(Qwen3RMSNorm, self.q_norm, self.k_norm)
+            norms = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight) if fused else {}
+        if fused and _takes_fused_rope(q, k, cos, sin, *norms.values()):
             half = cos.shape[-1] // 2
             if norms:
                 norms["eps"] = self.q_norm.variance_epsilon
