@@ -44,7 +44,7 @@ import torch
 
 from .d_stage_kv_cache import DStageKVCache
 from .decode_d_stage import _HALF, _dequantize_by_bits, _quantize_by_bits
-from .rope import _differentiated, qk_norm_rope
+from .rope import _TABLE_TYPES, _differentiated, qk_norm_rope
 from .sage_unified import sage_vertical_attention_v2
 from .vertical import compute_vertical_indices
 
@@ -197,7 +197,11 @@ def _quant_roundtrip_decode(q, k, v, mode: str, window_size: int, top_ratio: flo
 def _takes_fused_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *weights: torch.Tensor) -> bool:
     """Whether qk_norm_rope takes a module's rows [B, N, heads, D], its embedding [B or 1, N, R] and its norms'
     weights, with no gradient of any to record and no tangent to carry."""
-    if not q.is_cuda or q.dtype not in _HALF or q.shape[-1] not in (64, 128) or cos.dim() != 3 or cos.shape != sin.shape:
+    if not q.is_cuda or q.dtype not in _HALF or k.dtype != q.dtype or q.shape[-1] not in (64, 128) or cos.dim() != 3 or cos.shape != sin.shape:
+        return False
+    if cos.dtype not in _TABLE_TYPES or sin.dtype != cos.dtype or any(w.dtype not in (torch.float32, q.dtype) for w in weights):
+        return False
+    if any(type(t) is not torch.Tensor for t in (q, k, cos, sin)) or any(t.device != q.device for t in (k, cos, sin, *weights)):
         return False
     r = cos.shape[-1]
     if r % 16 or not 0 < r <= q.shape[-1] or cos.shape[0] not in (1, q.shape[0]) or cos.shape[1] != q.shape[1]:
@@ -218,8 +222,9 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
     attention module (src/patch/patch_llama.py:27-259, src/patch/patch_qwen.py).
     fused_rope: the head norms and the rotation in one launch (qk_norm_rope, rounded
     once) instead of the module's own torch operations, which round after each;
-    where a gradient is recorded or a tangent carried, on the CPU, or where q_norm or
-    k_norm has hooks or another forward, the module's own are used."""
+    where a gradient is recorded or a tangent carried, on the CPU, for types that it does
+    not take, or where q_norm or k_norm has hooks or another forward, the module's own
+    are used."""
     if family == "llama":
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb, eager_attention_forward
     elif family == "qwen":

@@ -113,3 +113,37 @@ def test_norms_of_another_class():
     k.load_state_dict(at.k_norm.state_dict())
     at.k_norm = k
     assert same(both(m, x))
+
+
+@pytest.mark.parametrize("what", ["weights in fp16", "weights in fp64", "one weight in fp64", "keys in fp32", "angles in fp64"])
+def test_types_that_the_rotation_does_not_take(what):
+    """What the modules compute without fused_rope, they compute with it."""
+    from hyquant_amd import patch
+    m, x = model()
+    at = m.model.layers[0].self_attn
+    if what == "keys in fp32":
+        at.k_proj.float()
+        project = at.k_proj.forward
+        at.k_proj.forward = lambda y: project(y.float())
+    elif what != "angles in fp64":
+        to = torch.float16 if "fp16" in what else torch.float64
+        for n in (at.k_norm,) if "one" in what else (at.q_norm, at.k_norm):
+            n.weight.data = n.weight.data.to(to)
+    cos, sin = m.model.rotary_emb(x, torch.arange(x.shape[1], device=DEV)[None])
+    if what == "angles in fp64":
+        cos, sin = cos.double(), sin.double()
+    keys = []
+
+    class Done(Exception):
+        pass
+
+    class Only:
+        def update(self, k, v, layer, kw):
+            keys.append(k)
+            raise Done                   # (the attention behind would want one type of all)
+
+    for fused in (False, True):
+        fwd = patch.build_attention_forward("qwen", mode="dense", window_size=W, top_ratio=0.05, fused_rope=fused)
+        with torch.no_grad(), pytest.raises(Done):
+            fwd(at, x, (cos, sin), past_key_values=Only())
+    assert keys[0].dtype == keys[1].dtype and torch.equal(*keys)
