@@ -223,8 +223,8 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
     fused_rope: the head norms and the rotation in one launch (qk_norm_rope, rounded
     once) instead of the module's own torch operations, which round after each;
     where a gradient is recorded or a tangent carried, on the CPU, for types that it does
-    not take, or where q_norm or k_norm has hooks or another forward, the module's own
-    are used."""
+    not take, or where q_norm or k_norm has hooks, another forward or another eps than
+    the other, the module's own are used."""
     if family == "llama":
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb, eager_attention_forward
     elif family == "qwen":
@@ -253,7 +253,7 @@ def build_attention_forward(family: str, *, mode: str, window_size: int, top_rat
         norms = {}
         fused = fused_rope
         if fused and family == "qwen":
-            fused = _only_norms(Qwen3RMSNorm, self.q_norm, self.k_norm)
+            fused = _only_norms(Qwen3RMSNorm, self.q_norm, self.k_norm) and self.q_norm.variance_epsilon == self.k_norm.variance_epsilon
             norms = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight) if fused else {}
         if fused and _takes_fused_rope(q, k, cos, sin, *norms.values()):
             half = cos.shape[-1] // 2

@@ -147,3 +147,18 @@ def test_types_that_the_rotation_does_not_take(what):
         with torch.no_grad(), pytest.raises(Done):
             fwd(at, x, (cos, sin), past_key_values=Only())
     assert keys[0].dtype == keys[1].dtype and torch.equal(*keys)
+
+
+@pytest.mark.parametrize("eps", [(1e-6, 0.5), (0.25, 1e-6), (0.5, 0.5)])
+def test_each_norm_has_its_own_eps(eps):
+    m, x = model()
+    at = m.model.layers[0].self_attn
+    at.q_norm.variance_epsilon, at.k_norm.variance_epsilon = eps
+    outs = both(m, x)
+    if eps[0] != eps[1]:
+        assert same(outs)
+    else:                                # (one launch for both; its roundings are others)
+        own, fused = outs
+        plain = both(model()[0], x)[0]
+        far = (own[1].double() - plain[1].double()).norm()
+        assert not same(outs) and (own[1].double() - fused[1].double()).norm() < far / 8
