@@ -775,9 +775,10 @@ int check_rope(const std::string& w, const hyq_rope_params* p, bool cache) {
     if (p->table_type < 0 || p->table_type > 2 || (p->weight_fp32 | 1) != 1 || (p->interleaved | 1) != 1) return fail(HYQ_EINVAL, w + "bad type or order");
     if (!(p->eps >= 0.0) || std::isinf(p->eps)) return fail(HYQ_EINVAL, w + "eps must be finite and >= 0");
     // (batch and n apart: their product may pass 64 bits; an append has up to four rows' threads for a key head)
-    const int64_t most = MOST_THREADS / (p->head_dim / 8), heads = std::max(p->q_heads + 4 * p->k_heads, 1);
-    if (p->n > most || p->batch > most || (p->n && p->batch > most / p->n) || p->batch * p->n > (most / heads) - 32)
-        return fail(HYQ_ENOTSUP, w + "more than " + std::to_string(most) + " rows");
+    const int64_t rows = MOST_THREADS / (p->head_dim / 8), heads = std::max(p->q_heads + (cache ? 4 : 1) * p->k_heads, 1);
+    const int64_t most = rows / heads - 32;
+    if (p->n > rows || p->batch > rows || (p->n && p->batch > rows / p->n) || p->batch * p->n > most)
+        return fail(HYQ_ENOTSUP, w + "more than " + std::to_string(most) + " tokens of " + std::to_string(p->q_heads) + " + " + std::to_string(p->k_heads) + " heads");
     if (p->batch == 0 || p->n == 0) return HYQ_OK;
     if (p->q_heads && (!p->q || !p->q_out)) return fail(HYQ_EINVAL, w + "null q");
     if (p->k_heads && (!p->k || (!cache && !p->k_out))) return fail(HYQ_EINVAL, w + "null k");
@@ -945,7 +946,8 @@ extern "C" int hyq_paged8_append(const uint16_t* k, int64_t k_stride_t, int64_t 
     if (kv_heads < 1 || kv_heads > 65535) return fail(HYQ_EINVAL, w + "key heads out of range");
     if (is_fp16 != 0 && is_fp16 != 1) return fail(HYQ_EINVAL, w + "is_fp16 must be 0 or 1");
     const int64_t most = MOST_THREADS / (head_dim / 8);
-    if (num_tokens > most / (4 * kv_heads) - 32) return fail(HYQ_ENOTSUP, w + "more than " + std::to_string(most) + " rows");
+    if (num_tokens > most / (4 * kv_heads) - 32)
+        return fail(HYQ_ENOTSUP, w + "more than " + std::to_string(most / (4 * kv_heads) - 32) + " tokens of " + std::to_string(kv_heads) + " heads");
     if (num_tokens == 0 || pool->num_pages == 0) return HYQ_OK;
     if (!k || !v || !slots || !aligned(slots, 8)) return fail(HYQ_EINVAL, w + "k, v or slots null or misaligned");
     if (!rows16(k, k_stride_t, k_stride_h, 0) || !rows16(v, v_stride_t, v_stride_h, 0))
