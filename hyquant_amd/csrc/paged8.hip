@@ -308,7 +308,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged8_attn_kerne
 //   PV  O^T[channel][row] = V^T . P'^T, P' = fp16(2^t) against the exact codes,
 //       V^T by transposing LDS reads.  M follows the row's own largest t, so that
 //       P' keeps to [0, 2^13]; rounding P' to 11 bits once is the only rounding
-//       between the scores and the output.  l sums 2^t / v_scale.
+//       between the scores and the output.  l sums 2^t / v_scale.  Against 64 bits
+//       and relative to the outputs, bf16 is off by 1.67e-3 (its own rounding
+//       1.66e-3), fp16 by 2.8e-4 (2.1e-4).  P' in two fp16 numbers, as above, leaves
+//       the outputs' own roundings and takes 453 us where this takes 344 (2048 tokens
+//       at 8192), 117 where this takes 98.6 (chunks beside decode steps).
 // Bound by the matrix pipe, the LDS reads that feed it and the VALU work beside it:
 // 2048 tokens at 8192 (309 GFLOP) take 334 to 339 us, 0.92 PFLOP/s where a large matrix
 // product reaches 1.33; of 347 us on another box the products with their LDS reads alone

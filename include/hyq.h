@@ -613,7 +613,8 @@ int hyq_paged8_gather(const int64_t* slots, int64_t num_tokens, int32_t kv_heads
  * s_stride_head, 1).  The codes enter the products as exact operands, a block's
  * scales as constants of the fp32 scores; a weight times its V scale is then
  * rounded once: for requests of at most 16 rows to the sum of two fp16 numbers
- * (2^-21), for larger requests to fp16 (2^-11).  A row that sees a key
+ * (2^-21), for larger requests to fp16 (2^-11, as much as an fp16 output's own
+ * rounding).  A row that sees a key
  * whose block's K or V scale is not within [2^-40, 2^48] is NaN, its lse too.
  */
 size_t hyq_paged8_attention_workspace_size(const hyq_paged_params* p);
