@@ -314,10 +314,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 4 : 3) void paged8_attn_kerne
 //       the outputs' own roundings and takes 453 us where this takes 344 (2048 tokens
 //       at 8192), 117 where this takes 98.6 (chunks beside decode steps).
 // Bound by the matrix pipe, the LDS reads that feed it and the VALU work beside it:
-// 2048 tokens at 8192 (309 GFLOP) take 334 to 339 us, 0.92 PFLOP/s where a large matrix
-// product reaches 1.33; of 347 us on another box the products with their LDS reads alone
-// took 224, with the conversion 267, with the softmax 311.  Both halves of a block are pipelined against
-// each other, and the first four wavefronts have priority, as in the 4-bit kernel.
+// 2048 tokens at 8192 (309 GFLOP) take 334 to 362 us by box, 0.85 to 0.92 PFLOP/s where
+// a large matrix product reaches 1.33; of 347 us on another box the products with their
+// LDS reads alone took 224, with the conversion 267, with the softmax 311.  Both halves
+// of a block are pipelined against each other, and the first four wavefronts have
+// priority, as in the 4-bit kernel.
 // Four wavefronts of 64 rows, one a SIMD, read LDS half as often but leave the pipes
 // to one instruction stream: 542 us.  K and V converted by different wavefronts, K's
 // offset taken off there: 342.
