@@ -475,7 +475,10 @@ __global__ __launch_bounds__(2 * D, 4) void paged8_append_kernel(RopeArgs a) {
     const bool gaps = __builtin_amdgcn_ballot_w64(in && slot < 0);       // (the same in all wavefronts)
     if (gaps) {
         // Tokens without a slot do not part a run: the lanes take the tokens that have
-        // one instead, the last before t0 and 32 from it on, however far apart.
+        // one instead, the last before t0 and 32 from it on, however far apart: 4000
+        // tokens without any beside 5 cost nothing that shows, 100000 0.2 ms.  (The whole
+        // workgroup's search takes 50 us there, and its code costs 1.3 to 3 of the 92 us
+        // of the 60 chunks.)
         uint64_t m = __builtin_amdgcn_ballot_w64(slot >= 0) & 0x1fffeu;
         if (!m) return;
         own = __builtin_popcountll(m);
